@@ -113,6 +113,24 @@ int sna_qkv_norm_rope_store(const void *qkv, int64_t qkv_stride, int64_t n_token
                             void *k_cache, void *v_cache, const float *k_scale, const float *v_scale,
                             int64_t num_blocks, int32_t page_size, int32_t cache_dtype, void *stream);
 
+/* The writer for rotary positions with several axes (time, height, width of images and video): the projection's output
+ * qkv [n_tokens, (num_q_heads + 2 num_kv_heads) * head_dim] bf16 (row stride qkv_stride), per-head RMSNorm of Q and K when
+ * the gammas [head_dim] bf16 are given (both or neither), pair i of a Q or K head (elements i and i + n_pairs) rotated by
+ * the angle positions[axes[i], t] * inv_freq[i], the elements past 2 n_pairs as they are, Q written to q_out, K and V
+ * stored at `slots` as sna_qkv_norm_rope_store stores them.
+ *   positions  [n_axes, n_tokens] int64 (row stride pos_stride), any values; n_axes 1 to 4.
+ *   inv_freq   [n_pairs] fp32; n_pairs a multiple of 8, at most head_dim / 2.
+ *   axes       HOST array [n_pairs], each below n_axes.
+ * Angles are formed in 64 bits; norm and rotation are fp32 and every output is rounded once (bf16, or e4m3fn(x / s)).
+ * cache_dtype SNA_DTYPE_BF16 or SNA_DTYPE_FP8_E4M3FN; head_dim 64 or 128.
+ * This has no reference counterpart (its rope takes one position a token, ops/attention/qkv_paged.py:56-60). */
+int sna_qkv_norm_mrope_store(const void *qkv, int64_t qkv_stride, int64_t n_tokens, int32_t num_q_heads,
+                             int32_t num_kv_heads, int32_t head_dim, const void *q_norm, const void *k_norm, float eps,
+                             const int64_t *positions, int64_t pos_stride, int32_t n_axes, const float *inv_freq,
+                             int32_t n_pairs, const uint8_t *axes, const int64_t *slots, void *q_out, void *k_cache,
+                             void *v_cache, const float *k_scale, const float *v_scale, int64_t num_blocks,
+                             int32_t page_size, int32_t cache_dtype, void *stream);
+
 /* Per-head absmax scales, s[h] = max |x[:, h, :]| / 448, or 1 for an all-zero head.
  *   x         [n_tokens, num_heads, head_dim] bf16.
  *   scale_out [num_heads] fp32.
@@ -441,6 +459,69 @@ int sna_prefill_attention_split(const void *q, const void *k_cache, const void *
                                 int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
                                 int64_t num_blocks, int32_t kv_dtype, void *workspace, int64_t workspace_bytes,
                                 void *stream);
+
+/* =====================================================================================================
+ * Attention weights of cached keys, and eviction by them
+ * ===================================================================================================== */
+
+/* The attention weight that the cached keys of one layer receive from a batch of queries, over the pool:
+ *   weights[r, g, j] (+)= sum over request r's queries i and the query heads h of KV head g of p(i, h, j),
+ * p the softmax probabilities that sna_prefill_attention uses (sinks and window included). Arguments as there; instead
+ * of an output:
+ *   weights   [R, num_kv_heads, width] fp32, strides row_stride and head_stride (at least width). accumulate != 0: the
+ *             requests' keys (valid ones below width) are added to, the rest is left as it is; 0: every column is
+ *             written, zero where there is no key.
+ *   workspace device, 16-byte aligned, at least sna_attention_weights_workspace_bytes bytes, any contents; calls that
+ *             share one on different streams race.
+ * Every sum runs in a fixed order: the same call gives the same bits. The queries' rows of q lie inside [0, n_tokens);
+ * offsets outside are cut. head_dim 64 or 128, any page size, num_q_heads / num_kv_heads <= 128.
+ * This has no reference counterpart. */
+int64_t sna_attention_weights_workspace_bytes(int32_t n_tokens, int32_t R, int32_t max_q_len, int32_t num_q_heads,
+                                              int32_t num_kv_heads, int32_t page_size, int32_t table_width,
+                                              int32_t width);
+int sna_prefill_attention_weights(const void *q, const void *k_cache, const float *k_scale, const int32_t *block_table,
+                                  int64_t table_stride, int32_t table_width, const int32_t *q_start,
+                                  const int32_t *prior_lens, int32_t n_tokens, int32_t R, int32_t max_q_len,
+                                  const float *sinks, float sm_scale, int32_t window, float *weights,
+                                  int64_t row_stride, int64_t head_stride, int32_t width, int32_t accumulate,
+                                  int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                                  int64_t num_blocks, int32_t kv_dtype, void *workspace, int64_t workspace_bytes,
+                                  void *stream);
+
+/* The same for a decode step: row b has one query q[b] (q [B, num_q_heads, head_dim]) at position seq_lens[b] - 1, whose
+ * key is in the pool already (the decode entry points store it at new_slots). A row of seq_len 0 or less has no keys. The
+ * workspace is that of n_tokens = R = B, max_q_len = 1. */
+int sna_decode_attention_weights(const void *q, const void *k_cache, const float *k_scale, const int32_t *block_table,
+                                 int64_t table_stride, int32_t table_width, const int32_t *seq_lens, int32_t B,
+                                 const float *sinks, float sm_scale, int32_t window, float *weights,
+                                 int64_t row_stride, int64_t head_stride, int32_t width, int32_t accumulate,
+                                 int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                                 int64_t num_blocks, int32_t kv_dtype, void *workspace, int64_t workspace_bytes,
+                                 void *stream);
+
+/* The tokens that each (row, KV head) keeps, by weight: a row of L = seq_lens[r] tokens (held to [0, width]) keeps all of
+ * them where L <= keep; else its first `first`, its last `recent`, and of the others the keep - first - recent of the
+ * largest weights (equal weights: the lowest position; -0 equals 0, NaN ranks above every number). Exact.
+ *   weights   [R, num_kv_heads, width] fp32 (strides as above).
+ *   kept      [R, num_kv_heads, keep] int32: the positions in ascending order, -1 past a short row's.
+ *   new_lens  [R] int32: min(L, keep).
+ *   weights_out [R, num_kv_heads, out_width] fp32 (out_width >= keep): the kept tokens' weights, then zeros; or NULL. It
+ *             may be `weights` itself (same address and strides), and overlaps it in no other way. */
+int sna_select_tokens(const float *weights, int64_t row_stride, int64_t head_stride, int32_t width,
+                      const int32_t *seq_lens, int32_t R, int32_t num_kv_heads, int32_t keep, int32_t first,
+                      int32_t recent, int32_t *kept, int32_t *new_lens, float *weights_out, int64_t out_row_stride,
+                      int64_t out_head_stride, int32_t out_width, void *stream);
+
+/* Moves the kept tokens' K and V together: token kept[r, g, i] of KV head g of row r, read through block_table, goes to
+ * position i of the row's pages in dst_table ([R, dst_width] int32), or in block_table's own (dst_table NULL: in place,
+ * where kept must ascend, as sna_select_tokens writes it). Entries of -1 move nothing, nor does a token whose source or
+ * target lies past its table or on an invalid page. Bytes move as they are (the scales are the head's). A page that two
+ * rows share may be read through both, not written: evict such rows to pages of their own, and let dst_table name no page
+ * that block_table names. head_dim 64 or 128; the caches as for sna_kv_store_mha. */
+int sna_compact_tokens(void *k_cache, void *v_cache, int64_t num_blocks, int32_t num_kv_heads, int32_t page_size,
+                       int32_t head_dim, int32_t cache_dtype, const int32_t *block_table, int64_t table_stride,
+                       int32_t table_width, const int32_t *dst_table, int64_t dst_stride, int32_t dst_width,
+                       const int32_t *kept, int32_t R, int32_t keep, void *stream);
 
 /* =====================================================================================================
  * DSA indexer (the step that picks the sparse decode's positions)

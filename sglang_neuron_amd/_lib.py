@@ -68,6 +68,8 @@ SIGNATURES = {
     "sna_kv_store_mha": (_I32, [_P, _P, _P, _I64, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P]),
     "sna_qkv_norm_rope_store": (_I32, [_P, _I64, _I64, _I32, _I32, _I32, _P, _P, ctypes.c_float, _P, _P, _I64, _P, _P,
                                         _P, _P, _P, _P, _I64, _I32, _I32, _P]),
+    "sna_qkv_norm_mrope_store": (_I32, [_P, _I64, _I64, _I32, _I32, _I32, _P, _P, _F32, _P, _I64, _I32, _P, _I32, _P, _P,
+                                        _P, _P, _P, _P, _P, _I64, _I32, _I32, _P]),
     "sna_absmax_workspace_bytes": (_I64, [_I64, _I32]),
     "sna_kv_absmax_scale": (_I32, [_P, _I64, _I32, _I32, _P, _P, _I64, _P]),
     "sna_kv_store_mla": (_I32, [_P, _P, _I64, _I32, _P, _P, _I64, _I32, _P]),
@@ -94,6 +96,15 @@ SIGNATURES = {
     "sna_prefill_attention_split": (_I32, [_P, _P, _P, _P, _P, _P, _I64, _I32, _P, _P, _I32, _I32, _P, _F32, _I32, _P,
                                      _I32, _I32, _I32, _I32, _I64, _I32, _P, _I64, _P]),
     "sna_prefill_workspace_bytes": (_I64, [_I32] * 8),
+    "sna_attention_weights_workspace_bytes": (_I64, [_I32] * 8),
+    "sna_prefill_attention_weights": (_I32, [_P, _P, _P, _P, _I64, _I32, _P, _P, _I32, _I32, _I32, _P, _F32, _I32, _P,
+                                             _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _I64, _I32, _P, _I64, _P]),
+    "sna_decode_attention_weights": (_I32, [_P, _P, _P, _P, _I64, _I32, _P, _I32, _P, _F32, _I32, _P, _I64, _I64, _I32,
+                                            _I32, _I32, _I32, _I32, _I32, _I64, _I32, _P, _I64, _P]),
+    "sna_select_tokens": (_I32, [_P, _I64, _I64, _I32, _P, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _I64, _I64, _I32,
+                                 _P]),
+    "sna_compact_tokens": (_I32, [_P, _P, _I64, _I32, _I32, _I32, _I32, _P, _I64, _I32, _P, _I64, _I32, _P, _I32, _I32,
+                                  _P]),
     "sna_index_key_store": (_I32, [_P, _P, _I64, _I32, _P, _I64, _P]),
     "sna_indexer_scores": (_I32, [_P, _P, _P, _P, _I64, _I32, _P, _I32, _I32, _I32, _I32, _I64, _I32, _P, _I64, _P]),
     "sna_page_items_wire_bytes": (_I64, [_P, _I32, _I64]),

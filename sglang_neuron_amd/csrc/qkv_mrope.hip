@@ -1,0 +1,234 @@
+// The QKV writer for rotary positions with several axes (time, height, width of images and video): per-head RMSNorm of Q
+// and K (optional), the rotation of pair i (elements i and i + rot / 2 of a head's first rot) by the angle
+//   positions[axis(i), t] * inv_freq[i],
+// Q written out and K / V stored into the paged MHA pool (bf16, or e4m3fn with per-KV-head scales), in one pass over the
+// projection's output.
+//
+// Angles are formed in turns in 64 bits (position * (inv_freq / 2 pi), less its whole part), so positions of any size keep
+// the fraction that 32 bits would lose; sine and cosine of the fraction are fp32. The norm and the rotation are fp32 and
+// each output is rounded once: Q and a bf16 pool to bf16, an FP8 pool to e4m3fn(x / s). (The one-axis writer rounds its
+// intermediate steps to bf16 as the reference's torch path does; this operator has no such path to follow.)
+//
+// A workgroup takes 8 tokens, two to a wave, and one group of 64 / (D / 8) consecutive heads; lane j of a head holds its
+// elements 8 j .. 8 j + 7 (one 16-byte load). The tokens' sines and cosines are computed once by the workgroup's threads
+// and passed through LDS. Bound by memory: every projection row is read once, every Q, K and V row written once.
+#include "sna_device.h"
+#include "sna_host.h"
+
+namespace sna {
+
+struct MropeArgs {
+  const uint16_t* qkv;  // [T, (Hq + 2 Hkv) D]
+  int64_t qkv_stride, T;
+  int32_t Hq, Hkv;
+  const uint16_t* q_norm;  // [D], or both null
+  const uint16_t* k_norm;
+  float eps;
+  const int64_t* positions;  // [A, T]
+  int64_t pos_stride;
+  const float* inv_freq;  // [half]
+  int32_t half;           // rotated pairs
+  uint64_t axes[2];       // 2 bits a pair
+  const int64_t* slots;
+  uint16_t* q_out;  // [T, Hq, D]
+  uint8_t* k_cache;
+  uint8_t* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t num_slots;
+  int32_t P;
+};
+
+constexpr int kMropeTokens = 8;  // of a workgroup
+
+// e4m3fn(clamp(x / s)) of two floats, as a 16-bit pair of bytes.
+__device__ __forceinline__ uint32_t mrope_fp8_pair(float x0, float x1, float s, float rs, bool rcp_ok) {
+  uint32_t b;
+  if (rcp_ok) b = quantize_pair_e4m3fn_hw_nonan(x0, x1, s, rs);
+  else b = f32_to_e4m3fn(clamp_fp8(x0 / s)) | f32_to_e4m3fn(clamp_fp8(x1 / s)) << 8;
+  if (x0 != x0) b = (b & 0xff00u) | (__float_as_uint(x0) >> 24 & 0x80u) | 0x7fu;
+  if (x1 != x1) b = (b & 0x00ffu) | ((__float_as_uint(x1) >> 24 & 0x80u) | 0x7fu) << 8;
+  return b;
+}
+
+template <bool FP8, int D>
+__global__ __launch_bounds__(256) void qkv_norm_mrope_store_kernel(MropeArgs a) {
+  constexpr int LPH = D / 8, HPW = 64 / LPH, U = kMropeTokens / 4;
+  __shared__ float sm_cos[kMropeTokens][D / 2], sm_sin[kMropeTokens][D / 2];
+  const int tid = threadIdx.x, lane = tid & 63, sub = lane % LPH;
+  const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)(tid >> 6));
+  const int32_t heads = a.Hq + 2 * a.Hkv;
+  const int32_t head = (int32_t)blockIdx.y * HPW + lane / LPH;
+  const bool head_ok = head < heads;
+  const bool is_q = head < a.Hq, is_k = !is_q && head < a.Hq + a.Hkv, roped = head < a.Hq + a.Hkv;
+  const int64_t tb = (int64_t)blockIdx.x * kMropeTokens, t0 = tb + wave * U;
+  uint4 w[U];
+#pragma unroll
+  for (int k = 0; k < U; ++k)
+    w[k] = t0 + k < a.T && head_ok ? ld16_stream(a.qkv + (t0 + k) * a.qkv_stride + (int64_t)head * D + 8 * sub)
+                                   : make_uint4(0, 0, 0, 0);
+  for (int p = tid; p < kMropeTokens * a.half; p += 256) {
+    const int k = p / a.half, i = p - k * a.half;
+    if (tb + k >= a.T) break;
+    const int axis = (int)(a.axes[i >> 5] >> (2 * (i & 31)) & 3);
+    const double turns = (double)a.positions[axis * a.pos_stride + tb + k] * ((double)a.inv_freq[i] * 0.15915494309189535);
+    const float f = 2.0f * (float)(turns - rint(turns));  // half turns, in [-1, 1]
+    sm_cos[k][i] = cospif(f);
+    sm_sin[k][i] = sinpif(f);
+  }
+  float gf[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) gf[e] = 1.0f;
+  if (a.q_norm && head_ok && roped) {
+    const uint4 gw = ld16((is_q ? a.q_norm : a.k_norm) + 8 * sub);
+    const uint32_t gg[4] = {gw.x, gw.y, gw.z, gw.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) gf[e] = bf16_bits_to_f32(gg[e / 2] >> (16 * (e & 1)) & 0xffffu);
+  }
+  const int32_t h = head - a.Hq - (is_k ? 0 : a.Hkv);  // the KV head (K and V lanes)
+  float scl = 1.0f, rs = 1.0f;
+  bool rcp_ok = false;
+  if (FP8 && head_ok && !is_q) {
+    scl = is_k ? a.k_scale[h] : a.v_scale[h];
+    rcp_ok = rcp_scale_ok(scl);
+    rs = rcp_ok ? 1.0f / scl : 1.0f;
+  }
+  uint8_t* const cache = is_k ? a.k_cache : a.v_cache;
+  // the rotation partner of the lane's elements, half elements away, and their sign
+  const bool rotated = roped && 8 * sub < 2 * a.half, first = 8 * sub < a.half;
+  const int partner = rotated ? lane + (first ? a.half / 8 : -(a.half / 8)) : lane;
+  const int pair0 = first ? 8 * sub : 8 * sub - a.half;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int64_t t = t0 + k;
+    if (t >= a.T) break;  // uniform
+    const uint32_t ww[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+    float x[8], y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = bf16_bits_to_f32(ww[e / 2] >> (16 * (e & 1)) & 0xffffu);
+    if (a.q_norm) {  // uniform
+      float ss = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+      for (int off = LPH / 2; off > 0; off >>= 1) ss += __shfl_xor(ss, off, 64);
+      const float inv = 1.0f / sqrtf(ss / (float)D + a.eps);
+      if (roped) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * gf[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float o = __shfl(x[e], partner, 64);
+      y[e] = x[e];
+      if (rotated) {
+        const float c = sm_cos[t - tb][pair0 + e], s = sm_sin[t - tb][pair0 + e];
+        y[e] = x[e] * c + (first ? -o : o) * s;
+      }
+    }
+    if (!head_ok) continue;
+    const uint4 b16 = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
+                                 pack_bf16x2(y[6], y[7]));
+    if (is_q) {
+      *reinterpret_cast<uint4*>(a.q_out + (t * a.Hq + head) * D + 8 * sub) = b16;
+      continue;
+    }
+    const int64_t slot = redirect_slot(a.slots[t], a.num_slots);
+    const int64_t page = slot / a.P;
+    const int64_t dst = ((page * a.Hkv + h) * a.P + (slot - page * a.P)) * D + 8 * sub;
+    if constexpr (FP8) {
+      *reinterpret_cast<uint2*>(cache + dst) =
+          make_uint2(mrope_fp8_pair(y[0], y[1], scl, rs, rcp_ok) | mrope_fp8_pair(y[2], y[3], scl, rs, rcp_ok) << 16,
+                     mrope_fp8_pair(y[4], y[5], scl, rs, rcp_ok) | mrope_fp8_pair(y[6], y[7], scl, rs, rcp_ok) << 16);
+    } else {
+      *reinterpret_cast<uint4*>(cache + 2 * dst) = b16;
+    }
+  }
+}
+
+}  // namespace sna
+
+using namespace sna;
+
+extern "C" int sna_qkv_norm_mrope_store(const void* qkv, int64_t qkv_stride, int64_t n_tokens, int32_t num_q_heads,
+                                        int32_t num_kv_heads, int32_t head_dim, const void* q_norm, const void* k_norm,
+                                        float eps, const int64_t* positions, int64_t pos_stride, int32_t n_axes,
+                                        const float* inv_freq, int32_t n_pairs, const uint8_t* axes,
+                                        const int64_t* slots, void* q_out, void* k_cache, void* v_cache,
+                                        const float* k_scale, const float* v_scale, int64_t num_blocks,
+                                        int32_t page_size, int32_t cache_dtype, void* stream) {
+  ApiGuard guard;
+  if (n_tokens < 0 || num_q_heads < 1 || num_kv_heads < 1 || page_size < 1 || num_blocks < 1)
+    return fail(SNA_ERR_INVALID_ARGUMENT,
+                "qkv_norm_mrope_store: bad sizes (tokens %lld, heads %d/%d, head_dim %d, page %d, blocks %lld)",
+                (long long)n_tokens, num_q_heads, num_kv_heads, head_dim, page_size, (long long)num_blocks);
+  if (head_dim != 64 && head_dim != 128)
+    return fail(SNA_ERR_UNSUPPORTED, "qkv_norm_mrope_store: head_dim %d (64 or 128 are built)", head_dim);
+  if (n_axes < 1 || n_axes > 4)
+    return fail(SNA_ERR_UNSUPPORTED, "qkv_norm_mrope_store: %d position axes (1 to 4)", n_axes);
+  if (n_pairs < 8 || n_pairs % 8 != 0 || 2 * n_pairs > head_dim)
+    return fail(SNA_ERR_UNSUPPORTED, "qkv_norm_mrope_store: %d rotated pairs (a multiple of 8, at most head_dim / 2 = %d)",
+                n_pairs, head_dim / 2);
+  if (qkv_stride < (int64_t)(num_q_heads + 2 * (int64_t)num_kv_heads) * head_dim || pos_stride < n_tokens)
+    return fail(SNA_ERR_INVALID_ARGUMENT, "qkv_norm_mrope_store: row strides %lld / %lld are shorter than a row",
+                (long long)qkv_stride, (long long)pos_stride);
+  if ((q_norm == nullptr) != (k_norm == nullptr))
+    return fail(SNA_ERR_INVALID_ARGUMENT, "qkv_norm_mrope_store: give both QK-norm gammas or neither");
+  if (cache_dtype == SNA_DTYPE_FP8_E4M3FN_MUL)
+    return fail(SNA_ERR_UNSUPPORTED, "qkv_norm_mrope_store: the writer divides by dequantization scales; for a pool of "
+                "multipliers m pass SNA_DTYPE_FP8_E4M3FN with the scales bf16(1 / m)");
+  if (cache_dtype != SNA_DTYPE_BF16 && cache_dtype != SNA_DTYPE_FP8_E4M3FN)
+    return fail(SNA_ERR_INVALID_ARGUMENT, "qkv_norm_mrope_store: unknown cache dtype %d", cache_dtype);
+  if (!axes) return fail(SNA_ERR_INVALID_ARGUMENT, "qkv_norm_mrope_store: null pointer");
+  MropeArgs a;
+  a.axes[0] = a.axes[1] = 0;
+  for (int32_t i = 0; i < n_pairs; ++i) {
+    if (axes[i] >= n_axes)
+      return fail(SNA_ERR_INVALID_ARGUMENT, "qkv_norm_mrope_store: pair %d on axis %d of %d", i, axes[i], n_axes);
+    a.axes[i >> 5] |= (uint64_t)axes[i] << (2 * (i & 31));
+  }
+  const bool fp8 = cache_dtype == SNA_DTYPE_FP8_E4M3FN;
+  if (n_tokens == 0) return SNA_OK;
+  if (!qkv || !positions || !inv_freq || !slots || !q_out || !k_cache || !v_cache || (fp8 && (!k_scale || !v_scale)))
+    return fail(SNA_ERR_INVALID_ARGUMENT, "qkv_norm_mrope_store: null pointer");
+  if (!(eps >= 0.0f)) return fail(SNA_ERR_INVALID_ARGUMENT, "qkv_norm_mrope_store: eps %g", (double)eps);
+  if (!aligned(qkv, 16) || qkv_stride % 8 || !aligned(q_out, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) ||
+      (q_norm && (!aligned(q_norm, 16) || !aligned(k_norm, 16))))
+    return fail(SNA_ERR_INVALID_ARGUMENT, "qkv_norm_mrope_store: tensors and row strides must be 16-byte aligned");
+  const int32_t hpw = 64 / (head_dim / 8);
+  // (32 bits number a launch's threads along a grid axis)
+  const int64_t token_blocks = (n_tokens + kMropeTokens - 1) / kMropeTokens;
+  const int64_t head_groups = (num_q_heads + 2 * (int64_t)num_kv_heads + hpw - 1) / hpw;
+  if (token_blocks >= 1 << 24 || head_groups > 65535)
+    return fail(SNA_ERR_INVALID_ARGUMENT, "qkv_norm_mrope_store: %lld tokens of %lld heads are too many for one launch",
+                (long long)n_tokens, num_q_heads + 2ll * num_kv_heads);
+  a.qkv = (const uint16_t*)qkv;
+  a.qkv_stride = qkv_stride;
+  a.T = n_tokens;
+  a.Hq = num_q_heads;
+  a.Hkv = num_kv_heads;
+  a.q_norm = (const uint16_t*)q_norm;
+  a.k_norm = (const uint16_t*)k_norm;
+  a.eps = eps;
+  a.positions = positions;
+  a.pos_stride = pos_stride;
+  a.inv_freq = inv_freq;
+  a.half = n_pairs;
+  a.slots = slots;
+  a.q_out = (uint16_t*)q_out;
+  a.k_cache = (uint8_t*)k_cache;
+  a.v_cache = (uint8_t*)v_cache;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.num_slots = num_blocks * page_size;
+  a.P = page_size;
+  const dim3 grid((unsigned)token_blocks, (unsigned)head_groups);
+  const hipStream_t s = (hipStream_t)stream;
+  if (fp8 && head_dim == 128) hipLaunchKernelGGL((qkv_norm_mrope_store_kernel<true, 128>), grid, dim3(256), 0, s, a);
+  else if (fp8) hipLaunchKernelGGL((qkv_norm_mrope_store_kernel<true, 64>), grid, dim3(256), 0, s, a);
+  else if (head_dim == 128) hipLaunchKernelGGL((qkv_norm_mrope_store_kernel<false, 128>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((qkv_norm_mrope_store_kernel<false, 64>), grid, dim3(256), 0, s, a);
+  return check_launch("qkv_norm_mrope_store");
+}

@@ -8,6 +8,7 @@ Reference interfaces each function stands in for are cited per function (paths u
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from typing import Optional, Sequence, Union
@@ -78,6 +79,22 @@ def _contig(t: Tensor, name: str, dtype: Optional[torch.dtype] = None) -> Tensor
 def _as(t: Tensor, dtype: torch.dtype) -> Tensor:
     """t converted to dtype, t itself when it already is (skipping Tensor.to's argument parsing on the hot path)."""
     return t if t.dtype == dtype else t.to(dtype)
+
+
+_same_device = contextlib.nullcontext()
+
+
+def _device_of(dev: torch.device):
+    """A context in which ``dev`` is the current device (nothing to do where it is already)."""
+    return _same_device if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _head_scales(scale: Optional[Tensor], G: int, name: str) -> Tensor:
+    """An FP8 cache's scales as [G] contiguous fp32 (one entry stands for all heads)."""
+    _need(scale is not None, lambda: f"an FP8 cache needs {name}")
+    scale = _as(scale.reshape(-1), torch.float32)
+    _need(scale.numel() in (1, G), lambda: f"{name} needs 1 or {G} entries (one per KV head)")
+    return _contig(scale if scale.numel() == G else scale.expand(G), name)
 
 
 def cache_dtype_code(dtype: torch.dtype, scales_multiply: bool = False) -> int:
@@ -185,6 +202,81 @@ def qkv_norm_rope_store(qkv: Tensor, *, cos: Tensor, sin: Tensor, num_q_heads: i
         _ptr(cos), _ptr(sin), cos.stride(0), _ptr(slots), _ptr(q_out), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
         _ptr(v_scale), nb, P, code, _stream(dev))
     _lib.check(rc, "qkv_norm_rope_store")
+    return q_out
+
+
+def mrope_axes(sections: Sequence[int], interleaved: bool = False) -> tuple[int, ...]:
+    """The position axis of each rotated pair, for qkv_norm_mrope_store: ``sections`` [A] gives the pairs of each axis,
+    one axis after another, or (``interleaved``) dealt in turn: pair i belongs to axis i mod A while that axis has pairs
+    left (i < A * sections[axis]), and to axis 0 else."""
+    sec = [int(n) for n in sections]
+    _need(1 <= len(sec) <= 4 and min(sec) >= 0 and sum(sec) > 0, lambda: f"1 to 4 sections of pairs, got {sections}")
+    if not interleaved:
+        return tuple(a for a, n in enumerate(sec) for _ in range(n))
+    A = len(sec)
+    axes = tuple(i % A if i < A * sec[i % A] else 0 for i in range(sum(sec)))
+    _need(all(axes.count(a) == n for a, n in enumerate(sec)),
+          lambda: f"sections {sections} cannot be dealt in turn: axis 0 needs the most pairs")
+    return axes
+
+
+def qkv_norm_mrope_store(qkv: Tensor, *, positions: Tensor, inv_freq: Tensor, axes: Sequence[int], num_q_heads: int,
+                         num_kv_heads: int, d_head: int, k_cache: Tensor, v_cache: Tensor, slot_mapping: Tensor,
+                         q_norm: Optional[Tensor] = None, k_norm: Optional[Tensor] = None, norm_eps: float = 1e-6,
+                         k_scale: Optional[Tensor] = None, v_scale: Optional[Tensor] = None,
+                         q_out: Optional[Tensor] = None) -> Tensor:
+    """The writer of qkv_norm_rope_store for rotary positions with several axes (images, video): pair i of a Q or K head
+    (elements i and i + n, n = len(inv_freq)) is rotated by the angle ``positions[axes[i], t] * inv_freq[i]``, elements
+    past 2 n stay. ``positions`` [A, T] int64 (A of 1 to 4), ``inv_freq`` [n] fp32 (n a multiple of 8, at most d / 2),
+    ``axes`` [n] host ints (mrope_axes). The other arguments are qkv_norm_rope_store's. Angles are formed in 64 bits, so
+    positions of any size serve; norm and rotation are fp32 and every output is rounded once. Returns Q [T, q, d] bf16; the
+    caches are written in place."""
+    dev = _on_gpu(qkv, positions, inv_freq, k_cache, v_cache, slot_mapping, q_norm, k_norm, k_scale, v_scale, q_out)
+    _need(k_cache.dim() == 4, lambda: f"caches [blocks, kv_heads, page, d], got {tuple(k_cache.shape)}")
+    nb, G, P, d = k_cache.shape
+    _need(G == num_kv_heads and d == d_head,
+          lambda: f"caches {tuple(k_cache.shape)} for {num_kv_heads} heads of {d_head}")
+    _need(v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype, "K and V caches differ")
+    _need(k_cache.is_contiguous() and v_cache.is_contiguous(), "caches must be contiguous")
+    width = (num_q_heads + 2 * num_kv_heads) * d_head
+    _need(qkv.dtype == torch.bfloat16 and qkv.dim() >= 1 and qkv.shape[-1] == width,
+          lambda: f"qkv must be bf16 [T, {width}], got {tuple(qkv.shape)}")
+    qkv = qkv if qkv.dim() == 2 else qkv.reshape(-1, width)
+    T = qkv.shape[0]
+    stride = qkv.stride(0) if T > 1 else width
+    _need(qkv.stride(1) == 1 and stride >= width and stride % 8 == 0,
+          lambda: f"qkv rows must have unit column stride and a row stride of a multiple of 8, got {qkv.stride()}")
+    _need(positions.dim() == 2 and positions.shape[1] == T, lambda: f"positions must be [axes, {T}]")
+    positions = _as(positions, torch.int64)
+    positions = positions if positions.stride(1) == 1 and positions.stride(0) >= T else positions.contiguous()
+    inv_freq = _contig(inv_freq.reshape(-1), "inv_freq", torch.float32)
+    n = inv_freq.numel()
+    _need(len(axes) == n, lambda: f"{len(axes)} axes for {n} rotated pairs")
+    _need(n == 0 or (min(axes) >= 0 and max(axes) < positions.shape[0]),
+          lambda: f"axes must lie in [0, {positions.shape[0]})")
+    slots = _contig(_as(slot_mapping.reshape(-1), torch.int64), "slot_mapping")
+    _need(slots.numel() == T, lambda: f"{slots.numel()} slots for {T} tokens")
+    _need((q_norm is None) == (k_norm is None), "give both QK-norm gammas or neither")
+    if q_norm is not None:
+        q_norm = _contig(q_norm.reshape(-1), "q_norm", torch.bfloat16)
+        k_norm = _contig(k_norm.reshape(-1), "k_norm", torch.bfloat16)
+        _need(q_norm.numel() == d_head and k_norm.numel() == d_head, lambda: f"QK-norm gammas need {d_head} entries")
+    code = cache_dtype_code(k_cache.dtype)
+    if code == _lib.DTYPE_FP8_E4M3FN:
+        k_scale, v_scale = _head_scales(k_scale, G, "k_scale"), _head_scales(v_scale, G, "v_scale")
+    else:
+        k_scale = v_scale = None
+    if q_out is None:
+        q_out = torch.empty(T, num_q_heads, d_head, dtype=torch.bfloat16, device=dev)
+    _need(q_out.shape == (T, num_q_heads, d_head) and q_out.dtype == torch.bfloat16 and q_out.is_contiguous(),
+          "bad q_out tensor")
+    with _device_of(dev):
+        rc = _lib.load().sna_qkv_norm_mrope_store(
+            _ptr(qkv), stride, T, num_q_heads, num_kv_heads, d_head, _ptr(q_norm), _ptr(k_norm), float(norm_eps),
+            _ptr(positions), max(positions.stride(0), T), positions.shape[0], _ptr(inv_freq), n, bytes(axes),
+            _ptr(slots), _ptr(q_out), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), nb, P, code,
+            _stream(dev))
+    _lib.check(rc, "qkv_norm_mrope_store")
     return q_out
 
 
@@ -777,6 +869,18 @@ def lse_combine(o_parts: Tensor, lse_parts: Tensor) -> tuple[Tensor, Tensor]:
 # prefill attention over the pool
 # ------------------------------------------------------------------------------------------------------------------
 
+def _check_q_start(host_q_start, R: int, T: int, max_q_len: int) -> None:
+    """Refuse a host copy of q_start that is not the R chunks' offsets in T rows, or holds a chunk past max_q_len."""
+    hq = [int(x) for x in torch.as_tensor(host_q_start).reshape(-1).tolist()]
+    _need(len(hq) == R + 1 and hq[0] == 0 and hq[-1] == T,
+          lambda: f"q_start must run from 0 to T = {T} over {R + 1} "
+          f"entries, got {hq[:4]}{'...' if len(hq) > 4 else ''} ending {hq[-1] if hq else None}")
+    lens = [hq[r + 1] - hq[r] for r in range(R)]
+    _need(min(lens, default=0) >= 0, "q_start must not decrease")
+    _need(max(lens, default=0) <= int(max_q_len),
+          lambda: f"a chunk of {max(lens)} queries exceeds max_q_len {max_q_len}")
+
+
 def prefill_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, q_start: Tensor,
                       prior_lens: Tensor, *, max_q_len: int, sm_scale: float, k_scale: Optional[Tensor] = None,
                       v_scale: Optional[Tensor] = None, sinks: Optional[Tensor] = None, window: int = 0,
@@ -805,14 +909,7 @@ def prefill_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: 
     pl = _contig(_as(prior_lens, torch.int32), "prior_lens")
     table = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32).contiguous()
     if host_q_start is not None:
-        hq = [int(x) for x in torch.as_tensor(host_q_start).reshape(-1).tolist()]
-        _need(len(hq) == R + 1 and hq[0] == 0 and hq[-1] == T,
-              lambda: f"q_start must run from 0 to T = {T} over {R + 1} "
-              f"entries, got {hq[:4]}{'...' if len(hq) > 4 else ''} ending {hq[-1] if hq else None}")
-        lens = [hq[r + 1] - hq[r] for r in range(R)]
-        _need(min(lens, default=0) >= 0, "q_start must not decrease")
-        _need(max(lens, default=0) <= int(max_q_len),
-              lambda: f"a chunk of {max(lens)} queries exceeds max_q_len {max_q_len}")
+        _check_q_start(host_q_start, R, T, max_q_len)
     code = cache_dtype_code(k_cache.dtype, scales_multiply)
     ks = vs = None
     if code != _lib.DTYPE_BF16:
@@ -861,6 +958,198 @@ def segmented_attention(q: Tensor, *, k_cache: Tensor, v_cache: Tensor, block_ta
         max_q_len=S, sm_scale=scale, k_scale=k_scale, v_scale=v_scale, sinks=None if sink is None else sink.reshape(-1),
         window=int(sliding_window or 0), host_q_start=[0, S])
     return out.transpose(0, 1).contiguous()
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# attention weights of cached keys, and eviction by them
+# ------------------------------------------------------------------------------------------------------------------
+
+def _weight_strides(weights: Tensor, R: int, G: int, what: str) -> tuple[int, int]:
+    """(row stride, head stride) of a [R, G, N] fp32 tensor whose rows do not overlap."""
+    _need(weights.dim() == 3 and weights.shape[0] == R and weights.shape[1] == G and weights.dtype == torch.float32,
+          lambda: f"{what} must be [{R}, {G}, N] fp32, got {tuple(weights.shape)} {weights.dtype}")
+    N = weights.shape[2]
+    _need(weights.stride(2) == 1 or N <= 1, lambda: f"{what} must have unit column stride")
+    row, head = (weights.stride(0) if R > 1 else N * G), (weights.stride(1) if G > 1 else N)
+    _need(head >= N and row >= N and (R <= 1 or G <= 1 or row >= head * G or head >= row * R),
+          lambda: f"{what}: rows of strides {weights.stride()} overlap")
+    return row, head
+
+
+def _attention_weights(what, q, T, R, k_cache, block_table, q_start, lens, max_q_len, sm_scale, k_scale, sinks, window,
+                       weights, scales_multiply) -> Tensor:
+    dev = _on_gpu(q, k_cache, block_table, q_start, lens, k_scale, sinks, weights)
+    _need(k_cache.dim() == 4 and k_cache.is_contiguous(), "the cache must be contiguous [blocks, kv_heads, page, d]")
+    H, d = q.shape[1:]
+    nb, G, P, dk = k_cache.shape
+    _need(dk == d, lambda: f"cache {tuple(k_cache.shape)} does not match q's head_dim {d}")
+    _need(H % G == 0, lambda: f"{H} query heads over {G} KV heads")
+    code = cache_dtype_code(k_cache.dtype, scales_multiply)
+    q = _contig(q, "q", torch.bfloat16)
+    _need(block_table.dim() == 2 and block_table.shape[0] == R, lambda: f"block_table must be [{R}, width]")
+    table = _as(block_table, torch.int32)
+    table = table if table.stride(1) == 1 else table.contiguous()
+    W = table.shape[1]
+    _need(W >= 1, "block_table has no columns")
+    lens = _contig(_as(lens.reshape(-1), torch.int32), "lens")
+    k_scale = None if code == _lib.DTYPE_BF16 else _head_scales(k_scale, G, "k_scale")
+    if sinks is not None:
+        sinks = _contig(_as(sinks.reshape(-1), torch.float32), "sinks")
+        _need(sinks.numel() == H, lambda: f"{sinks.numel()} sinks for {H} heads")
+    add = weights is not None
+    if add:
+        row, head = _weight_strides(weights, R, G, "weights")
+    else:
+        weights = torch.empty(R, G, W * P, dtype=torch.float32, device=dev)
+        row, head = G * W * P, W * P
+    N = weights.shape[2]
+    lib = _lib.load()
+    need = lib.sna_attention_weights_workspace_bytes(T, R, max_q_len, H, G, P, W, N)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    stride = max(table.stride(0), W)
+    with _device_of(dev):
+        if q_start is None:
+            rc = lib.sna_decode_attention_weights(
+                _ptr(q), _ptr(k_cache), _ptr(k_scale), _ptr(table), stride, W, _ptr(lens), R, _ptr(sinks),
+                float(sm_scale), int(window), _ptr(weights), row, head, N, int(add), H, G, d, P, nb, code, _ptr(ws),
+                need, _stream(dev))
+        else:
+            rc = lib.sna_prefill_attention_weights(
+                _ptr(q), _ptr(k_cache), _ptr(k_scale), _ptr(table), stride, W, _ptr(q_start), _ptr(lens), T, R,
+                max_q_len, _ptr(sinks), float(sm_scale), int(window), _ptr(weights), row, head, N, int(add), H, G, d, P,
+                nb, code, _ptr(ws), need, _stream(dev))
+    _lib.check(rc, what)
+    return weights
+
+
+def prefill_attention_weights(q: Tensor, k_cache: Tensor, block_table: Tensor, q_start: Tensor, prior_lens: Tensor, *,
+                              max_q_len: int, sm_scale: float, k_scale: Optional[Tensor] = None,
+                              sinks: Optional[Tensor] = None, window: int = 0, weights: Optional[Tensor] = None,
+                              host_q_start=None, scales_multiply: bool = False) -> Tensor:
+    """The attention weight that cached keys receive from a batch of chunks: [R, G, N] fp32, entry (r, g, j) the sum over
+    request r's queries and the query heads of KV head g of their softmax probability of key j. The arguments are
+    prefill_attention's (the chunk's keys are in the pool already), and the probabilities are those that it uses. A chunk
+    may be a prompt's last few queries alone (``prior_lens`` then counts every token before them): an observation window.
+
+    ``weights`` [R, G, N] fp32, when given, is added to and returned (keys past N get nothing, entries without a key stay
+    as they are); without it a new tensor of N = table width * page is returned, zero where there is no key. The same call
+    gives the same bits."""
+    _need(q.dim() == 3, lambda: f"q must be [T, H, d], got {tuple(q.shape)}")
+    T, R = q.shape[0], prior_lens.numel()
+    _need(q_start.numel() == R + 1, lambda: f"q_start must be [{R + 1}]")
+    if host_q_start is not None:
+        _check_q_start(host_q_start, R, T, max_q_len)
+    return _attention_weights("prefill_attention_weights", q, T, R, k_cache, block_table,
+                              _contig(_as(q_start.reshape(-1), torch.int32), "q_start"), prior_lens, int(max_q_len),
+                              sm_scale, k_scale, sinks, window, weights, scales_multiply)
+
+
+def decode_attention_weights(q: Tensor, k_cache: Tensor, block_table: Tensor, seq_lens: Tensor, *, sm_scale: float,
+                             k_scale: Optional[Tensor] = None, sinks: Optional[Tensor] = None, window: int = 0,
+                             weights: Optional[Tensor] = None, scales_multiply: bool = False) -> Tensor:
+    """prefill_attention_weights for a decode step: row b's one query q[b] (q [B, H, d]) at position seq_lens[b] - 1, its
+    key in the pool already (paged_decode_gqa stores it at ``new_slots``). Returns [B, G, N] fp32 as there."""
+    _need(q.dim() == 3, lambda: f"q must be [B, H, d], got {tuple(q.shape)}")
+    B = q.shape[0]
+    _need(seq_lens.numel() == B, lambda: f"{seq_lens.numel()} seq_lens for {B} rows")
+    return _attention_weights("decode_attention_weights", q, B, B, k_cache, block_table, None, seq_lens, 1, sm_scale,
+                              k_scale, sinks, window, weights, scales_multiply)
+
+
+def select_tokens(weights: Tensor, seq_lens: Tensor, *, keep: int, first: int = 0, recent: int = 0,
+                  weights_out: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
+    """The tokens that each (row, KV head) keeps, by weight: row r of L = seq_lens[r] tokens keeps all of them where L <=
+    ``keep``, else its ``first`` first ones, its ``recent`` last ones and, of the others, those of the largest
+    ``weights`` [R, G, N] fp32 (equal weights: the lowest position; NaN ranks above every number). Returns (kept
+    [R, G, keep] int32, ascending positions, -1 past a short row's; new_lens [R] int32 = min(L, keep)).
+
+    ``weights_out`` [R, G, M >= keep] fp32, when given, receives the kept tokens' weights and zeros after them; it may be
+    ``weights`` itself, so that the tokens written next start at zero."""
+    dev = _on_gpu(weights, seq_lens, weights_out)
+    _need(weights.dim() == 3, lambda: f"weights must be [R, G, N], got {tuple(weights.shape)}")
+    R, G, N = weights.shape
+    row, head = _weight_strides(weights, R, G, "weights")
+    lens = _contig(_as(seq_lens.reshape(-1), torch.int32), "seq_lens")
+    _need(lens.numel() == R, lambda: f"{lens.numel()} seq_lens for {R} rows")
+    keep, first, recent = int(keep), int(first), int(recent)
+    _need(keep >= 1 and first >= 0 and recent >= 0 and first + recent <= keep,
+          lambda: f"keep {keep} tokens of which {first} first and {recent} recent")
+    o_row = o_head = M = 0
+    if weights_out is not None:
+        o_row, o_head = _weight_strides(weights_out, R, G, "weights_out")
+        M = weights_out.shape[2]
+        _need(M >= keep, lambda: f"weights_out of {M} columns for {keep} tokens")
+        same = weights_out.data_ptr() == weights.data_ptr() and (o_row, o_head) == (row, head)
+        _need(same or not _overlap(weights, weights_out), "weights_out overlaps weights without being it")
+    kept = torch.empty(R, G, keep, dtype=torch.int32, device=dev)
+    new_lens = torch.empty(R, dtype=torch.int32, device=dev)
+    if R == 0 or G == 0:
+        return kept, new_lens
+    with _device_of(dev):
+        rc = _lib.load().sna_select_tokens(_ptr(weights), row, head, N, _ptr(lens), R, G, keep, first, recent,
+                                           _ptr(kept), _ptr(new_lens), _ptr(weights_out), o_row, o_head, M,
+                                           _stream(dev))
+    _lib.check(rc, "select_tokens")
+    return kept, new_lens
+
+
+def _overlap(a: Tensor, b: Tensor) -> bool:
+    """Whether the address ranges of two tensors meet."""
+    def span(t):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+        return t.data_ptr(), t.data_ptr() + last * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def compact_tokens(k_cache: Tensor, v_cache: Tensor, block_table: Tensor, kept: Tensor, *,
+                   dst_table: Optional[Tensor] = None) -> None:
+    """Move the kept tokens' K and V of one layer together: token ``kept[r, g, i]`` of KV head g of row r (read through
+    ``block_table`` [R, W]) to position i of the row's pages in ``dst_table`` [R, W'], or, without it, in place. ``kept``
+    [R, G, keep] int32 ascends (select_tokens), -1 entries move nothing. The caches [blocks, G, page, d] hold bf16 or FP8;
+    bytes move as they are. Afterwards the row holds its kept tokens at positions 0 .. in order, its pages past them are
+    free, and the decode entry points read it with the new length (a sliding window would count evicted positions no more).
+
+    Rows that share pages (a cached prefix) cannot be compacted in place: give them pages of their own in ``dst_table``,
+    which names no page of ``block_table``."""
+    dev = _on_gpu(k_cache, v_cache, block_table, kept, dst_table)
+    _need(k_cache.dim() == 4 and v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype,
+          "K and V caches differ")
+    _need(k_cache.is_contiguous() and v_cache.is_contiguous(), "caches must be contiguous")
+    _need(k_cache.data_ptr() != v_cache.data_ptr() or k_cache.numel() == 0, "K and V are one tensor")
+    nb, G, P, d = k_cache.shape
+    _need(kept.dim() == 3 and kept.shape[1] == G, lambda: f"kept must be [R, {G}, keep], got {tuple(kept.shape)}")
+    kept = _contig(kept, "kept", torch.int32)
+    R, _, keep = kept.shape
+    _need(block_table.dim() == 2 and block_table.shape[0] == R, lambda: f"block_table must be [{R}, width]")
+    table = _contig(_as(block_table, torch.int32), "block_table")
+    dst = None
+    if dst_table is not None:
+        _need(dst_table.dim() == 2 and dst_table.shape[0] == R, lambda: f"dst_table must be [{R}, width]")
+        _need(dst_table.shape[1] * P >= keep, lambda: f"dst_table of {dst_table.shape[1]} pages of {P} for {keep} tokens")
+        dst = _contig(_as(dst_table, torch.int32), "dst_table")
+    code = cache_dtype_code(k_cache.dtype)
+    if R == 0 or keep == 0:
+        return
+    with _device_of(dev):
+        rc = _lib.load().sna_compact_tokens(
+            _ptr(k_cache), _ptr(v_cache), nb, G, P, d, code, _ptr(table), table.shape[1], table.shape[1],
+            None if dst is None else _ptr(dst), 0 if dst is None else dst.shape[1], 0 if dst is None else dst.shape[1],
+            _ptr(kept), R, keep, _stream(dev))
+    _lib.check(rc, "compact_tokens")
+
+
+def evict_tokens(k_cache: Tensor, v_cache: Tensor, block_table: Tensor, seq_lens: Tensor, weights: Tensor, *, keep: int,
+                 first: int = 0, recent: int = 0, dst_table: Optional[Tensor] = None,
+                 weights_out: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
+    """Thin the rows of one layer's caches to ``keep`` tokens each by accumulated attention weight: select_tokens, then
+    compact_tokens. Every KV head of a row keeps a set of its own, the count is the row's. Returns (kept, new_lens)."""
+    G = k_cache.shape[1] if k_cache.dim() == 4 else -1
+    _need(weights.dim() == 3 and weights.shape[1] == G and block_table.shape[0] == weights.shape[0],
+          lambda: f"weights {tuple(weights.shape)} for {block_table.shape[0]} rows of {G} KV heads")
+    kept, new_lens = select_tokens(weights, seq_lens, keep=keep, first=first, recent=recent, weights_out=weights_out)
+    compact_tokens(k_cache, v_cache, block_table, kept, dst_table=dst_table)
+    return kept, new_lens
 
 
 # ------------------------------------------------------------------------------------------------------------------
