@@ -44,9 +44,11 @@ struct WeightsArgs {
   int32_t blocks;    // key blocks that the table's keys (and, when every column is written, the width) take
   float2* ws_part;   // [G, blocks, T * group] a block's (largest score in the log2 domain, sum)
   float2* ws_row;    // [G, T * group] a row's (largest score in the log2 domain, 1 / sum)
+  // few rows instead: ws_part is [R, G, blocks, max_q * group], and
+  float* ws_score;   // [R, G, max_q * group, blocks * 256] scores in the log2 domain, -inf where unseen
 };
 
-constexpr int kWeightKeys = 256;  // keys of a workgroup
+constexpr int kWeightKeys = 256;  // keys of a workgroup, 64 to a wave
 constexpr int kWeightRows = 32;   // query rows of a tile
 
 // A request's queries and keys: rows 0 .. S - 1 are tokens qa .. of q at positions prior + t; keys 0 .. n - 1.
@@ -70,19 +72,136 @@ __device__ __forceinline__ WeightsRequest weights_request(const WeightsArgs& a, 
   return q;
 }
 
+template <int D, int ESZ>
+struct WeightsGeo {
+  static constexpr int NS = D / 16;            // matrix steps of a score
+  static constexpr int ROWB = D * ESZ;         // bytes of a key
+  static constexpr int KCH = ROWB / 16;        // its 16-byte chunks
+  static constexpr int KEYB = 64 * ROWB;       // bytes of a wave's keys
+  static constexpr int QCH = D * 2 / 16;       // 16-byte chunks of a query row
+  static constexpr int TILE = kWeightRows * QCH;
+  // Rows of N chunks lie in LDS with chunk c of row r at c ^ swz(r), so that 16 lanes which read one chunk of 16
+  // consecutive rows touch every bank once.
+  static __device__ __forceinline__ int swz(int r, int n) { return (n >= 16 ? r : r / (16 / n)) & (n - 1); }
+};
+
+// The wave's 64 keys from k0 on, lane i's being key k0 + i: its first byte in the cache, or -1 where there is none.
+__device__ __forceinline__ int64_t weights_key_at(const WeightsArgs& a, int32_t r, int32_t g, int32_t key, int32_t n,
+                                                  int32_t row_bytes) {
+  if (key >= n) return -1;
+  const int32_t col = key / a.P;
+  const int64_t page = a.table[r * a.table_stride + col];
+  if (page < 0 || page >= a.num_blocks) return -1;
+  return ((page * a.G + g) * a.P + (key - col * a.P)) * (int64_t)row_bytes;
+}
+
+// The wave's 64 keys through LDS (whole rows by DMA, 1024 bytes an instruction) to A operands in registers: lane (g2, i)
+// feeds key 32 s + i, dims 16 c + 8 g2 .. of step c (bf16) or 32 (c / 2) + 16 g2 + 8 (c & 1) .. (FP8, as its 16-byte
+// chunks hold them). A key that is not there reads the cache's first row; what comes of it is masked or dropped.
+template <int D, int ESZ>
+__device__ __forceinline__ void weights_keys(const WeightsArgs& a, int64_t at, uint8_t* lds, uint32_t (&kf)[2][D / 16][4]) {
+  using Geo = WeightsGeo<D, ESZ>;
+  constexpr int RPD = 1024 / Geo::ROWB;
+  const int lane = threadIdx.x & 63, g2 = lane >> 5, i32 = lane & 31;
+  const int64_t from = at < 0 ? 0 : at;
+  const uint32_t base = lds_address((lds_ptr_t*)lds);
+#pragma unroll
+  for (int j = 0; j < 64 / RPD; ++j) {
+    const int row = j * RPD + lane / Geo::KCH, ch = lane % Geo::KCH ^ Geo::swz(row, Geo::KCH);
+    const uint32_t lo = __shfl((uint32_t)from, row, 64), hi = __shfl((uint32_t)(from >> 32), row, 64);
+    const uint8_t* src = a.k_cache + (int64_t)((uint64_t)hi << 32 | lo) + 16 * ch;
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane(base + 1024 * j);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m0), "v"(src) : "memory");
+  }
+  wait_vmcnt<0>();
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int row = 32 * s + i32;
+    const uint8_t* mine = lds + row * Geo::ROWB;
+    if constexpr (ESZ == 1) {
+#pragma unroll
+      for (int c = 0; c < Geo::NS / 2; ++c) {
+        const uint4 w = *reinterpret_cast<const uint4*>(mine + 16 * ((2 * c + g2) ^ Geo::swz(row, Geo::KCH)));
+        fp8x4_to_bf16x4(w.x, kf[s][2 * c][0], kf[s][2 * c][1]);
+        fp8x4_to_bf16x4(w.y, kf[s][2 * c][2], kf[s][2 * c][3]);
+        fp8x4_to_bf16x4(w.z, kf[s][2 * c + 1][0], kf[s][2 * c + 1][1]);
+        fp8x4_to_bf16x4(w.w, kf[s][2 * c + 1][2], kf[s][2 * c + 1][3]);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < Geo::NS; ++c) {
+        const uint4 w = *reinterpret_cast<const uint4*>(mine + 16 * ((2 * c + g2) ^ Geo::swz(row, Geo::KCH)));
+        kf[s][c][0] = w.x, kf[s][c][1] = w.y, kf[s][c][2] = w.z, kf[s][c][3] = w.w;
+      }
+    }
+  }
+}
+// The query chunk (8 dims) that meets lane group g2's K operand of step c.
+template <int ESZ>
+__device__ __forceinline__ int weights_chunk(int c, int g2) {
+  return ESZ == 1 ? 4 * (c / 2) + 2 * g2 + (c & 1) : 2 * c + g2;
+}
+
+// Log2-domain factor of a score.
+template <int ESZ>
+__device__ __forceinline__ float weights_scale(const WeightsArgs& a, int32_t g) {
+  double scale = (double)a.sm_scale * 1.4426950408889634;
+  if (ESZ == 1) scale = a.mul_scale ? scale / (double)a.k_scale[g] : scale * (double)a.k_scale[g];
+  return (float)scale;
+}
+
+// The keys of the wave's 64 (from kw on) that a row at position pos sees, as bits.
+__device__ __forceinline__ uint64_t weights_seen(const WeightsArgs& a, uint64_t valid, int64_t pos, int32_t kw) {
+  const int64_t hi = pos - kw;  // keys 0 .. hi
+  uint64_t seen = hi < 0 ? 0 : hi < 63 ? valid & ((2ull << hi) - 1) : valid;
+  if (a.window > 0) {
+    const int64_t lo = pos - a.window + 1 - kw;  // from key lo
+    seen = lo > 63 ? 0 : lo > 0 ? seen & (~0ull << lo) : seen;
+  }
+  return seen;
+}
+// Key of element e of lane group g2's sub-tile s.
+__device__ __forceinline__ constexpr int weights_key(int s, int e, int g2) { return 32 * s + 8 * (e / 4) + 4 * g2 + e % 4; }
+
+// (largest, sum of 2^(x - largest)) of two sets merged.
+__device__ __forceinline__ float2 weights_join(float2 p, float2 o) {
+  const float b = fmaxf(p.x, o.x);
+  return make_float2(b, p.y * __builtin_amdgcn_exp2f(p.x - b) + o.y * __builtin_amdgcn_exp2f(o.x - b));
+}
+
+// The lane's 32 scores x * c2 of one row as (largest, sum), with the lane's 32 away, which holds the row's other 32 keys.
+// ALL: every key is seen and c2 > 0; else the scores are left in x, scaled and -inf where unseen.
+template <bool ALL>
+__device__ __forceinline__ float2 weights_stats(f32x16_t (&x)[2], float c2, uint64_t seen, int g2) {
+  float mx = ALL ? -INFINITY : kNegBig, sum = 0.0f;
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      if (!ALL) x[s][e] = seen >> weights_key(s, e, g2) & 1 ? x[s][e] * c2 : -INFINITY;
+      mx = fmaxf(mx, x[s][e]);
+    }
+  if (ALL) mx *= c2;
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(ALL ? fmaf(x[s][e], c2, -mx) : x[s][e] - mx);
+  const float both = xor32_partner_max(mx);
+  return make_float2(both, xor32_partner_sum(sum * __builtin_amdgcn_exp2f(mx - both)));
+}
+
 enum WeightsPass { kStats, kSum };
 template <int D, int ESZ, WeightsPass PASS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void weights_tile_kernel(WeightsArgs a) {
-  constexpr bool FP8 = ESZ == 1;
-  constexpr int NS = D / 16;          // matrix steps of a score
-  constexpr int CH = D * 2 / 16;      // 16-byte chunks of a query row
-  constexpr int TILE = kWeightRows * CH;
-  constexpr int LD = TILE / 256;      // chunks of a tile that a thread moves
-  __shared__ uint4 sm_q[2][TILE];
-  __shared__ int64_t sm_key[kWeightKeys];  // a key's first byte in the cache, -1 where there is none
+  using Geo = WeightsGeo<D, ESZ>;
+  constexpr int NS = Geo::NS, CH = Geo::QCH, TILE = Geo::TILE;
+  constexpr int LD = TILE / 256;  // chunks of a tile that a thread moves
+  constexpr int BYTES = 4 * Geo::KEYB > 2 * TILE * 16 ? 4 * Geo::KEYB : 2 * TILE * 16;
+  __shared__ __attribute__((aligned(1024))) uint8_t sm[BYTES];  // the keys on their way to registers, then the row tiles
   __shared__ float sm_out[kWeightKeys];
   __shared__ float2 sm_part[2][4][kWeightRows];
+  uint4* const sm_q = reinterpret_cast<uint4*>(sm);
   const int tid = threadIdx.x, lane = tid & 63, g2 = lane >> 5, i32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t lin = xcd_order(blockIdx.x, gridDim.x);
@@ -99,16 +218,10 @@ void weights_tile_kernel(WeightsArgs a) {
     if (PASS == kSum && !a.add && k0 + tid < a.width) out[k0 + tid] = 0.0f;
     return;
   }
-  {
-    const int32_t key = k0 + tid;
-    int64_t at = -1;
-    if (key < rq.n) {
-      const int32_t col = key / a.P;
-      const int64_t page = a.table[r * a.table_stride + col];
-      if (page >= 0 && page < a.num_blocks) at = ((page * a.G + g) * a.P + (key - col * a.P)) * (int64_t)(D * ESZ);
-    }
-    sm_key[tid] = at;
-  }
+  const int64_t at = weights_key_at(a, r, g, k0 + tid, rq.n, Geo::ROWB);
+  const uint64_t valid = __ballot(at >= 0);
+  uint32_t kf[2][NS][4];
+  weights_keys<D, ESZ>(a, at, sm + wave * Geo::KEYB, kf);
   const int32_t m_end = t1 * a.group;
   const int32_t m0 = (t0 * a.group) & ~(kWeightRows - 1);
   const int32_t tiles = (m_end - m0 + kWeightRows - 1) / kWeightRows;
@@ -133,35 +246,7 @@ void weights_tile_kernel(WeightsArgs a) {
     }
   };
   load();
-  __syncthreads();
-  // the wave's keys as A operands: lane (g2, i) feeds key 32 s + i
-  uint32_t kf[2][NS][4];
-  uint64_t valid = 0;  // bit i: key 64 wave + i is there
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int64_t at = sm_key[64 * wave + 32 * s + i32];
-    valid |= (__ballot(at >= 0) & 0xffffffffull) << (32 * s);
-    const uint8_t* row = a.k_cache + at;
-    if constexpr (FP8) {
-#pragma unroll
-      for (int c = 0; c < NS / 2; ++c) {
-        const uint4 w = at >= 0 ? ld16(row + 32 * c + 16 * g2) : make_uint4(0, 0, 0, 0);
-        fp8x4_to_bf16x4(w.x, kf[s][2 * c][0], kf[s][2 * c][1]);
-        fp8x4_to_bf16x4(w.y, kf[s][2 * c][2], kf[s][2 * c][3]);
-        fp8x4_to_bf16x4(w.z, kf[s][2 * c + 1][0], kf[s][2 * c + 1][1]);
-        fp8x4_to_bf16x4(w.w, kf[s][2 * c + 1][2], kf[s][2 * c + 1][3]);
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < NS; ++c) {
-        const uint4 w = at >= 0 ? ld16(row + 32 * c + 16 * g2) : make_uint4(0, 0, 0, 0);
-        kf[s][c][0] = w.x, kf[s][c][1] = w.y, kf[s][c][2] = w.z, kf[s][c][3] = w.w;
-      }
-    }
-  }
-  double scale = (double)a.sm_scale * 1.4426950408889634;
-  if (FP8) scale = a.mul_scale ? scale / (double)a.k_scale[g] : scale * (double)a.k_scale[g];
-  const float c2 = (float)scale;
+  const float c2 = weights_scale<ESZ>(a, g);
   const int64_t rows = (int64_t)a.T * a.group;  // rows of a KV head
   float2* const part = a.ws_part + ((int64_t)g * a.blocks + kb) * rows + (int64_t)rq.qa * a.group;
   const float2* const row_of = a.ws_row + (int64_t)g * rows + (int64_t)rq.qa * a.group;
@@ -171,125 +256,231 @@ void weights_tile_kernel(WeightsArgs a) {
   for (int s = 0; s < 2; ++s)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[s][e] = 0.0f;
+  // the four waves' parts of tile i merged and written
+  auto write_part = [&](int32_t i) {
+    const int32_t m = m0 + kWeightRows * i + i32;
+    if (wave == (i & 3) && g2 == 0 && m < m_end) {
+      const float2(*p)[kWeightRows] = sm_part[i & 1];
+      part[m] = weights_join(weights_join(p[0][i32], p[1][i32]), weights_join(p[2][i32], p[3][i32]));
+    }
+  };
+  // (t, j): token and head of the lane's row, and of the tile's first and last rows
+  int32_t t = (m0 + i32) / a.group, j = m0 + i32 - t * a.group;
+  int32_t tf = m0 / a.group, jf = m0 - tf * a.group;
+  __syncthreads();  // every wave has its keys: the row tiles take their place
 
   for (int32_t i = 0; i < tiles; ++i) {
-    uint4* const slot = sm_q[i & 1];
+    uint4* const slot = sm_q + (i & 1) * TILE;
 #pragma unroll
     for (int l = 0; l < LD; ++l) {
       const int row = (tid + 256 * l) / CH, ch = tid % CH;
-      slot[row * CH + (ch ^ (row & (CH - 1)))] = ld[l];
+      slot[row * CH + (ch ^ Geo::swz(row, CH))] = ld[l];
     }
     __syncthreads();  // the slot was read two tiles ago: the barrier between covers it
     if (i + 1 < tiles) load();
     const int32_t m = m0 + kWeightRows * i + i32;  // this lane's row
     float2 rw = make_float2(0.0f, 0.0f);
     if (PASS == kSum && m < m_end) rw = row_of[m];
-    const int32_t t = m / a.group;
-    const int64_t pos = rq.prior + t;
+    if (PASS == kStats && i > 0) write_part(i - 1);
     f32x16_t x[2] = {};
 #pragma unroll
     for (int c = 0; c < NS; ++c) {
-      // chunk of 8 dims that the lane's K operand of step c holds
-      const int ch = FP8 ? 4 * (c / 2) + 2 * g2 + (c & 1) : 2 * c + g2;
-      const uint4 w = slot[i32 * CH + (ch ^ (i32 & (CH - 1)))];
+      const uint4 w = slot[i32 * CH + (weights_chunk<ESZ>(c, g2) ^ Geo::swz(i32, CH))];
       const uint32_t qf[4] = {w.x, w.y, w.z, w.w};
       x[0] = mfma_32x32x16_bf16(kf[0][c], qf, x[0]);
       x[1] = mfma_32x32x16_bf16(kf[1][c], qf, x[1]);
     }
-    // the keys that the lane's row sees, of the wave's 64
-    uint64_t seen = valid;
-    {
-      const int64_t hi = pos - kw;  // keys 0 .. hi of the wave
-      seen = m >= m_end || hi < 0 ? 0 : hi < 63 ? seen & ((2ull << hi) - 1) : seen;
-      if (a.window > 0) {
-        const int64_t lo = pos - a.window + 1 - kw;  // from key lo
-        seen = lo > 63 ? 0 : lo > 0 ? seen & (~0ull << lo) : seen;
-      }
-    }
-    const bool all = __all(seen == ~0ull);
+    // whether the tile's first row (and, in a window, its last) sees all of the wave's keys: scalar work
+    const int32_t te = tf + (jf + kWeightRows - 1) / a.group;
+    bool all = c2 > 0.0f && rq.prior + tf >= kw + 63 && (PASS == kSum || valid == ~0ull);
+    if (a.window > 0) all = all && rq.prior + te - a.window < kw;
     if constexpr (PASS == kStats) {
-      float mx = kNegBig, sum = 0.0f;
+      const float2 p = all ? weights_stats<true>(x, c2, 0, g2)
+                           : weights_stats<false>(x, c2, weights_seen(a, valid, rq.prior + t, kw), g2);
+      if (g2 == 0) sm_part[i & 1][wave][i32] = p;
+    } else if (all) {
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const bool on = all || (seen >> (32 * s + 8 * (e / 4) + 4 * g2 + e % 4) & 1);
-          x[s][e] = on ? x[s][e] * c2 : -INFINITY;
-          mx = fmaxf(mx, x[s][e]);
-        }
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(x[s][e] - mx);
-      // the row's other keys of the wave are the lane 32 away
-      const float om = __shfl_xor(mx, 32, 64), os = __shfl_xor(sum, 32, 64);
-      const float bm = fmaxf(mx, om);
-      sum = sum * __builtin_amdgcn_exp2f(mx - bm) + os * __builtin_amdgcn_exp2f(om - bm);
-      if (g2 == 0) sm_part[i & 1][wave][i32] = make_float2(bm, sum);
-      __syncthreads();
-      if (tid < kWeightRows && m0 + kWeightRows * i + tid < m_end) {
-        float2 p = sm_part[i & 1][0][tid];
-#pragma unroll
-        for (int w = 1; w < 4; ++w) {
-          const float2 o = sm_part[i & 1][w][tid];
-          const float b = fmaxf(p.x, o.x);
-          p.y = p.y * __builtin_amdgcn_exp2f(p.x - b) + o.y * __builtin_amdgcn_exp2f(o.x - b);
-          p.x = b;
-        }
-        part[m0 + kWeightRows * i + tid] = p;
-      }
+        for (int e = 0; e < 16; ++e)
+          acc[s][e] = fmaf(__builtin_amdgcn_exp2f(fmaf(x[s][e], c2, -rw.x)), rw.y, acc[s][e]);
     } else {
+      const uint64_t seen = m < m_end ? weights_seen(a, valid, rq.prior + t, kw) : 0;
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const bool on = all || (seen >> (32 * s + 8 * (e / 4) + 4 * g2 + e % 4) & 1);
-          const float p = __builtin_amdgcn_exp2f(x[s][e] * c2 - rw.x) * rw.y;
-          acc[s][e] += on ? p : 0.0f;
+          const float p = __builtin_amdgcn_exp2f(fmaf(x[s][e], c2, -rw.x)) * rw.y;
+          acc[s][e] += seen >> weights_key(s, e, g2) & 1 ? p : 0.0f;
         }
     }
+    t += step_t, j += step_j;
+    if (j >= a.group) j -= a.group, ++t;
+    tf += step_t, jf += step_j;
+    if (jf >= a.group) jf -= a.group, ++tf;
   }
-  if constexpr (PASS == kSum) {
+  if constexpr (PASS == kStats) {
+    __syncthreads();
+    write_part(tiles - 1);
+  } else {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        float v = acc[s][e];
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-        if (i32 == 0) sm_out[64 * wave + 32 * s + 8 * (e / 4) + 4 * g2 + e % 4] = v;
+        const float v = row16_sum(acc[s][e]);
+        const float both = v + __shfl_xor(v, 16, 64);
+        if (i32 == 0) sm_out[64 * wave + weights_key(s, e, g2)] = both;
       }
     __syncthreads();
     const int32_t key = k0 + tid;
     if (key < a.width) {
-      const float v = sm_key[tid] >= 0 ? sm_out[tid] : 0.0f;
+      const float v = at >= 0 ? sm_out[tid] : 0.0f;
       if (!a.add) out[key] = v;
-      else if (sm_key[tid] >= 0) out[key] += v;
+      else if (at >= 0) out[key] += v;
     }
   }
 }
 
-// A row's blocks merged: (its largest score M in the log2 domain, 1 / sum of 2^(score - M) with the sink's).
+// A row's blocks merged: (its largest score M in the log2 domain, 1 / sum of 2^(score - M) with the sink's). 32 rows a
+// workgroup, a row's blocks dealt to 8 threads.
 __global__ __launch_bounds__(256) void weights_merge_kernel(WeightsArgs a) {
+  __shared__ float2 sm[8][32];
   const int32_t r = blockIdx.z, g = blockIdx.y;
   const WeightsRequest rq = weights_request(a, r);
-  const int32_t m = blockIdx.x * 256 + threadIdx.x;
-  if (m >= rq.S * a.group) return;
+  const int i = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  if ((int32_t)blockIdx.x * 32 >= rq.S * a.group) return;  // uniform
+  const int32_t m = min((int32_t)blockIdx.x * 32 + i, rq.S * a.group - 1);
   const int32_t t = m / a.group, h = g * a.group + m - t * a.group;
   const int64_t pos = rq.prior + t;
   const int64_t rows = (int64_t)a.T * a.group;
   const int64_t row = (int64_t)rq.qa * a.group + m;
   // the blocks that hold keys it sees: each has written this row
   const int64_t hi = min(pos, (int64_t)rq.n - 1), lo = a.window > 0 ? max(pos - a.window + 1, (int64_t)0) : 0;
-  float M = kNegBig, S = 0.0f;
-  if (a.sinks) M = a.sinks[h] * kLog2e, S = 1.0f;
-  for (int32_t b = (int32_t)(lo / kWeightKeys); hi >= lo && b <= hi / kWeightKeys; ++b) {
-    const float2 p = a.ws_part[((int64_t)g * a.blocks + b) * rows + row];
-    const float n = fmaxf(M, p.x);
-    S = S * __builtin_amdgcn_exp2f(M - n) + p.y * __builtin_amdgcn_exp2f(p.x - n);
-    M = n;
+  float2 p = make_float2(kNegBig, 0.0f);
+  if (hi >= lo) {
+    const int32_t b1 = (int32_t)(hi / kWeightKeys);
+#pragma unroll 4
+    for (int32_t b = (int32_t)(lo / kWeightKeys) + slice; b <= b1; b += 8)
+      p = weights_join(p, a.ws_part[((int64_t)g * a.blocks + b) * rows + row]);
   }
-  a.ws_row[(int64_t)g * rows + row] = make_float2(M, S == 0.0f ? 0.0f : 1.0f / S);
+  sm[slice][i] = p;
+  __syncthreads();
+  if (slice == 0 && (int32_t)blockIdx.x * 32 + i < rq.S * a.group) {
+    for (int s = 1; s < 8; ++s) p = weights_join(p, sm[s][i]);
+    if (a.sinks) p = weights_join(p, make_float2(a.sinks[h] * kLog2e, 1.0f));
+    a.ws_row[(int64_t)g * rows + row] = make_float2(p.x, p.y == 0.0f ? 0.0f : 1.0f / p.y);
+  }
+}
+
+// Few rows (at most kScoreRows a request and KV head: a decode step): the scores themselves go to the workspace, so that
+// the keys are read once, and a second launch sums the probabilities from them.
+constexpr int kScoreRows = 16;
+template <int D, int ESZ>
+__global__ __launch_bounds__(256) void weights_score_kernel(WeightsArgs a) {
+  using Geo = WeightsGeo<D, ESZ>;
+  __shared__ __attribute__((aligned(1024))) uint8_t sm[4 * Geo::KEYB];
+  __shared__ float2 sm_part[4][32];
+  const int tid = threadIdx.x, lane = tid & 63, g2 = lane >> 5, i32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int32_t kb = (int32_t)(blockIdx.x % a.blocks), r = (int32_t)(blockIdx.x / a.blocks % a.R);
+  const int32_t g = (int32_t)(blockIdx.x / a.blocks / a.R);
+  const WeightsRequest rq = weights_request(a, r);
+  const int32_t k0 = kb * kWeightKeys, kw = k0 + 64 * wave;
+  // (a block before every row's window, or past the keys, is not read by the second launch)
+  if (k0 >= rq.n || rq.S == 0 || (a.window > 0 && (int64_t)k0 + kWeightKeys - 1 <= rq.prior - a.window)) return;  // uniform
+  const int64_t at = weights_key_at(a, r, g, k0 + tid, rq.n, Geo::ROWB);
+  const uint64_t valid = __ballot(at >= 0);
+  const int32_t m = i32, M = rq.S * a.group;
+  const int32_t t = m / a.group, j = m - t * a.group;
+  uint32_t qf[Geo::NS][4];
+  const uint16_t* row = a.q + ((int64_t)(rq.qa + t) * a.H + g * a.group + j) * D;
+#pragma unroll
+  for (int c = 0; c < Geo::NS; ++c) {
+    const uint4 w = m < M ? ld16(row + 8 * weights_chunk<ESZ>(c, g2)) : make_uint4(0, 0, 0, 0);
+    qf[c][0] = w.x, qf[c][1] = w.y, qf[c][2] = w.z, qf[c][3] = w.w;
+  }
+  uint32_t kf[2][Geo::NS][4];
+  weights_keys<D, ESZ>(a, at, sm + wave * Geo::KEYB, kf);
+  f32x16_t x[2] = {};
+#pragma unroll
+  for (int c = 0; c < Geo::NS; ++c) {
+    x[0] = mfma_32x32x16_bf16(kf[0][c], qf[c], x[0]);
+    x[1] = mfma_32x32x16_bf16(kf[1][c], qf[c], x[1]);
+  }
+  const float2 p = weights_stats<false>(x, weights_scale<ESZ>(a, g), weights_seen(a, valid, rq.prior + t, kw), g2);
+  const int32_t width = a.blocks * kWeightKeys, rows = a.max_q * a.group;
+  if (m < M) {
+    float* dst = a.ws_score + (((int64_t)r * a.G + g) * rows + m) * width + kw;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<float4*>(dst + weights_key(s, 4 * q, g2)) =
+            make_float4(x[s][4 * q], x[s][4 * q + 1], x[s][4 * q + 2], x[s][4 * q + 3]);
+  }
+  if (g2 == 0) sm_part[wave][i32] = p;
+  __syncthreads();
+  if (tid < M)
+    a.ws_part[(((int64_t)r * a.G + g) * a.blocks + kb) * rows + tid] =
+        weights_join(weights_join(sm_part[0][tid], sm_part[1][tid]), weights_join(sm_part[2][tid], sm_part[3][tid]));
+}
+
+// 1024 keys a workgroup, 4 to a thread: the rows' blocks merged (16 threads a row), then every key's probabilities summed.
+__global__ __launch_bounds__(256) void weights_from_scores_kernel(WeightsArgs a) {
+  __shared__ float2 sm[16][kScoreRows], sm_row[kScoreRows];
+  const int tid = threadIdx.x;
+  const int32_t r = blockIdx.z, g = blockIdx.y, k0 = blockIdx.x * 1024;
+  const WeightsRequest rq = weights_request(a, r);
+  const int32_t M = rq.S * a.group, rows = a.max_q * a.group;
+  float* const out = a.weights + r * a.w_row + g * a.w_head;
+  // the blocks that any row sees
+  const int64_t first = a.window > 0 ? max(rq.prior - a.window + 1, (int64_t)0) : 0;
+  const int32_t b0 = (int32_t)min(first / kWeightKeys, (int64_t)a.blocks), b1 = (rq.n + kWeightKeys - 1) / kWeightKeys;
+  if (k0 >= rq.n || M == 0 || (int64_t)k0 + 1023 < first) {  // uniform
+    if (!a.add)
+      for (int32_t k = k0 + tid; k < min(k0 + 1024, a.width); k += 256) out[k] = 0.0f;
+    return;
+  }
+  {
+    const int m = tid & (kScoreRows - 1), slice = tid / kScoreRows;
+    float2 p = make_float2(kNegBig, 0.0f);
+    if (m < M) {
+      const float2* part = a.ws_part + ((int64_t)r * a.G + g) * a.blocks * rows + m;
+#pragma unroll 4
+      for (int32_t b = b0 + slice; b < b1; b += 16) p = weights_join(p, part[(int64_t)b * rows]);
+    }
+    sm[slice][m] = p;
+    __syncthreads();
+    if (tid < M) {
+      for (int s = 1; s < 16; ++s) p = weights_join(p, sm[s][tid]);
+      if (a.sinks) p = weights_join(p, make_float2(a.sinks[g * a.group + tid % a.group] * kLog2e, 1.0f));
+      sm_row[tid] = make_float2(p.x, p.y == 0.0f ? 0.0f : 1.0f / p.y);
+    }
+    __syncthreads();
+  }
+  const int32_t key = k0 + 4 * tid;
+  if (key >= a.width) return;
+  float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (key / kWeightKeys >= b0 && key < rq.n) {
+    const int64_t width = (int64_t)a.blocks * kWeightKeys;
+    const float* src = a.ws_score + ((int64_t)r * a.G + g) * rows * width + key;
+#pragma unroll 4
+    for (int32_t m = 0; m < M; ++m) {
+      const float4 x = *reinterpret_cast<const float4*>(src + m * width);
+      const float2 rw = sm_row[m];
+      w.x = fmaf(__builtin_amdgcn_exp2f(x.x - rw.x), rw.y, w.x);
+      w.y = fmaf(__builtin_amdgcn_exp2f(x.y - rw.x), rw.y, w.y);
+      w.z = fmaf(__builtin_amdgcn_exp2f(x.z - rw.x), rw.y, w.z);
+      w.w = fmaf(__builtin_amdgcn_exp2f(x.w - rw.x), rw.y, w.w);
+    }
+  }
+  const float v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (key + e >= a.width) break;
+    if (!a.add) out[key + e] = v[e];
+    else if (key + e < rq.n) out[key + e] += v[e];
+  }
 }
 
 }  // namespace sna
@@ -305,12 +496,36 @@ int64_t weights_blocks(int32_t page_size, int32_t table_width, int32_t width) {
   return (keys + kWeightKeys - 1) / kWeightKeys;
 }
 
-int64_t weights_bytes(int64_t T, int32_t H, int64_t blocks) { return (blocks + 1) * T * H * (int64_t)sizeof(float2); }
+// How a launch works, and its workspace: few rows a request keep their scores (at most kScoreBytes of them), others
+// compute them twice.
+constexpr int64_t kScoreBytes = (int64_t)1 << 29;
+struct WeightsPlan {
+  int64_t blocks, part, rest, bytes;
+  bool scores;
+};
+WeightsPlan weights_plan(int64_t T, int64_t R, int64_t max_q, int32_t H, int32_t G, int32_t page_size,
+                         int32_t table_width, int32_t width) {
+  WeightsPlan p;
+  p.blocks = weights_blocks(page_size, table_width, width);
+  const int64_t rows = max_q * (H / G);
+  const int64_t score = rows <= kScoreRows ? R * G * rows * p.blocks * kWeightKeys * (int64_t)sizeof(float) : INT64_MAX;
+  p.scores = score <= kScoreBytes;
+  p.part = (p.scores ? R * G * rows : T * H) * p.blocks * (int64_t)sizeof(float2);
+  p.rest = p.scores ? score : T * H * (int64_t)sizeof(float2);
+  p.part = (p.part + 15) / 16 * 16;
+  p.bytes = p.part + p.rest;
+  return p;
+}
 
 template <int D, int ESZ>
 void launch_weights(const WeightsArgs& a, uint32_t wgs, hipStream_t s) {
+  if (a.ws_score) {
+    hipLaunchKernelGGL((weights_score_kernel<D, ESZ>), dim3(wgs), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(weights_from_scores_kernel, dim3((a.blocks + 3) / 4, a.G, a.R), dim3(256), 0, s, a);
+    return;
+  }
   hipLaunchKernelGGL((weights_tile_kernel<D, ESZ, kStats>), dim3(wgs), dim3(256), 0, s, a);
-  hipLaunchKernelGGL(weights_merge_kernel, dim3((unsigned)(((int64_t)a.max_q * a.group + 255) / 256), a.G, a.R), dim3(256),
+  hipLaunchKernelGGL(weights_merge_kernel, dim3((unsigned)(((int64_t)a.max_q * a.group + 31) / 32), a.G, a.R), dim3(256),
                      0, s, a);
   hipLaunchKernelGGL((weights_tile_kernel<D, ESZ, kSum>), dim3(wgs), dim3(256), 0, s, a);
 }
@@ -349,12 +564,14 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
   if (head_stride < width || row_stride < width)
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: weight strides %lld / %lld for %d columns", what, (long long)row_stride,
                 (long long)head_stride, width);
-  const int64_t blocks = weights_blocks(page_size, table_width, width);
+  max_q_len = std::max(max_q_len, 1);
+  const WeightsPlan plan = weights_plan(T, R, max_q_len, num_q_heads, num_kv_heads, page_size, table_width, width);
+  const int64_t blocks = plan.blocks;
   const int64_t wgs = blocks * R * num_kv_heads;
   if (wgs > kGridMax)
     return fail(SNA_ERR_UNSUPPORTED, "%s: %lld key blocks x %d requests x %d KV heads exceed the grid (split the batch)",
                 what, (long long)blocks, R, num_kv_heads);
-  const int64_t need = weights_bytes(T, num_q_heads, blocks);
+  const int64_t need = plan.bytes;
   if (workspace_bytes < need || (need > 0 && !workspace))
     return fail(SNA_ERR_WORKSPACE, "%s: workspace of %lld bytes, need %lld", what, (long long)workspace_bytes,
                 (long long)need);
@@ -381,13 +598,14 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
   a.G = num_kv_heads;
   a.P = page_size;
   a.group = group;
-  a.max_q = std::max(max_q_len, 1);
+  a.max_q = max_q_len;
   a.num_blocks = num_blocks;
   a.sm_scale = sm_scale;
   a.window = window;
   a.blocks = (int32_t)blocks;
-  a.ws_row = (float2*)workspace;
-  a.ws_part = a.ws_row + (int64_t)T * num_q_heads;
+  a.ws_part = (float2*)workspace;
+  a.ws_row = plan.scores ? nullptr : (float2*)((uint8_t*)workspace + plan.part);
+  a.ws_score = plan.scores ? (float*)((uint8_t*)workspace + plan.part) : nullptr;
   const hipStream_t s = (hipStream_t)stream;
   if (kv_dtype != SNA_DTYPE_BF16) {
     if (head_dim == 128) launch_weights<128, 1>(a, (uint32_t)wgs, s); else launch_weights<64, 1>(a, (uint32_t)wgs, s);
@@ -402,10 +620,10 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
 extern "C" int64_t sna_attention_weights_workspace_bytes(int32_t n_tokens, int32_t R, int32_t max_q_len,
                                                          int32_t num_q_heads, int32_t num_kv_heads, int32_t page_size,
                                                          int32_t table_width, int32_t width) {
-  if (n_tokens < 1 || R < 1 || max_q_len < 1 || num_q_heads < 1 || num_kv_heads < 1 ||
+  if (n_tokens < 0 || R < 1 || max_q_len < 0 || num_q_heads < 1 || num_kv_heads < 1 ||
       num_q_heads % num_kv_heads != 0 || page_size < 1 || table_width < 1 || width < 0)
     return 0;
-  return weights_bytes(n_tokens, num_q_heads, weights_blocks(page_size, table_width, width));
+  return weights_plan(n_tokens, R, std::max(max_q_len, 1), num_q_heads, num_kv_heads, page_size, table_width, width).bytes;
 }
 
 extern "C" int sna_prefill_attention_weights(const void* q, const void* k_cache, const float* k_scale,
