@@ -38,12 +38,15 @@ struct WeightsArgs {
   int32_t width;
   bool add;  // add to what is there instead of writing every column
   int32_t T, R, H, G, P, group, max_q;
+  uint64_t magic;  // ceil(2^32 / group): row / group = row * magic >> 32 while rows * group <= 2^32
   int64_t num_blocks;
   float sm_scale;
   int32_t window;
   int32_t blocks;    // key blocks that the table's keys (and, when every column is written, the width) take
   float2* ws_part;   // [G, blocks, T * group] a block's (largest score in the log2 domain, sum)
   float2* ws_row;    // [G, T * group] a row's (largest score in the log2 domain, 1 / sum)
+  int32_t splits, split_tokens;  // the queries are cut into so many runs of so many tokens (a multiple of 32)
+  float* ws_sum;     // [splits, R, G, blocks * 256] the runs' sums, with more than one
   // few rows instead: ws_part is [R, G, blocks, max_q * group], and
   float* ws_score;   // [R, G, max_q * group, blocks * 256] scores in the log2 domain, -inf where unseen
 };
@@ -95,6 +98,17 @@ __device__ __forceinline__ int64_t weights_key_at(const WeightsArgs& a, int32_t 
   return ((page * a.G + g) * a.P + (key - col * a.P)) * (int64_t)row_bytes;
 }
 
+// Loads straight into LDS (lane i's bytes at LDS address m0 + size * i) from an address per lane, kept in the caches: other
+// workgroups and the second pass read them again. Assembly, as the DMAs of sna_device.h are; waited for by wait_vmcnt.
+__device__ __forceinline__ void dma_global16_cached(const void* src, uint32_t lds) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m0), "v"(src) : "memory");
+}
+__device__ __forceinline__ void dma_global4(const void* src, uint32_t lds) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(m0), "v"(src) : "memory");
+}
+
 // The wave's 64 keys through LDS (whole rows by DMA, 1024 bytes an instruction) to A operands in registers: lane (g2, i)
 // feeds key 32 s + i, dims 16 c + 8 g2 .. of step c (bf16) or 32 (c / 2) + 16 g2 + 8 (c & 1) .. (FP8, as its 16-byte
 // chunks hold them). A key that is not there reads the cache's first row; what comes of it is masked or dropped.
@@ -109,9 +123,7 @@ __device__ __forceinline__ void weights_keys(const WeightsArgs& a, int64_t at, u
   for (int j = 0; j < 64 / RPD; ++j) {
     const int row = j * RPD + lane / Geo::KCH, ch = lane % Geo::KCH ^ Geo::swz(row, Geo::KCH);
     const uint32_t lo = __shfl((uint32_t)from, row, 64), hi = __shfl((uint32_t)(from >> 32), row, 64);
-    const uint8_t* src = a.k_cache + (int64_t)((uint64_t)hi << 32 | lo) + 16 * ch;
-    const uint32_t m0 = __builtin_amdgcn_readfirstlane(base + 1024 * j);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m0), "v"(src) : "memory");
+    dma_global16_cached(a.k_cache + (int64_t)((uint64_t)hi << 32 | lo) + 16 * ch, base + 1024 * j);
   }
   wait_vmcnt<0>();
 #pragma unroll
@@ -160,6 +172,9 @@ __device__ __forceinline__ uint64_t weights_seen(const WeightsArgs& a, uint64_t 
   }
   return seen;
 }
+// The lane's share of such bits: bit 8 q + r of word s is element 4 q + r of sub-tile s.
+__device__ __forceinline__ uint32_t weights_bits(uint64_t seen, int s, int g2) { return (uint32_t)(seen >> 32 * s) >> 4 * g2; }
+__device__ __forceinline__ constexpr uint32_t weights_bit(int e) { return 1u << (8 * (e / 4) + e % 4); }
 // Key of element e of lane group g2's sub-tile s.
 __device__ __forceinline__ constexpr int weights_key(int s, int e, int g2) { return 32 * s + 8 * (e / 4) + 4 * g2 + e % 4; }
 
@@ -175,12 +190,14 @@ template <bool ALL>
 __device__ __forceinline__ float2 weights_stats(f32x16_t (&x)[2], float c2, uint64_t seen, int g2) {
   float mx = ALL ? -INFINITY : kNegBig, sum = 0.0f;
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+  for (int s = 0; s < 2; ++s) {
+    const uint32_t bits = ALL ? 0 : weights_bits(seen, s, g2);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      if (!ALL) x[s][e] = seen >> weights_key(s, e, g2) & 1 ? x[s][e] * c2 : -INFINITY;
+      if (!ALL) x[s][e] = bits & weights_bit(e) ? x[s][e] * c2 : -INFINITY;
       mx = fmaxf(mx, x[s][e]);
     }
+  }
   if (ALL) mx *= c2;
 #pragma unroll
   for (int s = 0; s < 2; ++s)
@@ -191,71 +208,118 @@ __device__ __forceinline__ float2 weights_stats(f32x16_t (&x)[2], float c2, uint
 }
 
 enum WeightsPass { kStats, kSum };
+template <int D, int ESZ>
+struct WeightsRing {
+  using Geo = WeightsGeo<D, ESZ>;
+  static constexpr int SLOTS = 8;               // row tiles in LDS: one read, the others on their way
+  static constexpr int SLOTB = Geo::TILE * 16;  // bytes of a tile
+  static constexpr int LD = SLOTB / 4096;       // DMAs of a tile that a wave issues
+  // The keys take the ring's last slots (and, bf16 at D = 128, one slot more) on their way to registers; the EARLY first
+  // tiles are on their way beside them.
+  static constexpr int EARLY = SLOTS * SLOTB - 4 * Geo::KEYB > 0 ? (SLOTS * SLOTB - 4 * Geo::KEYB) / SLOTB : 1;
+  static constexpr int BYTES = EARLY * SLOTB + (4 * Geo::KEYB > (SLOTS - EARLY) * SLOTB ? 4 * Geo::KEYB
+                                                                                       : (SLOTS - EARLY) * SLOTB);
+};
 template <int D, int ESZ, WeightsPass PASS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void weights_tile_kernel(WeightsArgs a) {
   using Geo = WeightsGeo<D, ESZ>;
-  constexpr int NS = Geo::NS, CH = Geo::QCH, TILE = Geo::TILE;
-  constexpr int LD = TILE / 256;  // chunks of a tile that a thread moves
-  constexpr int BYTES = 4 * Geo::KEYB > 2 * TILE * 16 ? 4 * Geo::KEYB : 2 * TILE * 16;
-  __shared__ __attribute__((aligned(1024))) uint8_t sm[BYTES];  // the keys on their way to registers, then the row tiles
-  __shared__ float sm_out[kWeightKeys];
-  __shared__ float2 sm_part[2][4][kWeightRows];
-  uint4* const sm_q = reinterpret_cast<uint4*>(sm);
+  using Ring = WeightsRing<D, ESZ>;
+  constexpr int NS = Geo::NS, CH = Geo::QCH, SLOTS = Ring::SLOTS, LD = Ring::LD;
+  constexpr int DMAS = LD + (PASS == kSum);  // that a wave issues for a tile
+  __shared__ __attribute__((aligned(1024))) uint8_t sm[Ring::BYTES];
+  __shared__ float2 sm_row[PASS == kSum ? SLOTS : 1][kWeightRows];  // the tiles' rows of ws_row
+  __shared__ float sm_out[PASS == kSum ? kWeightKeys : 1];
+  __shared__ float2 sm_part[PASS == kStats ? 2 : 1][4][kWeightRows];
   const int tid = threadIdx.x, lane = tid & 63, g2 = lane >> 5, i32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t lin = xcd_order(blockIdx.x, gridDim.x);
-  const int32_t kb = (int32_t)(lin % a.blocks), r = (int32_t)(lin / a.blocks % a.R), g = (int32_t)(lin / a.blocks / a.R);
+  uint32_t lin = xcd_order(blockIdx.x, gridDim.x);
+  const int32_t kb = (int32_t)(lin % a.blocks);
+  lin /= a.blocks;
+  const int32_t run = (int32_t)(lin % a.splits), r = (int32_t)(lin / a.splits % a.R), g = (int32_t)(lin / a.splits / a.R);
   const WeightsRequest rq = weights_request(a, r);
   const int32_t k0 = kb * kWeightKeys;
-  // the rows that see any of the block's keys: tokens [t0, t1)
+  // the run's rows that see any of the block's keys: tokens [t0, t1)
   const int64_t last = (int64_t)min(k0 + kWeightKeys, rq.n) - 1;
-  int32_t t0 = (int32_t)min(max(k0 - rq.prior, (int64_t)0), (int64_t)rq.S), t1 = rq.S;
-  if (a.window > 0) t1 = (int32_t)min(max(last + a.window - rq.prior, (int64_t)0), (int64_t)rq.S);
+  const int64_t run0 = (int64_t)run * a.split_tokens;
+  const int32_t s0 = (int32_t)min(run0, (int64_t)rq.S), s1 = (int32_t)min(run0 + a.split_tokens, (int64_t)rq.S);
+  int32_t t0 = (int32_t)min(max(k0 - rq.prior, (int64_t)s0), (int64_t)s1), t1 = s1;
+  if (a.window > 0) t1 = (int32_t)min(max(last + a.window - rq.prior, (int64_t)s0), (int64_t)s1);
   if (k0 >= rq.n) t1 = t0;
-  float* const out = a.weights + r * a.w_row + g * a.w_head;
+  // where the block's sums go: the weights, or the run's part of them
+  const bool parts = a.splits > 1;
+  float* const out = parts ? a.ws_sum + (((int64_t)run * a.R + r) * a.G + g) * a.blocks * kWeightKeys
+                           : a.weights + r * a.w_row + g * a.w_head;
+  const int32_t width = parts ? a.blocks * kWeightKeys : a.width;
+  const bool add = a.add && !parts;
   if (t1 <= t0) {  // uniform
-    if (PASS == kSum && !a.add && k0 + tid < a.width) out[k0 + tid] = 0.0f;
+    if (PASS == kSum && !add && k0 + tid < width) out[k0 + tid] = 0.0f;
     return;
   }
-  const int64_t at = weights_key_at(a, r, g, k0 + tid, rq.n, Geo::ROWB);
-  const uint64_t valid = __ballot(at >= 0);
-  uint32_t kf[2][NS][4];
-  weights_keys<D, ESZ>(a, at, sm + wave * Geo::KEYB, kf);
+  auto token_of = [&](int32_t row) -> int32_t { return (int32_t)((uint64_t)(uint32_t)row * a.magic >> 32); };
   const int32_t m_end = t1 * a.group;
   const int32_t m0 = (t0 * a.group) & ~(kWeightRows - 1);
   const int32_t tiles = (m_end - m0 + kWeightRows - 1) / kWeightRows;
-  // this thread's chunks of a tile: row (tid + 256 l) / CH, chunk (tid + 256 l) % CH; the row's token and head move on by
-  // 32 rows a tile
-  const int32_t step_t = kWeightRows / a.group, step_j = kWeightRows - step_t * a.group;
-  int32_t ld_t[LD], ld_j[LD];
-  uint4 ld[LD];
-#pragma unroll
-  for (int l = 0; l < LD; ++l) {
-    const int32_t m = m0 + (tid + 256 * l) / CH;
-    ld_t[l] = m / a.group, ld_j[l] = m - ld_t[l] * a.group;
-  }
-  auto load = [&]() {
-#pragma unroll
-    for (int l = 0; l < LD; ++l) {
-      ld[l] = make_uint4(0, 0, 0, 0);
-      if (ld_t[l] < t1)
-        ld[l] = ld16(a.q + ((int64_t)(rq.qa + ld_t[l]) * a.H + g * a.group + ld_j[l]) * D + 8 * (tid % CH));
-      ld_t[l] += step_t, ld_j[l] += step_j;
-      if (ld_j[l] >= a.group) ld_j[l] -= a.group, ++ld_t[l];
-    }
-  };
-  load();
-  const float c2 = weights_scale<ESZ>(a, g);
   const int64_t rows = (int64_t)a.T * a.group;  // rows of a KV head
   float2* const part = a.ws_part + ((int64_t)g * a.blocks + kb) * rows + (int64_t)rq.qa * a.group;
   const float2* const row_of = a.ws_row + (int64_t)g * rows + (int64_t)rq.qa * a.group;
+  // Tile i to its slot by whole-row DMAs, chunk c of row r to c ^ swz(r). Where the heads of a token never straddle two
+  // tiles, every tile but the last lies a scalar step behind the one before; else, and in the last (rows past its end
+  // repeat the last one; they are dropped), the rows' tokens are found again.
+  const bool whole = kWeightRows % a.group == 0;
+  const uint16_t* const q0 = a.q + ((int64_t)rq.qa * a.H + g * a.group) * D;
+  const uint32_t ring = lds_address((lds_ptr_t*)sm);
+  constexpr int RPD = 64 / CH;  // rows a DMA fills
+  int32_t ld_row[LD], ld_ch[LD];
+  uint32_t ld_off[LD];
+#pragma unroll
+  for (int l = 0; l < LD; ++l) {
+    ld_row[l] = (LD * wave + l) * RPD + lane / CH;
+    ld_ch[l] = 16 * (lane % CH ^ Geo::swz(ld_row[l], CH));
+    const int32_t t = token_of(ld_row[l]);
+    ld_off[l] = (uint32_t)(t * a.H + ld_row[l] - t * a.group) * (2 * D) + ld_ch[l];
+  }
+  auto load = [&](int32_t i) {
+    const uint32_t slot = ring + (i & (SLOTS - 1)) * Ring::SLOTB + LD * wave * 1024;
+    const int32_t m = m0 + kWeightRows * i;
+    if (whole && i < tiles - 1) {  // uniform (m is a token's first row here)
+      const uint16_t* const base = q0 + (int64_t)token_of(m) * a.H * D;
+#pragma unroll
+      for (int l = 0; l < LD; ++l) dma_saddr16_cached(base, ld_off[l], slot + 1024 * l);
+    } else {
+#pragma unroll
+      for (int l = 0; l < LD; ++l) {
+        const int32_t row = min(m + ld_row[l], m_end - 1), t = token_of(row);
+        dma_global16_cached(reinterpret_cast<const uint8_t*>(q0 + ((int64_t)t * a.H + row - t * a.group) * D) + ld_ch[l],
+                            slot + 1024 * l);
+      }
+    }
+    if constexpr (PASS == kSum) {  // 8 of the tile's rows, two dwords each
+      if (lane < 16) {
+        const int32_t row = min(m + 8 * wave + lane / 2, m_end - 1);
+        dma_global4(reinterpret_cast<const float*>(row_of + row) + (lane & 1), lds_address((lds_ptr_t*)sm_row[i & (SLOTS - 1)]) + 64 * wave);
+      }
+    }
+  };
+  const int32_t early = min(tiles, Ring::EARLY);
+  for (int32_t i = 0; i < early; ++i) load(i);
+  const int64_t at = weights_key_at(a, r, g, k0 + tid, rq.n, Geo::ROWB);
+  const uint64_t valid = __ballot(at >= 0);
+  uint32_t kf[2][NS][4];
+  weights_keys<D, ESZ>(a, at, sm + Ring::EARLY * Ring::SLOTB + wave * Geo::KEYB, kf);
+  const float c2 = weights_scale<ESZ>(a, g);
   const int32_t kw = k0 + 64 * wave;  // the wave's first key
   float acc[2][16];
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[s][e] = 0.0f;
+  // a row's (largest, 1 / sum); one that drops every score past the last
+  auto row_stats = [&](int32_t i) -> float2 {
+    const float2 v = sm_row[i & (SLOTS - 1)][i32];
+    const int32_t m = m0 + kWeightRows * i;
+    return m + kWeightRows <= m_end || m + i32 < m_end ? v : make_float2(-kNegBig, 0.0f);
+  };
   // the four waves' parts of tile i merged and written
   auto write_part = [&](int32_t i) {
     const int32_t m = m0 + kWeightRows * i + i32;
@@ -264,25 +328,9 @@ void weights_tile_kernel(WeightsArgs a) {
       part[m] = weights_join(weights_join(p[0][i32], p[1][i32]), weights_join(p[2][i32], p[3][i32]));
     }
   };
-  // (t, j): token and head of the lane's row, and of the tile's first and last rows
-  int32_t t = (m0 + i32) / a.group, j = m0 + i32 - t * a.group;
-  int32_t tf = m0 / a.group, jf = m0 - tf * a.group;
-  __syncthreads();  // every wave has its keys: the row tiles take their place
-
-  for (int32_t i = 0; i < tiles; ++i) {
-    uint4* const slot = sm_q + (i & 1) * TILE;
-#pragma unroll
-    for (int l = 0; l < LD; ++l) {
-      const int row = (tid + 256 * l) / CH, ch = tid % CH;
-      slot[row * CH + (ch ^ Geo::swz(row, CH))] = ld[l];
-    }
-    __syncthreads();  // the slot was read two tiles ago: the barrier between covers it
-    if (i + 1 < tiles) load();
-    const int32_t m = m0 + kWeightRows * i + i32;  // this lane's row
-    float2 rw = make_float2(0.0f, 0.0f);
-    if (PASS == kSum && m < m_end) rw = row_of[m];
-    if (PASS == kStats && i > 0) write_part(i - 1);
-    f32x16_t x[2] = {};
+  auto products = [&](int32_t i, f32x16_t (&x)[2]) {
+    const uint4* const slot = reinterpret_cast<const uint4*>(sm + (i & (SLOTS - 1)) * Ring::SLOTB);
+    x[0] = x[1] = f32x16_t{};
 #pragma unroll
     for (int c = 0; c < NS; ++c) {
       const uint4 w = slot[i32 * CH + (weights_chunk<ESZ>(c, g2) ^ Geo::swz(i32, CH))];
@@ -290,34 +338,68 @@ void weights_tile_kernel(WeightsArgs a) {
       x[0] = mfma_32x32x16_bf16(kf[0][c], qf, x[0]);
       x[1] = mfma_32x32x16_bf16(kf[1][c], qf, x[1]);
     }
+  };
+  float2 rw = make_float2(0.0f, 0.0f);
+  // Tile i's scores x are worked on while the next tile's products run (past the last tile: of stale rows, dropped).
+  auto step = [&](int32_t i, f32x16_t (&x)[2], f32x16_t (&next)[2]) {
+    // tile i + 1 is in its slot once this wave's DMAs and the others' are (SLOTS - 2 later tiles may be on their way), and
+    // the barrier also says that tile i, whose slot tile i + SLOTS takes, is read
+    if (i + SLOTS <= tiles) wait_vmcnt<(SLOTS - 2) * DMAS>();
+    else wait_vmcnt<0>();
+    __syncthreads();
+    if (i + SLOTS < tiles) load(i + SLOTS);
+    float2 rn = rw;  // (read with the tile: its slot's next one may be on its way after the next barrier)
+    if (PASS == kSum) rn = row_stats(i + 1);
+    if (PASS == kStats && i > 0) write_part(i - 1);
     // whether the tile's first row (and, in a window, its last) sees all of the wave's keys: scalar work
-    const int32_t te = tf + (jf + kWeightRows - 1) / a.group;
-    bool all = c2 > 0.0f && rq.prior + tf >= kw + 63 && (PASS == kSum || valid == ~0ull);
-    if (a.window > 0) all = all && rq.prior + te - a.window < kw;
-    if constexpr (PASS == kStats) {
-      const float2 p = all ? weights_stats<true>(x, c2, 0, g2)
-                           : weights_stats<false>(x, c2, weights_seen(a, valid, rq.prior + t, kw), g2);
-      if (g2 == 0) sm_part[i & 1][wave][i32] = p;
-    } else if (all) {
+    const int32_t m = m0 + kWeightRows * i;
+    bool all = c2 > 0.0f && rq.prior + token_of(m) >= kw + 63 && (PASS == kSum || valid == ~0ull);
+    if (a.window > 0) all = all && rq.prior + token_of(m + kWeightRows - 1) - a.window < kw;
+    if (all) {
+      products(i + 1, next);
+      if constexpr (PASS == kStats) {
+        const float2 p = weights_stats<true>(x, c2, 0, g2);
+        if (g2 == 0) sm_part[i & 1][wave][i32] = p;
+      } else {
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          acc[s][e] = fmaf(__builtin_amdgcn_exp2f(fmaf(x[s][e], c2, -rw.x)), rw.y, acc[s][e]);
+          for (int e = 0; e < 16; ++e) x[s][e] = __builtin_amdgcn_exp2f(fmaf(x[s][e], c2, -rw.x));
+      }
     } else {
-      const uint64_t seen = m < m_end ? weights_seen(a, valid, rq.prior + t, kw) : 0;
+      const uint64_t seen = weights_seen(a, valid, rq.prior + token_of(m + i32), kw);
+      products(i + 1, next);
+      if constexpr (PASS == kStats) {
+        const float2 p = weights_stats<false>(x, c2, seen, g2);
+        if (g2 == 0) sm_part[i & 1][wave][i32] = p;
+      } else {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const uint32_t bits = weights_bits(seen, s, g2);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(x[s][e], c2, -rw.x));
+            x[s][e] = bits & weights_bit(e) ? p : 0.0f;
+          }
+        }
+      }
+    }
+    if constexpr (PASS == kSum) {
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(x[s][e], c2, -rw.x)) * rw.y;
-          acc[s][e] += seen >> weights_key(s, e, g2) & 1 ? p : 0.0f;
-        }
+        for (int e = 0; e < 16; ++e) acc[s][e] = fmaf(x[s][e], rw.y, acc[s][e]);
     }
-    t += step_t, j += step_j;
-    if (j >= a.group) j -= a.group, ++t;
-    tf += step_t, jf += step_j;
-    if (jf >= a.group) jf -= a.group, ++tf;
+    rw = rn;
+  };
+  __syncthreads();  // every wave has its keys (and, with them, its early tiles): the other tiles take their place
+  for (int32_t i = early; i < min(tiles, SLOTS); ++i) load(i);
+  f32x16_t x0[2], x1[2];
+  if (PASS == kSum) rw = row_stats(0);
+  products(0, x0);
+  for (int32_t i = 0; i < tiles; i += 2) {
+    step(i, x0, x1);
+    if (i + 1 < tiles) step(i + 1, x1, x0);
   }
   if constexpr (PASS == kStats) {
     __syncthreads();
@@ -333,12 +415,26 @@ void weights_tile_kernel(WeightsArgs a) {
       }
     __syncthreads();
     const int32_t key = k0 + tid;
-    if (key < a.width) {
+    if (key < width) {
       const float v = at >= 0 ? sm_out[tid] : 0.0f;
-      if (!a.add) out[key] = v;
+      if (!add) out[key] = v;
       else if (at >= 0) out[key] += v;
     }
   }
+}
+
+// The runs' sums of a key added in their order.
+__global__ __launch_bounds__(256) void weights_reduce_kernel(WeightsArgs a) {
+  const int32_t r = blockIdx.z, g = blockIdx.y, key = blockIdx.x * 256 + threadIdx.x;
+  const WeightsRequest rq = weights_request(a, r);
+  if (key >= a.width || (a.add && key >= rq.n)) return;
+  const int64_t step = (int64_t)a.R * a.G * a.blocks * kWeightKeys;
+  const float* src = a.ws_sum + ((int64_t)r * a.G + g) * a.blocks * kWeightKeys + key;
+  float v = 0.0f;
+#pragma unroll 4
+  for (int32_t s = 0; s < a.splits; ++s) v += src[s * step];
+  float* out = a.weights + r * a.w_row + g * a.w_head + key;
+  *out = a.add ? *out + v : v;
 }
 
 // A row's blocks merged: (its largest score M in the log2 domain, 1 / sum of 2^(score - M) with the sink's). 32 rows a
@@ -368,7 +464,8 @@ __global__ __launch_bounds__(256) void weights_merge_kernel(WeightsArgs a) {
   if (slice == 0 && (int32_t)blockIdx.x * 32 + i < rq.S * a.group) {
     for (int s = 1; s < 8; ++s) p = weights_join(p, sm[s][i]);
     if (a.sinks) p = weights_join(p, make_float2(a.sinks[h] * kLog2e, 1.0f));
-    a.ws_row[(int64_t)g * rows + row] = make_float2(p.x, p.y == 0.0f ? 0.0f : 1.0f / p.y);
+    // (a row that sees nothing: every score is dropped)
+    a.ws_row[(int64_t)g * rows + row] = p.y == 0.0f ? make_float2(-kNegBig, 0.0f) : make_float2(p.x, 1.0f / p.y);
   }
 }
 
@@ -454,7 +551,7 @@ __global__ __launch_bounds__(256) void weights_from_scores_kernel(WeightsArgs a)
     if (tid < M) {
       for (int s = 1; s < 16; ++s) p = weights_join(p, sm[s][tid]);
       if (a.sinks) p = weights_join(p, make_float2(a.sinks[g * a.group + tid % a.group] * kLog2e, 1.0f));
-      sm_row[tid] = make_float2(p.x, p.y == 0.0f ? 0.0f : 1.0f / p.y);
+      sm_row[tid] = p.y == 0.0f ? make_float2(-kNegBig, 0.0f) : make_float2(p.x, 1.0f / p.y);
     }
     __syncthreads();
   }
@@ -501,8 +598,11 @@ int64_t weights_blocks(int32_t page_size, int32_t table_width, int32_t width) {
 constexpr int64_t kScoreBytes = (int64_t)1 << 29;
 struct WeightsPlan {
   int64_t blocks, part, rest, bytes;
+  int32_t splits, split_tokens;
   bool scores;
 };
+constexpr int64_t kSplitRows = 2048;       // least rows of a run of queries
+constexpr int64_t kSplitWorkgroups = 4096; // runs are cut up to so many workgroups
 WeightsPlan weights_plan(int64_t T, int64_t R, int64_t max_q, int32_t H, int32_t G, int32_t page_size,
                          int32_t table_width, int32_t width) {
   WeightsPlan p;
@@ -512,8 +612,19 @@ WeightsPlan weights_plan(int64_t T, int64_t R, int64_t max_q, int32_t H, int32_t
   p.scores = score <= kScoreBytes;
   p.part = (p.scores ? R * G * rows : T * H) * p.blocks * (int64_t)sizeof(float2);
   p.rest = p.scores ? score : T * H * (int64_t)sizeof(float2);
+  const int64_t group = H / G;
+  p.splits = 1, p.split_tokens = (int32_t)max_q;
+  int64_t sum = 0;
+  if (!p.scores) {
+    const int64_t least = ((kSplitRows + group - 1) / group + kWeightRows - 1) / kWeightRows * kWeightRows;
+    const int64_t most = std::max<int64_t>(1, std::min((max_q + least - 1) / least, kSplitWorkgroups / (p.blocks * R * G)));
+    p.split_tokens = (int32_t)(((max_q + most - 1) / most + kWeightRows - 1) / kWeightRows * kWeightRows);
+    p.splits = (int32_t)((max_q + p.split_tokens - 1) / p.split_tokens);
+    if (p.splits > 1) sum = p.splits * R * G * p.blocks * kWeightKeys * (int64_t)sizeof(float);
+  }
   p.part = (p.part + 15) / 16 * 16;
-  p.bytes = p.part + p.rest;
+  p.rest = (p.rest + 15) / 16 * 16;
+  p.bytes = p.part + p.rest + sum;
   return p;
 }
 
@@ -528,6 +639,8 @@ void launch_weights(const WeightsArgs& a, uint32_t wgs, hipStream_t s) {
   hipLaunchKernelGGL(weights_merge_kernel, dim3((unsigned)(((int64_t)a.max_q * a.group + 31) / 32), a.G, a.R), dim3(256),
                      0, s, a);
   hipLaunchKernelGGL((weights_tile_kernel<D, ESZ, kSum>), dim3(wgs), dim3(256), 0, s, a);
+  if (a.splits > 1)
+    hipLaunchKernelGGL(weights_reduce_kernel, dim3((unsigned)((a.width + 255) / 256), a.G, a.R), dim3(256), 0, s, a);
 }
 
 int attention_weights(const char* what, const void* q, const void* k_cache, const float* k_scale,
@@ -561,13 +674,16 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %d requests x %d KV heads exceed the grid", what, R, num_kv_heads);
   if ((int64_t)T * group > INT32_MAX - kWeightRows)
     return fail(SNA_ERR_UNSUPPORTED, "%s: %d tokens of %d heads a KV head (split the batch)", what, T, group);
+  if ((int64_t)max_q_len * group * group > (int64_t)1 << 32)  // (the kernels' row / group is exact up to there)
+    return fail(SNA_ERR_UNSUPPORTED, "%s: chunks of up to %d tokens of %d heads a KV head (split them)", what, max_q_len,
+                group);
   if (head_stride < width || row_stride < width)
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: weight strides %lld / %lld for %d columns", what, (long long)row_stride,
                 (long long)head_stride, width);
   max_q_len = std::max(max_q_len, 1);
   const WeightsPlan plan = weights_plan(T, R, max_q_len, num_q_heads, num_kv_heads, page_size, table_width, width);
   const int64_t blocks = plan.blocks;
-  const int64_t wgs = blocks * R * num_kv_heads;
+  const int64_t wgs = blocks * R * num_kv_heads * plan.splits;
   if (wgs > kGridMax)
     return fail(SNA_ERR_UNSUPPORTED, "%s: %lld key blocks x %d requests x %d KV heads exceed the grid (split the batch)",
                 what, (long long)blocks, R, num_kv_heads);
@@ -598,6 +714,7 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
   a.G = num_kv_heads;
   a.P = page_size;
   a.group = group;
+  a.magic = ((1ull << 32) + group - 1) / group;
   a.max_q = max_q_len;
   a.num_blocks = num_blocks;
   a.sm_scale = sm_scale;
@@ -605,6 +722,9 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
   a.blocks = (int32_t)blocks;
   a.ws_part = (float2*)workspace;
   a.ws_row = plan.scores ? nullptr : (float2*)((uint8_t*)workspace + plan.part);
+  a.splits = plan.splits;
+  a.split_tokens = plan.split_tokens;
+  a.ws_sum = (float*)((uint8_t*)workspace + plan.part + plan.rest);
   a.ws_score = plan.scores ? (float*)((uint8_t*)workspace + plan.part) : nullptr;
   const hipStream_t s = (hipStream_t)stream;
   if (kv_dtype != SNA_DTYPE_BF16) {

@@ -100,6 +100,9 @@ CASES = [
     ("holes-window", 8, 2, 64, 16, [300, 400, 64], [300, 7, 64], True, 20, False, 40),
     ("page-7", 4, 2, 64, 7, [100, 30], [33, 30], False, 0, False, 0),
     ("long-window-of-queries", 4, 1, 128, 64, [3000], [32], True, 0, False, 0),
+    ("runs-of-queries", 64, 1, 64, 16, [100, 300], [100, 70], True, 0, True, 2),
+    ("runs-window", 96, 2, 128, 16, [150, 40], [150, 40], False, 33, False, 0),
+    ("many-tiles", 16, 1, 128, 16, [700], [530], True, 0, False, 0),
     ("many-rows", 2, 1, 64, 16, [5 + 13 * i for i in range(40)], [1 + i % 4 for i in range(40)], True, 0, False, 0),
 ]
 
@@ -174,6 +177,16 @@ def test_accumulates_into_strided_weights_and_leaves_the_rest():
     prefill(c, weights=t)
     want, reach = oracle(c, 320)
     check(c, t, want, reach, "transposed")
+
+
+def test_accumulates_runs_of_queries():
+    c = make(12, 64, 1, 64, 16, [100, 80], [90, 80], False)
+    w = torch.full((2, 1, 128), 3.0, device=DEV)
+    prefill(c, weights=w)
+    want, reach = oracle(c, 128)
+    off = (w.double().cpu() - (want + 3)).abs()
+    rel = 2 * (64 + 8) * 2.0 ** -24 * reach + (128 + 1 + 64 * 90) * 2.0 ** -24
+    assert bool((off <= want * rel + (3 + want) * 2.0 ** -24).all()) and bool((w[0, :, 100:] == 3).all())
 
 
 def test_multipliers_and_strided_queries():
