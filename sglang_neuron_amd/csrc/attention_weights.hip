@@ -16,6 +16,7 @@
 // normalization are values of the lane, and a key's sum over the rows stays in the lane's registers until the end.
 // Scores are fp32, exponentials in the log2 domain, every sum fp32; a key's rows are added in a fixed order.
 #include <algorithm>
+#include <type_traits>
 
 #include "sna_device.h"
 #include "sna_host.h"
@@ -230,7 +231,7 @@ void weights_tile_kernel(WeightsArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t sm[Ring::BYTES];
   __shared__ float2 sm_row[PASS == kSum ? SLOTS : 1][kWeightRows];  // the tiles' rows of ws_row
   __shared__ float sm_out[PASS == kSum ? kWeightKeys : 1];
-  __shared__ float2 sm_part[PASS == kStats ? 2 : 1][4][kWeightRows];
+  __shared__ float2 sm_part[PASS == kStats ? 4 : 1][4][kWeightRows];
   const int tid = threadIdx.x, lane = tid & 63, g2 = lane >> 5, i32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   uint32_t lin = xcd_order(blockIdx.x, gridDim.x);
@@ -263,41 +264,41 @@ void weights_tile_kernel(WeightsArgs a) {
   const int64_t rows = (int64_t)a.T * a.group;  // rows of a KV head
   float2* const part = a.ws_part + ((int64_t)g * a.blocks + kb) * rows + (int64_t)rq.qa * a.group;
   const float2* const row_of = a.ws_row + (int64_t)g * rows + (int64_t)rq.qa * a.group;
-  // Tile i to its slot by whole-row DMAs, chunk c of row r to c ^ swz(r). Where the heads of a token never straddle two
-  // tiles, every tile but the last lies a scalar step behind the one before; else, and in the last (rows past its end
-  // repeat the last one; they are dropped), the rows' tokens are found again.
+  // Tile i (in order) to its slot by whole-row DMAs, chunk c of row r to c ^ swz(r). Where the heads of a token never
+  // straddle two tiles, every tile but the last lies a scalar step behind the one before; else, and in the last (rows past
+  // its end repeat the last one; they are dropped), the rows' tokens are found again.
   const bool whole = kWeightRows % a.group == 0;
   const uint16_t* const q0 = a.q + ((int64_t)rq.qa * a.H + g * a.group) * D;
-  const uint32_t ring = lds_address((lds_ptr_t*)sm);
+  const uint32_t ring = lds_address((lds_ptr_t*)sm), ring_row = lds_address((lds_ptr_t*)sm_row);
   constexpr int RPD = 64 / CH;  // rows a DMA fills
-  int32_t ld_row[LD], ld_ch[LD];
+  const int64_t q_step = (int64_t)(kWeightRows / a.group) * a.H * D;
+  const uint16_t* q_tile = q0 + (int64_t)token_of(m0) * a.H * D;  // tile i's first row, where they are whole
   uint32_t ld_off[LD];
 #pragma unroll
   for (int l = 0; l < LD; ++l) {
-    ld_row[l] = (LD * wave + l) * RPD + lane / CH;
-    ld_ch[l] = 16 * (lane % CH ^ Geo::swz(ld_row[l], CH));
-    const int32_t t = token_of(ld_row[l]);
-    ld_off[l] = (uint32_t)(t * a.H + ld_row[l] - t * a.group) * (2 * D) + ld_ch[l];
+    const int32_t row = (LD * wave + l) * RPD + lane / CH, t = token_of(row);
+    ld_off[l] = (uint32_t)(t * a.H + row - t * a.group) * (2 * D) + 16 * (lane % CH ^ Geo::swz(row, CH));
   }
   auto load = [&](int32_t i) {
     const uint32_t slot = ring + (i & (SLOTS - 1)) * Ring::SLOTB + LD * wave * 1024;
-    const int32_t m = m0 + kWeightRows * i;
-    if (whole && i < tiles - 1) {  // uniform (m is a token's first row here)
-      const uint16_t* const base = q0 + (int64_t)token_of(m) * a.H * D;
+    if (whole && i < tiles - 1) {  // uniform
 #pragma unroll
-      for (int l = 0; l < LD; ++l) dma_saddr16_cached(base, ld_off[l], slot + 1024 * l);
+      for (int l = 0; l < LD; ++l) dma_saddr16_cached(q_tile, ld_off[l], slot + 1024 * l);
     } else {
 #pragma unroll
       for (int l = 0; l < LD; ++l) {
-        const int32_t row = min(m + ld_row[l], m_end - 1), t = token_of(row);
-        dma_global16_cached(reinterpret_cast<const uint8_t*>(q0 + ((int64_t)t * a.H + row - t * a.group) * D) + ld_ch[l],
+        const int32_t at = (LD * wave + l) * RPD + lane / CH;
+        const int32_t row = min(m0 + kWeightRows * i + at, m_end - 1), t = token_of(row);
+        dma_global16_cached(q0 + ((int64_t)t * a.H + row - t * a.group) * D + 8 * (lane % CH ^ Geo::swz(at, CH)),
                             slot + 1024 * l);
       }
     }
+    q_tile += q_step;
     if constexpr (PASS == kSum) {  // 8 of the tile's rows, two dwords each
       if (lane < 16) {
-        const int32_t row = min(m + 8 * wave + lane / 2, m_end - 1);
-        dma_global4(reinterpret_cast<const float*>(row_of + row) + (lane & 1), lds_address((lds_ptr_t*)sm_row[i & (SLOTS - 1)]) + 64 * wave);
+        const int32_t row = min(m0 + kWeightRows * i + 8 * wave + lane / 2, m_end - 1);
+        dma_global4(reinterpret_cast<const float*>(row_of + row) + (lane & 1),
+                    ring_row + (i & (SLOTS - 1)) * (kWeightRows * 8) + 64 * wave);
       }
     }
   };
@@ -314,96 +315,97 @@ void weights_tile_kernel(WeightsArgs a) {
   for (int s = 0; s < 2; ++s)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[s][e] = 0.0f;
-  // a row's (largest, 1 / sum); one that drops every score past the last
-  auto row_stats = [&](int32_t i) -> float2 {
-    const float2 v = sm_row[i & (SLOTS - 1)][i32];
-    const int32_t m = m0 + kWeightRows * i;
-    return m + kWeightRows <= m_end || m + i32 < m_end ? v : make_float2(-kNegBig, 0.0f);
-  };
+  // The pairs of tiles [f0, f1) whose every row sees all of the wave's keys (SUM does not mind keys that are not there:
+  // their sums are dropped): from the pair whose first token reaches the last key, to the one before a row past the end, or
+  // past the first key's window.
+  const int32_t pairs = (tiles + 1) / 2;
+  int32_t f0 = pairs, f1 = 0;
+  if (c2 > 0.0f && (PASS == kSum || valid == ~0ull)) {  // uniform
+    auto pair_from = [&](int64_t token) -> int32_t {  // the first pair that starts at or behind a token's first row
+      const int64_t row = min(max(token, (int64_t)t0), (int64_t)t1) * a.group - m0;
+      return (int32_t)((row + 2 * kWeightRows - 1) / (2 * kWeightRows));
+    };
+    f0 = max(pair_from(kw + 63 - rq.prior), 0);
+    f1 = (m_end - m0) / (2 * kWeightRows);
+    if (a.window > 0) {  // whole pairs of tokens below the first one that no longer sees key kw
+      const int64_t end = min(max((int64_t)kw + a.window - rq.prior, (int64_t)t0), (int64_t)t1) * a.group - m0;
+      f1 = min(f1, (int32_t)(max(end, (int64_t)0) / (2 * kWeightRows)));
+    }
+  }
+  f0 = __builtin_amdgcn_readfirstlane(f0), f1 = __builtin_amdgcn_readfirstlane(f1);
   // the four waves' parts of tile i merged and written
   auto write_part = [&](int32_t i) {
     const int32_t m = m0 + kWeightRows * i + i32;
     if (wave == (i & 3) && g2 == 0 && m < m_end) {
-      const float2(*p)[kWeightRows] = sm_part[i & 1];
+      const float2(*p)[kWeightRows] = sm_part[i & 3];
       part[m] = weights_join(weights_join(p[0][i32], p[1][i32]), weights_join(p[2][i32], p[3][i32]));
     }
   };
-  auto products = [&](int32_t i, f32x16_t (&x)[2]) {
+  float2 rw[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};  // the rows' (largest, 1 / sum) of two tiles
+  f32x16_t x[2][2];                                                   // and their scores
+  // The products of tile i, to x[i & 1] (past the last tile: of stale rows, dropped).
+  auto products = [&](int32_t i, int b) {
     const uint4* const slot = reinterpret_cast<const uint4*>(sm + (i & (SLOTS - 1)) * Ring::SLOTB);
-    x[0] = x[1] = f32x16_t{};
+    if (PASS == kSum) rw[b] = sm_row[i & (SLOTS - 1)][i32];
+    x[b][0] = x[b][1] = f32x16_t{};
 #pragma unroll
     for (int c = 0; c < NS; ++c) {
       const uint4 w = slot[i32 * CH + (weights_chunk<ESZ>(c, g2) ^ Geo::swz(i32, CH))];
       const uint32_t qf[4] = {w.x, w.y, w.z, w.w};
-      x[0] = mfma_32x32x16_bf16(kf[0][c], qf, x[0]);
-      x[1] = mfma_32x32x16_bf16(kf[1][c], qf, x[1]);
+      x[b][0] = mfma_32x32x16_bf16(kf[0][c], qf, x[b][0]);
+      x[b][1] = mfma_32x32x16_bf16(kf[1][c], qf, x[b][1]);
     }
   };
-  float2 rw = make_float2(0.0f, 0.0f);
-  // Tile i's scores x are worked on while the next tile's products run (past the last tile: of stale rows, dropped).
-  auto step = [&](int32_t i, f32x16_t (&x)[2], f32x16_t (&next)[2]) {
-    // tile i + 1 is in its slot once this wave's DMAs and the others' are (SLOTS - 2 later tiles may be on their way), and
-    // the barrier also says that tile i, whose slot tile i + SLOTS takes, is read
-    if (i + SLOTS <= tiles) wait_vmcnt<(SLOTS - 2) * DMAS>();
-    else wait_vmcnt<0>();
-    __syncthreads();
-    if (i + SLOTS < tiles) load(i + SLOTS);
-    float2 rn = rw;  // (read with the tile: its slot's next one may be on its way after the next barrier)
-    if (PASS == kSum) rn = row_stats(i + 1);
-    if (PASS == kStats && i > 0) write_part(i - 1);
-    // whether the tile's first row (and, in a window, its last) sees all of the wave's keys: scalar work
-    const int32_t m = m0 + kWeightRows * i;
-    bool all = c2 > 0.0f && rq.prior + token_of(m) >= kw + 63 && (PASS == kSum || valid == ~0ull);
-    if (a.window > 0) all = all && rq.prior + token_of(m + kWeightRows - 1) - a.window < kw;
-    if (all) {
-      products(i + 1, next);
-      if constexpr (PASS == kStats) {
-        const float2 p = weights_stats<true>(x, c2, 0, g2);
-        if (g2 == 0) sm_part[i & 1][wave][i32] = p;
-      } else {
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[s][e] = __builtin_amdgcn_exp2f(fmaf(x[s][e], c2, -rw.x));
-      }
+  // Tile i's scores, all of them seen, or those that weights_seen says.
+  auto work = [&](auto all, int32_t i, int b) {
+    constexpr bool ALL = decltype(all)::value;
+    const int32_t m = m0 + kWeightRows * i + i32;
+    const uint64_t seen = ALL || m >= m_end ? 0 : weights_seen(a, valid, rq.prior + token_of(m), kw);
+    if constexpr (PASS == kStats) {
+      const float2 p = weights_stats<ALL>(x[b], c2, seen, g2);
+      if (g2 == 0) sm_part[i & 3][wave][i32] = p;
     } else {
-      const uint64_t seen = weights_seen(a, valid, rq.prior + token_of(m + i32), kw);
-      products(i + 1, next);
-      if constexpr (PASS == kStats) {
-        const float2 p = weights_stats<false>(x, c2, seen, g2);
-        if (g2 == 0) sm_part[i & 1][wave][i32] = p;
-      } else {
+      const float inv = ALL || m < m_end ? rw[b].y : 0.0f;  // (past the last tile it is stale)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const uint32_t bits = weights_bits(seen, s, g2);
+      for (int s = 0; s < 2; ++s) {
+        const uint32_t bits = weights_bits(seen, s, g2);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(x[s][e], c2, -rw.x));
-            x[s][e] = bits & weights_bit(e) ? p : 0.0f;
-          }
+        for (int e = 0; e < 16; ++e) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(x[b][s][e], c2, -rw[b].x));
+          acc[s][e] = fmaf(ALL || bits & weights_bit(e) ? p : 0.0f, inv, acc[s][e]);
         }
       }
     }
-    if constexpr (PASS == kSum) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[s][e] = fmaf(x[s][e], rw.y, acc[s][e]);
+  };
+  // A pair of tiles, 2 p and 2 p + 1: each one's scores are worked on while the next one's products run.
+  auto pair = [&](auto all, int32_t p) {
+    // Tiles 2 p + 1 and 2 p + 2 are in their slots once this wave's DMAs and the others' are (the SLOTS - 4 later tiles may
+    // be on their way); the barrier also says that tile 2 p and those before, whose slots the next ones take, are read.
+    if (2 * p + SLOTS - 2 < tiles) wait_vmcnt<(SLOTS - 4) * DMAS>();
+    else wait_vmcnt<0>();
+    __syncthreads();
+    if (2 * p + SLOTS - 1 < tiles) load(2 * p + SLOTS - 1);
+    if (2 * p + SLOTS < tiles) load(2 * p + SLOTS);
+    if (PASS == kStats && p > 0) {
+      write_part(2 * p - 2);
+      write_part(2 * p - 1);
     }
-    rw = rn;
+    products(2 * p + 1, 1);
+    work(all, 2 * p, 0);
+    products(2 * p + 2, 0);
+    work(all, 2 * p + 1, 1);
   };
   __syncthreads();  // every wave has its keys (and, with them, its early tiles): the other tiles take their place
-  for (int32_t i = early; i < min(tiles, SLOTS); ++i) load(i);
-  f32x16_t x0[2], x1[2];
-  if (PASS == kSum) rw = row_stats(0);
-  products(0, x0);
-  for (int32_t i = 0; i < tiles; i += 2) {
-    step(i, x0, x1);
-    if (i + 1 < tiles) step(i + 1, x1, x0);
-  }
+  for (int32_t i = early; i < min(tiles, SLOTS - 1); ++i) load(i);
+  products(0, 0);
+  int32_t p = 0;
+  for (; p < min(f0, pairs); ++p) pair(std::false_type{}, p);
+  for (; p < f1; ++p) pair(std::true_type{}, p);
+  for (; p < pairs; ++p) pair(std::false_type{}, p);
   if constexpr (PASS == kStats) {
     __syncthreads();
-    write_part(tiles - 1);
+    write_part(2 * pairs - 2);
+    write_part(2 * pairs - 1);
   } else {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
