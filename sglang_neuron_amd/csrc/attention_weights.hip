@@ -319,6 +319,9 @@ void weights_tile_kernel(WeightsArgs a) {
   // their sums are dropped): from the pair whose first token reaches the last key, to the one before a row past the end, or
   // past the first key's window.
   const int32_t pairs = (tiles + 1) / 2;
+  // the first `unseen` pairs see none of the wave's keys
+  int32_t unseen = (int32_t)(max((min(kw - rq.prior, (int64_t)t1) * a.group - m0), (int64_t)0) / (2 * kWeightRows));
+  unseen = __builtin_amdgcn_readfirstlane(unseen);
   int32_t f0 = pairs, f1 = 0;
   if (c2 > 0.0f && (PASS == kSum || valid == ~0ull)) {  // uniform
     auto pair_from = [&](int64_t token) -> int32_t {  // the first pair that starts at or behind a token's first row
@@ -377,10 +380,10 @@ void weights_tile_kernel(WeightsArgs a) {
       }
     }
   };
-  // A pair of tiles, 2 p and 2 p + 1: each one's scores are worked on while the next one's products run.
-  auto pair = [&](auto all, int32_t p) {
-    // Tiles 2 p + 1 and 2 p + 2 are in their slots once this wave's DMAs and the others' are (the SLOTS - 4 later tiles may
-    // be on their way); the barrier also says that tile 2 p and those before, whose slots the next ones take, are read.
+  // Before a pair of tiles, 2 p and 2 p + 1: tiles 2 p + 1 and 2 p + 2 are in their slots once this wave's DMAs and the
+  // others' are (the SLOTS - 4 later tiles may be on their way); the barrier also says that tile 2 p and those before, whose
+  // slots the next ones take, are read.
+  auto ready = [&](int32_t p) {
     if (2 * p + SLOTS - 2 < tiles) wait_vmcnt<(SLOTS - 4) * DMAS>();
     else wait_vmcnt<0>();
     __syncthreads();
@@ -390,6 +393,10 @@ void weights_tile_kernel(WeightsArgs a) {
       write_part(2 * p - 2);
       write_part(2 * p - 1);
     }
+  };
+  // Each tile's scores are worked on while the next one's products run.
+  auto pair = [&](auto all, int32_t p) {
+    ready(p);
     products(2 * p + 1, 1);
     work(all, 2 * p, 0);
     products(2 * p + 2, 0);
@@ -397,8 +404,16 @@ void weights_tile_kernel(WeightsArgs a) {
   };
   __syncthreads();  // every wave has its keys (and, with them, its early tiles): the other tiles take their place
   for (int32_t i = early; i < min(tiles, SLOTS - 1); ++i) load(i);
-  products(0, 0);
+  if (unseen == 0) products(0, 0);
   int32_t p = 0;
+  for (; p < unseen; ++p) {
+    ready(p);
+    if (PASS == kStats && g2 == 0) {
+      const float2 none = make_float2(kNegBig, 0.0f);
+      sm_part[2 * p & 3][wave][i32] = sm_part[(2 * p + 1) & 3][wave][i32] = none;
+    }
+    if (p + 1 == unseen) products(2 * p + 2, 0);
+  }
   for (; p < min(f0, pairs); ++p) pair(std::false_type{}, p);
   for (; p < f1; ++p) pair(std::true_type{}, p);
   for (; p < pairs; ++p) pair(std::false_type{}, p);
