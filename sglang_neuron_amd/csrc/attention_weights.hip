@@ -110,14 +110,13 @@ __device__ __forceinline__ void dma_global4(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(m0), "v"(src) : "memory");
 }
 
-// The wave's 64 keys through LDS (whole rows by DMA, 1024 bytes an instruction) to A operands in registers: lane (g2, i)
-// feeds key 32 s + i, dims 16 c + 8 g2 .. of step c (bf16) or 32 (c / 2) + 16 g2 + 8 (c & 1) .. (FP8, as its 16-byte
-// chunks hold them). A key that is not there reads the cache's first row; what comes of it is masked or dropped.
+// The wave's 64 keys into LDS: whole rows by DMA, 1024 bytes an instruction, chunk c of row r to c ^ swz(r). A key that is
+// not there reads the cache's first row; what comes of it is masked or dropped.
 template <int D, int ESZ>
-__device__ __forceinline__ void weights_keys(const WeightsArgs& a, int64_t at, uint8_t* lds, uint32_t (&kf)[2][D / 16][4]) {
+__device__ __forceinline__ void weights_stage(const WeightsArgs& a, int64_t at, uint8_t* lds) {
   using Geo = WeightsGeo<D, ESZ>;
   constexpr int RPD = 1024 / Geo::ROWB;
-  const int lane = threadIdx.x & 63, g2 = lane >> 5, i32 = lane & 31;
+  const int lane = threadIdx.x & 63;
   const int64_t from = at < 0 ? 0 : at;
   const uint32_t base = lds_address((lds_ptr_t*)lds);
 #pragma unroll
@@ -126,6 +125,15 @@ __device__ __forceinline__ void weights_keys(const WeightsArgs& a, int64_t at, u
     const uint32_t lo = __shfl((uint32_t)from, row, 64), hi = __shfl((uint32_t)(from >> 32), row, 64);
     dma_global16_cached(a.k_cache + (int64_t)((uint64_t)hi << 32 | lo) + 16 * ch, base + 1024 * j);
   }
+}
+
+// The wave's 64 keys through LDS to A operands in registers: lane (g2, i) feeds key 32 s + i, dims 16 c + 8 g2 .. of step c
+// (bf16) or 32 (c / 2) + 16 g2 + 8 (c & 1) .. (FP8, as its 16-byte chunks hold them).
+template <int D, int ESZ>
+__device__ __forceinline__ void weights_keys(const WeightsArgs& a, int64_t at, uint8_t* lds, uint32_t (&kf)[2][D / 16][4]) {
+  using Geo = WeightsGeo<D, ESZ>;
+  const int lane = threadIdx.x & 63, g2 = lane >> 5, i32 = lane & 31;
+  weights_stage<D, ESZ>(a, at, lds);
   wait_vmcnt<0>();
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
@@ -489,12 +497,15 @@ __global__ __launch_bounds__(256) void weights_merge_kernel(WeightsArgs a) {
 // Few rows (at most kScoreRows a request and KV head: a decode step): the scores themselves go to the workspace, so that
 // the keys are read once, and a second launch sums the probabilities from them.
 constexpr int kScoreRows = 16;
+// 256 keys a workgroup, 64 to a wave, by v_mfma_f32_16x16x32_bf16: lane (g4, i) feeds key 16 s + i's dims 32 c + 8 g4 .. of
+// step c (FP8: 64 (c / 2) + 16 g4 + 8 (c & 1) ..) and holds the scores of row i and keys 16 s + 4 g4 + e.
 template <int D, int ESZ>
 __global__ __launch_bounds__(256) void weights_score_kernel(WeightsArgs a) {
   using Geo = WeightsGeo<D, ESZ>;
+  constexpr int NS = D / 32;  // matrix steps
   __shared__ __attribute__((aligned(1024))) uint8_t sm[4 * Geo::KEYB];
-  __shared__ float2 sm_part[4][32];
-  const int tid = threadIdx.x, lane = tid & 63, g2 = lane >> 5, i32 = lane & 31;
+  __shared__ float2 sm_part[4][kScoreRows];
+  const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, i16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int32_t kb = (int32_t)(blockIdx.x % a.blocks), r = (int32_t)(blockIdx.x / a.blocks % a.R);
   const int32_t g = (int32_t)(blockIdx.x / a.blocks / a.R);
@@ -504,35 +515,66 @@ __global__ __launch_bounds__(256) void weights_score_kernel(WeightsArgs a) {
   if (k0 >= rq.n || rq.S == 0 || (a.window > 0 && (int64_t)k0 + kWeightKeys - 1 <= rq.prior - a.window)) return;  // uniform
   const int64_t at = weights_key_at(a, r, g, k0 + tid, rq.n, Geo::ROWB);
   const uint64_t valid = __ballot(at >= 0);
-  const int32_t m = i32, M = rq.S * a.group;
+  uint8_t* const mine = sm + wave * Geo::KEYB;
+  weights_stage<D, ESZ>(a, at, mine);
+  const int32_t m = i16, M = rq.S * a.group;
   const int32_t t = m / a.group, j = m - t * a.group;
-  uint32_t qf[Geo::NS][4];
-  const uint16_t* row = a.q + ((int64_t)(rq.qa + t) * a.H + g * a.group + j) * D;
+  const uint16_t* row = a.q + ((int64_t)(rq.qa + min(t, rq.S - 1)) * a.H + g * a.group + j) * D;
+  uint4 qw[NS];
 #pragma unroll
-  for (int c = 0; c < Geo::NS; ++c) {
-    const uint4 w = m < M ? ld16(row + 8 * weights_chunk<ESZ>(c, g2)) : make_uint4(0, 0, 0, 0);
-    qf[c][0] = w.x, qf[c][1] = w.y, qf[c][2] = w.z, qf[c][3] = w.w;
-  }
-  uint32_t kf[2][Geo::NS][4];
-  weights_keys<D, ESZ>(a, at, sm + wave * Geo::KEYB, kf);
-  f32x16_t x[2] = {};
+  for (int c = 0; c < NS; ++c) qw[c] = ld16(row + 8 * (ESZ == 1 ? 8 * (c / 2) + 2 * g4 + (c & 1) : 4 * c + g4));
+  const float c2 = weights_scale<ESZ>(a, g);
+  wait_vmcnt<0>();
+  f32x4_t x[4];
 #pragma unroll
-  for (int c = 0; c < Geo::NS; ++c) {
-    x[0] = mfma_32x32x16_bf16(kf[0][c], qf[c], x[0]);
-    x[1] = mfma_32x32x16_bf16(kf[1][c], qf[c], x[1]);
+  for (int s = 0; s < 4; ++s) {
+    const int key = 16 * s + i16;
+    const uint8_t* k = mine + key * Geo::ROWB;
+    x[s] = f32x4_t{};
+#pragma unroll
+    for (int c = 0; c < NS; c += ESZ == 1 ? 2 : 1) {
+      const uint4 w = *reinterpret_cast<const uint4*>(k + 16 * ((4 * (ESZ == 1 ? c / 2 : c) + g4) ^ Geo::swz(key, Geo::KCH)));
+      const uint32_t q0[4] = {qw[c].x, qw[c].y, qw[c].z, qw[c].w};
+      if constexpr (ESZ == 1) {
+        const uint32_t q1[4] = {qw[c + 1].x, qw[c + 1].y, qw[c + 1].z, qw[c + 1].w};
+        uint32_t k0f[4], k1f[4];
+        fp8x4_to_bf16x4(w.x, k0f[0], k0f[1]);
+        fp8x4_to_bf16x4(w.y, k0f[2], k0f[3]);
+        fp8x4_to_bf16x4(w.z, k1f[0], k1f[1]);
+        fp8x4_to_bf16x4(w.w, k1f[2], k1f[3]);
+        x[s] = mfma_16x16x32_bf16(k0f, q0, x[s]);
+        x[s] = mfma_16x16x32_bf16(k1f, q1, x[s]);
+      } else {
+        const uint32_t kf[4] = {w.x, w.y, w.z, w.w};
+        x[s] = mfma_16x16x32_bf16(kf, q0, x[s]);
+      }
+    }
   }
-  const float2 p = weights_stats<false>(x, weights_scale<ESZ>(a, g), weights_seen(a, valid, rq.prior + t, kw), g2);
+  // scaled, -inf where unseen
+  const bool all = valid == ~0ull && rq.prior >= kw + 63 && (a.window <= 0 || rq.prior + rq.S - 1 - a.window < kw);  // uniform
+  const uint64_t seen = all ? 0 : weights_seen(a, valid, rq.prior + t, kw) >> 4 * g4;
+  float mx = kNegBig, sum = 0.0f;
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[s][e] *= c2;
+      if (!all) x[s][e] = seen >> (16 * s + e) & 1 ? x[s][e] : -INFINITY;
+      mx = fmaxf(mx, x[s][e]);
+    }
+  mx = max_across_groups(mx);
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(x[s][e] - mx);
+  sum = sum_across_groups(sum);
   const int32_t width = a.blocks * kWeightKeys, rows = a.max_q * a.group;
   if (m < M) {
-    float* dst = a.ws_score + (((int64_t)r * a.G + g) * rows + m) * width + kw;
+    float* dst = a.ws_score + (((int64_t)r * a.G + g) * rows + m) * width + kw + 4 * g4;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<float4*>(dst + weights_key(s, 4 * q, g2)) =
-            make_float4(x[s][4 * q], x[s][4 * q + 1], x[s][4 * q + 2], x[s][4 * q + 3]);
+    for (int s = 0; s < 4; ++s) *reinterpret_cast<f32x4_t*>(dst + 16 * s) = x[s];
   }
-  if (g2 == 0) sm_part[wave][i32] = p;
+  if (g4 == 0) sm_part[wave][m] = make_float2(mx, sum);
   __syncthreads();
   if (tid < M)
     a.ws_part[(((int64_t)r * a.G + g) * a.blocks + kb) * rows + tid] =
