@@ -49,7 +49,8 @@ struct WeightsArgs {
   int32_t splits, split_tokens;  // the queries are cut into so many runs of so many tokens (a multiple of 32)
   float* ws_sum;     // [splits, R, G, blocks * 256] the runs' sums, with more than one
   // few rows instead: ws_part is [R, G, blocks, max_q * group], and
-  float* ws_score;   // [R, G, max_q * group, blocks * 256] scores in the log2 domain, -inf where unseen
+  float* ws_score;   // [R, G, max_q * group, blocks * score_keys] scores in the log2 domain, -inf where unseen
+  int32_t span, score_keys;  // chunks of a workgroup, and their keys
 };
 
 constexpr int kWeightKeys = 256;  // keys of a workgroup, 64 to a wave
@@ -110,9 +111,9 @@ __device__ __forceinline__ void dma_global4(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(m0), "v"(src) : "memory");
 }
 
-// The wave's 64 keys into LDS: whole rows by DMA, 1024 bytes an instruction, chunk c of row r to c ^ swz(r). A key that is
+// N keys of a wave (lane i holding the place of key i mod N) into LDS: whole rows by DMA, 1024 bytes an instruction, chunk c of row r to c ^ swz(r). A key that is
 // not there reads the cache's first row; what comes of it is masked or dropped.
-template <int D, int ESZ>
+template <int D, int ESZ, int N>
 __device__ __forceinline__ void weights_stage(const WeightsArgs& a, int64_t at, uint8_t* lds) {
   using Geo = WeightsGeo<D, ESZ>;
   constexpr int RPD = 1024 / Geo::ROWB;
@@ -120,7 +121,7 @@ __device__ __forceinline__ void weights_stage(const WeightsArgs& a, int64_t at, 
   const int64_t from = at < 0 ? 0 : at;
   const uint32_t base = lds_address((lds_ptr_t*)lds);
 #pragma unroll
-  for (int j = 0; j < 64 / RPD; ++j) {
+  for (int j = 0; j < N / RPD; ++j) {
     const int row = j * RPD + lane / Geo::KCH, ch = lane % Geo::KCH ^ Geo::swz(row, Geo::KCH);
     const uint32_t lo = __shfl((uint32_t)from, row, 64), hi = __shfl((uint32_t)(from >> 32), row, 64);
     dma_global16_cached(a.k_cache + (int64_t)((uint64_t)hi << 32 | lo) + 16 * ch, base + 1024 * j);
@@ -133,7 +134,7 @@ template <int D, int ESZ>
 __device__ __forceinline__ void weights_keys(const WeightsArgs& a, int64_t at, uint8_t* lds, uint32_t (&kf)[2][D / 16][4]) {
   using Geo = WeightsGeo<D, ESZ>;
   const int lane = threadIdx.x & 63, g2 = lane >> 5, i32 = lane & 31;
-  weights_stage<D, ESZ>(a, at, lds);
+  weights_stage<D, ESZ, 64>(a, at, lds);
   wait_vmcnt<0>();
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
@@ -497,26 +498,49 @@ __global__ __launch_bounds__(256) void weights_merge_kernel(WeightsArgs a) {
 // Few rows (at most kScoreRows a request and KV head: a decode step): the scores themselves go to the workspace, so that
 // the keys are read once, and a second launch sums the probabilities from them.
 constexpr int kScoreRows = 16;
-// 256 keys a workgroup, 64 to a wave, by v_mfma_f32_16x16x32_bf16: lane (g4, i) feeds key 16 s + i's dims 32 c + 8 g4 .. of
-// step c (FP8: 64 (c / 2) + 16 g4 + 8 (c & 1) ..) and holds the scores of row i and keys 16 s + 4 g4 + e.
+// A workgroup of 4 waves takes `span` chunks of 4 x CK consecutive keys, CK to a wave; a wave's next chunk is on its way to
+// LDS while it works on one. By v_mfma_f32_16x16x32_bf16: lane (g4, i) feeds key 16 s + i's dims 32 c + 8 g4 .. of step c
+// (FP8: 64 (c / 2) + 16 g4 + 8 (c & 1) ..) and holds the scores of row i and keys 16 s + 4 g4 + e.
+constexpr int kScoreSpan = 8;  // most chunks
+template <int D, int ESZ>
+struct ScoreGeo {
+  static constexpr int CK = D * ESZ > 128 ? 32 : 64;  // keys of a wave's chunk: at most 8 KB
+};
 template <int D, int ESZ>
 __global__ __launch_bounds__(256) void weights_score_kernel(WeightsArgs a) {
   using Geo = WeightsGeo<D, ESZ>;
-  constexpr int NS = D / 32;  // matrix steps
-  __shared__ __attribute__((aligned(1024))) uint8_t sm[4 * Geo::KEYB];
+  constexpr int NS = D / 32;                     // matrix steps
+  constexpr int CK = ScoreGeo<D, ESZ>::CK, NT = CK / 16;
+  constexpr int DMAS = CK * Geo::ROWB / 1024;    // of a chunk
+  __shared__ __attribute__((aligned(1024))) uint8_t sm[4][2][CK * Geo::ROWB];
+  __shared__ int32_t sm_page[4][kScoreSpan][CK];  // the keys' pages, -1 where there is none
   __shared__ float2 sm_part[4][kScoreRows];
   const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, i16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int32_t kb = (int32_t)(blockIdx.x % a.blocks), r = (int32_t)(blockIdx.x / a.blocks % a.R);
   const int32_t g = (int32_t)(blockIdx.x / a.blocks / a.R);
   const WeightsRequest rq = weights_request(a, r);
-  const int32_t k0 = kb * kWeightKeys, kw = k0 + 64 * wave;
+  const int32_t keys = 4 * CK * a.span, k0 = kb * keys;
   // (a block before every row's window, or past the keys, is not read by the second launch)
-  if (k0 >= rq.n || rq.S == 0 || (a.window > 0 && (int64_t)k0 + kWeightKeys - 1 <= rq.prior - a.window)) return;  // uniform
-  const int64_t at = weights_key_at(a, r, g, k0 + tid, rq.n, Geo::ROWB);
-  const uint64_t valid = __ballot(at >= 0);
-  uint8_t* const mine = sm + wave * Geo::KEYB;
-  weights_stage<D, ESZ>(a, at, mine);
+  if (k0 >= rq.n || rq.S == 0 || (a.window > 0 && (int64_t)k0 + keys - 1 <= rq.prior - a.window)) return;  // uniform
+  const int32_t chunks = min(a.span, (rq.n - k0 + 4 * CK - 1) / (4 * CK));
+  auto key_of = [&](int32_t q) -> int32_t { return k0 + (4 * q + wave) * CK; };  // chunk q's first key
+  for (int32_t q = 0; q < chunks; ++q) {
+    const int32_t key = key_of(q) + lane % CK;
+    int32_t page = -1;
+    if (key < rq.n) {
+      page = a.table[r * a.table_stride + key / a.P];
+      if (page < 0 || page >= a.num_blocks) page = -1;
+    }
+    if (lane < CK) sm_page[wave][q][lane] = page;
+  }
+  auto stage = [&](int32_t q) -> uint64_t {
+    const int32_t key = key_of(q) + lane % CK, page = sm_page[wave][q][lane % CK];
+    const int64_t at = page < 0 ? -1 : (((int64_t)page * a.G + g) * a.P + key % a.P) * (int64_t)Geo::ROWB;
+    weights_stage<D, ESZ, CK>(a, at, sm[wave][q & 1]);
+    return __ballot(page >= 0);
+  };
+  uint64_t valid = stage(0), next = 0;
   const int32_t m = i16, M = rq.S * a.group;
   const int32_t t = m / a.group, j = m - t * a.group;
   const uint16_t* row = a.q + ((int64_t)(rq.qa + min(t, rq.S - 1)) * a.H + g * a.group + j) * D;
@@ -524,56 +548,69 @@ __global__ __launch_bounds__(256) void weights_score_kernel(WeightsArgs a) {
 #pragma unroll
   for (int c = 0; c < NS; ++c) qw[c] = ld16(row + 8 * (ESZ == 1 ? 8 * (c / 2) + 2 * g4 + (c & 1) : 4 * c + g4));
   const float c2 = weights_scale<ESZ>(a, g);
-  wait_vmcnt<0>();
-  f32x4_t x[4];
+  const int32_t width = a.blocks * keys, rows = a.max_q * a.group;
+  float* const dst = a.ws_score + (((int64_t)r * a.G + g) * rows + min(m, rows - 1)) * width + 4 * g4;
+  float2 best = make_float2(kNegBig, 0.0f);
+  for (int32_t q = 0; q < chunks; ++q) {
+    if (q + 1 < chunks) {
+      next = stage(q + 1);  // its slot's last chunk is read: this wave's own
+      wait_vmcnt<DMAS>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    const int32_t kw = key_of(q);
+    f32x4_t x[NT];
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    const int key = 16 * s + i16;
-    const uint8_t* k = mine + key * Geo::ROWB;
-    x[s] = f32x4_t{};
+    for (int s = 0; s < NT; ++s) {
+      const int key = 16 * s + i16;
+      const uint8_t* k = sm[wave][q & 1] + key * Geo::ROWB;
+      x[s] = f32x4_t{};
 #pragma unroll
-    for (int c = 0; c < NS; c += ESZ == 1 ? 2 : 1) {
-      const uint4 w = *reinterpret_cast<const uint4*>(k + 16 * ((4 * (ESZ == 1 ? c / 2 : c) + g4) ^ Geo::swz(key, Geo::KCH)));
-      const uint32_t q0[4] = {qw[c].x, qw[c].y, qw[c].z, qw[c].w};
-      if constexpr (ESZ == 1) {
-        const uint32_t q1[4] = {qw[c + 1].x, qw[c + 1].y, qw[c + 1].z, qw[c + 1].w};
-        uint32_t k0f[4], k1f[4];
-        fp8x4_to_bf16x4(w.x, k0f[0], k0f[1]);
-        fp8x4_to_bf16x4(w.y, k0f[2], k0f[3]);
-        fp8x4_to_bf16x4(w.z, k1f[0], k1f[1]);
-        fp8x4_to_bf16x4(w.w, k1f[2], k1f[3]);
-        x[s] = mfma_16x16x32_bf16(k0f, q0, x[s]);
-        x[s] = mfma_16x16x32_bf16(k1f, q1, x[s]);
-      } else {
-        const uint32_t kf[4] = {w.x, w.y, w.z, w.w};
-        x[s] = mfma_16x16x32_bf16(kf, q0, x[s]);
+      for (int c = 0; c < NS; c += ESZ == 1 ? 2 : 1) {
+        const uint4 w = *reinterpret_cast<const uint4*>(k + 16 * ((4 * (ESZ == 1 ? c / 2 : c) + g4) ^ Geo::swz(key, Geo::KCH)));
+        const uint32_t q0[4] = {qw[c].x, qw[c].y, qw[c].z, qw[c].w};
+        if constexpr (ESZ == 1) {
+          const uint32_t q1[4] = {qw[c + 1].x, qw[c + 1].y, qw[c + 1].z, qw[c + 1].w};
+          uint32_t ka[4], kc[4];
+          fp8x4_to_bf16x4(w.x, ka[0], ka[1]);
+          fp8x4_to_bf16x4(w.y, ka[2], ka[3]);
+          fp8x4_to_bf16x4(w.z, kc[0], kc[1]);
+          fp8x4_to_bf16x4(w.w, kc[2], kc[3]);
+          x[s] = mfma_16x16x32_bf16(ka, q0, x[s]);
+          x[s] = mfma_16x16x32_bf16(kc, q1, x[s]);
+        } else {
+          const uint32_t ka[4] = {w.x, w.y, w.z, w.w};
+          x[s] = mfma_16x16x32_bf16(ka, q0, x[s]);
+        }
       }
     }
-  }
-  // scaled, -inf where unseen
-  const bool all = valid == ~0ull && rq.prior >= kw + 63 && (a.window <= 0 || rq.prior + rq.S - 1 - a.window < kw);  // uniform
-  const uint64_t seen = all ? 0 : weights_seen(a, valid, rq.prior + t, kw) >> 4 * g4;
-  float mx = kNegBig, sum = 0.0f;
+    // scaled, -inf where unseen
+    constexpr uint64_t kAll = CK == 64 ? ~0ull : (1ull << CK % 64) - 1;
+    const bool all = (valid & kAll) == kAll && rq.prior >= kw + CK - 1 &&
+                     (a.window <= 0 || rq.prior + rq.S - 1 - a.window < kw);  // uniform
+    const uint64_t seen = all ? 0 : weights_seen(a, valid, rq.prior + t, kw) >> 4 * g4;
+    float mx = kNegBig, sum = 0.0f;
 #pragma unroll
-  for (int s = 0; s < 4; ++s)
+    for (int s = 0; s < NT; ++s)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[s][e] *= c2;
-      if (!all) x[s][e] = seen >> (16 * s + e) & 1 ? x[s][e] : -INFINITY;
-      mx = fmaxf(mx, x[s][e]);
+      for (int e = 0; e < 4; ++e) {
+        x[s][e] *= c2;
+        if (!all) x[s][e] = seen >> (16 * s + e) & 1 ? x[s][e] : -INFINITY;
+        mx = fmaxf(mx, x[s][e]);
+      }
+#pragma unroll
+    for (int s = 0; s < NT; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(x[s][e] - mx);
+    best = weights_join(best, make_float2(mx, sum));
+    if (m < M) {
+#pragma unroll
+      for (int s = 0; s < NT; ++s) *reinterpret_cast<f32x4_t*>(dst + kw + 16 * s) = x[s];
     }
-  mx = max_across_groups(mx);
-#pragma unroll
-  for (int s = 0; s < 4; ++s)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(x[s][e] - mx);
-  sum = sum_across_groups(sum);
-  const int32_t width = a.blocks * kWeightKeys, rows = a.max_q * a.group;
-  if (m < M) {
-    float* dst = a.ws_score + (((int64_t)r * a.G + g) * rows + m) * width + kw + 4 * g4;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) *reinterpret_cast<f32x4_t*>(dst + 16 * s) = x[s];
+    valid = next;
   }
+  const float mx = max_across_groups(best.x);
+  const float sum = sum_across_groups(best.y * __builtin_amdgcn_exp2f(best.x - mx));
   if (g4 == 0) sm_part[wave][m] = make_float2(mx, sum);
   __syncthreads();
   if (tid < M)
@@ -591,7 +628,8 @@ __global__ __launch_bounds__(256) void weights_from_scores_kernel(WeightsArgs a)
   float* const out = a.weights + r * a.w_row + g * a.w_head;
   // the blocks that any row sees
   const int64_t first = a.window > 0 ? max(rq.prior - a.window + 1, (int64_t)0) : 0;
-  const int32_t b0 = (int32_t)min(first / kWeightKeys, (int64_t)a.blocks), b1 = (rq.n + kWeightKeys - 1) / kWeightKeys;
+  const int32_t keys = a.score_keys;
+  const int32_t b0 = (int32_t)min(first / keys, (int64_t)a.blocks), b1 = (rq.n + keys - 1) / keys;
   if (k0 >= rq.n || M == 0 || (int64_t)k0 + 1023 < first) {  // uniform
     if (!a.add)
       for (int32_t k = k0 + tid; k < min(k0 + 1024, a.width); k += 256) out[k] = 0.0f;
@@ -617,8 +655,8 @@ __global__ __launch_bounds__(256) void weights_from_scores_kernel(WeightsArgs a)
   const int32_t key = k0 + 4 * tid;
   if (key >= a.width) return;
   float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (key / kWeightKeys >= b0 && key < rq.n) {
-    const int64_t width = (int64_t)a.blocks * kWeightKeys;
+  if (key >= (int64_t)b0 * keys && key < rq.n) {
+    const int64_t width = (int64_t)a.blocks * keys;
     const float* src = a.ws_score + ((int64_t)r * a.G + g) * rows * width + key;
 #pragma unroll 4
     for (int32_t m = 0; m < M; ++m) {
@@ -647,27 +685,39 @@ namespace {
 
 constexpr int64_t kGridMax = (1 << 24) - 1;  // workgroups of 256 threads: 32 bits number a launch's threads
 
-int64_t weights_blocks(int32_t page_size, int32_t table_width, int32_t width) {
-  const int64_t keys = std::max<int64_t>((int64_t)table_width * page_size, width);
-  return (keys + kWeightKeys - 1) / kWeightKeys;
+int64_t weights_blocks(int32_t page_size, int32_t table_width, int32_t width, int32_t keys) {
+  return (std::max<int64_t>((int64_t)table_width * page_size, width) + keys - 1) / keys;
 }
+int32_t score_chunk(int32_t head_dim, int32_t esz) { return head_dim * esz > 128 ? 32 : 64; }
 
 // How a launch works, and its workspace: few rows a request keep their scores (at most kScoreBytes of them), others
 // compute them twice.
 constexpr int64_t kScoreBytes = (int64_t)1 << 29;
 struct WeightsPlan {
   int64_t blocks, part, rest, bytes;
-  int32_t splits, split_tokens;
+  int32_t splits, split_tokens, span, score_keys;
   bool scores;
 };
+constexpr int64_t kScoreWorkgroups = 1024;  // a score launch's chunks are taken several to a workgroup from so many on
 constexpr int64_t kSplitRows = 2048;       // least rows of a run of queries
 constexpr int64_t kSplitWorkgroups = 4096; // runs are cut up to so many workgroups
 WeightsPlan weights_plan(int64_t T, int64_t R, int64_t max_q, int32_t H, int32_t G, int32_t page_size,
-                         int32_t table_width, int32_t width) {
+                         int32_t table_width, int32_t width, int32_t head_dim, int32_t esz) {
   WeightsPlan p;
-  p.blocks = weights_blocks(page_size, table_width, width);
+  p.score_keys = 0;
+  p.blocks = weights_blocks(page_size, table_width, width, kWeightKeys);
+  p.span = 1;
   const int64_t rows = max_q * (H / G);
-  const int64_t score = rows <= kScoreRows ? R * G * rows * p.blocks * kWeightKeys * (int64_t)sizeof(float) : INT64_MAX;
+  int64_t score = INT64_MAX;
+  if (rows <= kScoreRows) {
+    const int32_t chunk = 4 * score_chunk(head_dim, esz);
+    const int64_t chunks = weights_blocks(page_size, table_width, 0, chunk);
+    p.span = (int32_t)std::min<int64_t>(kScoreSpan, std::max<int64_t>(1, chunks * R * G / kScoreWorkgroups));
+    p.score_keys = chunk * p.span;
+    const int64_t blocks = (chunks + p.span - 1) / p.span;
+    score = R * G * rows * blocks * p.score_keys * (int64_t)sizeof(float);
+    if (score <= kScoreBytes) p.blocks = blocks;
+  }
   p.scores = score <= kScoreBytes;
   p.part = (p.scores ? R * G * rows : T * H) * p.blocks * (int64_t)sizeof(float2);
   p.rest = p.scores ? score : T * H * (int64_t)sizeof(float2);
@@ -691,7 +741,9 @@ template <int D, int ESZ>
 void launch_weights(const WeightsArgs& a, uint32_t wgs, hipStream_t s) {
   if (a.ws_score) {
     hipLaunchKernelGGL((weights_score_kernel<D, ESZ>), dim3(wgs), dim3(256), 0, s, a);
-    hipLaunchKernelGGL(weights_from_scores_kernel, dim3((a.blocks + 3) / 4, a.G, a.R), dim3(256), 0, s, a);
+    static_assert(ScoreGeo<D, ESZ>::CK == (D * ESZ > 128 ? 32 : 64), "score_chunk");
+    const int64_t cols = a.add ? (int64_t)a.blocks * a.score_keys : a.width;  // (every column is written, or the keys')
+    hipLaunchKernelGGL(weights_from_scores_kernel, dim3((unsigned)((cols + 1023) / 1024), a.G, a.R), dim3(256), 0, s, a);
     return;
   }
   hipLaunchKernelGGL((weights_tile_kernel<D, ESZ, kStats>), dim3(wgs), dim3(256), 0, s, a);
@@ -740,7 +792,8 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: weight strides %lld / %lld for %d columns", what, (long long)row_stride,
                 (long long)head_stride, width);
   max_q_len = std::max(max_q_len, 1);
-  const WeightsPlan plan = weights_plan(T, R, max_q_len, num_q_heads, num_kv_heads, page_size, table_width, width);
+  const WeightsPlan plan = weights_plan(T, R, max_q_len, num_q_heads, num_kv_heads, page_size, table_width, width,
+                                        head_dim, kv_dtype == SNA_DTYPE_BF16 ? 2 : 1);
   const int64_t blocks = plan.blocks;
   const int64_t wgs = blocks * R * num_kv_heads * plan.splits;
   if (wgs > kGridMax)
@@ -783,6 +836,8 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
   a.ws_row = plan.scores ? nullptr : (float2*)((uint8_t*)workspace + plan.part);
   a.splits = plan.splits;
   a.split_tokens = plan.split_tokens;
+  a.span = plan.span;
+  a.score_keys = plan.score_keys;
   a.ws_sum = (float*)((uint8_t*)workspace + plan.part + plan.rest);
   a.ws_score = plan.scores ? (float*)((uint8_t*)workspace + plan.part) : nullptr;
   const hipStream_t s = (hipStream_t)stream;
@@ -797,12 +852,14 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
 }  // namespace
 
 extern "C" int64_t sna_attention_weights_workspace_bytes(int32_t n_tokens, int32_t R, int32_t max_q_len,
-                                                         int32_t num_q_heads, int32_t num_kv_heads, int32_t page_size,
-                                                         int32_t table_width, int32_t width) {
+                                                         int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                                         int32_t page_size, int32_t table_width, int32_t width,
+                                                         int32_t kv_dtype) {
   if (n_tokens < 0 || R < 1 || max_q_len < 0 || num_q_heads < 1 || num_kv_heads < 1 ||
       num_q_heads % num_kv_heads != 0 || page_size < 1 || table_width < 1 || width < 0)
     return 0;
-  return weights_plan(n_tokens, R, std::max(max_q_len, 1), num_q_heads, num_kv_heads, page_size, table_width, width).bytes;
+  return weights_plan(n_tokens, R, std::max(max_q_len, 1), num_q_heads, num_kv_heads, page_size, table_width, width, head_dim,
+                      kv_dtype == SNA_DTYPE_BF16 ? 2 : 1).bytes;
 }
 
 extern "C" int sna_prefill_attention_weights(const void* q, const void* k_cache, const float* k_scale,

@@ -1004,7 +1004,7 @@ def _attention_weights(what, q, T, R, k_cache, block_table, q_start, lens, max_q
         row, head = G * W * P, W * P
     N = weights.shape[2]
     lib = _lib.load()
-    need = lib.sna_attention_weights_workspace_bytes(T, R, max_q_len, H, G, P, W, N)
+    need = lib.sna_attention_weights_workspace_bytes(T, R, max_q_len, H, G, d, P, W, N, code)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     stride = max(table.stride(0), W)
     with _device_of(dev):
