@@ -499,21 +499,19 @@ __global__ __launch_bounds__(256) void weights_merge_kernel(WeightsArgs a) {
 // the keys are read once, and a second launch sums the probabilities from them.
 constexpr int kScoreRows = 16;
 // A workgroup of 4 waves takes `span` chunks of 4 x CK consecutive keys, CK to a wave; a wave's next chunk is on its way to
-// LDS while it works on one. By v_mfma_f32_16x16x32_bf16: lane (g4, i) feeds key 16 s + i's dims 32 c + 8 g4 .. of step c
+// LDS while it works on one. (Keys of 64 bytes: one chunk a workgroup, whose 16 KB leave room for more workgroups: 128 rows
+// of 2048-8192 keys took 16 us so and 21 in spans; of 128 bytes, 64 rows of 4096, 72 and 64.) By v_mfma_f32_16x16x32_bf16: lane (g4, i) feeds key 16 s + i's dims 32 c + 8 g4 .. of step c
 // (FP8: 64 (c / 2) + 16 g4 + 8 (c & 1) ..) and holds the scores of row i and keys 16 s + 4 g4 + e.
-constexpr int kScoreSpan = 8;  // most chunks
-template <int D, int ESZ>
-struct ScoreGeo {
-  static constexpr int CK = D * ESZ > 128 ? 32 : 64;  // keys of a wave's chunk: at most 8 KB
-};
+constexpr int score_chunk(int row_bytes) { return row_bytes > 128 ? 32 : 64; }  // keys of a wave's chunk: at most 8 KB
+constexpr int score_span(int row_bytes) { return row_bytes > 64 ? 8 : 1; }      // most chunks
 template <int D, int ESZ>
 __global__ __launch_bounds__(256) void weights_score_kernel(WeightsArgs a) {
   using Geo = WeightsGeo<D, ESZ>;
   constexpr int NS = D / 32;                     // matrix steps
-  constexpr int CK = ScoreGeo<D, ESZ>::CK, NT = CK / 16;
+  constexpr int CK = score_chunk(Geo::ROWB), SPAN = score_span(Geo::ROWB), SLOTS = SPAN > 1 ? 2 : 1, NT = CK / 16;
   constexpr int DMAS = CK * Geo::ROWB / 1024;    // of a chunk
-  __shared__ __attribute__((aligned(1024))) uint8_t sm[4][2][CK * Geo::ROWB];
-  __shared__ int32_t sm_page[4][kScoreSpan][CK];  // the keys' pages, -1 where there is none
+  __shared__ __attribute__((aligned(1024))) uint8_t sm[4][SLOTS][CK * Geo::ROWB];
+  __shared__ int32_t sm_page[4][SPAN][CK];  // the keys' pages, -1 where there is none
   __shared__ float2 sm_part[4][kScoreRows];
   const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, i16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -523,7 +521,7 @@ __global__ __launch_bounds__(256) void weights_score_kernel(WeightsArgs a) {
   const int32_t keys = 4 * CK * a.span, k0 = kb * keys;
   // (a block before every row's window, or past the keys, is not read by the second launch)
   if (k0 >= rq.n || rq.S == 0 || (a.window > 0 && (int64_t)k0 + keys - 1 <= rq.prior - a.window)) return;  // uniform
-  const int32_t chunks = min(a.span, (rq.n - k0 + 4 * CK - 1) / (4 * CK));
+  const int32_t chunks = SPAN == 1 ? 1 : min(a.span, (rq.n - k0 + 4 * CK - 1) / (4 * CK));
   auto key_of = [&](int32_t q) -> int32_t { return k0 + (4 * q + wave) * CK; };  // chunk q's first key
   for (int32_t q = 0; q < chunks; ++q) {
     const int32_t key = key_of(q) + lane % CK;
@@ -537,7 +535,7 @@ __global__ __launch_bounds__(256) void weights_score_kernel(WeightsArgs a) {
   auto stage = [&](int32_t q) -> uint64_t {
     const int32_t key = key_of(q) + lane % CK, page = sm_page[wave][q][lane % CK];
     const int64_t at = page < 0 ? -1 : (((int64_t)page * a.G + g) * a.P + key % a.P) * (int64_t)Geo::ROWB;
-    weights_stage<D, ESZ, CK>(a, at, sm[wave][q & 1]);
+    weights_stage<D, ESZ, CK>(a, at, sm[wave][q & (SLOTS - 1)]);
     return __ballot(page >= 0);
   };
   uint64_t valid = stage(0), next = 0;
@@ -552,7 +550,7 @@ __global__ __launch_bounds__(256) void weights_score_kernel(WeightsArgs a) {
   float* const dst = a.ws_score + (((int64_t)r * a.G + g) * rows + min(m, rows - 1)) * width + 4 * g4;
   float2 best = make_float2(kNegBig, 0.0f);
   for (int32_t q = 0; q < chunks; ++q) {
-    if (q + 1 < chunks) {
+    if (SPAN > 1 && q + 1 < chunks) {
       next = stage(q + 1);  // its slot's last chunk is read: this wave's own
       wait_vmcnt<DMAS>();
     } else {
@@ -563,7 +561,7 @@ __global__ __launch_bounds__(256) void weights_score_kernel(WeightsArgs a) {
 #pragma unroll
     for (int s = 0; s < NT; ++s) {
       const int key = 16 * s + i16;
-      const uint8_t* k = sm[wave][q & 1] + key * Geo::ROWB;
+      const uint8_t* k = sm[wave][q & (SLOTS - 1)] + key * Geo::ROWB;
       x[s] = f32x4_t{};
 #pragma unroll
       for (int c = 0; c < NS; c += ESZ == 1 ? 2 : 1) {
@@ -688,7 +686,6 @@ constexpr int64_t kGridMax = (1 << 24) - 1;  // workgroups of 256 threads: 32 bi
 int64_t weights_blocks(int32_t page_size, int32_t table_width, int32_t width, int32_t keys) {
   return (std::max<int64_t>((int64_t)table_width * page_size, width) + keys - 1) / keys;
 }
-int32_t score_chunk(int32_t head_dim, int32_t esz) { return head_dim * esz > 128 ? 32 : 64; }
 
 // How a launch works, and its workspace: few rows a request keep their scores (at most kScoreBytes of them), others
 // compute them twice.
@@ -710,9 +707,9 @@ WeightsPlan weights_plan(int64_t T, int64_t R, int64_t max_q, int32_t H, int32_t
   const int64_t rows = max_q * (H / G);
   int64_t score = INT64_MAX;
   if (rows <= kScoreRows) {
-    const int32_t chunk = 4 * score_chunk(head_dim, esz);
+    const int32_t chunk = 4 * score_chunk(head_dim * esz);
     const int64_t chunks = weights_blocks(page_size, table_width, 0, chunk);
-    p.span = (int32_t)std::min<int64_t>(kScoreSpan, std::max<int64_t>(1, chunks * R * G / kScoreWorkgroups));
+    p.span = (int32_t)std::min<int64_t>(score_span(head_dim * esz), std::max<int64_t>(1, chunks * R * G / kScoreWorkgroups));
     p.score_keys = chunk * p.span;
     const int64_t blocks = (chunks + p.span - 1) / p.span;
     score = R * G * rows * blocks * p.score_keys * (int64_t)sizeof(float);
@@ -741,7 +738,6 @@ template <int D, int ESZ>
 void launch_weights(const WeightsArgs& a, uint32_t wgs, hipStream_t s) {
   if (a.ws_score) {
     hipLaunchKernelGGL((weights_score_kernel<D, ESZ>), dim3(wgs), dim3(256), 0, s, a);
-    static_assert(ScoreGeo<D, ESZ>::CK == (D * ESZ > 128 ? 32 : 64), "score_chunk");
     const int64_t cols = a.add ? (int64_t)a.blocks * a.score_keys : a.width;  // (every column is written, or the keys')
     hipLaunchKernelGGL(weights_from_scores_kernel, dim3((unsigned)((cols + 1023) / 1024), a.G, a.R), dim3(256), 0, s, a);
     return;
