@@ -506,11 +506,16 @@ int sna_decode_attention_weights(const void *q, const void *k_cache, const float
  *   kept      [R, num_kv_heads, keep] int32: the positions in ascending order, -1 past a short row's.
  *   new_lens  [R] int32: min(L, keep).
  *   weights_out [R, num_kv_heads, out_width] fp32 (out_width >= keep): the kept tokens' weights, then zeros; or NULL. It
- *             may be `weights` itself (same address and strides), and overlaps it in no other way. */
+ *             may be `weights` itself (same address and strides), and overlaps it in no other way.
+ *   workspace device, 16-byte aligned, at least sna_select_workspace_bytes bytes (in_place: weights_out is weights; 0 for
+ *             rows of up to 16384 columns, and it may be NULL then), any contents; calls that share one on different
+ *             streams race. */
+int64_t sna_select_workspace_bytes(int32_t R, int32_t num_kv_heads, int32_t width, int32_t keep, int32_t in_place);
 int sna_select_tokens(const float *weights, int64_t row_stride, int64_t head_stride, int32_t width,
                       const int32_t *seq_lens, int32_t R, int32_t num_kv_heads, int32_t keep, int32_t first,
                       int32_t recent, int32_t *kept, int32_t *new_lens, float *weights_out, int64_t out_row_stride,
-                      int64_t out_head_stride, int32_t out_width, void *stream);
+                      int64_t out_head_stride, int32_t out_width, void *workspace, int64_t workspace_bytes,
+                      void *stream);
 
 /* Moves the kept tokens' K and V together: token kept[r, g, i] of KV head g of row r, read through block_table, goes to
  * position i of the row's pages in dst_table ([R, dst_width] int32), or in block_table's own (dst_table NULL: in place,

@@ -101,8 +101,9 @@ SIGNATURES = {
                                              _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _I64, _I32, _P, _I64, _P]),
     "sna_decode_attention_weights": (_I32, [_P, _P, _P, _P, _I64, _I32, _P, _I32, _P, _F32, _I32, _P, _I64, _I64, _I32,
                                             _I32, _I32, _I32, _I32, _I32, _I64, _I32, _P, _I64, _P]),
+    "sna_select_workspace_bytes": (_I64, [_I32] * 5),
     "sna_select_tokens": (_I32, [_P, _I64, _I64, _I32, _P, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _I64, _I64, _I32,
-                                 _P]),
+                                 _P, _I64, _P]),
     "sna_compact_tokens": (_I32, [_P, _P, _I64, _I32, _I32, _I32, _I32, _P, _I64, _I32, _P, _I64, _I32, _P, _I32, _I32,
                                   _P]),
     "sna_index_key_store": (_I32, [_P, _P, _I64, _I32, _P, _I64, _P]),

@@ -3,10 +3,11 @@
 // the block table and the count, not the tokens.
 //
 //   select   Row r of L tokens keeps, where L > keep, its first `first` tokens, its last `recent` ones, and of the rest
-//            the keep - first - recent of the largest weights (ties: the lowest position; a NaN ranks above every
-//            number), in ascending order; else all L. One workgroup per (row, KV head) finds the threshold weight exactly
-//            by three histogram passes over the weights' order-preserving 32-bit keys (11, 11 and 10 bits, integer
-//            counts), then writes the positions at or above it by prefix counts.
+//            the keep - first - recent of the largest weights (ties: the lowest position; a NaN ranks above every number),
+//            in ascending order; else all L. The threshold weight is found exactly, by three histogram passes over the
+//            weights' order-preserving 32-bit keys (11, 11 and 10 bits, integer counts); the positions at or above it are
+//            then written by prefix counts. One workgroup per (row, KV head) does it all while it holds the row's
+//            candidates in registers (16384); a longer row takes one for every 16384, and a launch a pass.
 //   compact  Kept token i goes to position i of the row's (or another table's) pages. In place a target lies at or before
 //            its source, and at or after every earlier target, so one workgroup may walk a row's tokens in order,
 //            reading a whole tile before it writes it, without a copy elsewhere; the columns of a head's rows are
@@ -43,92 +44,298 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 constexpr int kSelectThreads = 1024;
-constexpr int kSelectBins = 2048;
+constexpr int kSelectBins = 2048, kSelectCopies = 4;  // a pass's histogram: a copy for every 4th lane,
+constexpr int kSelectCopy = kSelectBins + 16;         // 16 banks apart
+constexpr int kSelectMost = 16;                       // keys a thread holds, at most
+constexpr int32_t kSelectSegment = kSelectThreads * kSelectMost;  // candidates of a workgroup
+// Pass p looks at a key's bits [kSelectShift[p], kSelectShift[p - 1]).
+__device__ constexpr int kSelectShift[3] = {21, 10, 0};
+__device__ constexpr int kSelectBits[3] = {11, 11, 10};
 
-__global__ __launch_bounds__(kSelectThreads) void select_tokens_kernel(SelectArgs a) {
-  __shared__ uint32_t hist[kSelectBins];
-  __shared__ uint32_t wtot[16], wtie[16], pick[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int32_t g = blockIdx.x, r = blockIdx.y;
-  const int32_t L = min(max(a.lens[r], 0), a.width);
-  const float* const w = a.weights + r * a.w_row + g * a.w_head;
-  int32_t* const kept = a.kept + ((int64_t)r * a.G + g) * a.keep;
-  if (g == 0 && tid == 0) a.new_lens[r] = min(L, a.keep);
-  if (L <= a.keep) {  // uniform
-    for (int32_t i = tid; i < a.keep; i += kSelectThreads) kept[i] = i < L ? i : -1;
-  } else {
-    const int32_t lo = a.first, hi = L - a.recent;  // the candidates
-    uint32_t need = (uint32_t)(a.keep - a.first - a.recent);
-    for (int32_t i = tid; i < a.first; i += kSelectThreads) kept[i] = i;
-    for (int32_t i = tid; i < a.recent; i += kSelectThreads) kept[a.keep - a.recent + i] = hi + i;
-    uint32_t T = 0;  // the key of the last weight taken: bits found so far
-    if (need > 0) {
-      for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-        for (int i = tid; i < kSelectBins; i += kSelectThreads) hist[i] = 0;
-        __syncthreads();
-        for (int32_t i = lo + tid; i < hi; i += kSelectThreads) {
-          const uint32_t key = weight_key(w[i]);
-          // (the bits above this pass's are T's)
-          if (pass == 0 || (key ^ T) >> (shift + bits) == 0) atomicAdd(&hist[key >> shift & ((1u << bits) - 1)], 1u);
-        }
-        __syncthreads();
-        // the bin that holds the need-th largest: thread i owns bins top - 2 i and the one below it, largest first
-        const int top = kSelectBins - 1 - 2 * tid;
-        const uint32_t h0 = hist[top], h1 = hist[top - 1];
-        int32_t total;
-        const uint32_t incl = (uint32_t)wave_incl_scan_i32((int32_t)(h0 + h1), &total);
-        if (lane == 0) wtot[wave] = (uint32_t)total;
-        __syncthreads();
-        uint32_t before = incl - (h0 + h1);
-        for (int i = 0; i < wave; ++i) before += wtot[i];
-        if (before < need && need <= before + h0) pick[0] = (uint32_t)top, pick[1] = before;
-        if (before + h0 < need && need <= before + h0 + h1) pick[0] = (uint32_t)top - 1, pick[1] = before + h0;
-        __syncthreads();
-        T |= pick[0] << shift;
-        need -= pick[1];
-      }
-      // T is the key of the last weight taken, `need` how many of its ties are; each wave takes a run of the candidates
-      const int32_t per = ((hi - lo + 15) / 16 + 63) & ~63;
-      const int32_t a0 = min(lo + wave * per, hi), a1 = min(a0 + per, hi);
-      uint32_t above = 0, ties = 0;
-      for (int32_t i = a0 + lane; i < a1; i += 64) {
-        const uint32_t key = weight_key(w[i]);
-        above += key > T, ties += key == T;
-      }
-      int32_t n_above, n_ties;
-      wave_incl_scan_i32((int32_t)above, &n_above);
-      wave_incl_scan_i32((int32_t)ties, &n_ties);
-      if (lane == 0) wtot[wave] = (uint32_t)n_above, wtie[wave] = (uint32_t)n_ties;
-      __syncthreads();
-      uint32_t run_above = 0, run_ties = 0;
-      for (int i = 0; i < wave; ++i) run_above += wtot[i], run_ties += wtie[i];
-      const uint64_t below = (1ull << lane) - 1;
-      for (int32_t i0 = a0; i0 < a1; i0 += 64) {
-        const int32_t i = i0 + lane;
-        const uint32_t key = i < a1 ? weight_key(w[i]) : 0;
-        const bool gt = i < a1 && key > T, eq = i < a1 && key == T;
-        const uint64_t mg = __ballot(gt), me = __ballot(eq);
-        const uint32_t ranked = run_ties + (uint32_t)__popcll(me & below);  // ties before this one
-        const uint32_t at = run_above + (uint32_t)__popcll(mg & below) + min(ranked, need);
-        if (gt || (eq && ranked < need)) kept[a.first + at] = i;
-        run_above += (uint32_t)__popcll(mg), run_ties += (uint32_t)__popcll(me);
-      }
-    }
+// A row's candidates [lo, hi) (whole: there is nothing to choose).
+struct SelectRow {
+  const float* w;
+  int32_t L, n, lo, hi;
+  bool whole;  // every token is kept
+};
+__device__ __forceinline__ SelectRow select_row(const SelectArgs& a, int32_t g, int32_t r) {
+  SelectRow s;
+  s.w = a.weights + r * a.w_row + g * a.w_head;
+  s.L = min(max(a.lens[r], 0), a.width);
+  s.n = min(s.L, a.keep);
+  s.whole = s.L <= a.keep;
+  s.lo = a.first, s.hi = s.L - a.recent;
+  return s;
+}
+// The segment of them that a workgroup holds: E a thread, in position order wave by wave, 64 at a time. A place past the
+// candidates has key 0, below that of every weight: it is never among the largest.
+template <int E>
+struct SelectKeys {
+  float x[E];
+  uint32_t key[E];
+  int32_t first;  // the lane's first place
+  __device__ __forceinline__ void load(const SelectRow& s, int32_t segment) {
+    first = s.lo + (segment * (kSelectThreads / 64) + (int)(threadIdx.x >> 6)) * (64 * E) + (int)(threadIdx.x & 63);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = first + 64 * e < s.hi ? s.w[first + 64 * e] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) key[e] = first + 64 * e < s.hi ? weight_key(x[e]) : 0u;
   }
-  if (!a.out) return;
-  // The kept tokens' weights, in order: a tile is read before it is written, for `out` may be `weights` itself.
-  float* const out = a.out + r * a.o_row + g * a.o_head;
-  const int32_t n = min(L, a.keep);
+};
+
+struct SelectShared {
+  uint32_t hist[kSelectCopies * kSelectCopy];
+  uint32_t wave[16], other[16], third[16], pick[3];
+};
+__device__ __forceinline__ void select_clear(SelectShared& sm) {
+  for (int i = threadIdx.x; i < kSelectCopies * kSelectCopy / 4; i += kSelectThreads)
+    reinterpret_cast<uint4*>(sm.hist)[i] = make_uint4(0, 0, 0, 0);
+}
+template <int E>
+__device__ __forceinline__ void select_count(SelectShared& sm, const SelectKeys<E>& k, int pass, uint32_t T) {
+  uint32_t* const mine = sm.hist + (threadIdx.x & (kSelectCopies - 1)) * kSelectCopy;
+  const int shift = kSelectShift[pass], bits = kSelectBits[pass];
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (pass == 0 ? k.key[e] != 0 : k.key[e] >> (shift + bits) == T)
+      atomicAdd(&mine[k.key[e] >> shift & ((1u << bits) - 1)], 1u);
+}
+// Thread t's bins of the histogram, 2047 - 2 t and the one below it, copies added.
+__device__ __forceinline__ uint2 select_bins(const SelectShared& sm) {
+  uint2 h = make_uint2(0, 0);
+#pragma unroll
+  for (int c = 0; c < kSelectCopies; ++c) {
+    const uint2 v = *reinterpret_cast<const uint2*>(sm.hist + c * kSelectCopy + kSelectBins - 2 - 2 * (int)threadIdx.x);
+    h.x += v.y, h.y += v.x;
+  }
+  return h;
+}
+// Over the workgroup's bins, thread t holding counts h of bins 2047 - 2 t and below: the bin of the need-th largest key, the
+// keys in bins above it and its own, in sm.pick after the next barrier.
+__device__ __forceinline__ void select_find(SelectShared& sm, uint2 h, uint32_t need) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int32_t total;
+  const uint32_t incl = (uint32_t)wave_incl_scan_i32((int32_t)(h.x + h.y), &total);
+  if (lane == 0) sm.wave[wave] = (uint32_t)total;
   __syncthreads();
-  for (int32_t i0 = 0; i0 < n; i0 += kSelectThreads) {  // uniform
-    const int32_t i = i0 + tid;
-    const float v = i < n ? w[kept[i]] : 0.0f;
+  uint32_t before = incl - (h.x + h.y);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) before += i < wave ? sm.wave[i] : 0u;
+  const uint32_t top = (uint32_t)(kSelectBins - 1 - 2 * tid);
+  if (before < need && need <= before + h.x) sm.pick[0] = top, sm.pick[1] = before, sm.pick[2] = h.x;
+  before += h.x;
+  if (before < need && need <= before + h.y) sm.pick[0] = top - 1, sm.pick[1] = before, sm.pick[2] = h.y;
+}
+// Keys whose bits from `shift` on are above T, and the first `need` of those equal to it (`above` and `equal` of either lie
+// in segments before), go to kept from a.first on in position order, their weights to out (where there is one).
+template <int E>
+__device__ __forceinline__ void select_write(SelectShared& sm, const SelectArgs& a, const SelectKeys<E>& k, uint32_t T,
+                                             int shift, uint32_t need, uint32_t above, uint32_t equal, int32_t* kept,
+                                             float* out) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t n_above = 0, n_equal = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    n_above += (uint32_t)__popcll(__ballot(k.key[e] >> shift > T));
+    n_equal += (uint32_t)__popcll(__ballot(k.key[e] >> shift == T));
+  }
+  if (lane == 0) sm.wave[wave] = n_above, sm.other[wave] = n_equal;
+  __syncthreads();  // (also: the segment is read, so its places may be written)
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (i < wave) above += sm.wave[i], equal += sm.other[i];
+  const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const bool gt = k.key[e] >> shift > T, eq = k.key[e] >> shift == T;
+    const uint64_t mg = __ballot(gt), me = __ballot(eq);
+    const uint32_t pe = equal + (uint32_t)__popcll(me & below);
+    if (gt || (eq && pe < need)) {
+      const uint32_t to = (uint32_t)a.first + above + (uint32_t)__popcll(mg & below) + min(pe, need);
+      kept[to] = k.first + 64 * e;
+      if (out) out[to] = k.x[e];
+    }
+    above += (uint32_t)__popcll(mg), equal += (uint32_t)__popcll(me);
+  }
+}
+// What a row keeps without choosing: all of a short row, the first tokens of another. (out may be the weights themselves:
+// then these weights are in place.)
+__device__ __forceinline__ void select_first(const SelectArgs& a, const SelectRow& s, int32_t* kept, float* out) {
+  for (int32_t i = threadIdx.x; i < (s.whole ? a.keep : a.first); i += kSelectThreads) {
+    kept[i] = i < s.L ? i : -1;
+    if (out && out != s.w && i < s.L) out[i] = s.w[i];
+  }
+}
+// ... and the last ones: a tile is read before it is written, for out may be the weights themselves, and their candidates
+// have been read.
+__device__ __forceinline__ void select_recent(const SelectArgs& a, const SelectRow& s, int32_t* kept, float* out) {
+  const int32_t to = a.keep - a.recent;
+  for (int32_t i0 = 0; i0 < a.recent; i0 += kSelectThreads) {  // uniform
+    const int32_t i = i0 + threadIdx.x;
+    const float v = i < a.recent && out ? s.w[s.hi + i] : 0.0f;
     wait_vmcnt<0>();
     __syncthreads();
-    if (i < n) out[i] = v;
+    if (i < a.recent) {
+      kept[to + i] = s.hi + i;
+      if (out) out[to + i] = v;
+    }
   }
-  for (int32_t i = n + tid; i < a.out_width; i += kSelectThreads) out[i] = 0.0f;
+}
+
+// A row whose candidates one workgroup holds.
+template <int E>
+__global__ __launch_bounds__(kSelectThreads) void select_row_kernel(SelectArgs a) {
+  __shared__ SelectShared sm;
+  const int32_t g = blockIdx.x, r = blockIdx.y;
+  const SelectRow s = select_row(a, g, r);
+  int32_t* const kept = a.kept + ((int64_t)r * a.G + g) * a.keep;
+  float* const out = a.out ? a.out + r * a.o_row + g * a.o_head : nullptr;
+  if (g == 0 && threadIdx.x == 0) a.new_lens[r] = s.n;
+  select_first(a, s, kept, out);
+  uint32_t need = (uint32_t)(a.keep - a.first - a.recent);
+  if (!s.whole) {  // uniform
+    if (need > 0) {
+      SelectKeys<E> x;
+      x.load(s, 0);
+      select_clear(sm);
+      uint32_t T = 0;  // the threshold key's bits found so far
+      int pass = 0;
+      for (;; ++pass) {
+        __syncthreads();  // the histogram is clear
+        select_count(sm, x, pass, T);
+        __syncthreads();
+        const uint2 h = select_bins(sm);
+        select_find(sm, h, need);  // (its barrier: the bins are read)
+        select_clear(sm);
+        __syncthreads();
+        T = T << kSelectBits[pass] | sm.pick[0];
+        need -= sm.pick[1];
+        // (a bin that is taken whole: what is left of its bits does not matter)
+        if (pass == 2 || sm.pick[2] == need) break;
+      }
+      select_write(sm, a, x, T, kSelectShift[pass], need, 0, 0, kept, out);
+    }
+    select_recent(a, s, kept, out);
+  }
+  if (out) {
+    __syncthreads();
+    for (int32_t i = s.n + threadIdx.x; i < a.out_width; i += kSelectThreads) out[i] = 0.0f;
+  }
+}
+
+// A longer row takes S workgroups of kSelectSegment candidates, one launch a pass: a segment's histogram goes to the
+// workspace, the next launch adds the row's up.
+struct SelectLong {
+  uint32_t* hist[3];  // [R, G, S, 2048]
+  uint32_t* above;    // [R, G, S] a segment's keys above the bits found before the last pass
+  uint32_t* state;    // [3, R, G, 2] the bits found before each pass, and how many keys are still to be found
+  float* kept_w;      // [R, G, keep] the kept weights of a row that is thinned in place, or null
+  int32_t S;
+};
+// The row's histogram of pass `pass` added over its segments (thread t's bins), the threshold's bits and count brought up to
+// it, and this segment's keys above its bin added to what is above already. prior: the same of the segments before this one.
+struct SelectFound {
+  uint32_t T, need, above, prior_above, prior_equal;
+};
+__device__ __forceinline__ SelectFound select_fold(SelectShared& sm, const SelectArgs& a, const SelectLong& b, int32_t row,
+                                                   int32_t seg, int pass) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  SelectFound f;
+  const uint32_t* const state = b.state + 2 * ((int64_t)pass * a.R * a.G + row);
+  f.T = pass > 0 ? state[0] : 0u;
+  f.need = pass > 0 ? state[1] : (uint32_t)(a.keep - a.first - a.recent);
+  const uint2* h = reinterpret_cast<const uint2*>(b.hist[pass]) + (int64_t)row * b.S * (kSelectBins / 2) + tid;
+  uint2 all = make_uint2(0, 0), mine = make_uint2(0, 0), prior = make_uint2(0, 0);
+#pragma unroll 8
+  for (int32_t i = 0; i < b.S; ++i) {
+    const uint2 v = h[(int64_t)i * (kSelectBins / 2)];
+    all.x += v.x, all.y += v.y;
+    if (i < seg) prior.x += v.x, prior.y += v.y;
+    if (i == seg) mine = v;
+  }
+  select_find(sm, all, f.need);
+  __syncthreads();
+  const uint32_t bin = sm.pick[0], top = (uint32_t)(kSelectBins - 1 - 2 * tid);
+  f.T = f.T << kSelectBits[pass] | bin;
+  f.need -= sm.pick[1];
+  // counts above the bin, and in it, of this segment and of those before
+  const uint32_t mine_above = (top > bin ? mine.x : 0u) + (top - 1 > bin && top > 0 ? mine.y : 0u);
+  const uint32_t prior_above = (top > bin ? prior.x : 0u) + (top - 1 > bin && top > 0 ? prior.y : 0u);
+  const uint32_t prior_equal = top == bin ? prior.x : top - 1 == bin ? prior.y : 0u;
+  int32_t m, p, e;
+  wave_incl_scan_i32((int32_t)mine_above, &m);
+  wave_incl_scan_i32((int32_t)prior_above, &p);
+  wave_incl_scan_i32((int32_t)prior_equal, &e);
+  __syncthreads();  // sm.wave is read
+  if (lane == 0) sm.wave[wave] = (uint32_t)m, sm.other[wave] = (uint32_t)p, sm.third[wave] = (uint32_t)e;
+  __syncthreads();
+  f.above = f.prior_above = f.prior_equal = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) f.above += sm.wave[i], f.prior_above += sm.other[i], f.prior_equal += sm.third[i];
+  __syncthreads();
+  return f;
+}
+
+template <int PASS>
+__global__ __launch_bounds__(kSelectThreads) void select_hist_kernel(SelectArgs a, SelectLong b) {
+  __shared__ SelectShared sm;
+  const int32_t seg = blockIdx.x, g = blockIdx.y, r = blockIdx.z, row = r * a.G + g;
+  const SelectRow s = select_row(a, g, r);
+  if (s.whole || a.keep == a.first + a.recent) return;  // uniform
+  SelectKeys<kSelectMost> x;
+  x.load(s, seg);
+  uint32_t T = 0;
+  if constexpr (PASS > 0) {
+    const SelectFound f = select_fold(sm, a, b, row, seg, PASS - 1);
+    T = f.T;
+    if (threadIdx.x == 0) {
+      uint32_t* const above = b.above + (int64_t)row * b.S + seg;
+      *above = PASS == 1 ? f.above : *above + f.above;
+      uint32_t* const state = b.state + 2 * ((int64_t)PASS * a.R * a.G + row);
+      if (seg == 0) state[0] = f.T, state[1] = f.need;
+    }
+  }
+  select_clear(sm);
+  __syncthreads();
+  select_count(sm, x, PASS, T);
+  __syncthreads();
+  reinterpret_cast<uint2*>(b.hist[PASS])[((int64_t)row * b.S + seg) * (kSelectBins / 2) + threadIdx.x] = select_bins(sm);
+}
+
+__global__ __launch_bounds__(kSelectThreads) void select_write_kernel(SelectArgs a, SelectLong b) {
+  __shared__ SelectShared sm;
+  const int32_t seg = blockIdx.x, g = blockIdx.y, r = blockIdx.z, row = r * a.G + g;
+  const SelectRow s = select_row(a, g, r);
+  int32_t* const kept = a.kept + (int64_t)row * a.keep;
+  float* out = a.out ? a.out + r * a.o_row + g * a.o_head : nullptr;
+  // a row that is thinned in place: its weights go by the workspace, for other workgroups still read them
+  if (b.kept_w && !s.whole) out = b.kept_w + (int64_t)row * a.keep;
+  if (seg == 0) {
+    if (g == 0 && threadIdx.x == 0) a.new_lens[r] = s.n;
+    select_first(a, s, kept, out);
+    if (!s.whole) select_recent(a, s, kept, out);
+  }
+  if (!s.whole && a.keep > a.first + a.recent) {  // uniform
+    SelectKeys<kSelectMost> x;
+    x.load(s, seg);
+    const SelectFound f = select_fold(sm, a, b, row, seg, 2);
+    uint32_t above = f.prior_above;
+    for (int32_t i = 0; i < seg; ++i) above += b.above[(int64_t)row * b.S + i];
+    select_write(sm, a, x, f.T, 0, f.need, above, f.prior_equal, kept, out);
+  }
+  if (out && !(b.kept_w && !s.whole))
+    for (int32_t i = s.n + seg * kSelectThreads + threadIdx.x; i < a.out_width; i += b.S * kSelectThreads) out[i] = 0.0f;
+}
+
+// The rows thinned in place: their kept weights, then zeros.
+__global__ __launch_bounds__(kSelectThreads) void select_place_kernel(SelectArgs a, SelectLong b) {
+  const int32_t g = blockIdx.y, r = blockIdx.z;
+  const SelectRow s = select_row(a, g, r);
+  if (s.whole) return;
+  float* const out = a.out + r * a.o_row + g * a.o_head;
+  const float* const from = b.kept_w + ((int64_t)r * a.G + g) * a.keep;
+  for (int32_t i = blockIdx.x * kSelectThreads + threadIdx.x; i < a.out_width; i += gridDim.x * kSelectThreads)
+    out[i] = i < a.keep ? from[i] : 0.0f;
 }
 
 struct CompactArgs {
@@ -197,10 +404,29 @@ __global__ __launch_bounds__(kCompactThreads) void compact_tokens_kernel(Compact
 
 using namespace sna;
 
+namespace {
+
+// The workspace of a launch whose rows may be longer than one workgroup holds: histograms, counts and thresholds, and the
+// kept weights where rows are thinned in place.
+int64_t select_segments(int32_t width) { return ((int64_t)width + kSelectSegment - 1) / kSelectSegment; }
+int64_t select_bytes(int64_t rows, int32_t width, int32_t keep, bool in_place) {
+  if (width <= kSelectSegment) return 0;
+  return rows * (select_segments(width) * (3 * kSelectBins + 1) + 3 * 2 + (in_place ? keep : 0)) * 4;
+}
+
+}  // namespace
+
+extern "C" int64_t sna_select_workspace_bytes(int32_t R, int32_t num_kv_heads, int32_t width, int32_t keep,
+                                              int32_t in_place) {
+  if (R < 1 || num_kv_heads < 1 || width < 1 || keep < 1) return 0;
+  return select_bytes((int64_t)R * num_kv_heads, width, keep, in_place != 0);
+}
+
 extern "C" int sna_select_tokens(const float* weights, int64_t row_stride, int64_t head_stride, int32_t width,
                                  const int32_t* seq_lens, int32_t R, int32_t num_kv_heads, int32_t keep, int32_t first,
                                  int32_t recent, int32_t* kept, int32_t* new_lens, float* weights_out,
-                                 int64_t out_row_stride, int64_t out_head_stride, int32_t out_width, void* stream) {
+                                 int64_t out_row_stride, int64_t out_head_stride, int32_t out_width, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
   ApiGuard guard;
   if (R < 0 || num_kv_heads < 1 || width < 1 || keep < 1 || first < 0 || recent < 0 || (int64_t)first + recent > keep ||
       row_stride < width || head_stride < width)
@@ -211,10 +437,22 @@ extern "C" int sna_select_tokens(const float* weights, int64_t row_stride, int64
   if (weights_out && (out_width < keep || out_row_stride < out_width || out_head_stride < out_width))
     return fail(SNA_ERR_INVALID_ARGUMENT, "select_tokens: weights_out of %d columns (strides %lld / %lld) for %d tokens",
                 out_width, (long long)out_row_stride, (long long)out_head_stride, keep);
+  if (width > INT32_MAX - kSelectSegment || (weights_out && out_width > INT32_MAX - (1 << 20)))
+    return fail(SNA_ERR_UNSUPPORTED, "select_tokens: %d columns, %d out (under 2^31)", width, out_width);
   if (R == 0) return SNA_OK;
   if (!weights || !seq_lens || !kept || !new_lens)
     return fail(SNA_ERR_INVALID_ARGUMENT, "select_tokens: null pointer");
-  if (R > 65535) return fail(SNA_ERR_INVALID_ARGUMENT, "select_tokens: %d rows exceed the grid", R);
+  if (R > 65535 || num_kv_heads > 65535)
+    return fail(SNA_ERR_INVALID_ARGUMENT, "select_tokens: %d rows x %d KV heads exceed the grid", R, num_kv_heads);
+  const bool in_place = weights_out == weights && weights_out;
+  if (in_place && (out_row_stride != row_stride || out_head_stride != head_stride))
+    return fail(SNA_ERR_INVALID_ARGUMENT, "select_tokens: weights_out is weights with other strides");
+  const int64_t rows = (int64_t)R * num_kv_heads, need = select_bytes(rows, width, keep, in_place);
+  if (workspace_bytes < need || (need > 0 && !workspace))
+    return fail(SNA_ERR_WORKSPACE, "select_tokens: workspace of %lld bytes, need %lld", (long long)workspace_bytes,
+                (long long)need);
+  if (need > 0 && !aligned(workspace, 16))
+    return fail(SNA_ERR_INVALID_ARGUMENT, "select_tokens: the workspace must be 16-byte aligned");
   SelectArgs a;
   a.weights = weights;
   a.w_row = row_stride;
@@ -232,7 +470,31 @@ extern "C" int sna_select_tokens(const float* weights, int64_t row_stride, int64
   a.o_row = out_row_stride;
   a.o_head = out_head_stride;
   a.out_width = out_width;
-  hipLaunchKernelGGL(select_tokens_kernel, dim3(num_kv_heads, R), dim3(kSelectThreads), 0, (hipStream_t)stream, a);
+  const hipStream_t s = (hipStream_t)stream;
+  const dim3 block(kSelectThreads), grid(num_kv_heads, R);
+  if (width <= kSelectSegment / 4) {
+    hipLaunchKernelGGL((select_row_kernel<kSelectMost / 4>), grid, block, 0, s, a);
+  } else if (width <= kSelectSegment / 2) {
+    hipLaunchKernelGGL((select_row_kernel<kSelectMost / 2>), grid, block, 0, s, a);
+  } else if (width <= kSelectSegment) {
+    hipLaunchKernelGGL((select_row_kernel<kSelectMost>), grid, block, 0, s, a);
+  } else {
+    SelectLong b;
+    b.S = (int32_t)select_segments(width);
+    const int64_t bins = rows * b.S * kSelectBins;
+    b.hist[0] = (uint32_t*)workspace;
+    b.hist[1] = b.hist[0] + bins;
+    b.hist[2] = b.hist[1] + bins;
+    b.above = b.hist[2] + bins;
+    b.state = b.above + rows * b.S;
+    b.kept_w = in_place ? (float*)(b.state + rows * 6) : nullptr;
+    const dim3 parts(b.S, num_kv_heads, R);
+    hipLaunchKernelGGL((select_hist_kernel<0>), parts, block, 0, s, a, b);
+    hipLaunchKernelGGL((select_hist_kernel<1>), parts, block, 0, s, a, b);
+    hipLaunchKernelGGL((select_hist_kernel<2>), parts, block, 0, s, a, b);
+    hipLaunchKernelGGL(select_write_kernel, parts, block, 0, s, a, b);
+    if (in_place) hipLaunchKernelGGL(select_place_kernel, parts, block, 0, s, a, b);
+  }
   return check_launch("select_tokens");
 }
 

@@ -1075,6 +1075,7 @@ def select_tokens(weights: Tensor, seq_lens: Tensor, *, keep: int, first: int = 
     _need(keep >= 1 and first >= 0 and recent >= 0 and first + recent <= keep,
           lambda: f"keep {keep} tokens of which {first} first and {recent} recent")
     o_row = o_head = M = 0
+    same = False
     if weights_out is not None:
         o_row, o_head = _weight_strides(weights_out, R, G, "weights_out")
         M = weights_out.shape[2]
@@ -1085,10 +1086,12 @@ def select_tokens(weights: Tensor, seq_lens: Tensor, *, keep: int, first: int = 
     new_lens = torch.empty(R, dtype=torch.int32, device=dev)
     if R == 0 or G == 0:
         return kept, new_lens
+    lib = _lib.load()
+    need = lib.sna_select_workspace_bytes(R, G, N, keep, int(same))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
     with _device_of(dev):
-        rc = _lib.load().sna_select_tokens(_ptr(weights), row, head, N, _ptr(lens), R, G, keep, first, recent,
-                                           _ptr(kept), _ptr(new_lens), _ptr(weights_out), o_row, o_head, M,
-                                           _stream(dev))
+        rc = lib.sna_select_tokens(_ptr(weights), row, head, N, _ptr(lens), R, G, keep, first, recent, _ptr(kept),
+                                   _ptr(new_lens), _ptr(weights_out), o_row, o_head, M, _ptr(ws), need, _stream(dev))
     _lib.check(rc, "select_tokens")
     return kept, new_lens
 

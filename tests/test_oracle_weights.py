@@ -118,8 +118,19 @@ def test_select_refusals(bad):
     a = dict(w=P, row=16, head=8, N=8, lens=P, R=2, G=2, keep=5, first=1, recent=1, kept=P, new=P, out=None, orow=16,
              ohead=8, M=8) | bad
     rc = _lib.load().sna_select_tokens(a["w"], a["row"], a["head"], a["N"], a["lens"], a["R"], a["G"], a["keep"], a["first"],
-                                       a["recent"], a["kept"], a["new"], a["out"], a["orow"], a["ohead"], a["M"], None)
+                                       a["recent"], a["kept"], a["new"], a["out"], a["orow"], a["ohead"], a["M"], None, 0,
+                                       None)
     assert rc == -1, _lib.last_error()
+
+
+def test_select_workspace_refusals():
+    lib = _lib.load()
+    assert lib.sna_select_workspace_bytes(2, 2, 16384, 5, 1) == 0
+    need, more = (lib.sna_select_workspace_bytes(2, 2, 40000, 5, p) for p in (0, 1))
+    assert 0 < need < more
+    for ws, size in ((None, need), (P, need - 1), (P + 4, need)):
+        rc = lib.sna_select_tokens(P, 80000, 40000, 40000, P, 2, 2, 5, 1, 1, P, P, None, 0, 0, 0, ws, size, None)
+        assert rc in (-1, -2) and "workspace" in _lib.last_error()
 
 
 @pytest.mark.parametrize("bad,code", [(dict(R=-1), -1), (dict(G=0), -1), (dict(nb=0), -1), (dict(page=0), -1),
