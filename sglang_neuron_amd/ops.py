@@ -8,7 +8,6 @@ Reference interfaces each function stands in for are cited per function (paths u
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 from typing import Optional, Sequence, Union
@@ -81,12 +80,20 @@ def _as(t: Tensor, dtype: torch.dtype) -> Tensor:
     return t if t.dtype == dtype else t.to(dtype)
 
 
-_same_device = contextlib.nullcontext()
+def _launch(dev: torch.device, fn, what: str, *args) -> None:
+    """fn(*args, stream) on ``dev``'s current stream, with ``dev`` the current device (a null stream means the current
+    device's), its status checked."""
+    idx = dev.index
+    if idx == _current_device():
+        rc = fn(*args, _raw_stream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, _raw_stream(idx))
+    if rc:
+        _lib.check(rc, what)
 
 
-def _device_of(dev: torch.device):
-    """A context in which ``dev`` is the current device (nothing to do where it is already)."""
-    return _same_device if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _head_scales(scale: Optional[Tensor], G: int, name: str) -> Tensor:
@@ -231,36 +238,46 @@ def qkv_norm_mrope_store(qkv: Tensor, *, positions: Tensor, inv_freq: Tensor, ax
     ``axes`` [n] host ints (mrope_axes). The other arguments are qkv_norm_rope_store's. Angles are formed in 64 bits, so
     positions of any size serve; norm and rotation are fp32 and every output is rounded once. Returns Q [T, q, d] bf16; the
     caches are written in place."""
+    # (conditions are tested here and messages built by _need only where one fails: the checks of a small call cost as much
+    # as its kernel)
     dev = _on_gpu(qkv, positions, inv_freq, k_cache, v_cache, slot_mapping, q_norm, k_norm, k_scale, v_scale, q_out)
-    _need(k_cache.dim() == 4, lambda: f"caches [blocks, kv_heads, page, d], got {tuple(k_cache.shape)}")
-    nb, G, P, d = k_cache.shape
-    _need(G == num_kv_heads and d == d_head,
-          lambda: f"caches {tuple(k_cache.shape)} for {num_kv_heads} heads of {d_head}")
-    _need(v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype, "K and V caches differ")
-    _need(k_cache.is_contiguous() and v_cache.is_contiguous(), "caches must be contiguous")
+    shape = k_cache.shape
+    if len(shape) != 4 or shape[1] != num_kv_heads or shape[3] != d_head:
+        _need(False, f"caches {tuple(shape)} for {num_kv_heads} heads of {d_head}: [blocks, kv_heads, page, d]")
+    nb, G, P, d = shape
+    if v_cache.shape != shape or v_cache.dtype != k_cache.dtype:
+        _need(False, "K and V caches differ")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        _need(False, "caches must be contiguous")
     width = (num_q_heads + 2 * num_kv_heads) * d_head
-    _need(qkv.dtype == torch.bfloat16 and qkv.dim() >= 1 and qkv.shape[-1] == width,
-          lambda: f"qkv must be bf16 [T, {width}], got {tuple(qkv.shape)}")
+    if qkv.dtype != torch.bfloat16 or qkv.dim() < 1 or qkv.shape[-1] != width:
+        _need(False, f"qkv must be bf16 [T, {width}], got {tuple(qkv.shape)} {qkv.dtype}")
     qkv = qkv if qkv.dim() == 2 else qkv.reshape(-1, width)
     T = qkv.shape[0]
-    stride = qkv.stride(0) if T > 1 else width
-    _need(qkv.stride(1) == 1 and stride >= width and stride % 8 == 0,
-          lambda: f"qkv rows must have unit column stride and a row stride of a multiple of 8, got {qkv.stride()}")
-    _need(positions.dim() == 2 and positions.shape[1] == T, lambda: f"positions must be [axes, {T}]")
+    stride, col = qkv.stride()
+    if T <= 1:
+        stride = width
+    if col != 1 or stride < width or stride % 8:
+        _need(False, f"qkv rows must have unit column stride and a row stride of a multiple of 8, got {qkv.stride()}")
+    if positions.dim() != 2 or positions.shape[1] != T:
+        _need(False, f"positions must be [axes, {T}]")
     positions = _as(positions, torch.int64)
-    positions = positions if positions.stride(1) == 1 and positions.stride(0) >= T else positions.contiguous()
-    inv_freq = _contig(inv_freq.reshape(-1), "inv_freq", torch.float32)
-    n = inv_freq.numel()
-    _need(len(axes) == n, lambda: f"{len(axes)} axes for {n} rotated pairs")
-    _need(n == 0 or (min(axes) >= 0 and max(axes) < positions.shape[0]),
-          lambda: f"axes must lie in [0, {positions.shape[0]})")
-    slots = _contig(_as(slot_mapping.reshape(-1), torch.int64), "slot_mapping")
-    _need(slots.numel() == T, lambda: f"{slots.numel()} slots for {T} tokens")
-    _need((q_norm is None) == (k_norm is None), "give both QK-norm gammas or neither")
+    if positions.stride(1) != 1 or positions.stride(0) < T:
+        positions = positions.contiguous()
+    inv_freq = _contig(inv_freq if inv_freq.dim() == 1 else inv_freq.reshape(-1), "inv_freq", torch.float32)
+    n = inv_freq.shape[0]
+    if len(axes) != n or (n > 0 and not (min(axes) >= 0 and max(axes) < positions.shape[0])):
+        _need(False, f"{len(axes)} axes for {n} rotated pairs, each in [0, {positions.shape[0]})")
+    slots = _contig(_as(slot_mapping if slot_mapping.dim() == 1 else slot_mapping.reshape(-1), torch.int64), "slot_mapping")
+    if slots.shape[0] != T:
+        _need(False, f"{slots.shape[0]} slots for {T} tokens")
+    if (q_norm is None) != (k_norm is None):
+        _need(False, "give both QK-norm gammas or neither")
     if q_norm is not None:
-        q_norm = _contig(q_norm.reshape(-1), "q_norm", torch.bfloat16)
-        k_norm = _contig(k_norm.reshape(-1), "k_norm", torch.bfloat16)
-        _need(q_norm.numel() == d_head and k_norm.numel() == d_head, lambda: f"QK-norm gammas need {d_head} entries")
+        q_norm = _contig(q_norm if q_norm.dim() == 1 else q_norm.reshape(-1), "q_norm", torch.bfloat16)
+        k_norm = _contig(k_norm if k_norm.dim() == 1 else k_norm.reshape(-1), "k_norm", torch.bfloat16)
+        if q_norm.shape[0] != d_head or k_norm.shape[0] != d_head:
+            _need(False, f"QK-norm gammas need {d_head} entries")
     code = cache_dtype_code(k_cache.dtype)
     if code == _lib.DTYPE_FP8_E4M3FN:
         k_scale, v_scale = _head_scales(k_scale, G, "k_scale"), _head_scales(v_scale, G, "v_scale")
@@ -268,15 +285,12 @@ def qkv_norm_mrope_store(qkv: Tensor, *, positions: Tensor, inv_freq: Tensor, ax
         k_scale = v_scale = None
     if q_out is None:
         q_out = torch.empty(T, num_q_heads, d_head, dtype=torch.bfloat16, device=dev)
-    _need(q_out.shape == (T, num_q_heads, d_head) and q_out.dtype == torch.bfloat16 and q_out.is_contiguous(),
-          "bad q_out tensor")
-    with _device_of(dev):
-        rc = _lib.load().sna_qkv_norm_mrope_store(
-            _ptr(qkv), stride, T, num_q_heads, num_kv_heads, d_head, _ptr(q_norm), _ptr(k_norm), float(norm_eps),
-            _ptr(positions), max(positions.stride(0), T), positions.shape[0], _ptr(inv_freq), n, bytes(axes),
-            _ptr(slots), _ptr(q_out), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), nb, P, code,
-            _stream(dev))
-    _lib.check(rc, "qkv_norm_mrope_store")
+    elif q_out.shape != (T, num_q_heads, d_head) or q_out.dtype != torch.bfloat16 or not q_out.is_contiguous():
+        _need(False, "bad q_out tensor")
+    _launch(dev, _lib.load().sna_qkv_norm_mrope_store, "qkv_norm_mrope_store", qkv.data_ptr(), stride, T, num_q_heads,
+            num_kv_heads, d_head, _ptr(q_norm), _ptr(k_norm), norm_eps, positions.data_ptr(),
+            max(positions.stride(0), T), positions.shape[0], inv_freq.data_ptr(), n, bytes(axes), slots.data_ptr(),
+            q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), nb, P, code)
     return q_out
 
 
@@ -966,59 +980,61 @@ def segmented_attention(q: Tensor, *, k_cache: Tensor, v_cache: Tensor, block_ta
 
 def _weight_strides(weights: Tensor, R: int, G: int, what: str) -> tuple[int, int]:
     """(row stride, head stride) of a [R, G, N] fp32 tensor whose rows do not overlap."""
-    _need(weights.dim() == 3 and weights.shape[0] == R and weights.shape[1] == G and weights.dtype == torch.float32,
-          lambda: f"{what} must be [{R}, {G}, N] fp32, got {tuple(weights.shape)} {weights.dtype}")
-    N = weights.shape[2]
-    _need(weights.stride(2) == 1 or N <= 1, lambda: f"{what} must have unit column stride")
-    row, head = (weights.stride(0) if R > 1 else N * G), (weights.stride(1) if G > 1 else N)
-    _need(head >= N and row >= N and (R <= 1 or G <= 1 or row >= head * G or head >= row * R),
-          lambda: f"{what}: rows of strides {weights.stride()} overlap")
+    shape = weights.shape
+    if len(shape) != 3 or shape[0] != R or shape[1] != G or weights.dtype != torch.float32:
+        _need(False, f"{what} must be [{R}, {G}, N] fp32, got {tuple(shape)} {weights.dtype}")
+    N = shape[2]
+    row, head, col = weights.stride()
+    row, head = (row if R > 1 else N * G), (head if G > 1 else N)
+    if col != 1 and N > 1:
+        _need(False, f"{what} must have unit column stride")
+    if head < N or row < N or (R > 1 and G > 1 and row < head * G and head < row * R):
+        _need(False, f"{what}: rows of strides {weights.stride()} overlap")
     return row, head
 
 
 def _attention_weights(what, q, T, R, k_cache, block_table, q_start, lens, max_q_len, sm_scale, k_scale, sinks, window,
                        weights, scales_multiply) -> Tensor:
     dev = _on_gpu(q, k_cache, block_table, q_start, lens, k_scale, sinks, weights)
-    _need(k_cache.dim() == 4 and k_cache.is_contiguous(), "the cache must be contiguous [blocks, kv_heads, page, d]")
-    H, d = q.shape[1:]
-    nb, G, P, dk = k_cache.shape
-    _need(dk == d, lambda: f"cache {tuple(k_cache.shape)} does not match q's head_dim {d}")
-    _need(H % G == 0, lambda: f"{H} query heads over {G} KV heads")
+    _, H, d = q.shape
+    shape = k_cache.shape
+    if len(shape) != 4 or not k_cache.is_contiguous() or shape[3] != d or H % shape[1]:
+        _need(False, f"the cache must be contiguous [blocks, kv_heads, page, {d}] with kv_heads dividing {H}, got "
+              f"{tuple(shape)}")
+    nb, G, P, _ = shape
     code = cache_dtype_code(k_cache.dtype, scales_multiply)
     q = _contig(q, "q", torch.bfloat16)
-    _need(block_table.dim() == 2 and block_table.shape[0] == R, lambda: f"block_table must be [{R}, width]")
+    if block_table.dim() != 2 or block_table.shape[0] != R or block_table.shape[1] < 1:
+        _need(False, f"block_table must be [{R}, width]")
     table = _as(block_table, torch.int32)
     table = table if table.stride(1) == 1 else table.contiguous()
     W = table.shape[1]
-    _need(W >= 1, "block_table has no columns")
-    lens = _contig(_as(lens.reshape(-1), torch.int32), "lens")
+    lens = _contig(_as(lens if lens.dim() == 1 else lens.reshape(-1), torch.int32), "lens")
     k_scale = None if code == _lib.DTYPE_BF16 else _head_scales(k_scale, G, "k_scale")
     if sinks is not None:
         sinks = _contig(_as(sinks.reshape(-1), torch.float32), "sinks")
-        _need(sinks.numel() == H, lambda: f"{sinks.numel()} sinks for {H} heads")
+        if sinks.shape[0] != H:
+            _need(False, f"{sinks.shape[0]} sinks for {H} heads")
     add = weights is not None
     if add:
         row, head = _weight_strides(weights, R, G, "weights")
+        N = weights.shape[2]
     else:
-        weights = torch.empty(R, G, W * P, dtype=torch.float32, device=dev)
-        row, head = G * W * P, W * P
-    N = weights.shape[2]
+        N = W * P
+        row, head = G * N, N
+        weights = torch.empty(R, G, N, dtype=torch.float32, device=dev)
     lib = _lib.load()
     need = lib.sna_attention_weights_workspace_bytes(T, R, max_q_len, H, G, d, P, W, N, code)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     stride = max(table.stride(0), W)
-    with _device_of(dev):
-        if q_start is None:
-            rc = lib.sna_decode_attention_weights(
-                _ptr(q), _ptr(k_cache), _ptr(k_scale), _ptr(table), stride, W, _ptr(lens), R, _ptr(sinks),
-                float(sm_scale), int(window), _ptr(weights), row, head, N, int(add), H, G, d, P, nb, code, _ptr(ws),
-                need, _stream(dev))
-        else:
-            rc = lib.sna_prefill_attention_weights(
-                _ptr(q), _ptr(k_cache), _ptr(k_scale), _ptr(table), stride, W, _ptr(q_start), _ptr(lens), T, R,
-                max_q_len, _ptr(sinks), float(sm_scale), int(window), _ptr(weights), row, head, N, int(add), H, G, d, P,
-                nb, code, _ptr(ws), need, _stream(dev))
-    _lib.check(rc, what)
+    if q_start is None:
+        _launch(dev, lib.sna_decode_attention_weights, what, q.data_ptr(), k_cache.data_ptr(), _ptr(k_scale),
+                table.data_ptr(), stride, W, lens.data_ptr(), R, _ptr(sinks), sm_scale, window, weights.data_ptr(), row,
+                head, N, add, H, G, d, P, nb, code, ws.data_ptr(), need)
+    else:
+        _launch(dev, lib.sna_prefill_attention_weights, what, q.data_ptr(), k_cache.data_ptr(), _ptr(k_scale),
+                table.data_ptr(), stride, W, q_start.data_ptr(), lens.data_ptr(), T, R, max_q_len, _ptr(sinks), sm_scale,
+                window, weights.data_ptr(), row, head, N, add, H, G, d, P, nb, code, ws.data_ptr(), need)
     return weights
 
 
@@ -1049,9 +1065,9 @@ def decode_attention_weights(q: Tensor, k_cache: Tensor, block_table: Tensor, se
                              weights: Optional[Tensor] = None, scales_multiply: bool = False) -> Tensor:
     """prefill_attention_weights for a decode step: row b's one query q[b] (q [B, H, d]) at position seq_lens[b] - 1, its
     key in the pool already (paged_decode_gqa stores it at ``new_slots``). Returns [B, G, N] fp32 as there."""
-    _need(q.dim() == 3, lambda: f"q must be [B, H, d], got {tuple(q.shape)}")
+    if q.dim() != 3 or seq_lens.numel() != q.shape[0]:
+        _need(False, f"q must be [B, H, d] with one of seq_lens a row, got {tuple(q.shape)} and {tuple(seq_lens.shape)}")
     B = q.shape[0]
-    _need(seq_lens.numel() == B, lambda: f"{seq_lens.numel()} seq_lens for {B} rows")
     return _attention_weights("decode_attention_weights", q, B, B, k_cache, block_table, None, seq_lens, 1, sm_scale,
                               k_scale, sinks, window, weights, scales_multiply)
 
@@ -1066,43 +1082,45 @@ def select_tokens(weights: Tensor, seq_lens: Tensor, *, keep: int, first: int = 
     ``weights_out`` [R, G, M >= keep] fp32, when given, receives the kept tokens' weights and zeros after them; it may be
     ``weights`` itself, so that the tokens written next start at zero."""
     dev = _on_gpu(weights, seq_lens, weights_out)
-    _need(weights.dim() == 3, lambda: f"weights must be [R, G, N], got {tuple(weights.shape)}")
+    if weights.dim() != 3:
+        _need(False, f"weights must be [R, G, N], got {tuple(weights.shape)}")
     R, G, N = weights.shape
     row, head = _weight_strides(weights, R, G, "weights")
-    lens = _contig(_as(seq_lens.reshape(-1), torch.int32), "seq_lens")
-    _need(lens.numel() == R, lambda: f"{lens.numel()} seq_lens for {R} rows")
-    keep, first, recent = int(keep), int(first), int(recent)
-    _need(keep >= 1 and first >= 0 and recent >= 0 and first + recent <= keep,
-          lambda: f"keep {keep} tokens of which {first} first and {recent} recent")
+    lens = _contig(_as(seq_lens if seq_lens.dim() == 1 else seq_lens.reshape(-1), torch.int32), "seq_lens")
+    if lens.shape[0] != R:
+        _need(False, f"{lens.shape[0]} seq_lens for {R} rows")
+    if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
+        _need(False, f"keep {keep} tokens of which {first} first and {recent} recent")
     o_row = o_head = M = 0
     same = False
     if weights_out is not None:
         o_row, o_head = _weight_strides(weights_out, R, G, "weights_out")
         M = weights_out.shape[2]
-        _need(M >= keep, lambda: f"weights_out of {M} columns for {keep} tokens")
+        if M < keep:
+            _need(False, f"weights_out of {M} columns for {keep} tokens")
         same = weights_out.data_ptr() == weights.data_ptr() and (o_row, o_head) == (row, head)
-        _need(same or not _overlap(weights, weights_out), "weights_out overlaps weights without being it")
+        if not same and _overlap(weights, weights_out):
+            _need(False, "weights_out overlaps weights without being it")
     kept = torch.empty(R, G, keep, dtype=torch.int32, device=dev)
     new_lens = torch.empty(R, dtype=torch.int32, device=dev)
     if R == 0 or G == 0:
         return kept, new_lens
     lib = _lib.load()
-    need = lib.sna_select_workspace_bytes(R, G, N, keep, int(same))
+    need = lib.sna_select_workspace_bytes(R, G, N, keep, same)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    with _device_of(dev):
-        rc = lib.sna_select_tokens(_ptr(weights), row, head, N, _ptr(lens), R, G, keep, first, recent, _ptr(kept),
-                                   _ptr(new_lens), _ptr(weights_out), o_row, o_head, M, _ptr(ws), need, _stream(dev))
-    _lib.check(rc, "select_tokens")
+    _launch(dev, lib.sna_select_tokens, "select_tokens", weights.data_ptr(), row, head, N, lens.data_ptr(), R, G, keep,
+            first, recent, kept.data_ptr(), new_lens.data_ptr(), _ptr(weights_out), o_row, o_head, M, _ptr(ws), need)
     return kept, new_lens
 
 
 def _overlap(a: Tensor, b: Tensor) -> bool:
     """Whether the address ranges of two tensors meet."""
-    def span(t):
-        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
-        return t.data_ptr(), t.data_ptr() + last * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+
+    def end(t):
+        return t.data_ptr() + (sum([(n - 1) * s for n, s in zip(t.shape, t.stride())]) + 1) * t.element_size()
+    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
 
 
 def compact_tokens(k_cache: Tensor, v_cache: Tensor, block_table: Tensor, kept: Tensor, *,
@@ -1116,30 +1134,33 @@ def compact_tokens(k_cache: Tensor, v_cache: Tensor, block_table: Tensor, kept: 
     Rows that share pages (a cached prefix) cannot be compacted in place: give them pages of their own in ``dst_table``,
     which names no page of ``block_table``."""
     dev = _on_gpu(k_cache, v_cache, block_table, kept, dst_table)
-    _need(k_cache.dim() == 4 and v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype,
-          "K and V caches differ")
-    _need(k_cache.is_contiguous() and v_cache.is_contiguous(), "caches must be contiguous")
-    _need(k_cache.data_ptr() != v_cache.data_ptr() or k_cache.numel() == 0, "K and V are one tensor")
-    nb, G, P, d = k_cache.shape
-    _need(kept.dim() == 3 and kept.shape[1] == G, lambda: f"kept must be [R, {G}, keep], got {tuple(kept.shape)}")
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != k_cache.dtype:
+        _need(False, "K and V caches differ")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        _need(False, "caches must be contiguous")
+    if k_cache.data_ptr() == v_cache.data_ptr() and k_cache.numel() > 0:
+        _need(False, "K and V are one tensor")
+    nb, G, P, d = shape
+    if kept.dim() != 3 or kept.shape[1] != G:
+        _need(False, f"kept must be [R, {G}, keep], got {tuple(kept.shape)}")
     kept = _contig(kept, "kept", torch.int32)
     R, _, keep = kept.shape
-    _need(block_table.dim() == 2 and block_table.shape[0] == R, lambda: f"block_table must be [{R}, width]")
+    if block_table.dim() != 2 or block_table.shape[0] != R:
+        _need(False, f"block_table must be [{R}, width]")
     table = _contig(_as(block_table, torch.int32), "block_table")
-    dst = None
+    W = table.shape[1]
+    to, V = None, 0
     if dst_table is not None:
-        _need(dst_table.dim() == 2 and dst_table.shape[0] == R, lambda: f"dst_table must be [{R}, width]")
-        _need(dst_table.shape[1] * P >= keep, lambda: f"dst_table of {dst_table.shape[1]} pages of {P} for {keep} tokens")
+        if dst_table.dim() != 2 or dst_table.shape[0] != R or dst_table.shape[1] * P < keep:
+            _need(False, f"dst_table must be [{R}, pages of {P} for {keep} tokens], got {tuple(dst_table.shape)}")
         dst = _contig(_as(dst_table, torch.int32), "dst_table")
-    code = cache_dtype_code(k_cache.dtype)
+        if dst_table.data_ptr() != block_table.data_ptr():  # (else it is in place)
+            to, V = dst.data_ptr(), dst.shape[1]
     if R == 0 or keep == 0:
         return
-    with _device_of(dev):
-        rc = _lib.load().sna_compact_tokens(
-            _ptr(k_cache), _ptr(v_cache), nb, G, P, d, code, _ptr(table), table.shape[1], table.shape[1],
-            None if dst is None else _ptr(dst), 0 if dst is None else dst.shape[1], 0 if dst is None else dst.shape[1],
-            _ptr(kept), R, keep, _stream(dev))
-    _lib.check(rc, "compact_tokens")
+    _launch(dev, _lib.load().sna_compact_tokens, "compact_tokens", k_cache.data_ptr(), v_cache.data_ptr(), nb, G, P, d,
+            cache_dtype_code(k_cache.dtype), table.data_ptr(), W, W, to, V, V, kept.data_ptr(), R, keep)
 
 
 def evict_tokens(k_cache: Tensor, v_cache: Tensor, block_table: Tensor, seq_lens: Tensor, weights: Tensor, *, keep: int,
@@ -1147,9 +1168,8 @@ def evict_tokens(k_cache: Tensor, v_cache: Tensor, block_table: Tensor, seq_lens
                  weights_out: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
     """Thin the rows of one layer's caches to ``keep`` tokens each by accumulated attention weight: select_tokens, then
     compact_tokens. Every KV head of a row keeps a set of its own, the count is the row's. Returns (kept, new_lens)."""
-    G = k_cache.shape[1] if k_cache.dim() == 4 else -1
-    _need(weights.dim() == 3 and weights.shape[1] == G and block_table.shape[0] == weights.shape[0],
-          lambda: f"weights {tuple(weights.shape)} for {block_table.shape[0]} rows of {G} KV heads")
+    if k_cache.dim() != 4 or weights.dim() != 3 or weights.shape[:2] != (block_table.shape[0], k_cache.shape[1]):
+        _need(False, f"weights {tuple(weights.shape)} for {block_table.shape[0]} rows of caches {tuple(k_cache.shape)}")
     kept, new_lens = select_tokens(weights, seq_lens, keep=keep, first=first, recent=recent, weights_out=weights_out)
     compact_tokens(k_cache, v_cache, block_table, kept, dst_table=dst_table)
     return kept, new_lens
