@@ -9,9 +9,13 @@
 // each output is rounded once: Q and a bf16 pool to bf16, an FP8 pool to e4m3fn(x / s). (The one-axis writer rounds its
 // intermediate steps to bf16 as the reference's torch path does; this operator has no such path to follow.)
 //
-// A workgroup takes 8 tokens, two to a wave, and one group of 64 / (D / 8) consecutive heads; lane j of a head holds its
-// elements 8 j .. 8 j + 7 (one 16-byte load). The tokens' sines and cosines are computed once by the workgroup's threads
-// and passed through LDS. Bound by memory: every projection row is read once, every Q, K and V row written once.
+// A workgroup takes 8 tokens, two to a wave, and a run of heads, 64 / (D / 8) at a time: lane j of a head holds its elements
+// 8 j .. 8 j + 7 (one 16-byte load), the next heads' rows are on their way while these are worked on. The tokens' sines and
+// cosines are computed once by the workgroup's threads (one each for two pairs of a token at D = 128) and handed round
+// through LDS; a lane keeps its own in registers for every head. Bound by memory: every projection row is read once, every
+// Q, K and V row written once.
+#include <algorithm>
+
 #include "sna_device.h"
 #include "sna_host.h"
 
@@ -37,6 +41,7 @@ struct MropeArgs {
   const float* v_scale;
   int64_t num_slots;
   int32_t P;
+  int32_t groups;  // head groups (of 64 / (D / 8) heads) that a workgroup takes
 };
 
 constexpr int kMropeTokens = 8;  // of a workgroup
@@ -51,24 +56,35 @@ __device__ __forceinline__ uint32_t mrope_fp8_pair(float x0, float x1, float s, 
   return b;
 }
 
-template <bool FP8, int D>
+// FULL: every element of a head is rotated (its partner is the lane half a head away).
+template <bool FP8, int D, bool FULL>
 __global__ __launch_bounds__(256) void qkv_norm_mrope_store_kernel(MropeArgs a) {
   constexpr int LPH = D / 8, HPW = 64 / LPH, U = kMropeTokens / 4;
-  __shared__ float sm_cos[kMropeTokens][D / 2], sm_sin[kMropeTokens][D / 2];
+  __shared__ __attribute__((aligned(16))) float sm_cos[kMropeTokens][D / 2], sm_sin[kMropeTokens][D / 2];
   const int tid = threadIdx.x, lane = tid & 63, sub = lane % LPH;
   const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)(tid >> 6));
   const int32_t heads = a.Hq + 2 * a.Hkv;
-  const int32_t head = (int32_t)blockIdx.y * HPW + lane / LPH;
-  const bool head_ok = head < heads;
-  const bool is_q = head < a.Hq, is_k = !is_q && head < a.Hq + a.Hkv, roped = head < a.Hq + a.Hkv;
   const int64_t tb = (int64_t)blockIdx.x * kMropeTokens, t0 = tb + wave * U;
+  const int32_t g0 = blockIdx.y * a.groups, g1 = min(g0 + a.groups, (heads + HPW - 1) / HPW);
+  const int32_t half = FULL ? D / 2 : a.half;
   uint4 w[U];
+  auto load = [&](int32_t grp) {
+    const int32_t head = grp * HPW + lane / LPH;
 #pragma unroll
-  for (int k = 0; k < U; ++k)
-    w[k] = t0 + k < a.T && head_ok ? ld16_stream(a.qkv + (t0 + k) * a.qkv_stride + (int64_t)head * D + 8 * sub)
-                                   : make_uint4(0, 0, 0, 0);
-  for (int p = tid; p < kMropeTokens * a.half; p += 256) {
-    const int k = p / a.half, i = p - k * a.half;
+    for (int k = 0; k < U; ++k)
+      w[k] = t0 + k < a.T && head < heads ? ld16_stream(a.qkv + (t0 + k) * a.qkv_stride + (int64_t)head * D + 8 * sub)
+                                          : make_uint4(0, 0, 0, 0);
+  };
+  load(g0);
+  int64_t kv_at[U];  // the tokens' elements in a pool of one KV head (redirected as the pool's store redirects)
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int64_t slot = t0 + k < a.T ? redirect_slot(a.slots[t0 + k], a.num_slots) : 0;
+    const int64_t page = slot / a.P;
+    kv_at[k] = (page * a.Hkv * a.P + (slot - page * a.P)) * D + 8 * sub;
+  }
+  for (int p = tid; p < kMropeTokens * half; p += 256) {
+    const int k = p / half, i = p - k * half;
     if (tb + k >= a.T) break;
     const int axis = (int)(a.axes[i >> 5] >> (2 * (i & 31)) & 3);
     const double turns = (double)a.positions[axis * a.pos_stride + tb + k] * ((double)a.inv_freq[i] * 0.15915494309189535);
@@ -76,77 +92,100 @@ __global__ __launch_bounds__(256) void qkv_norm_mrope_store_kernel(MropeArgs a) 
     sm_cos[k][i] = cospif(f);
     sm_sin[k][i] = sinpif(f);
   }
-  float gf[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) gf[e] = 1.0f;
-  if (a.q_norm && head_ok && roped) {
-    const uint4 gw = ld16((is_q ? a.q_norm : a.k_norm) + 8 * sub);
-    const uint32_t gg[4] = {gw.x, gw.y, gw.z, gw.w};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) gf[e] = bf16_bits_to_f32(gg[e / 2] >> (16 * (e & 1)) & 0xffffu);
-  }
-  const int32_t h = head - a.Hq - (is_k ? 0 : a.Hkv);  // the KV head (K and V lanes)
-  float scl = 1.0f, rs = 1.0f;
-  bool rcp_ok = false;
-  if (FP8 && head_ok && !is_q) {
-    scl = is_k ? a.k_scale[h] : a.v_scale[h];
-    rcp_ok = rcp_scale_ok(scl);
-    rs = rcp_ok ? 1.0f / scl : 1.0f;
-  }
-  uint8_t* const cache = is_k ? a.k_cache : a.v_cache;
-  // the rotation partner of the lane's elements, half elements away, and their sign
-  const bool rotated = roped && 8 * sub < 2 * a.half, first = 8 * sub < a.half;
-  const int partner = rotated ? lane + (first ? a.half / 8 : -(a.half / 8)) : lane;
-  const int pair0 = first ? 8 * sub : 8 * sub - a.half;
   __syncthreads();
+  // the rotation partner of the lane's elements, half elements away; the lane's cosines and signed sines
+  const bool rotated = FULL || 8 * sub < 2 * half, first = 8 * sub < half;
+  const int partner = rotated ? lane + (first ? half / 8 : -(half / 8)) : lane;
+  const int pair0 = rotated ? (first ? 8 * sub : 8 * sub - half) : 0;
+  float cs[U][8], sn[U][8];
 #pragma unroll
-  for (int k = 0; k < U; ++k) {
-    const int64_t t = t0 + k;
-    if (t >= a.T) break;  // uniform
-    const uint32_t ww[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-    float x[8], y[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = bf16_bits_to_f32(ww[e / 2] >> (16 * (e & 1)) & 0xffffu);
-    if (a.q_norm) {  // uniform
-      float ss = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-      for (int off = LPH / 2; off > 0; off >>= 1) ss += __shfl_xor(ss, off, 64);
-      const float inv = 1.0f / sqrtf(ss / (float)D + a.eps);
-      if (roped) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * gf[e];
-      }
-    }
+  for (int k = 0; k < U; ++k)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float o = __shfl(x[e], partner, 64);
-      y[e] = x[e];
-      if (rotated) {
-        const float c = sm_cos[t - tb][pair0 + e], s = sm_sin[t - tb][pair0 + e];
-        y[e] = x[e] * c + (first ? -o : o) * s;
+      cs[k][e] = rotated ? sm_cos[wave * U + k][pair0 + e] : 1.0f;
+      const float v = rotated ? sm_sin[wave * U + k][pair0 + e] : 0.0f;
+      sn[k][e] = first ? -v : v;
+    }
+  for (int32_t grp = g0; grp < g1; ++grp) {  // uniform
+    const int32_t head = grp * HPW + lane / LPH;
+    const bool head_ok = head < heads;
+    const bool is_q = head < a.Hq, is_k = !is_q && head < a.Hq + a.Hkv, roped = head < a.Hq + a.Hkv;
+    const int32_t h = head - a.Hq - (is_k ? 0 : a.Hkv);  // the KV head (K and V lanes)
+    uint4 cur[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) cur[k] = w[k];
+    if (grp + 1 < g1) load(grp + 1);
+    float gf[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) gf[e] = 1.0f;
+    if (a.q_norm && head_ok && roped) {
+      const uint4 gw = ld16((is_q ? a.q_norm : a.k_norm) + 8 * sub);
+      const uint32_t gg[4] = {gw.x, gw.y, gw.z, gw.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) gf[e] = bf16_bits_to_f32(gg[e / 2] >> (16 * (e & 1)) & 0xffffu);
+    }
+    float scl = 1.0f, rs = 1.0f;
+    bool rcp_ok = false;
+    if (FP8 && head_ok && !is_q) {
+      scl = is_k ? a.k_scale[h] : a.v_scale[h];
+      rcp_ok = rcp_scale_ok(scl);
+      rs = rcp_ok ? 1.0f / scl : 1.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int64_t t = t0 + k;
+      if (t >= a.T) break;  // uniform
+      const uint32_t ww[4] = {cur[k].x, cur[k].y, cur[k].z, cur[k].w};
+      float x[8], y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = e & 1 ? __uint_as_float(ww[e / 2] & 0xffff0000u) : bf16_bits_to_f32(ww[e / 2]);
+      if (a.q_norm) {  // uniform
+        float ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+        if constexpr (LPH == 16) {
+          ss = row16_sum(ss);
+        } else {
+#pragma unroll
+          for (int off = LPH / 2; off > 0; off >>= 1) ss += __shfl_xor(ss, off, 64);
+        }
+        if (roped) {
+          const float inv = __builtin_amdgcn_rsqf(ss * (1.0f / D) + a.eps);  // (1 ulp)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * gf[e];
+        }
       }
-    }
-    if (!head_ok) continue;
-    const uint4 b16 = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
-                                 pack_bf16x2(y[6], y[7]));
-    if (is_q) {
-      *reinterpret_cast<uint4*>(a.q_out + (t * a.Hq + head) * D + 8 * sub) = b16;
-      continue;
-    }
-    const int64_t slot = redirect_slot(a.slots[t], a.num_slots);
-    const int64_t page = slot / a.P;
-    const int64_t dst = ((page * a.Hkv + h) * a.P + (slot - page * a.P)) * D + 8 * sub;
-    if constexpr (FP8) {
-      *reinterpret_cast<uint2*>(cache + dst) =
-          make_uint2(mrope_fp8_pair(y[0], y[1], scl, rs, rcp_ok) | mrope_fp8_pair(y[2], y[3], scl, rs, rcp_ok) << 16,
-                     mrope_fp8_pair(y[4], y[5], scl, rs, rcp_ok) | mrope_fp8_pair(y[6], y[7], scl, rs, rcp_ok) << 16);
-    } else {
-      *reinterpret_cast<uint4*>(cache + 2 * dst) = b16;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float o;
+        if constexpr (FULL && LPH == 16)
+          o = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x[e]), 0x128, 0xf, 0xf, true));  // row_ror:8
+        else
+          o = __shfl(x[e], partner, 64);
+        y[e] = roped ? fmaf(x[e], cs[k][e], o * sn[k][e]) : x[e];
+      }
+      if (!head_ok) continue;
+      const uint4 b16 = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
+                                   pack_bf16x2(y[6], y[7]));
+      if (is_q) {
+        *reinterpret_cast<uint4*>(a.q_out + (t * a.Hq + head) * D + 8 * sub) = b16;
+        continue;
+      }
+      uint8_t* const cache = is_k ? a.k_cache : a.v_cache;
+      const int64_t dst = kv_at[k] + (int64_t)h * a.P * D;
+      if constexpr (FP8) {
+        *reinterpret_cast<uint2*>(cache + dst) =
+            make_uint2(mrope_fp8_pair(y[0], y[1], scl, rs, rcp_ok) | mrope_fp8_pair(y[2], y[3], scl, rs, rcp_ok) << 16,
+                       mrope_fp8_pair(y[4], y[5], scl, rs, rcp_ok) | mrope_fp8_pair(y[6], y[7], scl, rs, rcp_ok) << 16);
+      } else {
+        *reinterpret_cast<uint4*>(cache + 2 * dst) = b16;
+      }
     }
   }
 }
+
+// Workgroups that a launch is worth: a token block's heads are shared out until there are so many.
+constexpr int64_t kMropeWorkgroups = 1024;
 
 }  // namespace sna
 
@@ -224,11 +263,18 @@ extern "C" int sna_qkv_norm_mrope_store(const void* qkv, int64_t qkv_stride, int
   a.v_scale = v_scale;
   a.num_slots = num_blocks * page_size;
   a.P = page_size;
-  const dim3 grid((unsigned)token_blocks, (unsigned)head_groups);
+  const int64_t parts = std::min(head_groups, (kMropeWorkgroups + token_blocks - 1) / token_blocks);
+  a.groups = (int32_t)((head_groups + parts - 1) / parts);
+  const dim3 grid((unsigned)token_blocks, (unsigned)((head_groups + a.groups - 1) / a.groups));
   const hipStream_t s = (hipStream_t)stream;
-  if (fp8 && head_dim == 128) hipLaunchKernelGGL((qkv_norm_mrope_store_kernel<true, 128>), grid, dim3(256), 0, s, a);
-  else if (fp8) hipLaunchKernelGGL((qkv_norm_mrope_store_kernel<true, 64>), grid, dim3(256), 0, s, a);
-  else if (head_dim == 128) hipLaunchKernelGGL((qkv_norm_mrope_store_kernel<false, 128>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((qkv_norm_mrope_store_kernel<false, 64>), grid, dim3(256), 0, s, a);
+  const bool full = 2 * n_pairs == head_dim;
+#define SNA_MROPE_LAUNCH(F, DD)                                                                                        \
+  if (full) hipLaunchKernelGGL((qkv_norm_mrope_store_kernel<F, DD, true>), grid, dim3(256), 0, s, a);                  \
+  else hipLaunchKernelGGL((qkv_norm_mrope_store_kernel<F, DD, false>), grid, dim3(256), 0, s, a)
+  if (fp8 && head_dim == 128) { SNA_MROPE_LAUNCH(true, 128); }
+  else if (fp8) { SNA_MROPE_LAUNCH(true, 64); }
+  else if (head_dim == 128) { SNA_MROPE_LAUNCH(false, 128); }
+  else { SNA_MROPE_LAUNCH(false, 64); }
+#undef SNA_MROPE_LAUNCH
   return check_launch("qkv_norm_mrope_store");
 }
