@@ -128,17 +128,25 @@ __device__ __forceinline__ void weights_stage(const WeightsArgs& a, int64_t at, 
   }
 }
 
-// The wave's 64 keys through LDS to A operands in registers: lane (g2, i) feeds key 32 s + i, dims 16 c + 8 g2 .. of step c
-// (bf16) or 32 (c / 2) + 16 g2 + 8 (c & 1) .. (FP8, as its 16-byte chunks hold them).
-template <int D, int ESZ>
+// The wave's 64 keys through LDS (STEP at a time) to A operands in registers: lane (g2, i) feeds key 32 s + i, dims 16 c + 8
+// g2 .. of step c (bf16) or 32 (c / 2) + 16 g2 + 8 (c & 1) .. (FP8, as its 16-byte chunks hold them).
+template <int D, int ESZ, int STEP>
 __device__ __forceinline__ void weights_keys(const WeightsArgs& a, int64_t at, uint8_t* lds, uint32_t (&kf)[2][D / 16][4]) {
   using Geo = WeightsGeo<D, ESZ>;
   const int lane = threadIdx.x & 63, g2 = lane >> 5, i32 = lane & 31;
-  weights_stage<D, ESZ, 64>(a, at, lds);
-  wait_vmcnt<0>();
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    const int row = 32 * s + i32;
+    if (STEP == 64 ? s == 0 : true) {
+      int64_t from = at;
+      if constexpr (STEP == 32) {  // keys 32 s .. 32 s + 31, in both halves of the wave
+        const uint32_t lo = __shfl((uint32_t)at, 32 * s + i32, 64), hi = __shfl((uint32_t)(at >> 32), 32 * s + i32, 64);
+        from = (int64_t)((uint64_t)hi << 32 | lo);
+        if (s > 0) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the first ones are read
+      }
+      weights_stage<D, ESZ, STEP>(a, from, lds);
+      wait_vmcnt<0>();
+    }
+    const int row = STEP == 64 ? 32 * s + i32 : i32;
     const uint8_t* mine = lds + row * Geo::ROWB;
     if constexpr (ESZ == 1) {
 #pragma unroll
@@ -221,17 +229,16 @@ enum WeightsPass { kStats, kSum };
 template <int D, int ESZ>
 struct WeightsRing {
   using Geo = WeightsGeo<D, ESZ>;
-  static constexpr int SLOTS = 8;               // row tiles in LDS: one read, the others on their way
+  static constexpr int SLOTS = 4;               // row tiles in LDS: a pair that is read, a pair on its way
   static constexpr int SLOTB = Geo::TILE * 16;  // bytes of a tile
   static constexpr int LD = SLOTB / 4096;       // DMAs of a tile that a wave issues
-  // The keys take the ring's last slots (and, bf16 at D = 128, one slot more) on their way to registers; the EARLY first
-  // tiles are on their way beside them.
-  static constexpr int EARLY = SLOTS * SLOTB - 4 * Geo::KEYB > 0 ? (SLOTS * SLOTB - 4 * Geo::KEYB) / SLOTB : 1;
-  static constexpr int BYTES = EARLY * SLOTB + (4 * Geo::KEYB > (SLOTS - EARLY) * SLOTB ? 4 * Geo::KEYB
-                                                                                       : (SLOTS - EARLY) * SLOTB);
+  // The keys pass through the second pair's slots (and beyond) while the first pair is on its way.
+  static constexpr int STEP = Geo::ROWB > 128 ? 32 : 64;  // keys of a wave at a time: three workgroups fit a CU's LDS
+  static constexpr int STAGE = STEP * Geo::ROWB;
+  static constexpr int BYTES = 2 * SLOTB + (4 * STAGE > 2 * SLOTB ? 4 * STAGE : 2 * SLOTB);
 };
 template <int D, int ESZ, WeightsPass PASS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3)))
 void weights_tile_kernel(WeightsArgs a) {
   using Geo = WeightsGeo<D, ESZ>;
   using Ring = WeightsRing<D, ESZ>;
@@ -311,12 +318,12 @@ void weights_tile_kernel(WeightsArgs a) {
       }
     }
   };
-  const int32_t early = min(tiles, Ring::EARLY);
-  for (int32_t i = 0; i < early; ++i) load(i);
+  load(0);
+  if (tiles > 1) load(1);
   const int64_t at = weights_key_at(a, r, g, k0 + tid, rq.n, Geo::ROWB);
   const uint64_t valid = __ballot(at >= 0);
   uint32_t kf[2][NS][4];
-  weights_keys<D, ESZ>(a, at, sm + Ring::EARLY * Ring::SLOTB + wave * Geo::KEYB, kf);
+  weights_keys<D, ESZ, Ring::STEP>(a, at, sm + 2 * Ring::SLOTB + wave * Ring::STAGE, kf);
   const float c2 = weights_scale<ESZ>(a, g);
   const int32_t kw = k0 + 64 * wave;  // the wave's first key
   float acc[2][16];
@@ -353,67 +360,67 @@ void weights_tile_kernel(WeightsArgs a) {
       part[m] = weights_join(weights_join(p[0][i32], p[1][i32]), weights_join(p[2][i32], p[3][i32]));
     }
   };
-  float2 rw[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};  // the rows' (largest, 1 / sum) of two tiles
-  f32x16_t x[2][2];                                                   // and their scores
-  // The products of tile i, to x[i & 1] (past the last tile: of stale rows, dropped).
-  auto products = [&](int32_t i, int b) {
+  float2 rw = make_float2(0.0f, 0.0f);  // the lane's row's (largest, 1 / sum) of a tile
+  f32x16_t x[2];                        // and its scores
+  // The products of tile i (past the last tile: of stale rows, dropped).
+  auto products = [&](int32_t i) {
     const uint4* const slot = reinterpret_cast<const uint4*>(sm + (i & (SLOTS - 1)) * Ring::SLOTB);
-    if (PASS == kSum) rw[b] = sm_row[i & (SLOTS - 1)][i32];
-    x[b][0] = x[b][1] = f32x16_t{};
+    if (PASS == kSum) rw = sm_row[i & (SLOTS - 1)][i32];
+    x[0] = x[1] = f32x16_t{};
 #pragma unroll
     for (int c = 0; c < NS; ++c) {
       const uint4 w = slot[i32 * CH + (weights_chunk<ESZ>(c, g2) ^ Geo::swz(i32, CH))];
       const uint32_t qf[4] = {w.x, w.y, w.z, w.w};
-      x[b][0] = mfma_32x32x16_bf16(kf[0][c], qf, x[b][0]);
-      x[b][1] = mfma_32x32x16_bf16(kf[1][c], qf, x[b][1]);
+      x[0] = mfma_32x32x16_bf16(kf[0][c], qf, x[0]);
+      x[1] = mfma_32x32x16_bf16(kf[1][c], qf, x[1]);
     }
   };
   // Tile i's scores, all of them seen, or those that weights_seen says.
-  auto work = [&](auto all, int32_t i, int b) {
+  auto work = [&](auto all, int32_t i) {
     constexpr bool ALL = decltype(all)::value;
     const int32_t m = m0 + kWeightRows * i + i32;
     const uint64_t seen = ALL || m >= m_end ? 0 : weights_seen(a, valid, rq.prior + token_of(m), kw);
     if constexpr (PASS == kStats) {
-      const float2 p = weights_stats<ALL>(x[b], c2, seen, g2);
+      const float2 p = weights_stats<ALL>(x, c2, seen, g2);
       if (g2 == 0) sm_part[i & 3][wave][i32] = p;
     } else {
-      const float inv = ALL || m < m_end ? rw[b].y : 0.0f;  // (past the last tile it is stale)
+      const float inv = ALL || m < m_end ? rw.y : 0.0f;  // (past the last tile it is stale)
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const uint32_t bits = weights_bits(seen, s, g2);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(x[b][s][e], c2, -rw[b].x));
+          const float p = __builtin_amdgcn_exp2f(fmaf(x[s][e], c2, -rw.x));
           acc[s][e] = fmaf(ALL || bits & weights_bit(e) ? p : 0.0f, inv, acc[s][e]);
         }
       }
+      // (here, not after the next tile's products: or both tiles' scores would be held)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) asm volatile("" : "+v"(acc[s][e]));
     }
   };
-  // Before a pair of tiles, 2 p and 2 p + 1: tiles 2 p + 1 and 2 p + 2 are in their slots once this wave's DMAs and the
-  // others' are (the SLOTS - 4 later tiles may be on their way); the barrier also says that tile 2 p and those before, whose
-  // slots the next ones take, are read.
+  // Before a pair of tiles, 2 p and 2 p + 1: they are in their slots once this wave's DMAs and the others' are; the barrier
+  // also says that the pair before, whose slots the next pair takes, is read (and, at first, every wave's keys are).
   auto ready = [&](int32_t p) {
-    if (2 * p + SLOTS - 2 < tiles) wait_vmcnt<(SLOTS - 4) * DMAS>();
-    else wait_vmcnt<0>();
+    wait_vmcnt<0>();
     __syncthreads();
-    if (2 * p + SLOTS - 1 < tiles) load(2 * p + SLOTS - 1);
-    if (2 * p + SLOTS < tiles) load(2 * p + SLOTS);
+    if (2 * p + 2 < tiles) load(2 * p + 2);
+    if (2 * p + 3 < tiles) load(2 * p + 3);
     if (PASS == kStats && p > 0) {
       write_part(2 * p - 2);
       write_part(2 * p - 1);
     }
   };
-  // Each tile's scores are worked on while the next one's products run.
   auto pair = [&](auto all, int32_t p) {
     ready(p);
-    products(2 * p + 1, 1);
-    work(all, 2 * p, 0);
-    products(2 * p + 2, 0);
-    work(all, 2 * p + 1, 1);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      products(2 * p + b);
+      work(all, 2 * p + b);
+    }
   };
-  __syncthreads();  // every wave has its keys (and, with them, its early tiles): the other tiles take their place
-  for (int32_t i = early; i < min(tiles, SLOTS - 1); ++i) load(i);
-  if (unseen == 0) products(0, 0);
   int32_t p = 0;
   for (; p < unseen; ++p) {
     ready(p);
@@ -421,7 +428,6 @@ void weights_tile_kernel(WeightsArgs a) {
       const float2 none = make_float2(kNegBig, 0.0f);
       sm_part[2 * p & 3][wave][i32] = sm_part[(2 * p + 1) & 3][wave][i32] = none;
     }
-    if (p + 1 == unseen) products(2 * p + 2, 0);
   }
   for (; p < min(f0, pairs); ++p) pair(std::false_type{}, p);
   for (; p < f1; ++p) pair(std::true_type{}, p);
