@@ -471,8 +471,9 @@ int sna_prefill_attention_split(const void *q, const void *k_cache, const void *
  *   weights   [R, num_kv_heads, width] fp32, strides row_stride and head_stride (at least width). accumulate != 0: the
  *             requests' keys (valid ones below width) are added to, the rest is left as it is; 0: every column is
  *             written, zero where there is no key.
- *   workspace device, 16-byte aligned, at least sna_attention_weights_workspace_bytes bytes, any contents; calls that
- *             share one on different streams race.
+ *   workspace device, 16-byte aligned, at least sna_attention_weights_workspace_bytes bytes for the call's own
+ *             sizes (a smaller batch can need more than a larger one), any contents; calls that share one on different
+ *             streams race.
  * Every sum runs in a fixed order: the same call gives the same bits. The queries' rows of q lie inside [0, n_tokens);
  * offsets outside are cut. head_dim 64 or 128, any page size, num_q_heads / num_kv_heads <= 128.
  * This has no reference counterpart. */

@@ -622,6 +622,11 @@ __global__ __launch_bounds__(256) void weights_score_kernel(WeightsArgs a) {
         weights_join(weights_join(sm_part[0][tid], sm_part[1][tid]), weights_join(sm_part[2][tid], sm_part[3][tid]));
 }
 
+// A score's probability by its row's (largest, 1 / sum): none for an unseen one, whatever the row's sum is.
+__device__ __forceinline__ float weights_p(float x, float2 row) {
+  return x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - row.x) * row.y;
+}
+
 // 1024 keys a workgroup, 4 to a thread: the rows' blocks merged (16 threads a row), then every key's probabilities summed.
 __global__ __launch_bounds__(256) void weights_from_scores_kernel(WeightsArgs a) {
   __shared__ float2 sm[16][kScoreRows], sm_row[kScoreRows];
@@ -666,10 +671,10 @@ __global__ __launch_bounds__(256) void weights_from_scores_kernel(WeightsArgs a)
     for (int32_t m = 0; m < M; ++m) {
       const float4 x = *reinterpret_cast<const float4*>(src + m * width);
       const float2 rw = sm_row[m];
-      w.x = fmaf(__builtin_amdgcn_exp2f(x.x - rw.x), rw.y, w.x);
-      w.y = fmaf(__builtin_amdgcn_exp2f(x.y - rw.x), rw.y, w.y);
-      w.z = fmaf(__builtin_amdgcn_exp2f(x.z - rw.x), rw.y, w.z);
-      w.w = fmaf(__builtin_amdgcn_exp2f(x.w - rw.x), rw.y, w.w);
+      w.x += weights_p(x.x, rw);
+      w.y += weights_p(x.y, rw);
+      w.z += weights_p(x.z, rw);
+      w.w += weights_p(x.w, rw);
     }
   }
   const float v[4] = {w.x, w.y, w.z, w.w};
@@ -678,6 +683,168 @@ __global__ __launch_bounds__(256) void weights_from_scores_kernel(WeightsArgs a)
     if (key + e >= a.width) break;
     if (!a.add) out[key + e] = v[e];
     else if (key + e < rq.n) out[key + e] += v[e];
+  }
+}
+
+// Few rows whose scores fit LDS (FLOATS of them, with the row's page ids): one workgroup of 16 waves reads all of a (request,
+// KV head)'s keys, straight to registers, 64 (or 32) to a wave at a time and the next ones on their way, keeps the scores in
+// LDS, and turns them into the keys' weights there: one launch, every key read once and nothing else but the weights moved.
+// Lanes as in weights_score_kernel.
+constexpr int kRowThreads = 1024;
+constexpr int kRowPad = 16;  // floats between two rows of scores, on top of their keys: 16 banks apart
+template <int D, int ESZ, int FLOATS>
+__global__ __launch_bounds__(kRowThreads) void weights_row_kernel(WeightsArgs a) {
+  using Geo = WeightsGeo<D, ESZ>;
+  constexpr int NS = D / 32, CK = score_chunk(Geo::ROWB), NT = CK / 16, NL = Geo::KCH / 4, WAVES = kRowThreads / 64;
+  __shared__ __attribute__((aligned(16))) float sm[FLOATS];
+  __shared__ float sm_wave[WAVES][kScoreRows];
+  __shared__ float2 sm_row[kScoreRows];
+  const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, i16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int32_t r = (int32_t)(blockIdx.x / a.G), g = (int32_t)(blockIdx.x % a.G);
+  const WeightsRequest rq = weights_request(a, r);
+  const int32_t M = rq.S * a.group, rows = a.max_q * a.group;
+  float* const out = a.weights + r * a.w_row + g * a.w_head;
+  // keys [lo, n): from the 64 that hold the first one that any row sees
+  const int32_t lo = a.window > 0 ? (int32_t)min(max(rq.prior - a.window + 1, (int64_t)0), (int64_t)rq.n) & ~63 : 0;
+  if (M == 0 || rq.n <= lo) {  // uniform
+    if (!a.add)
+      for (int32_t k = tid; k < a.width; k += kRowThreads) out[k] = 0.0f;
+    return;
+  }
+  const int32_t cols = (rq.n - lo + 63) & ~63;
+  float* const score = sm;  // [rows, pitch]
+  const int32_t pitch = a.score_keys + kRowPad;
+  int32_t* const page_of = reinterpret_cast<int32_t*>(sm + rows * pitch);  // of the pages from lo's on, -1 where invalid
+  const int32_t c0 = lo / a.P;
+  for (int32_t c = tid; c <= (rq.n - 1) / a.P - c0; c += kRowThreads) {
+    const int32_t page = a.table[r * a.table_stride + c0 + c];
+    page_of[c] = page >= 0 && page < a.num_blocks ? page : -1;
+  }
+  const int32_t m = i16, t = m / a.group, j = m - t * a.group;
+  const uint16_t* const row = a.q + ((int64_t)(rq.qa + min(t, rq.S - 1)) * a.H + g * a.group + j) * D;
+  uint32_t qf[NS][4];
+#pragma unroll
+  for (int c = 0; c < NS; ++c) {
+    const uint4 w = ld16(row + 8 * (ESZ == 1 ? 8 * (c / 2) + 2 * g4 + (c & 1) : 4 * c + g4));
+    qf[c][0] = w.x, qf[c][1] = w.y, qf[c][2] = w.z, qf[c][3] = w.w;
+  }
+  const float c2 = weights_scale<ESZ>(a, g);
+  const uint64_t p_magic = ((1ull << 32) + a.P - 1) / a.P;  // key / P = key * magic >> 32: keys * P < 2^32 here
+  __syncthreads();
+  // (One copy of each step's code, none unrolled over the rows: a launch this short pays for every line of code it fetches.)
+  uint4 cur[NT][NL], next[NT][NL];
+  uint64_t valid = 0, valid_next = 0;
+  float best = kNegBig;
+  const int32_t end = lo + cols;
+  for (int32_t kw = lo + (wave - WAVES) * CK; kw < end; kw += WAVES * CK) {  // (the first round only loads)
+    const int32_t ahead = kw + WAVES * CK;
+    if (ahead < end) {  // uniform: the wave's next keys to registers, and which of them are there
+      valid_next = 0;
+#pragma unroll
+      for (int s = 0; s < NT; ++s) {
+        const int32_t key = ahead + 16 * s + i16;
+        const int32_t col = (int32_t)((uint32_t)key * p_magic >> 32);
+        const int32_t page = key < rq.n ? page_of[col - c0] : -1;
+        valid_next |= (uint64_t)(__ballot(page >= 0) & 0xffff) << 16 * s;
+        // (a key that is not there reads the cache's first row: masked)
+        const int64_t at = page < 0 ? 0 : (((int64_t)page * a.G + g) * a.P + (key - col * a.P)) * (int64_t)Geo::ROWB;
+#pragma unroll
+        for (int c = 0; c < NL; ++c) next[s][c] = ld16_stream(a.k_cache + at + 16 * (4 * c + g4));
+      }
+    }
+    if (kw >= lo) {
+      constexpr uint64_t kAll = CK == 64 ? ~0ull : (1ull << CK % 64) - 1;
+      const bool all = valid == kAll && rq.prior >= kw + CK - 1 && (a.window <= 0 || rq.prior + rq.S - 1 - a.window < kw);  // uniform
+      const uint64_t seen = all ? ~0ull : weights_seen(a, valid, rq.prior + t, kw) >> 4 * g4;
+#pragma unroll
+      for (int s = 0; s < NT; ++s) {
+        f32x4_t x = {};
+#pragma unroll
+        for (int c = 0; c < NL; ++c) {
+          const uint4 w = cur[s][c];
+          if constexpr (ESZ == 1) {
+            uint32_t ka[4], kb[4];
+            fp8x4_to_bf16x4(w.x, ka[0], ka[1]);
+            fp8x4_to_bf16x4(w.y, ka[2], ka[3]);
+            fp8x4_to_bf16x4(w.z, kb[0], kb[1]);
+            fp8x4_to_bf16x4(w.w, kb[2], kb[3]);
+            x = mfma_16x16x32_bf16(ka, qf[2 * c], x);
+            x = mfma_16x16x32_bf16(kb, qf[2 * c + 1], x);
+          } else {
+            const uint32_t ka[4] = {w.x, w.y, w.z, w.w};
+            x = mfma_16x16x32_bf16(ka, qf[c], x);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = seen >> (16 * s + e) & 1 ? x[e] * c2 : -INFINITY;
+          best = fmaxf(best, x[e]);
+        }
+        if (m < M) *reinterpret_cast<f32x4_t*>(score + m * pitch + (kw - lo) + 16 * s + 4 * g4) = x;
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < NT; ++s)
+#pragma unroll
+      for (int c = 0; c < NL; ++c) cur[s][c] = next[s][c];
+    valid = valid_next;
+  }
+  best = max_across_groups(best);
+  if (g4 == 0) sm_wave[wave][m] = best;
+  __syncthreads();
+  if (tid < M) {  // the rows' largest, and their sinks' share of the sum
+    const float sink = a.sinks ? a.sinks[g * a.group + tid % a.group] * kLog2e : -INFINITY;
+    float v = a.sinks ? sink : kNegBig;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) v = fmaxf(v, sm_wave[w][tid]);
+    sm_row[tid] = make_float2(v, __builtin_amdgcn_exp2f(sink - v));
+  }
+  __syncthreads();
+  // Exponentials in place, four keys a thread, and the rows' sums.
+#pragma unroll 1
+  for (int i = 0; i < M; ++i) {
+    const float top = sm_row[i].x;
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int32_t c = 4 * tid; c < cols; c += 4 * kRowThreads) {
+      float4* const at = reinterpret_cast<float4*>(score + i * pitch + c);
+      float4 x = *at;
+      x.x = __builtin_amdgcn_exp2f(x.x - top), x.y = __builtin_amdgcn_exp2f(x.y - top);
+      x.z = __builtin_amdgcn_exp2f(x.z - top), x.w = __builtin_amdgcn_exp2f(x.w - top);
+      *at = x;
+      sum += (x.x + x.y) + (x.z + x.w);
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) sm_wave[wave][i] = sum;
+  }
+  __syncthreads();
+  if (tid < M) {
+    float v = sm_row[tid].y;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) v += sm_wave[w][tid];
+    sm_row[tid].y = v == 0.0f ? 0.0f : 1.0f / v;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int32_t c = 4 * tid; c < cols; c += 4 * kRowThreads) {
+    float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+    for (int i = 0; i < M; ++i) {
+      const float4 x = *reinterpret_cast<const float4*>(score + i * pitch + c);
+      const float inv = sm_row[i].y;
+      // (an exponential of 0 adds nothing, whatever the row's sum is: an unseen key's)
+      w[0] += x.x == 0.0f ? 0.0f : x.x * inv, w[1] += x.y == 0.0f ? 0.0f : x.y * inv;
+      w[2] += x.z == 0.0f ? 0.0f : x.z * inv, w[3] += x.w == 0.0f ? 0.0f : x.w * inv;
+    }
+    const int32_t key = lo + c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (key + e < min(rq.n, a.width)) out[key + e] = a.add ? out[key + e] + w[e] : w[e];
+  }
+  if (!a.add) {
+    for (int32_t k = tid; k < min(lo, a.width); k += kRowThreads) out[k] = 0.0f;
+    for (int32_t k = rq.n + tid; k < a.width; k += kRowThreads) out[k] = 0.0f;
   }
 }
 
@@ -700,7 +867,15 @@ struct WeightsPlan {
   int64_t blocks, part, rest, bytes;
   int32_t splits, split_tokens, span, score_keys;
   bool scores;
+  int32_t row_floats;  // the LDS of weights_row_kernel where that serves, else 0
 };
+// weights_row_kernel serves where the scores fit LDS, the (request, KV head) pairs leave at most a quarter of its
+// workgroups' places on the chip empty, and the tables are long enough that a workgroup of 16 waves is worth starting.
+// Against two launches (us, heads 32/8 of 128, e4m3fn, all keys full): 256 pairs of 2048 keys 21.8 : 24.5, 512 of 8192
+// 132 : 156, 256 of 4096 with heads 8/1 of 64 21 : 29; without these bounds 264 pairs of 4096 would take 60 : 46 (the last
+// 8 a second turn), 1024 of 100 to 1024 bf16 keys 58 : 47 and 64 of 2048 13 : 9 (a CU alone reads 256 KB in 8 us).
+constexpr int64_t kRowPairs = 256, kRowKeys = 2048;  // the CUs, and the least keys of a table
+constexpr int32_t kRowFloats[2] = {18432, 36864};    // LDS of two workgroups a CU, or one
 constexpr int64_t kScoreWorkgroups = 1024;  // a score launch's chunks are taken several to a workgroup from so many on
 constexpr int64_t kSplitRows = 2048;       // least rows of a run of queries
 constexpr int64_t kSplitWorkgroups = 4096; // runs are cut up to so many workgroups
@@ -708,6 +883,20 @@ WeightsPlan weights_plan(int64_t T, int64_t R, int64_t max_q, int32_t H, int32_t
                          int32_t table_width, int32_t width, int32_t head_dim, int32_t esz) {
   WeightsPlan p;
   p.score_keys = 0;
+  p.row_floats = 0;
+  p.splits = 1, p.split_tokens = (int32_t)max_q;
+  const int64_t table_keys = ((int64_t)table_width * page_size + 63) / 64 * 64;
+  const int64_t floats = max_q * (H / G) * (table_keys + kRowPad) + table_width, pairs = R * G;
+  if (max_q * (H / G) <= kScoreRows && floats <= kRowFloats[1] && table_keys >= kRowKeys) {
+    const bool half = floats <= kRowFloats[0];
+    const int64_t slots = half ? 2 * kRowPairs : kRowPairs, turns = (pairs + slots - 1) / slots;
+    if (pairs >= kRowPairs && (turns == 1 || 4 * pairs >= 3 * turns * slots)) {
+      p.row_floats = kRowFloats[half ? 0 : 1];
+      p.blocks = 1, p.span = 1, p.part = p.rest = p.bytes = 0, p.scores = false;
+      p.score_keys = (int32_t)table_keys;
+      return p;
+    }
+  }
   p.blocks = weights_blocks(page_size, table_width, width, kWeightKeys);
   p.span = 1;
   const int64_t rows = max_q * (H / G);
@@ -741,7 +930,14 @@ WeightsPlan weights_plan(int64_t T, int64_t R, int64_t max_q, int32_t H, int32_t
 }
 
 template <int D, int ESZ>
-void launch_weights(const WeightsArgs& a, uint32_t wgs, hipStream_t s) {
+void launch_weights(const WeightsArgs& a, uint32_t wgs, int32_t row_floats, hipStream_t s) {
+  if (row_floats > 0) {
+    if (row_floats == kRowFloats[0])
+      hipLaunchKernelGGL((weights_row_kernel<D, ESZ, kRowFloats[0]>), dim3(a.R * a.G), dim3(kRowThreads), 0, s, a);
+    else
+      hipLaunchKernelGGL((weights_row_kernel<D, ESZ, kRowFloats[1]>), dim3(a.R * a.G), dim3(kRowThreads), 0, s, a);
+    return;
+  }
   if (a.ws_score) {
     hipLaunchKernelGGL((weights_score_kernel<D, ESZ>), dim3(wgs), dim3(256), 0, s, a);
     const int64_t cols = a.add ? (int64_t)a.blocks * a.score_keys : a.width;  // (every column is written, or the keys')
@@ -775,7 +971,7 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
   if (group > 128) return fail(SNA_ERR_UNSUPPORTED, "%s: %d query heads per KV head (at most 128)", what, group);
   if (kv_dtype != SNA_DTYPE_FP8_E4M3FN && kv_dtype != SNA_DTYPE_FP8_E4M3FN_MUL && kv_dtype != SNA_DTYPE_BF16)
     return fail(SNA_ERR_UNSUPPORTED, "%s: KV dtype %d (FP8 e4m3fn or bf16)", what, kv_dtype);
-  if ((int64_t)table_width * page_size > INT32_MAX - kWeightKeys || width > INT32_MAX - kWeightKeys)
+  if ((int64_t)table_width * page_size > INT32_MAX - (1 << 16) || width > INT32_MAX - (1 << 16))
     return fail(SNA_ERR_UNSUPPORTED, "%s: a table of %d pages of %d, a width of %d (under 2^31 keys)", what, table_width,
                 page_size, width);
   if (R == 0 || width == 0) return SNA_OK;
@@ -798,7 +994,7 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
                                         head_dim, kv_dtype == SNA_DTYPE_BF16 ? 2 : 1);
   const int64_t blocks = plan.blocks;
   const int64_t wgs = blocks * R * num_kv_heads * plan.splits;
-  if (wgs > kGridMax)
+  if (wgs > kGridMax / 4)
     return fail(SNA_ERR_UNSUPPORTED, "%s: %lld key blocks x %d requests x %d KV heads exceed the grid (split the batch)",
                 what, (long long)blocks, R, num_kv_heads);
   const int64_t need = plan.bytes;
@@ -844,9 +1040,9 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
   a.ws_score = plan.scores ? (float*)((uint8_t*)workspace + plan.part) : nullptr;
   const hipStream_t s = (hipStream_t)stream;
   if (kv_dtype != SNA_DTYPE_BF16) {
-    if (head_dim == 128) launch_weights<128, 1>(a, (uint32_t)wgs, s); else launch_weights<64, 1>(a, (uint32_t)wgs, s);
+    if (head_dim == 128) launch_weights<128, 1>(a, (uint32_t)wgs, plan.row_floats, s); else launch_weights<64, 1>(a, (uint32_t)wgs, plan.row_floats, s);
   } else {
-    if (head_dim == 128) launch_weights<128, 2>(a, (uint32_t)wgs, s); else launch_weights<64, 2>(a, (uint32_t)wgs, s);
+    if (head_dim == 128) launch_weights<128, 2>(a, (uint32_t)wgs, plan.row_floats, s); else launch_weights<64, 2>(a, (uint32_t)wgs, plan.row_floats, s);
   }
   return check_launch(what);
 }

@@ -16,7 +16,7 @@ import pytest
 import torch
 
 from oracle import weights as ow
-from sglang_neuron_amd import ops
+from sglang_neuron_amd import _lib, ops
 from sglang_neuron_amd.attention import NeuronAttnBackend
 from sglang_neuron_amd.mem_cache import NeuronMHATokenToKVPool
 from tests.conftest import announce
@@ -144,6 +144,106 @@ def test_decode_weights(H, G, d, P, lens, fp8, window, sinks):
     got = ops.decode_attention_weights(*args, **kw)
     check(c, got, want, reach, "decode")
     assert torch.equal(got, ops.decode_attention_weights(*args, **kw))
+
+
+def few_rows(R, H, G, d, P, most, queries, fp8, holes=0, seed=0, table_width=None):
+    """R requests of 0 to ``most`` keys (the first has them all) and up to ``queries`` queries each."""
+    g = torch.Generator().manual_seed(seed + R + d + P)
+    counts = [min(queries, 1 + int(x)) for x in torch.randint(0, queries, (R,), generator=g)]
+    lens = [most] + [max(c, int(x)) for c, x in zip(counts[1:], torch.randint(1, most // 4, (R - 1,), generator=g))]
+    counts[-1] = 0
+    c = make(seed + R + P, H, G, d, P, lens, counts, fp8, holes=holes)
+    if table_width:
+        wide = torch.full((R, table_width), -1, dtype=torch.int32)
+        wide[:, :c.table.shape[1]] = c.table
+        c.table = wide
+    return c
+
+
+# Few query rows a request, in the forms that their number, the tables' width and the batch choose between.
+@pytest.mark.parametrize("R,H,G,d,P,most,queries,fp8,window,sinks,holes,table_width", [
+    (130, 4, 2, 64, 16, 2100, 1, True, 0, False, 0, None),    # a row's scores in LDS: two workgroups a CU
+    (64, 8, 4, 128, 7, 2060, 3, False, 0, True, 20, None),    # the same, odd pages
+    (64, 16, 4, 64, 48, 2200, 3, False, 300, True, 20, None), # one workgroup a CU
+    (128, 32, 2, 128, 32, 2050, 1, True, 70, False, 5, None),
+    (40, 56, 8, 64, 1, 2080, 2, True, 0, True, 0, None),      # pages of one token
+    (512, 4, 2, 64, 16, 2111, 2, False, 2000, False, 9, None),  # two turns of workgroups
+    (160, 16, 8, 64, 16, 900, 2, False, 0, False, 9, None),   # several chunks a workgroup, scores through memory
+    (160, 16, 8, 128, 16, 700, 1, True, 200, True, 9, None),
+    (3, 16, 2, 128, 16, 2500, 2, False, 0, True, 3, 4000),    # tables much wider than the keys
+    (4, 64, 8, 64, 16, 700, 2, True, 0, False, 3, 17000),     # scores past the workspace's bound: computed twice
+])
+def test_few_rows(R, H, G, d, P, most, queries, fp8, window, sinks, holes, table_width):
+    announce(f"few rows {R} {H} {G} {d} {P} {most} {queries} {fp8}")
+    c = few_rows(R, H, G, d, P, most, queries, fp8, holes, table_width=table_width)
+    sk = torch.randn(H, generator=torch.Generator().manual_seed(5)) if sinks else None
+    sg = None if sk is None else sk.to(DEV)
+    keys, full = max(c.lens), c.table.shape[1] * P
+    want, reach = oracle(c, full, sinks=sk, window=window)
+    got = prefill(c, sinks=sg, window=window)
+    check(c, got, want, reach, "written")
+    assert got.shape[2] == full and bool((got[want.to(DEV) == 0] == 0).all())
+    assert torch.equal(got, prefill(c, sinks=sg, window=window, host=False))
+    rel = 2 * (d + 8) * 2.0 ** -24 * reach + (128 + -(-keys // 256) + max(c.counts) * H // G) * 2.0 ** -24
+    for width in (keys + 99, keys - 30):  # added to: wider than the keys, and narrower
+        base = torch.full((R, G + 1, width + 5), -2.0, device=DEV)
+        w = base[:, :G, 3:3 + width]
+        w.fill_(3.0)
+        prefill(c, sinks=sg, window=window, weights=w)
+        part = torch.zeros(R, G, width, dtype=torch.float64)
+        part[..., :min(width, full)] = want[..., :width]
+        # (adding rounds once more: half a step of at most 3 + W)
+        assert bool(((w.double().cpu() - (part + 3)).abs() <= part * rel + (part + 3) * 2.0 ** -24).all())
+        rest = torch.arange(width, device=DEV) >= torch.tensor(c.lens, device=DEV)[:, None]
+        assert bool((w[rest[:, None].expand(R, G, width)] == 3).all())
+        assert bool((base[:, G] == -2).all() and (base[..., :3] == -2).all() and (base[..., 3 + width:] == -2).all())
+
+
+@pytest.mark.parametrize("R,H,G,counts", [(64, 8, 4, 1), (3, 8, 4, 1), (3, 8, 4, 40)])
+@pytest.mark.parametrize("width", [2500, 1900])
+def test_written_widths_at_the_c_entry(R, H, G, counts, width):
+    """The C entry writes any number of columns: fewer than the table's keys, or more."""
+    c = few_rows(R, H, G, 64, 16, 2070, counts, False, seed=8)
+    q, k, table = c.q.to(DEV), c.k.to(DEV), c.table.to(DEV)
+    start, prior = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (c.start, c.prior))
+    out = torch.full((R, G, width + 3), -2.0, device=DEV)
+    lib = _lib.load()
+    sizes = (len(q), R, max(c.counts))
+    need = lib.sna_attention_weights_workspace_bytes(*sizes, H, G, 64, 16, table.shape[1], width, _lib.DTYPE_BF16)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    rc = lib.sna_prefill_attention_weights(
+        q.data_ptr(), k.data_ptr(), None, table.data_ptr(), table.shape[1], table.shape[1], start.data_ptr(),
+        prior.data_ptr(), *sizes, None, c.scale, 0, out.data_ptr(), G * (width + 3), width + 3, width, 0, H, G, 64, 16,
+        k.shape[0], _lib.DTYPE_BF16, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    want, reach = oracle(c, width)
+    check(c, out[..., :width], want, reach, "written")
+    assert bool((out[..., width:] == -2).all())
+
+
+def test_few_rows_bad_pages_and_nan():
+    """The kernel that keeps a row's scores in LDS: pages past the pool, rows that see nothing, a NaN of a visible key."""
+    c = few_rows(64, 8, 4, 64, 16, 2100, 1, False, seed=3)
+    c.table[1, 0], c.table[2] = 10 ** 6, -1
+    c.lens[3] = c.prior[3] = 0
+    lens = torch.tensor(c.lens, dtype=torch.int32, device=DEV)
+    c.counts = [1] * 64
+    c.start = list(range(65))
+    g = torch.Generator().manual_seed(6)
+    c.q = torch.randn(64, 8, 64, generator=g).to(torch.bfloat16)
+    c.prior = [n - 1 for n in c.lens]
+    want, reach = oracle(c, c.table.shape[1] * 16)
+    want[3] = 0
+    args = (c.q.to(DEV), c.k.to(DEV), c.table.to(DEV), lens)
+    got = ops.decode_attention_weights(*args, sm_scale=c.scale)
+    check(c, got, want, reach, "bad pages")
+    assert bool((got[2:4] == 0).all())
+    args[1][int(c.table[0, 5]), 1, 3] = float("nan")
+    got = ops.decode_attention_weights(*args, sm_scale=c.scale).cpu()
+    assert bool(got[0, 1, :2100].isnan().all()) and bool((got[0, 1, 2100:] == 0).all())
+    got[0, 1] = 0
+    want[0, 1] = 0
+    check(c, got, want, reach, "beside a NaN")
 
 
 def test_decode_rows_without_keys():

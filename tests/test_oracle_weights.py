@@ -103,6 +103,8 @@ def _weights_call(fn="sna_prefill_attention_weights", **kw):
 def test_weights_refusals(fn, bad, code):
     if fn.endswith("decode_attention_weights") and "T" in bad:
         pytest.skip("a decode step has one token a row")
+    if code == -2:  # (a table that is too wide for the launch that needs no workspace)
+        bad = bad | dict(tw=4096, ts=4096)
     assert _weights_call(fn, **bad) == code, _lib.last_error()
 
 
