@@ -529,6 +529,16 @@ int sna_compact_tokens(void *k_cache, void *v_cache, int64_t num_blocks, int32_t
                        int32_t table_width, const int32_t *dst_table, int64_t dst_stride, int32_t dst_width,
                        const int32_t *kept, int32_t R, int32_t keep, void *stream);
 
+/* sna_select_tokens and then sna_compact_tokens on what it kept, by their arguments: nothing is launched, and so no weight
+ * rewritten, unless both accept them. */
+int sna_evict_tokens(void *k_cache, void *v_cache, int64_t num_blocks, int32_t num_kv_heads, int32_t page_size,
+                     int32_t head_dim, int32_t cache_dtype, const int32_t *block_table, int64_t table_stride,
+                     int32_t table_width, const int32_t *dst_table, int64_t dst_stride, int32_t dst_width,
+                     const float *weights, int64_t row_stride, int64_t head_stride, int32_t width,
+                     const int32_t *seq_lens, int32_t R, int32_t keep, int32_t first, int32_t recent, int32_t *kept,
+                     int32_t *new_lens, float *weights_out, int64_t out_row_stride, int64_t out_head_stride,
+                     int32_t out_width, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* =====================================================================================================
  * DSA indexer (the step that picks the sparse decode's positions)
  * ===================================================================================================== */

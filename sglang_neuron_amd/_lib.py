@@ -106,6 +106,8 @@ SIGNATURES = {
                                  _P, _I64, _P]),
     "sna_compact_tokens": (_I32, [_P, _P, _I64, _I32, _I32, _I32, _I32, _P, _I64, _I32, _P, _I64, _I32, _P, _I32, _I32,
                                   _P]),
+    "sna_evict_tokens": (_I32, [_P, _P, _I64, _I32, _I32, _I32, _I32, _P, _I64, _I32, _P, _I64, _I32, _P, _I64, _I64, _I32,
+                                _P, _I32, _I32, _I32, _I32, _P, _P, _P, _I64, _I64, _I32, _P, _I64, _P]),
     "sna_index_key_store": (_I32, [_P, _P, _I64, _I32, _P, _I64, _P]),
     "sna_indexer_scores": (_I32, [_P, _P, _P, _P, _I64, _I32, _P, _I32, _I32, _I32, _I32, _I64, _I32, _P, _I64, _P]),
     "sna_page_items_wire_bytes": (_I64, [_P, _I32, _I64]),

@@ -422,38 +422,61 @@ extern "C" int64_t sna_select_workspace_bytes(int32_t R, int32_t num_kv_heads, i
   return select_bytes((int64_t)R * num_kv_heads, width, keep, in_place != 0);
 }
 
-extern "C" int sna_select_tokens(const float* weights, int64_t row_stride, int64_t head_stride, int32_t width,
-                                 const int32_t* seq_lens, int32_t R, int32_t num_kv_heads, int32_t keep, int32_t first,
-                                 int32_t recent, int32_t* kept, int32_t* new_lens, float* weights_out,
-                                 int64_t out_row_stride, int64_t out_head_stride, int32_t out_width, void* workspace,
-                                 int64_t workspace_bytes, void* stream) {
-  ApiGuard guard;
+namespace {
+
+// Both operators' arguments are checked, and their launches laid out, before either is launched.
+struct SelectLaunch {
+  SelectArgs a;
+  SelectLong b;
+  void run(hipStream_t s) const {
+    const dim3 block(kSelectThreads), grid(a.G, a.R);
+    if (a.width <= kSelectSegment / 4) {
+      hipLaunchKernelGGL((select_row_kernel<kSelectMost / 4>), grid, block, 0, s, a);
+    } else if (a.width <= kSelectSegment / 2) {
+      hipLaunchKernelGGL((select_row_kernel<kSelectMost / 2>), grid, block, 0, s, a);
+    } else if (a.width <= kSelectSegment) {
+      hipLaunchKernelGGL((select_row_kernel<kSelectMost>), grid, block, 0, s, a);
+    } else {
+      const dim3 parts(b.S, a.G, a.R);
+      hipLaunchKernelGGL((select_hist_kernel<0>), parts, block, 0, s, a, b);
+      hipLaunchKernelGGL((select_hist_kernel<1>), parts, block, 0, s, a, b);
+      hipLaunchKernelGGL((select_hist_kernel<2>), parts, block, 0, s, a, b);
+      hipLaunchKernelGGL(select_write_kernel, parts, block, 0, s, a, b);
+      if (b.kept_w) hipLaunchKernelGGL(select_place_kernel, parts, block, 0, s, a, b);
+    }
+  }
+};
+
+int plan_select(const char* what, const float* weights, int64_t row_stride, int64_t head_stride, int32_t width,
+                const int32_t* seq_lens, int32_t R, int32_t num_kv_heads, int32_t keep, int32_t first, int32_t recent,
+                int32_t* kept, int32_t* new_lens, float* weights_out, int64_t out_row_stride, int64_t out_head_stride,
+                int32_t out_width, void* workspace, int64_t workspace_bytes, SelectLaunch* to) {
   if (R < 0 || num_kv_heads < 1 || width < 1 || keep < 1 || first < 0 || recent < 0 || (int64_t)first + recent > keep ||
       row_stride < width || head_stride < width)
     return fail(SNA_ERR_INVALID_ARGUMENT,
-                "select_tokens: bad sizes (R %d, KV heads %d, width %d, strides %lld / %lld, keep %d of which first %d "
-                "and recent %d)", R, num_kv_heads, width, (long long)row_stride, (long long)head_stride, keep, first,
+                "%s: bad sizes (R %d, KV heads %d, width %d, strides %lld / %lld, keep %d of which first %d "
+                "and recent %d)", what, R, num_kv_heads, width, (long long)row_stride, (long long)head_stride, keep, first,
                 recent);
   if (weights_out && (out_width < keep || out_row_stride < out_width || out_head_stride < out_width))
-    return fail(SNA_ERR_INVALID_ARGUMENT, "select_tokens: weights_out of %d columns (strides %lld / %lld) for %d tokens",
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: weights_out of %d columns (strides %lld / %lld) for %d tokens", what,
                 out_width, (long long)out_row_stride, (long long)out_head_stride, keep);
   if (width > INT32_MAX - kSelectSegment || (weights_out && out_width > INT32_MAX - (1 << 20)))
-    return fail(SNA_ERR_UNSUPPORTED, "select_tokens: %d columns, %d out (under 2^31)", width, out_width);
+    return fail(SNA_ERR_UNSUPPORTED, "%s: %d columns, %d out (under 2^31)", what, width, out_width);
   if (R == 0) return SNA_OK;
   if (!weights || !seq_lens || !kept || !new_lens)
-    return fail(SNA_ERR_INVALID_ARGUMENT, "select_tokens: null pointer");
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   if (R > 65535 || num_kv_heads > 65535)
-    return fail(SNA_ERR_INVALID_ARGUMENT, "select_tokens: %d rows x %d KV heads exceed the grid", R, num_kv_heads);
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %d rows x %d KV heads exceed the grid", what, R, num_kv_heads);
   const bool in_place = weights_out == weights && weights_out;
   if (in_place && (out_row_stride != row_stride || out_head_stride != head_stride))
-    return fail(SNA_ERR_INVALID_ARGUMENT, "select_tokens: weights_out is weights with other strides");
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: weights_out is weights with other strides", what);
   const int64_t rows = (int64_t)R * num_kv_heads, need = select_bytes(rows, width, keep, in_place);
   if (workspace_bytes < need || (need > 0 && !workspace))
-    return fail(SNA_ERR_WORKSPACE, "select_tokens: workspace of %lld bytes, need %lld", (long long)workspace_bytes,
+    return fail(SNA_ERR_WORKSPACE, "%s: workspace of %lld bytes, need %lld", what, (long long)workspace_bytes,
                 (long long)need);
   if (need > 0 && !aligned(workspace, 16))
-    return fail(SNA_ERR_INVALID_ARGUMENT, "select_tokens: the workspace must be 16-byte aligned");
-  SelectArgs a;
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", what);
+  SelectArgs& a = to->a;
   a.weights = weights;
   a.w_row = row_stride;
   a.w_head = head_stride;
@@ -470,16 +493,9 @@ extern "C" int sna_select_tokens(const float* weights, int64_t row_stride, int64
   a.o_row = out_row_stride;
   a.o_head = out_head_stride;
   a.out_width = out_width;
-  const hipStream_t s = (hipStream_t)stream;
-  const dim3 block(kSelectThreads), grid(num_kv_heads, R);
-  if (width <= kSelectSegment / 4) {
-    hipLaunchKernelGGL((select_row_kernel<kSelectMost / 4>), grid, block, 0, s, a);
-  } else if (width <= kSelectSegment / 2) {
-    hipLaunchKernelGGL((select_row_kernel<kSelectMost / 2>), grid, block, 0, s, a);
-  } else if (width <= kSelectSegment) {
-    hipLaunchKernelGGL((select_row_kernel<kSelectMost>), grid, block, 0, s, a);
-  } else {
-    SelectLong b;
+  SelectLong& b = to->b;
+  b = {};
+  if (need > 0) {
     b.S = (int32_t)select_segments(width);
     const int64_t bins = rows * b.S * kSelectBins;
     b.hist[0] = (uint32_t*)workspace;
@@ -488,39 +504,41 @@ extern "C" int sna_select_tokens(const float* weights, int64_t row_stride, int64
     b.above = b.hist[2] + bins;
     b.state = b.above + rows * b.S;
     b.kept_w = in_place ? (float*)(b.state + rows * 6) : nullptr;
-    const dim3 parts(b.S, num_kv_heads, R);
-    hipLaunchKernelGGL((select_hist_kernel<0>), parts, block, 0, s, a, b);
-    hipLaunchKernelGGL((select_hist_kernel<1>), parts, block, 0, s, a, b);
-    hipLaunchKernelGGL((select_hist_kernel<2>), parts, block, 0, s, a, b);
-    hipLaunchKernelGGL(select_write_kernel, parts, block, 0, s, a, b);
-    if (in_place) hipLaunchKernelGGL(select_place_kernel, parts, block, 0, s, a, b);
   }
-  return check_launch("select_tokens");
+  return SNA_OK;
 }
 
-extern "C" int sna_compact_tokens(void* k_cache, void* v_cache, int64_t num_blocks, int32_t num_kv_heads,
-                                  int32_t page_size, int32_t head_dim, int32_t cache_dtype, const int32_t* block_table,
-                                  int64_t table_stride, int32_t table_width, const int32_t* dst_table,
-                                  int64_t dst_stride, int32_t dst_width, const int32_t* kept, int32_t R, int32_t keep,
-                                  void* stream) {
-  ApiGuard guard;
+struct CompactLaunch {
+  CompactArgs a;
+  dim3 grid;
+  void run(hipStream_t s) const { hipLaunchKernelGGL(compact_tokens_kernel, grid, dim3(kCompactThreads), 0, s, a); }
+};
+
+int plan_compact(const char* what, void* k_cache, void* v_cache, int64_t num_blocks, int32_t num_kv_heads,
+                 int32_t page_size, int32_t head_dim, int32_t cache_dtype, const int32_t* block_table,
+                 int64_t table_stride, int32_t table_width, const int32_t* dst_table, int64_t dst_stride,
+                 int32_t dst_width, const int32_t* kept, int32_t R, int32_t keep, CompactLaunch* to) {
   if (R < 0 || num_kv_heads < 1 || num_blocks < 1 || page_size < 1 || keep < 1 || table_width < 1 ||
       table_stride < table_width || (dst_table && (dst_width < 1 || dst_stride < dst_width)))
     return fail(SNA_ERR_INVALID_ARGUMENT,
-                "compact_tokens: bad sizes (R %d, KV heads %d, blocks %lld, page %d, keep %d, tables %d and %d wide, "
-                "strides %lld and %lld)", R, num_kv_heads, (long long)num_blocks, page_size, keep, table_width,
+                "%s: bad sizes (R %d, KV heads %d, blocks %lld, page %d, keep %d, tables %d and %d wide, "
+                "strides %lld and %lld)", what, R, num_kv_heads, (long long)num_blocks, page_size, keep, table_width,
                 dst_width, (long long)table_stride, (long long)dst_stride);
-  if (dst_table == block_table) dst_table = nullptr;  // in place
+  if (dst_table == block_table && dst_table) {
+    if (R > 1 && dst_stride != table_stride)
+      return fail(SNA_ERR_INVALID_ARGUMENT, "%s: dst_table is block_table with another stride", what);
+    dst_table = nullptr;  // in place
+  }
   if (head_dim != 64 && head_dim != 128)
-    return fail(SNA_ERR_UNSUPPORTED, "compact_tokens: head_dim %d (64 or 128)", head_dim);
+    return fail(SNA_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", what, head_dim);
   if (cache_dtype != SNA_DTYPE_BF16 && cache_dtype != SNA_DTYPE_FP8_E4M3FN && cache_dtype != SNA_DTYPE_FP8_E4M3FN_MUL)
-    return fail(SNA_ERR_UNSUPPORTED, "compact_tokens: KV dtype %d (FP8 e4m3fn or bf16)", cache_dtype);
+    return fail(SNA_ERR_UNSUPPORTED, "%s: KV dtype %d (FP8 e4m3fn or bf16)", what, cache_dtype);
   if (R == 0) return SNA_OK;
   if (!k_cache || !v_cache || !block_table || !kept)
-    return fail(SNA_ERR_INVALID_ARGUMENT, "compact_tokens: null pointer");
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   if (!aligned(k_cache, 16) || !aligned(v_cache, 16))
-    return fail(SNA_ERR_INVALID_ARGUMENT, "compact_tokens: the caches must be 16-byte aligned");
-  CompactArgs a;
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: the caches must be 16-byte aligned", what);
+  CompactArgs& a = to->a;
   a.k_cache = (uint8_t*)k_cache;
   a.v_cache = (uint8_t*)v_cache;
   a.num_blocks = num_blocks;
@@ -541,8 +559,62 @@ extern "C" int sna_compact_tokens(void* k_cache, void* v_cache, int64_t num_bloc
   a.chunks = dst_table ? (int32_t)std::min<int64_t>(((int64_t)keep + per - 1) / per, 65535) : 1;
   const int64_t y = (int64_t)a.slices * num_kv_heads * 2;
   if (R > 65535 || y > 65535)
-    return fail(SNA_ERR_INVALID_ARGUMENT, "compact_tokens: %d rows x %d KV heads exceed the grid", R, num_kv_heads);
-  hipLaunchKernelGGL(compact_tokens_kernel, dim3(a.chunks, (unsigned)y, R), dim3(kCompactThreads), 0, (hipStream_t)stream,
-                     a);
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %d rows x %d KV heads exceed the grid", what, R, num_kv_heads);
+  to->grid = dim3(a.chunks, (unsigned)y, R);
+  return SNA_OK;
+}
+
+}  // namespace
+
+extern "C" int sna_select_tokens(const float* weights, int64_t row_stride, int64_t head_stride, int32_t width,
+                                 const int32_t* seq_lens, int32_t R, int32_t num_kv_heads, int32_t keep, int32_t first,
+                                 int32_t recent, int32_t* kept, int32_t* new_lens, float* weights_out,
+                                 int64_t out_row_stride, int64_t out_head_stride, int32_t out_width, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+  ApiGuard guard;
+  SelectLaunch select;
+  const int rc = plan_select("select_tokens", weights, row_stride, head_stride, width, seq_lens, R, num_kv_heads, keep,
+                             first, recent, kept, new_lens, weights_out, out_row_stride, out_head_stride, out_width,
+                             workspace, workspace_bytes, &select);
+  if (rc || R == 0) return rc;
+  select.run((hipStream_t)stream);
+  return check_launch("select_tokens");
+}
+
+extern "C" int sna_compact_tokens(void* k_cache, void* v_cache, int64_t num_blocks, int32_t num_kv_heads,
+                                  int32_t page_size, int32_t head_dim, int32_t cache_dtype, const int32_t* block_table,
+                                  int64_t table_stride, int32_t table_width, const int32_t* dst_table,
+                                  int64_t dst_stride, int32_t dst_width, const int32_t* kept, int32_t R, int32_t keep,
+                                  void* stream) {
+  ApiGuard guard;
+  CompactLaunch compact;
+  const int rc = plan_compact("compact_tokens", k_cache, v_cache, num_blocks, num_kv_heads, page_size, head_dim,
+                              cache_dtype, block_table, table_stride, table_width, dst_table, dst_stride, dst_width,
+                              kept, R, keep, &compact);
+  if (rc || R == 0) return rc;
+  compact.run((hipStream_t)stream);
   return check_launch("compact_tokens");
+}
+
+extern "C" int sna_evict_tokens(void* k_cache, void* v_cache, int64_t num_blocks, int32_t num_kv_heads,
+                                int32_t page_size, int32_t head_dim, int32_t cache_dtype, const int32_t* block_table,
+                                int64_t table_stride, int32_t table_width, const int32_t* dst_table, int64_t dst_stride,
+                                int32_t dst_width, const float* weights, int64_t row_stride, int64_t head_stride,
+                                int32_t width, const int32_t* seq_lens, int32_t R, int32_t keep, int32_t first,
+                                int32_t recent, int32_t* kept, int32_t* new_lens, float* weights_out,
+                                int64_t out_row_stride, int64_t out_head_stride, int32_t out_width, void* workspace,
+                                int64_t workspace_bytes, void* stream) {
+  ApiGuard guard;
+  SelectLaunch select;
+  CompactLaunch compact;
+  int rc = plan_select("evict_tokens", weights, row_stride, head_stride, width, seq_lens, R, num_kv_heads, keep, first,
+                       recent, kept, new_lens, weights_out, out_row_stride, out_head_stride, out_width, workspace,
+                       workspace_bytes, &select);
+  if (rc == SNA_OK)
+    rc = plan_compact("evict_tokens", k_cache, v_cache, num_blocks, num_kv_heads, page_size, head_dim, cache_dtype,
+                      block_table, table_stride, table_width, dst_table, dst_stride, dst_width, kept, R, keep, &compact);
+  if (rc || R == 0) return rc;
+  select.run((hipStream_t)stream);
+  compact.run((hipStream_t)stream);
+  return check_launch("evict_tokens");
 }

@@ -1077,11 +1077,20 @@ def select_tokens(weights: Tensor, seq_lens: Tensor, *, keep: int, first: int = 
     """The tokens that each (row, KV head) keeps, by weight: row r of L = seq_lens[r] tokens keeps all of them where L <=
     ``keep``, else its ``first`` first ones, its ``recent`` last ones and, of the others, those of the largest
     ``weights`` [R, G, N] fp32 (equal weights: the lowest position; NaN ranks above every number). Returns (kept
-    [R, G, keep] int32, ascending positions, -1 past a short row's; new_lens [R] int32 = min(L, keep)).
+    [R, G, keep] int32, ascending positions, -1 past a short row's; new_lens [R] int32 = min(L, keep)). A length past N
+    counts as N: tokens without a weight are not kept.
 
     ``weights_out`` [R, G, M >= keep] fp32, when given, receives the kept tokens' weights and zeros after them; it may be
     ``weights`` itself, so that the tokens written next start at zero."""
     dev = _on_gpu(weights, seq_lens, weights_out)
+    args, (kept, new_lens), _keep = _select_args(dev, weights, seq_lens, keep, first, recent, weights_out)
+    if kept.shape[0] and kept.shape[1]:
+        _launch(dev, _lib.load().sna_select_tokens, "select_tokens", *args)
+    return kept, new_lens
+
+
+def _select_args(dev, weights, seq_lens, keep, first, recent, weights_out):
+    """(sna_select_tokens' arguments, its results, tensors that they point into)."""
     if weights.dim() != 3:
         _need(False, f"weights must be [R, G, N], got {tuple(weights.shape)}")
     R, G, N = weights.shape
@@ -1103,14 +1112,13 @@ def select_tokens(weights: Tensor, seq_lens: Tensor, *, keep: int, first: int = 
             _need(False, "weights_out overlaps weights without being it")
     kept = torch.empty(R, G, keep, dtype=torch.int32, device=dev)
     new_lens = torch.empty(R, dtype=torch.int32, device=dev)
-    if R == 0 or G == 0:
-        return kept, new_lens
-    lib = _lib.load()
-    need = lib.sna_select_workspace_bytes(R, G, N, keep, same)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    _launch(dev, lib.sna_select_tokens, "select_tokens", weights.data_ptr(), row, head, N, lens.data_ptr(), R, G, keep,
-            first, recent, kept.data_ptr(), new_lens.data_ptr(), _ptr(weights_out), o_row, o_head, M, _ptr(ws), need)
-    return kept, new_lens
+    need, ws = 0, None
+    if R > 0 and G > 0:
+        need = _lib.load().sna_select_workspace_bytes(R, G, N, keep, same)
+        if need > 0:
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    return (weights.data_ptr(), row, head, N, lens.data_ptr(), R, G, keep, first, recent, kept.data_ptr(),
+            new_lens.data_ptr(), _ptr(weights_out), o_row, o_head, M, _ptr(ws), need), (kept, new_lens), (lens, ws)
 
 
 def _overlap(a: Tensor, b: Tensor) -> bool:
@@ -1130,37 +1138,45 @@ def compact_tokens(k_cache: Tensor, v_cache: Tensor, block_table: Tensor, kept: 
     [R, G, keep] int32 ascends (select_tokens), -1 entries move nothing. The caches [blocks, G, page, d] hold bf16 or FP8;
     bytes move as they are. Afterwards the row holds its kept tokens at positions 0 .. in order, its pages past them are
     free, and the decode entry points read it with the new length (a sliding window would count evicted positions no more).
+    The keys stay rotated by the positions that they were stored with, so the row's next token is rotated by the number of
+    tokens that came before it, not by the new length.
 
     Rows that share pages (a cached prefix) cannot be compacted in place: give them pages of their own in ``dst_table``,
     which names no page of ``block_table``."""
     dev = _on_gpu(k_cache, v_cache, block_table, kept, dst_table)
+    if k_cache.dim() != 4 or kept.dim() != 3 or kept.shape[1] != k_cache.shape[1]:
+        _need(False, f"kept must be [R, KV heads, keep] for caches {tuple(k_cache.shape)}, got {tuple(kept.shape)}")
+    kept = _contig(kept, "kept", torch.int32)
+    R, _, keep = kept.shape
+    args, _keep = _compact_args(k_cache, v_cache, block_table, R, keep, dst_table)
+    if R == 0 or keep == 0:
+        return
+    _launch(dev, _lib.load().sna_compact_tokens, "compact_tokens", *args, kept.data_ptr(), R, keep)
+
+
+def _compact_args(k_cache, v_cache, block_table, R, keep, dst_table):
+    """(sna_compact_tokens' arguments up to the kept tokens, tensors that they point into)."""
     shape = k_cache.shape
     if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != k_cache.dtype:
         _need(False, "K and V caches differ")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         _need(False, "caches must be contiguous")
-    if k_cache.data_ptr() == v_cache.data_ptr() and k_cache.numel() > 0:
-        _need(False, "K and V are one tensor")
+    if abs(k_cache.data_ptr() - v_cache.data_ptr()) < k_cache.numel() * k_cache.element_size():
+        _need(False, "K and V are one tensor, or overlap")
     nb, G, P, d = shape
-    if kept.dim() != 3 or kept.shape[1] != G:
-        _need(False, f"kept must be [R, {G}, keep], got {tuple(kept.shape)}")
-    kept = _contig(kept, "kept", torch.int32)
-    R, _, keep = kept.shape
     if block_table.dim() != 2 or block_table.shape[0] != R:
         _need(False, f"block_table must be [{R}, width]")
     table = _contig(_as(block_table, torch.int32), "block_table")
     W = table.shape[1]
-    to, V = None, 0
+    dst, to, V = None, None, 0
     if dst_table is not None:
         if dst_table.dim() != 2 or dst_table.shape[0] != R or dst_table.shape[1] * P < keep:
             _need(False, f"dst_table must be [{R}, pages of {P} for {keep} tokens], got {tuple(dst_table.shape)}")
-        dst = _contig(_as(dst_table, torch.int32), "dst_table")
-        if dst_table.data_ptr() != block_table.data_ptr():  # (else it is in place)
-            to, V = dst.data_ptr(), dst.shape[1]
-    if R == 0 or keep == 0:
-        return
-    _launch(dev, _lib.load().sna_compact_tokens, "compact_tokens", k_cache.data_ptr(), v_cache.data_ptr(), nb, G, P, d,
-            cache_dtype_code(k_cache.dtype), table.data_ptr(), W, W, to, V, V, kept.data_ptr(), R, keep)
+        if dst_table.data_ptr() != block_table.data_ptr() or (R > 1 and dst_table.stride(0) != block_table.stride(0)):
+            dst = _contig(_as(dst_table, torch.int32), "dst_table")
+            to, V = dst.data_ptr(), dst.shape[1]  # (else it is the same rows' first pages: in place)
+    return (k_cache.data_ptr(), v_cache.data_ptr(), nb, G, P, d, cache_dtype_code(k_cache.dtype), table.data_ptr(), W, W,
+            to, V, V), (table, dst)
 
 
 def evict_tokens(k_cache: Tensor, v_cache: Tensor, block_table: Tensor, seq_lens: Tensor, weights: Tensor, *, keep: int,
@@ -1168,11 +1184,17 @@ def evict_tokens(k_cache: Tensor, v_cache: Tensor, block_table: Tensor, seq_lens
                  weights_out: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
     """Thin the rows of one layer's caches to ``keep`` tokens each by accumulated attention weight: select_tokens, then
     compact_tokens. Every KV head of a row keeps a set of its own, the count is the row's. Returns (kept, new_lens)."""
+    dev = _on_gpu(k_cache, v_cache, block_table, seq_lens, weights, dst_table, weights_out)
     if k_cache.dim() != 4 or weights.dim() != 3 or weights.shape[:2] != (block_table.shape[0], k_cache.shape[1]):
         _need(False, f"weights {tuple(weights.shape)} for {block_table.shape[0]} rows of caches {tuple(k_cache.shape)}")
-    kept, new_lens = select_tokens(weights, seq_lens, keep=keep, first=first, recent=recent, weights_out=weights_out)
-    compact_tokens(k_cache, v_cache, block_table, kept, dst_table=dst_table)
-    return kept, new_lens
+    R, G, N = weights.shape
+    caches, _c = _compact_args(k_cache, v_cache, block_table, R, keep, dst_table)
+    (w, row, head, _, lens, _, _, _, _, _, *out), results, _s = _select_args(dev, weights, seq_lens, keep, first, recent,
+                                                                           weights_out)
+    if R > 0 and G > 0:
+        _launch(dev, _lib.load().sna_evict_tokens, "evict_tokens", *caches, w, row, head, N, lens, R, keep, first, recent,
+                *out)
+    return results
 
 
 # ------------------------------------------------------------------------------------------------------------------

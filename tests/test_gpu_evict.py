@@ -239,6 +239,39 @@ def test_refusals():
         ops.compact_tokens(z(5, 2, 16, 32, dtype=torch.bfloat16), z(5, 2, 16, 32, dtype=torch.bfloat16), t, kept)
 
 
+def test_a_refused_eviction_leaves_the_weights():
+    """Nothing of an eviction runs unless all of its arguments are good: weights_out is the weights themselves here."""
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=DEV)  # noqa: E731
+    t, lens = torch.zeros(2, 4, dtype=torch.int32, device=DEV), torch.full((2,), 64, dtype=torch.int32, device=DEV)
+    w = _weights(1, 2, 2, 64, "plain").to(DEV)
+    was = w.clone()
+    for k, v, dst in ((z(5, 2, 16, 32), z(5, 2, 16, 32), None), (z(5, 2, 16, 64), z(5, 2, 8, 64), None),
+                      (z(5, 2, 16, 64), z(5, 2, 16, 64), t[:, :1])):
+        with pytest.raises(ValueError):
+            ops.evict_tokens(k, v, t, lens, w, keep=20, weights_out=w, dst_table=dst)
+    both = z(6, 2, 16, 64)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.evict_tokens(both[:5], both[1:], t, lens, w, keep=20, weights_out=w)
+    with pytest.raises(ValueError, match="another stride"):
+        ops.evict_tokens(z(5, 2, 16, 64), z(5, 2, 16, 64), t, lens, w, keep=20, weights_out=w,
+                         dst_table=t.view(-1)[:6].view(2, 3))
+    torch.cuda.synchronize()
+    assert torch.equal(w, was)
+
+
+def test_the_first_pages_of_the_table_as_target_are_in_place():
+    table = _table(1, [6, 5], 20, 6)
+    k, v = _cache(5, 20, 2, 16, 64, False), _cache(6, 20, 2, 16, 64, False)
+    w = _weights(7, 2, 2, 96, "plain")
+    lens = torch.tensor([96, 77], dtype=torch.int32, device=DEV)
+    dk, dv, dt = k.to(DEV), v.to(DEV), table.to(DEV)
+    kept, new = ops.evict_tokens(dk, dv, dt, lens, w.to(DEV), keep=40, dst_table=dt[:, :3])
+    want, _ = ow.select_tokens(w, [96, 77], 40, 0, 0)
+    assert torch.equal(kept.cpu(), want) and new.tolist() == [40, 40]
+    assert torch.equal(_bytes(dk), _bytes(ow.compact_tokens(k.view(torch.int16), table, want)))
+    assert torch.equal(_bytes(dv), _bytes(ow.compact_tokens(v.view(torch.int16), table, want)))
+
+
 def test_graph_and_side_stream():
     P, G, d, R = 16, 2, 128, 3
     lens, keep = [400, 100, 50], 64

@@ -149,6 +149,22 @@ def test_compact_refusals(bad, code):
     assert rc == code, _lib.last_error()
 
 
+@pytest.mark.parametrize("bad,code,what", [(dict(d=80), -4, "head_dim"), (dict(k=P + 8), -1, "aligned"),
+                                           (dict(tw=0), -1, "bad sizes"), (dict(keep=0), -1, "bad sizes"),
+                                           (dict(lens=None), -1, "null"), (dict(table=None), -1, "null"),
+                                           (dict(out=P, M=4), -1, "weights_out"), (dict(N=20000, row=40000, head=20000), -2,
+                                                                                  "workspace"),
+                                           (dict(dst=P, dstride=3, table=P, R=2), -1, "another stride")])
+def test_evict_refuses_before_either_launch(bad, code, what):
+    a = dict(k=P, v=P, nb=4, G=2, page=16, d=64, dtype=0, table=P, ts=2, tw=2, dst=None, dstride=2, dw=2, w=P, row=16, head=8,
+             N=8, lens=P, R=1, keep=5, first=1, recent=1, kept=P, new=P, out=None, M=8) | bad
+    rc = _lib.load().sna_evict_tokens(a["k"], a["v"], a["nb"], a["G"], a["page"], a["d"], a["dtype"], a["table"], a["ts"],
+                                      a["tw"], a["dst"], a["dstride"], a["dw"], a["w"], a["row"], a["head"], a["N"],
+                                      a["lens"], a["R"], a["keep"], a["first"], a["recent"], a["kept"], a["new"], a["out"],
+                                      16, 8, a["M"], None, 0, None)
+    assert rc == code and what in _lib.last_error(), _lib.last_error()
+
+
 @pytest.mark.parametrize("bad,code", [(dict(T=-1), -1), (dict(Hq=0), -1), (dict(d=96), -4), (dict(A=0), -4),
                                       (dict(A=5), -4), (dict(n=4), -4), (dict(n=72), -4), (dict(stride=8), -1),
                                       (dict(pstride=3), -1), (dict(kn=None), -1), (dict(dtype=2), -4),
