@@ -479,7 +479,7 @@ int sna_prefill_attention_split(const void *q, const void *k_cache, const void *
  * This has no reference counterpart. */
 int64_t sna_attention_weights_workspace_bytes(int32_t n_tokens, int32_t R, int32_t max_q_len, int32_t num_q_heads,
                                               int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
-                                              int32_t table_width, int32_t width, int32_t kv_dtype);
+                                              int32_t table_width, int32_t width, int32_t kv_dtype, int32_t window);
 int sna_prefill_attention_weights(const void *q, const void *k_cache, const float *k_scale, const int32_t *block_table,
                                   int64_t table_stride, int32_t table_width, const int32_t *q_start,
                                   const int32_t *prior_lens, int32_t n_tokens, int32_t R, int32_t max_q_len,

@@ -96,7 +96,7 @@ SIGNATURES = {
     "sna_prefill_attention_split": (_I32, [_P, _P, _P, _P, _P, _P, _I64, _I32, _P, _P, _I32, _I32, _P, _F32, _I32, _P,
                                      _I32, _I32, _I32, _I32, _I64, _I32, _P, _I64, _P]),
     "sna_prefill_workspace_bytes": (_I64, [_I32] * 8),
-    "sna_attention_weights_workspace_bytes": (_I64, [_I32] * 10),
+    "sna_attention_weights_workspace_bytes": (_I64, [_I32] * 11),
     "sna_prefill_attention_weights": (_I32, [_P, _P, _P, _P, _I64, _I32, _P, _P, _I32, _I32, _I32, _P, _F32, _I32, _P,
                                              _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _I64, _I32, _P, _I64, _P]),
     "sna_decode_attention_weights": (_I32, [_P, _P, _P, _P, _I64, _I32, _P, _I32, _P, _F32, _I32, _P, _I64, _I64, _I32,

@@ -258,7 +258,8 @@ void weights_tile_kernel(WeightsArgs a) {
   const int32_t k0 = kb * kWeightKeys;
   // the run's rows that see any of the block's keys: tokens [t0, t1)
   const int64_t last = (int64_t)min(k0 + kWeightKeys, rq.n) - 1;
-  const int64_t run0 = (int64_t)run * a.split_tokens;
+  // (the runs' tokens count from the 32 with the first one that sees the block)
+  const int64_t run0 = (min(max(k0 - rq.prior, (int64_t)0), (int64_t)rq.S) & ~31) + (int64_t)run * a.split_tokens;
   const int32_t s0 = (int32_t)min(run0, (int64_t)rq.S), s1 = (int32_t)min(run0 + a.split_tokens, (int64_t)rq.S);
   int32_t t0 = (int32_t)min(max(k0 - rq.prior, (int64_t)s0), (int64_t)s1), t1 = s1;
   if (a.window > 0) t1 = (int32_t)min(max(last + a.window - rq.prior, (int64_t)s0), (int64_t)s1);
@@ -877,10 +878,12 @@ struct WeightsPlan {
 constexpr int64_t kRowPairs = 256, kRowKeys = 2048;  // the CUs, and the least keys of a table
 constexpr int32_t kRowFloats[2] = {18432, 36864};    // LDS of two workgroups a CU, or one
 constexpr int64_t kScoreWorkgroups = 1024;  // a score launch's chunks are taken several to a workgroup from so many on
-constexpr int64_t kSplitRows = 2048;       // least rows of a run of queries
-constexpr int64_t kSplitWorkgroups = 4096; // runs are cut up to so many workgroups
+// Queries are cut into runs of at least so many rows while that makes no more than so many workgroups: by 4 tiles up to two
+// rounds of the 3 workgroups that a CU holds, by 8 up to four. One run each: 635 queries of 8 heads over 2270 keys 100 us
+// (29 cut), 300 of a window of 128 86 (39), 1024 of 32 heads over 8192 keys 327 (293), 4 x 2048 over 4096 keys 497 (470).
+constexpr int64_t kRunRows[2] = {128, 256}, kRunWorkgroups[2] = {1536, 3072};
 WeightsPlan weights_plan(int64_t T, int64_t R, int64_t max_q, int32_t H, int32_t G, int32_t page_size,
-                         int32_t table_width, int32_t width, int32_t head_dim, int32_t esz) {
+                         int32_t table_width, int32_t width, int32_t head_dim, int32_t esz, int32_t window) {
   WeightsPlan p;
   p.score_keys = 0;
   p.row_floats = 0;
@@ -917,10 +920,16 @@ WeightsPlan weights_plan(int64_t T, int64_t R, int64_t max_q, int32_t H, int32_t
   p.splits = 1, p.split_tokens = (int32_t)max_q;
   int64_t sum = 0;
   if (!p.scores) {
-    const int64_t least = ((kSplitRows + group - 1) / group + kWeightRows - 1) / kWeightRows * kWeightRows;
-    const int64_t most = std::max<int64_t>(1, std::min((max_q + least - 1) / least, kSplitWorkgroups / (p.blocks * R * G)));
-    p.split_tokens = (int32_t)(((max_q + most - 1) / most + kWeightRows - 1) / kWeightRows * kWeightRows);
-    p.splits = (int32_t)((max_q + p.split_tokens - 1) / p.split_tokens);
+    // the tokens that can see one block, from a multiple of 32 on, and the blocks that any can see
+    const int64_t most_tokens = window > 0 ? std::min<int64_t>(max_q, (int64_t)kWeightKeys + window + 31) : max_q;
+    const int64_t seen = window > 0 ? std::min<int64_t>(p.blocks, (max_q + window) / kWeightKeys + 2) : p.blocks;
+    auto runs = [&](int64_t rows, int64_t workgroups) {
+      const int64_t least = ((rows + group - 1) / group + kWeightRows - 1) / kWeightRows * kWeightRows;
+      return std::min((most_tokens + least - 1) / least, workgroups / (seen * R * G));
+    };
+    const int64_t most = std::max<int64_t>({1, runs(kRunRows[0], kRunWorkgroups[0]), runs(kRunRows[1], kRunWorkgroups[1])});
+    p.split_tokens = (int32_t)(((most_tokens + most - 1) / most + kWeightRows - 1) / kWeightRows * kWeightRows);
+    p.splits = (int32_t)((most_tokens + p.split_tokens - 1) / p.split_tokens);
     if (p.splits > 1) sum = p.splits * R * G * p.blocks * kWeightKeys * (int64_t)sizeof(float);
   }
   p.part = (p.part + 15) / 16 * 16;
@@ -991,7 +1000,7 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
                 (long long)head_stride, width);
   max_q_len = std::max(max_q_len, 1);
   const WeightsPlan plan = weights_plan(T, R, max_q_len, num_q_heads, num_kv_heads, page_size, table_width, width,
-                                        head_dim, kv_dtype == SNA_DTYPE_BF16 ? 2 : 1);
+                                        head_dim, kv_dtype == SNA_DTYPE_BF16 ? 2 : 1, window);
   const int64_t blocks = plan.blocks;
   const int64_t wgs = blocks * R * num_kv_heads * plan.splits;
   if (wgs > kGridMax / 4)
@@ -1052,12 +1061,12 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
 extern "C" int64_t sna_attention_weights_workspace_bytes(int32_t n_tokens, int32_t R, int32_t max_q_len,
                                                          int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                                                          int32_t page_size, int32_t table_width, int32_t width,
-                                                         int32_t kv_dtype) {
+                                                         int32_t kv_dtype, int32_t window) {
   if (n_tokens < 0 || R < 1 || max_q_len < 0 || num_q_heads < 1 || num_kv_heads < 1 ||
       num_q_heads % num_kv_heads != 0 || page_size < 1 || table_width < 1 || width < 0)
     return 0;
   return weights_plan(n_tokens, R, std::max(max_q_len, 1), num_q_heads, num_kv_heads, page_size, table_width, width, head_dim,
-                      kv_dtype == SNA_DTYPE_BF16 ? 2 : 1).bytes;
+                      kv_dtype == SNA_DTYPE_BF16 ? 2 : 1, window).bytes;
 }
 
 extern "C" int sna_prefill_attention_weights(const void* q, const void* k_cache, const float* k_scale,

@@ -1024,7 +1024,7 @@ def _attention_weights(what, q, T, R, k_cache, block_table, q_start, lens, max_q
         row, head = G * N, N
         weights = torch.empty(R, G, N, dtype=torch.float32, device=dev)
     lib = _lib.load()
-    need = lib.sna_attention_weights_workspace_bytes(T, R, max_q_len, H, G, d, P, W, N, code)
+    need = lib.sna_attention_weights_workspace_bytes(T, R, max_q_len, H, G, d, P, W, N, code, window)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     stride = max(table.stride(0), W)
     if q_start is None:

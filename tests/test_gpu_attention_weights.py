@@ -102,6 +102,10 @@ CASES = [
     ("long-window-of-queries", 4, 1, 128, 64, [3000], [32], True, 0, False, 0),
     ("runs-of-queries", 64, 1, 64, 16, [100, 300], [100, 70], True, 0, True, 2),
     ("runs-window", 96, 2, 128, 16, [150, 40], [150, 40], False, 33, False, 0),
+    ("runs-far-window", 8, 1, 64, 16, [5000, 300, 90], [600, 300, 45], False, 128, True, 4),
+    ("runs-wide-window", 8, 1, 64, 16, [1500, 900], [700, 31], True, 300, False, 0),
+    ("runs-group-3", 12, 4, 128, 16, [2000, 700, 1], [333, 700, 1], True, 0, True, 3),
+    ("runs-odd-prior", 8, 1, 64, 16, [777, 1333], [500, 65], False, 0, False, 0),
     ("many-tiles", 16, 1, 128, 16, [700], [530], True, 0, False, 0),
     ("many-rows", 2, 1, 64, 16, [5 + 13 * i for i in range(40)], [1 + i % 4 for i in range(40)], True, 0, False, 0),
 ]
@@ -209,7 +213,7 @@ def test_written_widths_at_the_c_entry(R, H, G, counts, width):
     out = torch.full((R, G, width + 3), -2.0, device=DEV)
     lib = _lib.load()
     sizes = (len(q), R, max(c.counts))
-    need = lib.sna_attention_weights_workspace_bytes(*sizes, H, G, 64, 16, table.shape[1], width, _lib.DTYPE_BF16)
+    need = lib.sna_attention_weights_workspace_bytes(*sizes, H, G, 64, 16, table.shape[1], width, _lib.DTYPE_BF16, 0)
     ws = torch.empty(need, dtype=torch.uint8, device=DEV)
     rc = lib.sna_prefill_attention_weights(
         q.data_ptr(), k.data_ptr(), None, table.data_ptr(), table.shape[1], table.shape[1], start.data_ptr(),
