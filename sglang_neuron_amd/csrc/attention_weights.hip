@@ -5,16 +5,27 @@
 // sees the keys (p - window, p] (all up to p without a window) that lie on valid pages; a query that sees none adds
 // nothing. It is what an eviction by accumulated weight ranks the keys by.
 //
-// A probability needs its row's sum over all keys before it can be added to its key's, so the scores are computed twice:
-//   weights_tile_kernel<STATS>  per block of 256 keys and query row: the largest score and the sum of exp(score - largest)
-//   weights_merge_kernel        per query row: the blocks merged to the row's largest score and 1 / its whole sum
-//   weights_tile_kernel<SUM>    per key: the probabilities summed over the rows
-// Rows are (query token, head) pairs of one KV head, token-major (row = t * group + j). A workgroup of 4 waves owns 256
-// keys of one (request, KV head), 64 to a wave, held as bf16 matrix operands in registers (an e4m3fn value is a bf16
-// value); the rows pass in tiles of 32 through a 2-slot LDS ring that the waves share. The product is S^T[key, row] =
-// K[key, :] . Q[row, :] by v_mfma_f32_32x32x16_bf16, so a lane holds 16 keys of one row: the row's maximum, sum and
-// normalization are values of the lane, and a key's sum over the rows stays in the lane's registers until the end.
-// Scores are fp32, exponentials in the log2 domain, every sum fp32; a key's rows are added in a fixed order.
+// A probability needs its row's sum over all keys before it can be added to its key's. Three forms, by the number of query
+// rows ((query token, head) pairs of one KV head, token-major: row = t * group + j) and how the batch fills the chip:
+//   many rows   the scores are computed twice, key-stationary:
+//     weights_tile_kernel<kStats>  per block of 256 keys and query row: the largest score, the sum of exp(score - largest)
+//     weights_merge_kernel         per query row: the blocks merged to the row's largest score and 1 / its whole sum
+//     weights_tile_kernel<kSum>    per key: the probabilities summed over a run of the rows
+//     weights_reduce_kernel        per key: the runs' sums added, where the queries are cut into runs
+//   up to 16 rows, as in a decode step: the keys are read once
+//     weights_score_kernel         the scores to a workspace, and each block's (largest, sum)
+//     weights_from_scores_kernel   the blocks merged, the probabilities of a key summed
+//   the same, with (request, KV head) pairs enough to fill the chip:
+//     weights_row_kernel           a pair's scores in the LDS of one workgroup: one launch
+// Scores are fp32, exponentials in the log2 domain, every sum fp32; sums run in a fixed order, without atomics.
+//
+// Measured (us of kernels; heads 32/8 of 128, e4m3fn, pages of 16, where not said): 64 rows of 4096 keys 65.6, 273 MB of
+// keys at 4.2 TB/s (HBM: a plain copy reaches 4.8); 8 rows of 128-1024 bf16 keys, heads 16/8, 5.2 + 4.4 (two launches and
+// their chains of round trips); 128 rows of 2048-8192 keys, heads 8/1 of 64, 17 + 8 (the same, ragged); 32 queries over
+// each of 3001 to 16384 keys 22.8 + 5 + 26.8 and 64 over 131071 bf16 keys 103 + 10 + 112 (the keys are read twice, at 2.6
+// TB/s, beside exponentials and products); 4 x 2048 queries after 2048 each 470-490 in all, the first pass a little over
+// half: products take 37% (41% in the second pass) of a SIMD's cycles and VALU instructions 61% (57%), which together is
+// all of them: a wave's matrix instructions and the other waves' VALU hardly overlap here.
 #include <algorithm>
 #include <type_traits>
 
@@ -50,7 +61,7 @@ struct WeightsArgs {
   float* ws_sum;     // [splits, R, G, blocks * 256] the runs' sums, with more than one
   // few rows instead: ws_part is [R, G, blocks, max_q * group], and
   float* ws_score;   // [R, G, max_q * group, blocks * score_keys] scores in the log2 domain, -inf where unseen
-  int32_t span, score_keys;  // chunks of a workgroup, and their keys
+  int32_t span, score_keys;  // chunks of a workgroup, and their keys (weights_row_kernel: a row's keys in LDS)
 };
 
 constexpr int kWeightKeys = 256;  // keys of a workgroup, 64 to a wave
@@ -111,8 +122,8 @@ __device__ __forceinline__ void dma_global4(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(m0), "v"(src) : "memory");
 }
 
-// N keys of a wave (lane i holding the place of key i mod N) into LDS: whole rows by DMA, 1024 bytes an instruction, chunk c of row r to c ^ swz(r). A key that is
-// not there reads the cache's first row; what comes of it is masked or dropped.
+// N keys of a wave (lane i holding the place of key i mod N) into LDS: whole rows by DMA, 1024 bytes an instruction, chunk
+// c of row r to c ^ swz(r). A key that is not there reads the cache's first row; what comes of it is masked or dropped.
 template <int D, int ESZ, int N>
 __device__ __forceinline__ void weights_stage(const WeightsArgs& a, int64_t at, uint8_t* lds) {
   using Geo = WeightsGeo<D, ESZ>;
@@ -225,6 +236,14 @@ __device__ __forceinline__ float2 weights_stats(f32x16_t (&x)[2], float c2, uint
   return make_float2(both, xor32_partner_sum(sum * __builtin_amdgcn_exp2f(mx - both)));
 }
 
+// Many rows. A workgroup of 4 waves owns 256 keys of one (request, KV head), 64 to a wave, held as bf16 matrix operands in
+// registers (an e4m3fn value is a bf16 value); the rows of its run pass in tiles of 32 through a ring of two pairs of tiles
+// in LDS that the waves share, filled by DMA, one barrier a pair. The product is S^T[key, row] = K[key, :] . Q[row, :] by
+// v_mfma_f32_32x32x16_bf16, so a lane holds 16 keys of one row twice: the row's maximum, sum and normalization are values of
+// the lane, and a key's sum over the rows stays in the lane's registers until the end, where it is added across the lanes
+// once. A tile costs a wave 32 exponentials a lane (8 cycles each), as many fused multiply-adds, and at head_dim 128 16
+// products of 32 cycles. Products and exponentials of one wave take turns, on three waves a SIMD. (The next tile's products
+// among the exponentials, on two waves a SIMD, took 620 us for 4 x 2048 after 2048 where this took 590.) Pairs of tiles that all of the wave's keys are seen by take a path without masks.
 enum WeightsPass { kStats, kSum };
 template <int D, int ESZ>
 struct WeightsRing {
@@ -507,8 +526,9 @@ __global__ __launch_bounds__(256) void weights_merge_kernel(WeightsArgs a) {
 constexpr int kScoreRows = 16;
 // A workgroup of 4 waves takes `span` chunks of 4 x CK consecutive keys, CK to a wave; a wave's next chunk is on its way to
 // LDS while it works on one. (Keys of 64 bytes: one chunk a workgroup, whose 16 KB leave room for more workgroups: 128 rows
-// of 2048-8192 keys took 16 us so and 21 in spans; of 128 bytes, 64 rows of 4096, 72 and 64.) By v_mfma_f32_16x16x32_bf16: lane (g4, i) feeds key 16 s + i's dims 32 c + 8 g4 .. of step c
-// (FP8: 64 (c / 2) + 16 g4 + 8 (c & 1) ..) and holds the scores of row i and keys 16 s + 4 g4 + e.
+// of 2048-8192 keys took 16 us so and 21 in spans; of 128 bytes, 64 rows of 4096, 72 and 64.) By v_mfma_f32_16x16x32_bf16:
+// lane (g4, i) feeds key 16 s + i's dims 32 c + 8 g4 .. of step c (FP8: 64 (c / 2) + 16 g4 + 8 (c & 1) ..) and holds the
+// scores of row i and keys 16 s + 4 g4 + e.
 constexpr int score_chunk(int row_bytes) { return row_bytes > 128 ? 32 : 64; }  // keys of a wave's chunk: at most 8 KB
 constexpr int score_span(int row_bytes) { return row_bytes > 64 ? 8 : 1; }      // most chunks
 template <int D, int ESZ>
@@ -756,7 +776,8 @@ __global__ __launch_bounds__(kRowThreads) void weights_row_kernel(WeightsArgs a)
     }
     if (kw >= lo) {
       constexpr uint64_t kAll = CK == 64 ? ~0ull : (1ull << CK % 64) - 1;
-      const bool all = valid == kAll && rq.prior >= kw + CK - 1 && (a.window <= 0 || rq.prior + rq.S - 1 - a.window < kw);  // uniform
+      const bool all = valid == kAll && rq.prior >= kw + CK - 1 &&
+                       (a.window <= 0 || rq.prior + rq.S - 1 - a.window < kw);  // uniform
       const uint64_t seen = all ? ~0ull : weights_seen(a, valid, rq.prior + t, kw) >> 4 * g4;
 #pragma unroll
       for (int s = 0; s < NT; ++s) {
@@ -811,10 +832,13 @@ __global__ __launch_bounds__(kRowThreads) void weights_row_kernel(WeightsArgs a)
     for (int32_t c = 4 * tid; c < cols; c += 4 * kRowThreads) {
       float4* const at = reinterpret_cast<float4*>(score + i * pitch + c);
       float4 x = *at;
-      x.x = __builtin_amdgcn_exp2f(x.x - top), x.y = __builtin_amdgcn_exp2f(x.y - top);
-      x.z = __builtin_amdgcn_exp2f(x.z - top), x.w = __builtin_amdgcn_exp2f(x.w - top);
+      const float4 p = make_float4(__builtin_amdgcn_exp2f(x.x - top), __builtin_amdgcn_exp2f(x.y - top),
+                                   __builtin_amdgcn_exp2f(x.z - top), __builtin_amdgcn_exp2f(x.w - top));
+      sum += (p.x + p.y) + (p.z + p.w);
+      // (an unseen key's is kept as -1: it adds nothing, whatever the row's sum is)
+      x.x = x.x == -INFINITY ? -1.0f : p.x, x.y = x.y == -INFINITY ? -1.0f : p.y;
+      x.z = x.z == -INFINITY ? -1.0f : p.z, x.w = x.w == -INFINITY ? -1.0f : p.w;
       *at = x;
-      sum += (x.x + x.y) + (x.z + x.w);
     }
     sum = wave_sum(sum);
     if (lane == 0) sm_wave[wave][i] = sum;
@@ -834,9 +858,8 @@ __global__ __launch_bounds__(kRowThreads) void weights_row_kernel(WeightsArgs a)
     for (int i = 0; i < M; ++i) {
       const float4 x = *reinterpret_cast<const float4*>(score + i * pitch + c);
       const float inv = sm_row[i].y;
-      // (an exponential of 0 adds nothing, whatever the row's sum is: an unseen key's)
-      w[0] += x.x == 0.0f ? 0.0f : x.x * inv, w[1] += x.y == 0.0f ? 0.0f : x.y * inv;
-      w[2] += x.z == 0.0f ? 0.0f : x.z * inv, w[3] += x.w == 0.0f ? 0.0f : x.w * inv;
+      w[0] += x.x < 0.0f ? 0.0f : x.x * inv, w[1] += x.y < 0.0f ? 0.0f : x.y * inv;
+      w[2] += x.z < 0.0f ? 0.0f : x.z * inv, w[3] += x.w < 0.0f ? 0.0f : x.w * inv;
     }
     const int32_t key = lo + c;
 #pragma unroll
@@ -861,7 +884,7 @@ int64_t weights_blocks(int32_t page_size, int32_t table_width, int32_t width, in
   return (std::max<int64_t>((int64_t)table_width * page_size, width) + keys - 1) / keys;
 }
 
-// How a launch works, and its workspace: few rows a request keep their scores (at most kScoreBytes of them), others
+// How a launch works, and its workspace: few rows a request keep their scores while these take 512 MB at most, others
 // compute them twice.
 constexpr int64_t kScoreBytes = (int64_t)1 << 29;
 struct WeightsPlan {
@@ -877,7 +900,7 @@ struct WeightsPlan {
 // 8 a second turn), 1024 of 100 to 1024 bf16 keys 58 : 47 and 64 of 2048 13 : 9 (a CU alone reads 256 KB in 8 us).
 constexpr int64_t kRowPairs = 256, kRowKeys = 2048;  // the CUs, and the least keys of a table
 constexpr int32_t kRowFloats[2] = {18432, 36864};    // LDS of two workgroups a CU, or one
-constexpr int64_t kScoreWorkgroups = 1024;  // a score launch's chunks are taken several to a workgroup from so many on
+constexpr int64_t kScoreWorkgroups = 1024;  // a score launch has so many at least before one takes several chunks
 // Queries are cut into runs of at least so many rows while that makes no more than so many workgroups: by 4 tiles up to two
 // rounds of the 3 workgroups that a CU holds, by 8 up to four. One run each: 635 queries of 8 heads over 2270 keys 100 us
 // (29 cut), 300 of a window of 128 86 (39), 1024 of 32 heads over 8192 keys 327 (293), 4 x 2048 over 4096 keys 497 (470).
@@ -889,9 +912,9 @@ WeightsPlan weights_plan(int64_t T, int64_t R, int64_t max_q, int32_t H, int32_t
   p.row_floats = 0;
   p.splits = 1, p.split_tokens = (int32_t)max_q;
   const int64_t table_keys = ((int64_t)table_width * page_size + 63) / 64 * 64;
-  const int64_t floats = max_q * (H / G) * (table_keys + kRowPad) + table_width, pairs = R * G;
-  if (max_q * (H / G) <= kScoreRows && floats <= kRowFloats[1] && table_keys >= kRowKeys) {
-    const bool half = floats <= kRowFloats[0];
+  const int64_t group = H / G, rows = max_q * group, pairs = R * G;
+  if (rows <= kScoreRows && table_keys >= kRowKeys && rows * (table_keys + kRowPad) + table_width <= kRowFloats[1]) {
+    const bool half = rows * (table_keys + kRowPad) + table_width <= kRowFloats[0];
     const int64_t slots = half ? 2 * kRowPairs : kRowPairs, turns = (pairs + slots - 1) / slots;
     if (pairs >= kRowPairs && (turns == 1 || 4 * pairs >= 3 * turns * slots)) {
       p.row_floats = kRowFloats[half ? 0 : 1];
@@ -902,7 +925,6 @@ WeightsPlan weights_plan(int64_t T, int64_t R, int64_t max_q, int32_t H, int32_t
   }
   p.blocks = weights_blocks(page_size, table_width, width, kWeightKeys);
   p.span = 1;
-  const int64_t rows = max_q * (H / G);
   int64_t score = INT64_MAX;
   if (rows <= kScoreRows) {
     const int32_t chunk = 4 * score_chunk(head_dim * esz);
@@ -916,15 +938,13 @@ WeightsPlan weights_plan(int64_t T, int64_t R, int64_t max_q, int32_t H, int32_t
   p.scores = score <= kScoreBytes;
   p.part = (p.scores ? R * G * rows : T * H) * p.blocks * (int64_t)sizeof(float2);
   p.rest = p.scores ? score : T * H * (int64_t)sizeof(float2);
-  const int64_t group = H / G;
-  p.splits = 1, p.split_tokens = (int32_t)max_q;
   int64_t sum = 0;
   if (!p.scores) {
     // the tokens that can see one block, from a multiple of 32 on, and the blocks that any can see
     const int64_t most_tokens = window > 0 ? std::min<int64_t>(max_q, (int64_t)kWeightKeys + window + 31) : max_q;
     const int64_t seen = window > 0 ? std::min<int64_t>(p.blocks, (max_q + window) / kWeightKeys + 2) : p.blocks;
-    auto runs = [&](int64_t rows, int64_t workgroups) {
-      const int64_t least = ((rows + group - 1) / group + kWeightRows - 1) / kWeightRows * kWeightRows;
+    auto runs = [&](int64_t fewest, int64_t workgroups) {
+      const int64_t least = ((fewest + group - 1) / group + kWeightRows - 1) / kWeightRows * kWeightRows;
       return std::min((most_tokens + least - 1) / least, workgroups / (seen * R * G));
     };
     const int64_t most = std::max<int64_t>({1, runs(kRunRows[0], kRunWorkgroups[0]), runs(kRunRows[1], kRunWorkgroups[1])});
@@ -974,6 +994,7 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
                 "%s: bad sizes (tokens %d, R %d, max_q_len %d, heads %d / %d, window %d, blocks %lld, table %d wide, "
                 "stride %lld, width %d, page %d)", what, T, R, max_q_len, num_q_heads, num_kv_heads, window,
                 (long long)num_blocks, table_width, (long long)table_stride, width, page_size);
+  max_q_len = std::max(std::min(max_q_len, T), 1);
   const int32_t group = num_q_heads / num_kv_heads;
   if (head_dim != 64 && head_dim != 128)
     return fail(SNA_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", what, head_dim);
@@ -998,7 +1019,9 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
   if (head_stride < width || row_stride < width)
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: weight strides %lld / %lld for %d columns", what, (long long)row_stride,
                 (long long)head_stride, width);
-  max_q_len = std::max(max_q_len, 1);
+  if (((int64_t)max_q_len * group + kWeightRows - 1) / kWeightRows > kGridMax)
+    return fail(SNA_ERR_UNSUPPORTED, "%s: chunks of up to %d tokens of %d heads a KV head exceed the grid (split them)",
+                what, max_q_len, group);
   const WeightsPlan plan = weights_plan(T, R, max_q_len, num_q_heads, num_kv_heads, page_size, table_width, width,
                                         head_dim, kv_dtype == SNA_DTYPE_BF16 ? 2 : 1, window);
   const int64_t blocks = plan.blocks;
@@ -1049,9 +1072,11 @@ int attention_weights(const char* what, const void* q, const void* k_cache, cons
   a.ws_score = plan.scores ? (float*)((uint8_t*)workspace + plan.part) : nullptr;
   const hipStream_t s = (hipStream_t)stream;
   if (kv_dtype != SNA_DTYPE_BF16) {
-    if (head_dim == 128) launch_weights<128, 1>(a, (uint32_t)wgs, plan.row_floats, s); else launch_weights<64, 1>(a, (uint32_t)wgs, plan.row_floats, s);
+    if (head_dim == 128) launch_weights<128, 1>(a, (uint32_t)wgs, plan.row_floats, s);
+    else launch_weights<64, 1>(a, (uint32_t)wgs, plan.row_floats, s);
   } else {
-    if (head_dim == 128) launch_weights<128, 2>(a, (uint32_t)wgs, plan.row_floats, s); else launch_weights<64, 2>(a, (uint32_t)wgs, plan.row_floats, s);
+    if (head_dim == 128) launch_weights<128, 2>(a, (uint32_t)wgs, plan.row_floats, s);
+    else launch_weights<64, 2>(a, (uint32_t)wgs, plan.row_floats, s);
   }
   return check_launch(what);
 }
@@ -1065,8 +1090,8 @@ extern "C" int64_t sna_attention_weights_workspace_bytes(int32_t n_tokens, int32
   if (n_tokens < 0 || R < 1 || max_q_len < 0 || num_q_heads < 1 || num_kv_heads < 1 ||
       num_q_heads % num_kv_heads != 0 || page_size < 1 || table_width < 1 || width < 0)
     return 0;
-  return weights_plan(n_tokens, R, std::max(max_q_len, 1), num_q_heads, num_kv_heads, page_size, table_width, width, head_dim,
-                      kv_dtype == SNA_DTYPE_BF16 ? 2 : 1, window).bytes;
+  return weights_plan(n_tokens, R, std::max(std::min(max_q_len, n_tokens), 1), num_q_heads, num_kv_heads, page_size,
+                      table_width, width, head_dim, kv_dtype == SNA_DTYPE_BF16 ? 2 : 1, window).bytes;
 }
 
 extern "C" int sna_prefill_attention_weights(const void* q, const void* k_cache, const float* k_scale,

@@ -248,6 +248,21 @@ def test_few_rows_bad_pages_and_nan():
     got[0, 1] = 0
     want[0, 1] = 0
     check(c, got, want, reach, "beside a NaN")
+    # most exponentials of a row underflow: a NaN of its sum reaches them all the same, in every form
+    for n in (64, 4):
+        few = ops.decode_attention_weights(args[0][:n], args[1], args[2][:n], lens[:n], sm_scale=40.0).cpu()
+        assert bool(few[0, 1, :2100].isnan().all()) and bool((few[0, :, 2100:] == 0).all())
+        assert bool(torch.isfinite(few[0, [0, 2, 3]]).all()) and bool(torch.isfinite(few[1:]).all())
+
+
+def test_a_longest_query_count_past_the_tokens():
+    """max_q_len is an upper bound: any that holds gives the same weights."""
+    c = make(29, 8, 2, 64, 16, [300, 40], [40, 3], False)
+    dev = [t.to(DEV) for t in (c.q, c.k, c.table)]
+    start, prior = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (c.start, c.prior))
+    want, reach = oracle(c, c.table.shape[1] * 16)
+    for most in (40, 43, 10 ** 6, 2 ** 31 - 1):
+        check(c, ops.prefill_attention_weights(*dev, start, prior, max_q_len=most, sm_scale=c.scale), want, reach, str(most))
 
 
 def test_decode_rows_without_keys():
