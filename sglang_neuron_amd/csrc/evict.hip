@@ -14,7 +14,10 @@
 //            independent, so several workgroups share a row by columns, and K and V are apart. To other pages nothing
 //            orders the tokens and the tiles go to workgroups of their own.
 // Both are bound by memory (latency for few rows): select reads 4 bytes a token and head, compact reads and writes the
-// kept rows.
+// kept rows. Measured (us, 8 KV heads): select of one row of 1000 tokens 7.4 (a chain of 3 histograms on one CU), of 32 rows
+// of up to 8192 12.7, of 4 rows of 50001 to 131072 7 + 9 + 10 + 17 (three passes and the writer, each one round trip and the
+// row's histograms); compact to other pages of 32 x 1024 e4m3fn tokens of 128 24, 5.6 TB/s read and written, of 4 x 8192 bf16
+// 62, 4.3 TB/s (a plain copy: 4.8), in place 26 and 94.
 #include <algorithm>
 
 #include "sna_device.h"
@@ -355,10 +358,19 @@ struct CompactArgs {
   int32_t chunks;  // workgroups that share a row's tokens (1 in place)
 };
 
-constexpr int kCompactThreads = 256;
+// In place a workgroup walks all of a row's tokens (of some columns), and large tiles make it few round trips: 4096 tokens of
+// 16384 (one row, 8 KV heads of 128, bf16) took 58 us by 256 threads and 28 by 1024, 8192 of 32768 (4 rows) 142 and 94. To
+// other pages the tiles are shared out, and small ones start sooner.
+constexpr int kCompactThreads = 256, kCompactInPlace = 1024;
 constexpr int kCompactUnroll = 4;  // 16-byte pieces a thread holds
+// In place a workgroup takes 128 bytes of a token's row where that makes so many workgroups at least, else 64 where that makes
+// so few, else 32. In us by 32 / 64 / 128 (heads of 128): 1024 workgroups of 128 bytes (32 rows, 1024 of 8192 tokens, bf16)
+// 134 / 88 / 69, 512 (the same, e4m3fn) 63 / 36 / 26, 128 (4 rows, 8192 of 32768, bf16) 123 / 93 / 126, 128 (8 rows, e4m3fn)
+// 18 / 12 / 16, 32 (one row) 21 / 28 / 46. (Whole rows of 256 bytes: 66 where 128 take 69, and 81 where 32 take 21.)
+constexpr int64_t kCompactWide = 512, kCompactFew = 128;
 
-__global__ __launch_bounds__(kCompactThreads) void compact_tokens_kernel(CompactArgs a) {
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void compact_tokens_kernel(CompactArgs a) {
   const int32_t chunk = blockIdx.x;
   const int32_t slice = blockIdx.y % a.slices, g = blockIdx.y / a.slices % a.G, kv = blockIdx.y / a.slices / a.G;
   const int32_t r = blockIdx.z;
@@ -369,13 +381,13 @@ __global__ __launch_bounds__(kCompactThreads) void compact_tokens_kernel(Compact
   const int32_t* const src_row = a.table + r * a.table_stride;
   const int32_t* const dst_row = a.dst + r * a.dst_stride;
   const int32_t col = (threadIdx.x & (pieces - 1)) * 16 + slice * (a.row_bytes / a.slices);
-  const int32_t per = kCompactThreads * kCompactUnroll >> sh;  // tokens of a tile
+  const int32_t per = THREADS * kCompactUnroll >> sh;  // tokens of a tile
   for (int32_t i0 = chunk * per; i0 < a.keep; i0 += a.chunks * per) {  // uniform
     uint4 v[kCompactUnroll];
     uint8_t* to[kCompactUnroll];
 #pragma unroll
     for (int u = 0; u < kCompactUnroll; ++u) {
-      const int32_t i = i0 + ((u * kCompactThreads + (int32_t)threadIdx.x) >> sh);
+      const int32_t i = i0 + ((u * THREADS + (int32_t)threadIdx.x) >> sh);
       to[u] = nullptr;
       v[u] = make_uint4(0, 0, 0, 0);
       const int32_t from = i < a.keep ? kept[i] : -1;
@@ -390,7 +402,7 @@ __global__ __launch_bounds__(kCompactThreads) void compact_tokens_kernel(Compact
       to[u] = dst;
       v[u] = ld16(src);
     }
-    if (a.chunks == 1) {  // in place: the tile is read before any of it is written
+    if (THREADS == kCompactInPlace) {  // in place: the tile is read before any of it is written
       wait_vmcnt<0>();
       __syncthreads();
     }
@@ -430,6 +442,8 @@ struct SelectLaunch {
   SelectLong b;
   void run(hipStream_t s) const {
     const dim3 block(kSelectThreads), grid(a.G, a.R);
+    // (no more keys a thread than the widest row can need: 32 rows of 8192 took 11.7 us with 8 and 14.1 with 16, 64 of 2048
+    // 8.9 with 4 and 13.1 with 16)
     if (a.width <= kSelectSegment / 4) {
       hipLaunchKernelGGL((select_row_kernel<kSelectMost / 4>), grid, block, 0, s, a);
     } else if (a.width <= kSelectSegment / 2) {
@@ -511,7 +525,10 @@ int plan_select(const char* what, const float* weights, int64_t row_stride, int6
 struct CompactLaunch {
   CompactArgs a;
   dim3 grid;
-  void run(hipStream_t s) const { hipLaunchKernelGGL(compact_tokens_kernel, grid, dim3(kCompactThreads), 0, s, a); }
+  void run(hipStream_t s) const {
+    if (a.dst == a.table) hipLaunchKernelGGL((compact_tokens_kernel<kCompactInPlace>), grid, dim3(kCompactInPlace), 0, s, a);
+    else hipLaunchKernelGGL((compact_tokens_kernel<kCompactThreads>), grid, dim3(kCompactThreads), 0, s, a);
+  }
 };
 
 int plan_compact(const char* what, void* k_cache, void* v_cache, int64_t num_blocks, int32_t num_kv_heads,
@@ -554,9 +571,16 @@ int plan_compact(const char* what, void* k_cache, void* v_cache, int64_t num_blo
   a.kept = kept;
   a.R = R;
   a.keep = keep;
-  a.slices = dst_table ? 1 : a.row_bytes / 64;
-  const int32_t per = kCompactThreads * kCompactUnroll / (a.row_bytes / a.slices / 16);
-  a.chunks = dst_table ? (int32_t)std::min<int64_t>(((int64_t)keep + per - 1) / per, 65535) : 1;
+  if (dst_table) {
+    const int32_t per = kCompactThreads * kCompactUnroll / (a.row_bytes / 16);
+    a.slices = 1;
+    a.chunks = (int32_t)std::min<int64_t>(((int64_t)keep + per - 1) / per, 65535);
+  } else {
+    const int64_t columns = 2 * (int64_t)R * num_kv_heads * a.row_bytes;
+    const int32_t bytes = columns >= 128 * kCompactWide ? 128 : columns >= 64 * kCompactFew ? 64 : 32;
+    a.slices = std::max(a.row_bytes / bytes, 1);
+    a.chunks = 1;
+  }
   const int64_t y = (int64_t)a.slices * num_kv_heads * 2;
   if (R > 65535 || y > 65535)
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %d rows x %d KV heads exceed the grid", what, R, num_kv_heads);

@@ -13,7 +13,8 @@
 // 8 j .. 8 j + 7 (one 16-byte load), the next heads' rows are on their way while these are worked on. The tokens' sines and
 // cosines are computed once by the workgroup's threads (one each for two pairs of a token at D = 128) and handed round
 // through LDS; a lane keeps its own in registers for every head. Bound by memory: every projection row is read once, every
-// Q, K and V row written once.
+// Q, K and V row written once: 185 MB for 8192 tokens of heads 32/8 of 128 to an e4m3fn pool in 42 us, 4.4 TB/s, where a
+// plain copy reaches 4.8; few tokens by one launch's round trips (4.7 us).
 #include <algorithm>
 
 #include "sna_device.h"
@@ -184,7 +185,9 @@ __global__ __launch_bounds__(256) void qkv_norm_mrope_store_kernel(MropeArgs a) 
   }
 }
 
-// Workgroups that a launch is worth: a token block's heads are shared out until there are so many.
+// A token block's heads are shared out until a launch has so many workgroups: 8 tokens of heads 16/8 of 128 take 4.7 us so and
+// 10.4 with a workgroup for all heads, 1531 of heads 24/4 of 64 6.0 and 7.9; 8192 tokens of heads 32/8 of 128 take 42 with
+// their heads in one workgroup and 56 with one a head group, which computes their angles each time.
 constexpr int64_t kMropeWorkgroups = 1024;
 
 }  // namespace sna

@@ -105,7 +105,10 @@ def _table(seed, pages, nb, width, first=1):
 @pytest.mark.parametrize("G,P,d,fp8,lens,keep", [
     (1, 16, 64, True, [5], 2), (2, 16, 128, True, [300, 40, 1], 37), (2, 16, 128, False, [300, 40, 0], 37),
     (3, 7, 64, False, [100, 99], 64), (1, 128, 128, False, [3000, 2500], 2000), (8, 16, 64, True, [900] * 5, 512),
-    (2, 64, 128, True, [9000], 4500), (1, 16, 128, False, [1200], 1199)])
+    (2, 64, 128, True, [9000], 4500), (1, 16, 128, False, [1200], 1199),
+    # in place by columns of 64 and of 128 bytes, more than a tile of each
+    (2, 16, 128, False, [1400, 5, 1101] * 7, 1100), (8, 16, 128, True, [520 + 10 * i for i in range(32)], 515),
+    (2, 48, 128, False, [600] * 64, 513)])
 @pytest.mark.parametrize("where", ["in-place", "other-pages"])
 def test_compact(G, P, d, fp8, lens, keep, where):
     announce(f"compact {where} {lens} -> {keep}")
