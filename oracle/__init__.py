@@ -26,5 +26,7 @@ How each function is pinned (tests/test_oracle_*.py):
   qkv      RoPE at angle 0 is the identity and at a quarter turn the exact rotate-half; RoPE against complex
            multiplication in float64 within its three bf16 roundings; RMSNorm of a constant-magnitude head against
            its closed form; the writes against the pinned MHA store.
+  weights  (no reference counterpart) closed forms of equal keys with a window and a sink; selection of hand-made rows;
+           compaction of a hand-made table; the rotation against complex multiplication.
 Nothing here is "parity unpinned"; see the tests for the pin of each function.
 """

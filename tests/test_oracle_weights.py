@@ -36,6 +36,15 @@ def test_selection_against_a_hand_made_row():
     assert kept[0, 0].tolist() == [0, 1, 2, -1, -1] and new == [3]
 
 
+def test_compaction_of_a_hand_made_table():
+    cache = torch.arange(4 * 2 * 2).view(4, 1, 2, 2)  # token o of page p: [4 p + 2 o, 4 p + 2 o + 1]
+    out = ow.compact_tokens(cache, torch.tensor([[2, 1, 3]]), torch.tensor([[[0, 3, 4, -1]]]))
+    assert out[2, 0].tolist() == [[8, 9], [6, 7]] and out[1, 0].tolist() == [[12, 13], [6, 7]]
+    assert torch.equal(out[3], cache[3]) and torch.equal(out[0], cache[0])
+    out = ow.compact_tokens(cache, torch.tensor([[2, 1, -1]]), torch.tensor([[[1, 2, 4]]]), torch.tensor([[3, 9]]))
+    assert out[3, 0].tolist() == [[10, 11], [4, 5]] and torch.equal(out[:3], cache[:3])
+
+
 def test_mrope_rotation_is_complex_multiplication():
     g = torch.Generator().manual_seed(1)
     x = torch.randn(3, 3 * 4, generator=g).double()
