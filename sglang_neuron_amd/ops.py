@@ -998,7 +998,7 @@ def _attention_weights(what, q, T, R, k_cache, block_table, q_start, lens, max_q
     dev = _on_gpu(q, k_cache, block_table, q_start, lens, k_scale, sinks, weights)
     _, H, d = q.shape
     shape = k_cache.shape
-    if len(shape) != 4 or not k_cache.is_contiguous() or shape[3] != d or H % shape[1]:
+    if len(shape) != 4 or not k_cache.is_contiguous() or shape[3] != d or shape[1] < 1 or H % shape[1]:
         _need(False, f"the cache must be contiguous [blocks, kv_heads, page, {d}] with kv_heads dividing {H}, got "
               f"{tuple(shape)}")
     nb, G, P, _ = shape

@@ -328,6 +328,22 @@ def test_a_chunk_of_its_own_sums_to_its_rows():
     assert bool(((got - want).abs() <= want * (128 + 8 + 2800) * 2.0 ** -24).all())
 
 
+@pytest.mark.parametrize("R,counts", [(4, 1), (64, 1), (2, 40)])
+def test_cache_offsets_past_32_bits(R, counts):
+    """The same pages far behind 4 GiB of a pool give the same bits, in every form."""
+    c = few_rows(R, 8, 4, 128, 16, 2060, counts, False, seed=31)
+    nb, page = len(c.k), c.k[0].numel() * 2
+    far = (2 ** 32 + 2 ** 30) // page
+    k = torch.zeros(far + nb, *c.k.shape[1:], dtype=torch.bfloat16, device=DEV)
+    k[far:] = c.k.to(DEV)
+    start, prior = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (c.start, c.prior))
+    table = c.table.to(DEV)
+    got = ops.prefill_attention_weights(c.q.to(DEV), k, torch.where(table >= 0, table + far, table), start, prior,
+                                        max_q_len=max(c.counts), sm_scale=c.scale)
+    near = prefill(c)
+    assert torch.equal(got, near) and bool((near[0] > 0).any())
+
+
 def test_bad_offsets_and_lengths_stay_inside():
     """Device offsets outside q, chunks past max_q_len and lengths past the table are cut, never followed."""
     c = make(17, 8, 2, 64, 16, [64, 64], [8, 8], False, junk=False)

@@ -275,6 +275,27 @@ def test_the_first_pages_of_the_table_as_target_are_in_place():
     assert torch.equal(_bytes(dv), _bytes(ow.compact_tokens(v.view(torch.int16), table, want)))
 
 
+@pytest.mark.parametrize("where", ["in-place", "other-pages"])
+def test_cache_offsets_past_32_bits(where):
+    """Tokens move between pages far behind 4 GiB of a pool as between the first ones."""
+    P, G, d, lens, keep = 64, 8, 128, [900, 333], 100
+    pages = [15, 6]
+    near = _table(1, pages, 22 + 4, 15)
+    dst = _table(2, [2, 2], 4, 2, first=0) + 22 if where == "other-pages" else None
+    near = torch.where(near >= 22, -1, near)  # (the last four are the targets': holes)
+    k, v = _cache(3, 26, G, P, d, False), _cache(4, 26, G, P, d, False)
+    kept, _ = ow.select_tokens(_weights(5, 2, G, 900, "plain"), lens, keep, 2, 10)
+    far = (2 ** 32 + 2 ** 30) // (G * P * d * 2)
+    big = [torch.zeros(far + 26, G, P, d, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    for b, t in zip(big, (k, v)):
+        b[far:] = t.to(DEV)
+    up = lambda t: None if t is None else torch.where(t >= 0, t + far, t).to(DEV)  # noqa: E731
+    ops.compact_tokens(*big, up(near), kept.to(DEV), dst_table=up(dst))
+    assert torch.equal(_bytes(big[0][far:]), _bytes(ow.compact_tokens(k.view(torch.int16), near, kept, dst)))
+    assert torch.equal(_bytes(big[1][far:]), _bytes(ow.compact_tokens(v.view(torch.int16), near, kept, dst)))
+    assert not bool(big[0][:far].any())
+
+
 def test_graph_and_side_stream():
     P, G, d, R = 16, 2, 128, 3
     lens, keep = [400, 100, 50], 64

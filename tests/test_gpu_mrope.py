@@ -142,6 +142,28 @@ def test_strides_slots_and_nan():
     assert bool((kc.view(torch.uint8)[0, :, 1:] == 0).all())  # only slot 0 of the reserved page is written
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_cache_offsets_past_32_bits(fp8):
+    """Slots far behind 4 GiB of a pool receive what the first ones do."""
+    T, Hq, Hkv, d, P = 40, 8, 4, 128, 16
+    qkv, pos, inv, gam, slots, k, v, sc = _make(11, T, Hq, Hkv, d, P, fp8, True, 128, 3, 77)
+    axes = ops.mrope_axes([16, 24, 24])
+    q, kc, vc = _run(qkv, pos, inv, axes, Hq, Hkv, d, k, v, slots, gam, sc)
+    far = (2 ** 32 + 2 ** 30) // (k[0].numel() * k.element_size())
+    big = [torch.zeros(far + len(k), Hkv, P, d, dtype=torch.uint8 if fp8 else torch.int16, device=DEV).view(k.dtype)
+           for _ in range(2)]
+    raw = lambda t: t.view(torch.uint8 if fp8 else torch.int16)  # noqa: E731
+    for b, t in zip(big, (k, v)):
+        raw(b)[far:] = raw(t).to(DEV)
+    got = ops.qkv_norm_mrope_store(
+        qkv.to(DEV), positions=pos.to(DEV), inv_freq=inv.to(DEV), axes=axes, num_q_heads=Hq, num_kv_heads=Hkv, d_head=d,
+        k_cache=big[0], v_cache=big[1], slot_mapping=(slots + far * P).to(DEV), q_norm=gam[0].to(DEV),
+        k_norm=gam[1].to(DEV), k_scale=sc[0].to(DEV) if fp8 else None, v_scale=sc[1].to(DEV) if fp8 else None)
+    assert torch.equal(got.cpu(), q)
+    assert torch.equal(raw(big[0])[far:].cpu(), raw(kc)) and torch.equal(raw(big[1])[far:].cpu(), raw(vc))
+    assert not bool(raw(big[0])[:far].any())
+
+
 def test_refusals_and_empty():
     T, Hq, Hkv, d, P = 4, 2, 1, 64, 16
     qkv, pos, inv, gam, slots, k, v, sc = _make(7, T, Hq, Hkv, d, P, True, False, 64, 2, 0)
