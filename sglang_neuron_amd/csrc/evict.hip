@@ -15,7 +15,7 @@
 //            orders the tokens and the tiles go to workgroups of their own.
 // Both are bound by memory (latency for few rows): select reads 4 bytes a token and head, compact reads and writes the
 // kept rows. Measured (us, 8 KV heads): select of one row of 1000 tokens 7.4 (a chain of 3 histograms on one CU), of 32 rows
-// of up to 8192 12.7, of 4 rows of 50001 to 131072 7 + 9 + 10 + 17 (three passes and the writer, each one round trip and the
+// of up to 8192 12.7, of 4 rows of 50001 to 131072 7 + 9 + 10 + 14 (three passes and the writer, each one round trip and the
 // row's histograms); compact to other pages of 32 x 1024 e4m3fn tokens of 128 24, 5.6 TB/s read and written, of 4 x 8192 bf16
 // 62, 4.3 TB/s (a plain copy: 4.8), in place 26 and 94.
 #include <algorithm>
@@ -316,14 +316,16 @@ __global__ __launch_bounds__(kSelectThreads) void select_write_kernel(SelectArgs
   if (seg == 0) {
     if (g == 0 && threadIdx.x == 0) a.new_lens[r] = s.n;
     select_first(a, s, kept, out);
-    if (!s.whole) select_recent(a, s, kept, out);
   }
+  if (seg == 1 && !s.whole) select_recent(a, s, kept, out);  // (there are two at least; another than the first's)
   if (!s.whole && a.keep > a.first + a.recent) {  // uniform
     SelectKeys<kSelectMost> x;
     x.load(s, seg);
     const SelectFound f = select_fold(sm, a, b, row, seg, 2);
     uint32_t above = f.prior_above;
-    for (int32_t i = 0; i < seg; ++i) above += b.above[(int64_t)row * b.S + i];
+    const uint32_t* const counts = b.above + (int64_t)row * b.S;
+#pragma unroll 8
+    for (int32_t i = 0; i < seg; ++i) above += counts[i];
     select_write(sm, a, x, f.T, 0, f.need, above, f.prior_equal, kept, out);
   }
   if (out && !(b.kept_w && !s.whole))
