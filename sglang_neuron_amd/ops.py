@@ -9,6 +9,7 @@ Reference interfaces each function stands in for are cited per function (paths u
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional, Sequence, Union
 
@@ -266,8 +267,9 @@ def qkv_norm_mrope_store(qkv: Tensor, *, positions: Tensor, inv_freq: Tensor, ax
         positions = positions.contiguous()
     inv_freq = _contig(inv_freq if inv_freq.dim() == 1 else inv_freq.reshape(-1), "inv_freq", torch.float32)
     n = inv_freq.shape[0]
-    if len(axes) != n or (n > 0 and not (min(axes) >= 0 and max(axes) < positions.shape[0])):
-        _need(False, f"{len(axes)} axes for {n} rotated pairs, each in [0, {positions.shape[0]})")
+    if len(axes) != n:
+        _need(False, f"{len(axes)} axes for {n} rotated pairs")
+    axes = bytes(axes)  # (ValueError outside [0, 256); the library refuses the others that are no axis)
     slots = _contig(_as(slot_mapping if slot_mapping.dim() == 1 else slot_mapping.reshape(-1), torch.int64), "slot_mapping")
     if slots.shape[0] != T:
         _need(False, f"{slots.shape[0]} slots for {T} tokens")
@@ -289,7 +291,7 @@ def qkv_norm_mrope_store(qkv: Tensor, *, positions: Tensor, inv_freq: Tensor, ax
         _need(False, "bad q_out tensor")
     _launch(dev, _lib.load().sna_qkv_norm_mrope_store, "qkv_norm_mrope_store", qkv.data_ptr(), stride, T, num_q_heads,
             num_kv_heads, d_head, _ptr(q_norm), _ptr(k_norm), norm_eps, positions.data_ptr(),
-            max(positions.stride(0), T), positions.shape[0], inv_freq.data_ptr(), n, bytes(axes), slots.data_ptr(),
+            max(positions.stride(0), T), positions.shape[0], inv_freq.data_ptr(), n, axes, slots.data_ptr(),
             q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), nb, P, code)
     return q_out
 
@@ -993,6 +995,12 @@ def _weight_strides(weights: Tensor, R: int, G: int, what: str) -> tuple[int, in
     return row, head
 
 
+@functools.lru_cache(maxsize=1024)
+def _weights_workspace(*sizes: int) -> int:
+    """sna_attention_weights_workspace_bytes, a function of sizes alone (a decode loop asks for the same ones)."""
+    return _lib.load().sna_attention_weights_workspace_bytes(*sizes)
+
+
 def _attention_weights(what, q, T, R, k_cache, block_table, q_start, lens, max_q_len, sm_scale, k_scale, sinks, window,
                        weights, scales_multiply) -> Tensor:
     dev = _on_gpu(q, k_cache, block_table, q_start, lens, k_scale, sinks, weights)
@@ -1024,7 +1032,8 @@ def _attention_weights(what, q, T, R, k_cache, block_table, q_start, lens, max_q
         row, head = G * N, N
         weights = torch.empty(R, G, N, dtype=torch.float32, device=dev)
     lib = _lib.load()
-    need = lib.sna_attention_weights_workspace_bytes(T, R, max_q_len, H, G, d, P, W, N, code, window)
+    window = int(window)
+    need = _weights_workspace(T, R, max_q_len, H, G, d, P, W, N, code, window)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     stride = max(table.stride(0), W)
     if q_start is None:
@@ -1089,6 +1098,12 @@ def select_tokens(weights: Tensor, seq_lens: Tensor, *, keep: int, first: int = 
     return kept, new_lens
 
 
+@functools.lru_cache(maxsize=1024)
+def _select_workspace(*sizes: int) -> int:
+    """sna_select_workspace_bytes, a function of sizes alone."""
+    return _lib.load().sna_select_workspace_bytes(*sizes)
+
+
 def _select_args(dev, weights, seq_lens, keep, first, recent, weights_out):
     """(sna_select_tokens' arguments, its results, tensors that they point into)."""
     if weights.dim() != 3:
@@ -1114,7 +1129,7 @@ def _select_args(dev, weights, seq_lens, keep, first, recent, weights_out):
     new_lens = torch.empty(R, dtype=torch.int32, device=dev)
     need, ws = 0, None
     if R > 0 and G > 0:
-        need = _lib.load().sna_select_workspace_bytes(R, G, N, keep, same)
+        need = _select_workspace(R, G, N, keep, same)
         if need > 0:
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
     return (weights.data_ptr(), row, head, N, lens.data_ptr(), R, G, keep, first, recent, kept.data_ptr(),
