@@ -23,9 +23,10 @@
 // keys at 4.2 TB/s (HBM: a plain copy reaches 4.8); 8 rows of 128-1024 bf16 keys, heads 16/8, 5.2 + 4.4 (two launches and
 // their chains of round trips); 128 rows of 2048-8192 keys, heads 8/1 of 64, 17 + 8 (the same, ragged); 32 queries over
 // each of 3001 to 16384 keys 22.8 + 5 + 26.8 (three launches' chains of loads) and 64 over 131071 bf16 keys 105 + 10 + 115
-// (products 28-31% and VALU 50-56% of the cycles, the keys read twice at 2.6 TB/s); 4 x 2048 queries after 2048 each 470-490 in all, the first pass a little over
-// half: products take 37% (41% in the second pass) of a SIMD's cycles and VALU instructions 61% (57%), which together is
-// all of them: a wave's matrix instructions and the other waves' VALU hardly overlap here.
+// (products 28-31% and VALU 50-56% of the cycles, the keys read twice at 2.6 TB/s); 4 x 2048 queries after 2048 each 470-490
+// in all, the first pass a little over half: products take 37% (41% in the second pass) of a SIMD's cycles and VALU
+// instructions 61% (57%), which together is all of them: a wave's matrix instructions and the other waves' VALU hardly
+// overlap here.
 #include <algorithm>
 #include <type_traits>
 
@@ -243,7 +244,8 @@ __device__ __forceinline__ float2 weights_stats(f32x16_t (&x)[2], float c2, uint
 // the lane, and a key's sum over the rows stays in the lane's registers until the end, where it is added across the lanes
 // once. A tile costs a wave 32 exponentials a lane (8 cycles each), as many fused multiply-adds, and at head_dim 128 16
 // products of 32 cycles. Products and exponentials of one wave take turns, on three waves a SIMD. (The next tile's products
-// among the exponentials, on two waves a SIMD, took 620 us for 4 x 2048 after 2048 where this took 590.) Pairs of tiles that all of the wave's keys are seen by take a path without masks.
+// among the exponentials, on two waves a SIMD, took 620 us for 4 x 2048 after 2048 where this took 590.) Pairs of tiles whose
+// rows see all of the wave's keys take a path without masks.
 enum WeightsPass { kStats, kSum };
 template <int D, int ESZ>
 struct WeightsRing {
@@ -902,9 +904,9 @@ constexpr int64_t kRowPairs = 256, kRowKeys = 2048;  // the CUs, and the least k
 constexpr int32_t kRowFloats[2] = {18432, 36864};    // LDS of two workgroups a CU, or one
 constexpr int64_t kScoreWorkgroups = 1024;  // a score launch has so many at least before one takes several chunks
 // Queries are cut into runs of at least so many rows while that makes no more than so many workgroups: by 4 tiles up to two
-// rounds of the 3 workgroups that a CU holds, by 8 up to four. One run each: 635 queries of 8 heads over 2270 keys 100 us
-// (29 cut), 300 of a window of 128 86 (39), 1024 of 32 heads over 8192 keys 327 (293), 4 x 2048 over 4096 keys 497 (470).
-constexpr int64_t kRunRows[2] = {128, 256}, kRunWorkgroups[2] = {1536, 3072};
+// rounds of the 3 workgroups that a CU holds, by 8 up to ten a CU. One run each: 635 queries of 8 heads over 2270 keys 100 us
+// (29 cut), 300 of a window of 128 86 (39), 1024 of 32 heads over 8192 keys 327 (295), 4 x 2048 over 4096 keys 497 (479).
+constexpr int64_t kRunRows[2] = {128, 256}, kRunWorkgroups[2] = {1536, 2560};
 WeightsPlan weights_plan(int64_t T, int64_t R, int64_t max_q, int32_t H, int32_t G, int32_t page_size,
                          int32_t table_width, int32_t width, int32_t head_dim, int32_t esz, int32_t window) {
   WeightsPlan p;
