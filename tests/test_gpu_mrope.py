@@ -164,6 +164,81 @@ def test_cache_offsets_past_32_bits(fp8):
     assert not bool(raw(big[0])[:far].any())
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_an_image_prompt_written_weighed_thinned_and_read(fp8):
+    """A prompt of text, an image's patches and text goes in by the writer, its keys are weighed by its last queries, the
+    cache is thinned in place, and the next token is written behind it at the position that follows the prompt's: its
+    attention and weights equal, bit for bit, those over a fresh cache that holds the kept rows alone."""
+    Hq, G, d, P, keep, scale = 8, 2, 128, 16, 70, 128 ** -0.5
+    lens = [300, 41]
+    R, T = len(lens), sum(lens)
+    g = torch.Generator().manual_seed(21)
+    rows = torch.randn(T + R, (Hq + 2 * G) * d, generator=g).to(torch.bfloat16).to(DEV)
+    inv = (10000.0 ** (-torch.arange(64) / 64)).float().to(DEV)
+    axes = ops.mrope_axes([16, 24, 24])
+    gam = [torch.rand(d, generator=g).add(0.5).to(torch.bfloat16).to(DEV) for _ in range(2)]
+    pos, after = [], []
+    for n in lens:
+        text, side = n // 4, 5
+        patches = n // 2
+        p = torch.stack([torch.arange(n)] * 3)
+        at = torch.arange(patches)
+        p[:, text:text + patches] = text + torch.stack([at * 0, at // side, at % side])
+        p[:, text + patches:] = int(p[:, :text + patches].max()) + 1 + torch.arange(n - text - patches)
+        pos.append(p)
+        after.append(p[:, -1:] + 1)
+    pos, after = torch.cat(pos, 1).to(DEV), torch.cat(after, 1).to(DEV)
+    pages = [-(-(n + 1) // P) for n in lens]
+    nb = 1 + sum(pages)
+    perm = (torch.randperm(nb - 1, generator=g) + 1).tolist()
+    table = torch.full((R, max(pages)), -1, dtype=torch.int32)
+    for r, n in enumerate(pages):
+        table[r, :n] = torch.tensor([perm.pop() for _ in range(n)])
+    table = table.to(DEV)
+    slot = lambda r, i: table[r, i // P].long() * P + i % P  # noqa: E731
+    slots = torch.cat([slot(r, torch.arange(n, device=DEV)) for r, n in enumerate(lens)])
+    cache = [torch.zeros(nb, G, P, d, dtype=FP8 if fp8 else torch.bfloat16, device=DEV) for _ in range(2)]
+    sc = [torch.full((G,), 0.02, device=DEV) if fp8 else None for _ in range(2)]
+
+    def write(x, at, where, kc, vc):
+        return ops.qkv_norm_mrope_store(x, positions=at, inv_freq=inv, axes=axes, num_q_heads=Hq, num_kv_heads=G, d_head=d,
+                                        k_cache=kc, v_cache=vc, slot_mapping=where, q_norm=gam[0], k_norm=gam[1],
+                                        k_scale=sc[0], v_scale=sc[1])
+
+    q = write(rows[:T], pos, slots, *cache)
+    whole = [c.clone() for c in cache]
+    last = torch.cat([torch.arange(n - 16, n) + sum(lens[:r]) for r, n in enumerate(lens)]).to(DEV)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    w = ops.prefill_attention_weights(q[last], cache[0], table, i32([0, 16, 32]), i32([n - 16 for n in lens]), max_q_len=16,
+                                      sm_scale=scale, k_scale=sc[0])
+    # without sinks every query's probabilities sum to 1: fp32 sums of at most 300 keys and 64 rows of scores whose products
+    # add up to at most scale * (1.5 * sqrt(d))^2 < 26 (normed rows times gammas under 1.5)
+    total = w.double().sum(-1)
+    assert bool(((total - 16 * Hq // G).abs() <= 16 * Hq // G * (2 * (d + 8) * 26 + 400) * 2.0 ** -24).all())
+    kept, new = ops.evict_tokens(*cache, table, i32(lens), w, keep=keep, first=4, recent=16, weights_out=w)
+    assert new.tolist() == [70, 41]
+    fresh = [torch.zeros_like(c) for c in cache]
+    raw = lambda t: t.view(torch.uint8 if fp8 else torch.int16)  # noqa: E731
+    for r in range(R):
+        n = int(new[r])
+        to = slot(r, torch.arange(n, device=DEV))
+        for h in range(G):
+            src = slot(r, kept[r, h, :n].long())
+            for a, b in zip(fresh, whole):
+                raw(a)[to // P, h, to % P] = raw(b)[src // P, h, src % P]
+    step = torch.stack([slot(r, new[r]) for r in range(R)])
+    outs = []
+    for kc, vc in (cache, fresh):
+        sq = write(rows[T:], after, step, kc, vc)
+        k, v = (raw(c)[step // P, :, step % P].view(c.dtype) for c in (kc, vc))
+        at = ops.decode_attention_weights(sq, kc, table, new + 1, sm_scale=scale, k_scale=sc[0])
+        out = ops.prefill_attention(sq, kc, vc, table, i32([0, 1, 2]), new, max_q_len=1, sm_scale=scale, k_scale=sc[0],
+                                    v_scale=sc[1])
+        outs.append((sq, raw(k), raw(v), at, out))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert bool((outs[0][3][0, :, :71] > 0).all()) and bool((outs[0][3][0, :, 71:] == 0).all())
+
+
 def test_refusals_and_empty():
     T, Hq, Hkv, d, P = 4, 2, 1, 64, 16
     qkv, pos, inv, gam, slots, k, v, sc = _make(7, T, Hq, Hkv, d, P, True, False, 64, 2, 0)
