@@ -22,7 +22,7 @@
 // Measured (us of kernels; heads 32/8 of 128, e4m3fn, pages of 16, where not said): 64 rows of 4096 keys 65.6, 273 MB of
 // keys at 4.2 TB/s (HBM: a plain copy reaches 4.8); 8 rows of 128-1024 bf16 keys, heads 16/8, 5.2 + 4.4 (two launches and
 // their chains of round trips); 128 rows of 2048-8192 keys, heads 8/1 of 64, 17 + 8 (the same, ragged); 32 queries over
-// each of 3001 to 16384 keys 22.8 + 5 + 26.8 (three launches' chains of loads) and 64 over 131071 bf16 keys 105 + 10 + 115
+// each of 3001 to 16384 keys 22.8 + 5 + 26.8 (three launches' chains of loads) and 64 over 131071 bf16 keys 105 + 6 + 115
 // (products 28-31% and VALU 50-56% of the cycles, the keys read twice at 2.6 TB/s); 4 x 2048 queries after 2048 each 470-490
 // in all, the first pass a little over half: products take 37% (41% in the second pass) of a SIMD's cycles and VALU
 // instructions 61% (57%), which together is all of them: a wave's matrix instructions and the other waves' VALU hardly
@@ -491,15 +491,17 @@ __global__ __launch_bounds__(256) void weights_reduce_kernel(WeightsArgs a) {
   *out = a.add ? *out + v : v;
 }
 
-// A row's blocks merged: (its largest score M in the log2 domain, 1 / sum of 2^(score - M) with the sink's). 32 rows a
-// workgroup, a row's blocks dealt to 8 threads.
+// A row's blocks merged: (its largest score M in the log2 domain, 1 / sum of 2^(score - M) with the sink's). ROWS rows a
+// workgroup, a row's blocks dealt to 256 / ROWS threads.
+template <int ROWS>
 __global__ __launch_bounds__(256) void weights_merge_kernel(WeightsArgs a) {
-  __shared__ float2 sm[8][32];
+  constexpr int SLICES = 256 / ROWS;
+  __shared__ float2 sm[SLICES][ROWS];
   const int32_t r = blockIdx.z, g = blockIdx.y;
   const WeightsRequest rq = weights_request(a, r);
-  const int i = threadIdx.x & 31, slice = threadIdx.x >> 5;
-  if ((int32_t)blockIdx.x * 32 >= rq.S * a.group) return;  // uniform
-  const int32_t m = min((int32_t)blockIdx.x * 32 + i, rq.S * a.group - 1);
+  const int i = threadIdx.x % ROWS, slice = threadIdx.x / ROWS;
+  if ((int32_t)blockIdx.x * ROWS >= rq.S * a.group) return;  // uniform
+  const int32_t m = min((int32_t)blockIdx.x * ROWS + i, rq.S * a.group - 1);
   const int32_t t = m / a.group, h = g * a.group + m - t * a.group;
   const int64_t pos = rq.prior + t;
   const int64_t rows = (int64_t)a.T * a.group;
@@ -510,13 +512,13 @@ __global__ __launch_bounds__(256) void weights_merge_kernel(WeightsArgs a) {
   if (hi >= lo) {
     const int32_t b1 = (int32_t)(hi / kWeightKeys);
 #pragma unroll 4
-    for (int32_t b = (int32_t)(lo / kWeightKeys) + slice; b <= b1; b += 8)
+    for (int32_t b = (int32_t)(lo / kWeightKeys) + slice; b <= b1; b += SLICES)
       p = weights_join(p, a.ws_part[((int64_t)g * a.blocks + b) * rows + row]);
   }
   sm[slice][i] = p;
   __syncthreads();
-  if (slice == 0 && (int32_t)blockIdx.x * 32 + i < rq.S * a.group) {
-    for (int s = 1; s < 8; ++s) p = weights_join(p, sm[s][i]);
+  if (slice == 0 && (int32_t)blockIdx.x * ROWS + i < rq.S * a.group) {
+    for (int s = 1; s < SLICES; ++s) p = weights_join(p, sm[s][i]);
     if (a.sinks) p = weights_join(p, make_float2(a.sinks[h] * kLog2e, 1.0f));
     // (a row that sees nothing: every score is dropped)
     a.ws_row[(int64_t)g * rows + row] = p.y == 0.0f ? make_float2(-kNegBig, 0.0f) : make_float2(p.x, 1.0f / p.y);
@@ -960,6 +962,10 @@ WeightsPlan weights_plan(int64_t T, int64_t R, int64_t max_q, int32_t H, int32_t
   return p;
 }
 
+// Up to so many rows (of all requests and KV heads) are merged 8 to a workgroup, a row's blocks by 32 threads, else 32 and by
+// 8: 2048 rows of 512 blocks take 6.1 us by 8 and 10.7 by 32, 4096 rows of 12 to 64 blocks 5.3 and 5.2, 262144 of 8 to 16
+// blocks 37 and 10.
+constexpr int64_t kMergeFewRows = 16384;
 template <int D, int ESZ>
 void launch_weights(const WeightsArgs& a, uint32_t wgs, int32_t row_floats, hipStream_t s) {
   if (row_floats > 0) {
@@ -976,8 +982,11 @@ void launch_weights(const WeightsArgs& a, uint32_t wgs, int32_t row_floats, hipS
     return;
   }
   hipLaunchKernelGGL((weights_tile_kernel<D, ESZ, kStats>), dim3(wgs), dim3(256), 0, s, a);
-  hipLaunchKernelGGL(weights_merge_kernel, dim3((unsigned)(((int64_t)a.max_q * a.group + 31) / 32), a.G, a.R), dim3(256),
-                     0, s, a);
+  const int64_t rows = (int64_t)a.max_q * a.group;
+  if (rows * a.G * a.R <= kMergeFewRows)
+    hipLaunchKernelGGL((weights_merge_kernel<8>), dim3((unsigned)((rows + 7) / 8), a.G, a.R), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((weights_merge_kernel<32>), dim3((unsigned)((rows + 31) / 32), a.G, a.R), dim3(256), 0, s, a);
   hipLaunchKernelGGL((weights_tile_kernel<D, ESZ, kSum>), dim3(wgs), dim3(256), 0, s, a);
   if (a.splits > 1)
     hipLaunchKernelGGL(weights_reduce_kernel, dim3((unsigned)((a.width + 255) / 256), a.G, a.R), dim3(256), 0, s, a);

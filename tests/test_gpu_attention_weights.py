@@ -107,6 +107,7 @@ CASES = [
     ("runs-group-3", 12, 4, 128, 16, [2000, 700, 1], [333, 700, 1], True, 0, True, 3),
     ("runs-odd-prior", 8, 1, 64, 16, [777, 1333], [500, 65], False, 0, False, 0),
     ("many-tiles", 16, 1, 128, 16, [700], [530], True, 0, False, 0),
+    ("many-rows-merged", 16, 2, 64, 16, [700, 650], [700, 300], True, 0, True, 2),
     ("many-rows", 2, 1, 64, 16, [5 + 13 * i for i in range(40)], [1 + i % 4 for i in range(40)], True, 0, False, 0),
 ]
 
