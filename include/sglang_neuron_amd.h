@@ -472,10 +472,12 @@ int sna_prefill_attention_split(const void *q, const void *k_cache, const void *
  *             requests' keys (valid ones below width) are added to, the rest is left as it is; 0: every column is
  *             written, zero where there is no key.
  *   workspace device, 16-byte aligned, at least sna_attention_weights_workspace_bytes bytes for the call's own
- *             sizes (a smaller batch can need more than a larger one), any contents; calls that share one on different
- *             streams race.
- * Every sum runs in a fixed order: the same call gives the same bits. The queries' rows of q lie inside [0, n_tokens);
- * offsets outside are cut. head_dim 64 or 128, any page size, num_q_heads / num_kv_heads <= 128.
+ *             sizes (a smaller batch can need more than a larger one; chunks take 8 bytes a token, query head and 256 keys
+ *             of the table's width, so long ones over wide tables are better passed in turn), any contents; calls that
+ *             share one on different streams race.
+ * q_start ascends (chunks that share rows of q share their statistics: such weights mean nothing). Every sum runs in a
+ * fixed order: the same call gives the same bits. The queries' rows of q lie inside [0, n_tokens); offsets outside are
+ * cut. head_dim 64 or 128, any page size, num_q_heads / num_kv_heads <= 128.
  * This has no reference counterpart. */
 int64_t sna_attention_weights_workspace_bytes(int32_t n_tokens, int32_t R, int32_t max_q_len, int32_t num_q_heads,
                                               int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
