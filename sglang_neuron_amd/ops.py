@@ -81,6 +81,15 @@ def _as(t: Tensor, dtype: torch.dtype) -> Tensor:
     return t if t.dtype == dtype else t.to(dtype)
 
 
+def _strided_rows(t: Tensor) -> tuple[Tensor, int]:
+    """(t [R, N], or its contiguous copy where its columns are apart or its rows share elements (an expanded table), its row
+    stride, at least N): row r's elements lie at r * stride .. r * stride + N - 1, all inside the tensor."""
+    N, stride = t.shape[1], t.stride(0)
+    if stride >= N and t.stride(1) == 1:
+        return t, stride
+    return t.contiguous(), N
+
+
 def _launch(dev: torch.device, fn, what: str, *args) -> None:
     """fn(*args, stream) on ``dev``'s current stream, with ``dev`` the current device (a null stream means the current
     device's), its status checked."""
@@ -262,9 +271,7 @@ def qkv_norm_mrope_store(qkv: Tensor, *, positions: Tensor, inv_freq: Tensor, ax
         _need(False, f"qkv rows must have unit column stride and a row stride of a multiple of 8, got {qkv.stride()}")
     if positions.dim() != 2 or positions.shape[1] != T:
         _need(False, f"positions must be [axes, {T}]")
-    positions = _as(positions, torch.int64)
-    if positions.stride(1) != 1 or positions.stride(0) < T:
-        positions = positions.contiguous()
+    positions, pos_stride = _strided_rows(_as(positions, torch.int64))
     inv_freq = _contig(inv_freq if inv_freq.dim() == 1 else inv_freq.reshape(-1), "inv_freq", torch.float32)
     n = inv_freq.shape[0]
     if len(axes) != n:
@@ -291,7 +298,7 @@ def qkv_norm_mrope_store(qkv: Tensor, *, positions: Tensor, inv_freq: Tensor, ax
         _need(False, "bad q_out tensor")
     _launch(dev, _lib.load().sna_qkv_norm_mrope_store, "qkv_norm_mrope_store", qkv.data_ptr(), stride, T, num_q_heads,
             num_kv_heads, d_head, _ptr(q_norm), _ptr(k_norm), norm_eps, positions.data_ptr(),
-            max(positions.stride(0), T), positions.shape[0], inv_freq.data_ptr(), n, axes, slots.data_ptr(),
+            pos_stride, positions.shape[0], inv_freq.data_ptr(), n, axes, slots.data_ptr(),
             q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), nb, P, code)
     return q_out
 
@@ -1014,8 +1021,7 @@ def _attention_weights(what, q, T, R, k_cache, block_table, q_start, lens, max_q
     q = _contig(q, "q", torch.bfloat16)
     if block_table.dim() != 2 or block_table.shape[0] != R or block_table.shape[1] < 1:
         _need(False, f"block_table must be [{R}, width]")
-    table = _as(block_table, torch.int32)
-    table = table if table.stride(1) == 1 else table.contiguous()
+    table, stride = _strided_rows(_as(block_table, torch.int32))
     W = table.shape[1]
     lens = _contig(_as(lens if lens.dim() == 1 else lens.reshape(-1), torch.int32), "lens")
     k_scale = None if code == _lib.DTYPE_BF16 else _head_scales(k_scale, G, "k_scale")
@@ -1035,7 +1041,6 @@ def _attention_weights(what, q, T, R, k_cache, block_table, q_start, lens, max_q
     window = int(window)
     need = _weights_workspace(T, R, max_q_len, H, G, d, P, W, N, code, window)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    stride = max(table.stride(0), W)
     if q_start is None:
         _launch(dev, lib.sna_decode_attention_weights, what, q.data_ptr(), k_cache.data_ptr(), _ptr(k_scale),
                 table.data_ptr(), stride, W, lens.data_ptr(), R, _ptr(sinks), sm_scale, window, weights.data_ptr(), row,
