@@ -237,6 +237,12 @@ def mrope_axes(sections: Sequence[int], interleaved: bool = False) -> tuple[int,
     return axes
 
 
+def _axis_bytes(axes: Sequence[int]) -> bytes:
+    """One byte a pair, element by element: bytes() of an array would be its memory. (ValueError outside [0, 256); the
+    library refuses what else is no axis.)"""
+    return axes if type(axes) is bytes else bytes(list(axes))
+
+
 def qkv_norm_mrope_store(qkv: Tensor, *, positions: Tensor, inv_freq: Tensor, axes: Sequence[int], num_q_heads: int,
                          num_kv_heads: int, d_head: int, k_cache: Tensor, v_cache: Tensor, slot_mapping: Tensor,
                          q_norm: Optional[Tensor] = None, k_norm: Optional[Tensor] = None, norm_eps: float = 1e-6,
@@ -274,9 +280,9 @@ def qkv_norm_mrope_store(qkv: Tensor, *, positions: Tensor, inv_freq: Tensor, ax
     positions, pos_stride = _strided_rows(_as(positions, torch.int64))
     inv_freq = _contig(inv_freq if inv_freq.dim() == 1 else inv_freq.reshape(-1), "inv_freq", torch.float32)
     n = inv_freq.shape[0]
+    axes = _axis_bytes(axes)
     if len(axes) != n:
         _need(False, f"{len(axes)} axes for {n} rotated pairs")
-    axes = bytes(axes)  # (ValueError outside [0, 256); the library refuses the others that are no axis)
     slots = _contig(_as(slot_mapping if slot_mapping.dim() == 1 else slot_mapping.reshape(-1), torch.int64), "slot_mapping")
     if slots.shape[0] != T:
         _need(False, f"{slots.shape[0]} slots for {T} tokens")

@@ -2,6 +2,9 @@
 
 from __future__ import annotations
 
+import array
+
+import numpy as np
 import pytest
 import torch
 
@@ -25,3 +28,17 @@ def test_strided_rows_stay_inside_their_tensor(R, N):
     # rows apart are taken where they lie
     t, stride = ops._strided_rows(views[1])
     assert t.data_ptr() == views[1].data_ptr() or R * N == 0
+
+
+def test_axes_are_read_element_by_element():
+    axes = ops.mrope_axes([16, 24, 24])
+    for same in (axes, list(axes), bytes(axes), bytearray(axes), np.array(axes), np.array(axes, dtype=np.int8),
+                 np.repeat(np.arange(3), [16, 24, 24]), array.array("i", axes), memoryview(array.array("q", axes)),
+                 torch.tensor(axes), torch.tensor(axes, dtype=torch.uint8)):
+        assert ops._axis_bytes(same) == bytes(axes), type(same)
+    for bad in ([300], [-1], np.array([256]), np.array([-1])):
+        with pytest.raises(ValueError):
+            ops._axis_bytes(bad)
+    for bad in ([0.0, 1.0], np.array([0.0, 1.0])):
+        with pytest.raises(TypeError):
+            ops._axis_bytes(bad)
