@@ -406,14 +406,15 @@ void weights_tile_kernel(WeightsArgs a) {
       const float2 p = weights_stats<ALL>(x, c2, seen, g2);
       if (g2 == 0) sm_part[i & 3][wave][i32] = p;
     } else {
-      const float inv = ALL || m < m_end ? rw.y : 0.0f;  // (past the last tile it is stale)
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const uint32_t bits = weights_bits(seen, s, g2);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float p = __builtin_amdgcn_exp2f(fmaf(x[s][e], c2, -rw.x));
-          acc[s][e] = fmaf(ALL || bits & weights_bit(e) ? p : 0.0f, inv, acc[s][e]);
+          // (an unseen key keeps its sum, whatever the row's is: NaN, or stale past the last tile)
+          const float sum = fmaf(p, rw.y, acc[s][e]);
+          acc[s][e] = ALL || bits & weights_bit(e) ? sum : acc[s][e];
         }
       }
       // (here, not after the next tile's products: or both tiles' scores would be held)

@@ -9,7 +9,7 @@ import torch
 
 from sglang_neuron_amd import ops
 from tests.conftest import announce
-from tests.test_gpu_attention_weights import DEV, make
+from tests.test_gpu_attention_weights import DEV, check, few_rows, make, oracle, prefill
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +45,55 @@ def test_requests_on_one_table_row(form, H, G, R, queries, keys):
     alone = _table_call(c, one.as_strided((1, W), (0, 1)), q[:queries], [0, queries], lens[:1], queries)
     whole = _table_call(c, one.contiguous(), q[:queries], [0, queries], lens[:1], queries)
     assert all(torch.equal(x, y) for x, y in zip(alone, whole)) and bool((whole[0] > 0).any())
+
+
+def _compare(c, clean, sinks=None, window=0):
+    """The oracle's NaN pattern, and its values elsewhere (``clean``: the same case without what is not finite, whose scores
+    bound the rounding)."""
+    width = c.table.shape[1] * c.P
+    _, reach = oracle(clean, width, sinks=sinks, window=window)
+    want, _ = oracle(c, width, sinks=sinks, window=window)
+    got = prefill(c, sinks=None if sinks is None else sinks.to(DEV), window=window)
+    assert torch.equal(got.isnan().cpu(), want.isnan())
+    check(c, torch.where(got.isnan(), 0.0, got), want.nan_to_num(0.0), reach, "finite keys")
+    return want
+
+
+def _pair(build):
+    return build(), build()
+
+
+@pytest.mark.parametrize("name,build", [
+    ("scores", lambda: make(43, 4, 2, 64, 16, [700, 60], [3, 1], False)),
+    ("lds", lambda: few_rows(64, 8, 4, 64, 16, 2100, 3, False, seed=4)),
+    ("many", lambda: make(43, 8, 2, 64, 16, [700, 60], [40, 3], False)),
+    ("many-fp8", lambda: make(43, 6, 2, 128, 16, [900, 60], [70, 3], True)),
+    ("runs", lambda: make(43, 64, 1, 64, 16, [300, 100], [90, 70], False)),
+])
+def test_a_query_that_is_nan_reaches_no_later_key(name, build):
+    announce(f"NaN query {name}")
+    c, clean = _pair(build)
+    assert c.counts[0] > 1
+    c.q[c.start[0], 1, 3] = float("nan")
+    want = _compare(c, clean)
+    first = c.lens[0] - c.counts[0]  # the NaN query's position
+    assert bool(want[0, 0, :first + 1].isnan().any()) and bool(torch.isfinite(want[0, :, first + 1:]).all())
+
+
+@pytest.mark.parametrize("name,build,window,key", [
+    ("scores", lambda: make(47, 4, 2, 64, 16, [300, 60], [3, 1], False), 50, 249),
+    ("lds", lambda: few_rows(64, 8, 4, 64, 16, 2100, 3, False, seed=4), 100, 1999),
+    ("many", lambda: make(47, 8, 2, 64, 16, [600, 90], [600, 40], False), 100, 20),
+    ("many-fp8", lambda: make(47, 8, 2, 128, 16, [600, 90], [600, 40], True), 30, 300),
+    ("runs", lambda: make(47, 96, 2, 128, 16, [300, 40], [300, 40], False), 33, 60),
+])
+def test_a_key_that_is_nan_reaches_no_key_outside_its_windows(name, build, window, key):
+    announce(f"NaN key {name}")
+    c, clean = _pair(build)
+    c.k[int(c.table[0, key // 16]), 0, key % 16, 5] = float("nan")
+    want = _compare(c, clean, window=window)
+    bad = want[0, 0].isnan().nonzero()[:, 0]
+    # the queries that see it are at key .. key + window - 1 (the chunk's own ones), and so are the keys that they see
+    lo, hi = max(key, c.lens[0] - c.counts[0]), min(key + window - 1, c.lens[0] - 1)
+    assert bad.tolist() == list(range(max(lo - window + 1, 0), hi + 1))
+    assert bool(torch.isfinite(want[0, 1]).all())
