@@ -228,7 +228,7 @@ __device__ __forceinline__ float2 weights_stats(f32x16_t (&x)[2], float c2, uint
       mx = fmaxf(mx, x[s][e]);
     }
   }
-  if (ALL) mx *= c2;
+  if (ALL) mx = fmaxf(mx * c2, kNegBig);  // (32 scores of -inf have the sum 0, as where there are masks)
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll

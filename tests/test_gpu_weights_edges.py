@@ -4,6 +4,8 @@ test_gpu_attention_weights.py."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -97,3 +99,25 @@ def test_a_key_that_is_nan_reaches_no_key_outside_its_windows(name, build, windo
     lo, hi = max(key, c.lens[0] - c.counts[0]), min(key + window - 1, c.lens[0] - 1)
     assert bad.tolist() == list(range(max(lo - window + 1, 0), hi + 1))
     assert bool(torch.isfinite(want[0, 1]).all())
+
+
+@pytest.mark.parametrize("name,build", [
+    ("scores", lambda: make(53, 4, 2, 64, 16, [700, 60], [3, 1], False)),
+    ("lds", lambda: few_rows(64, 8, 4, 64, 16, 2100, 1, False, seed=4)),
+    ("many", lambda: make(53, 8, 2, 64, 16, [700, 400], [40, 300], False)),
+    ("runs", lambda: make(53, 64, 1, 128, 16, [300, 200], [90, 70], False)),
+])
+def test_keys_whose_scores_are_minus_infinity(name, build):
+    """They get nothing, and nothing from their rows is lost, where they fill a block of keys and where they do not."""
+    announce(f"infinite keys {name}")
+    c, clean = _pair(build)
+    c.q[..., 0] = clean.q[..., 0] = -1.0
+    keys = [*range(64, 192), 200, 203]
+    for j in keys:
+        c.k[int(c.table[0, j // 16]), :, j % 16, 0] = math.inf
+    width = c.table.shape[1] * c.P
+    _, reach = oracle(clean, width)
+    want, _ = oracle(c, width)
+    got = prefill(c)
+    assert bool(torch.isfinite(got).all()) and bool((got[0, :, keys] == 0).all())
+    check(c, got, want, reach, "beside them")
