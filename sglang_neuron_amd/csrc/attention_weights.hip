@@ -27,6 +27,8 @@
 // in all, the first pass a little over half: products take 37% (41% in the second pass) of a SIMD's cycles and VALU
 // instructions 61% (57%), which together is all of them: a wave's matrix instructions and the other waves' VALU hardly
 // overlap here.
+#include <float.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -207,6 +209,13 @@ __device__ __forceinline__ uint32_t weights_bits(uint64_t seen, int s, int g2) {
 __device__ __forceinline__ constexpr uint32_t weights_bit(int e) { return 1u << (8 * (e / 4) + e % 4); }
 // Key of element e of lane group g2's sub-tile s.
 __device__ __forceinline__ constexpr int weights_key(int s, int e, int g2) { return 32 * s + 8 * (e / 4) + 4 * g2 + e % 4; }
+
+// Head h's sink in the log2 domain. One past the largest number takes its rows whole, as the largest does: infinity less
+// itself would be NaN.
+__device__ __forceinline__ float weights_sink(const WeightsArgs& a, int32_t h) {
+  const float x = a.sinks[h] * kLog2e;
+  return x > FLT_MAX ? FLT_MAX : x;
+}
 
 // (largest, sum of 2^(x - largest)) of two sets merged.
 __device__ __forceinline__ float2 weights_join(float2 p, float2 o) {
@@ -520,7 +529,7 @@ __global__ __launch_bounds__(256) void weights_merge_kernel(WeightsArgs a) {
   __syncthreads();
   if (slice == 0 && (int32_t)blockIdx.x * ROWS + i < rq.S * a.group) {
     for (int s = 1; s < SLICES; ++s) p = weights_join(p, sm[s][i]);
-    if (a.sinks) p = weights_join(p, make_float2(a.sinks[h] * kLog2e, 1.0f));
+    if (a.sinks) p = weights_join(p, make_float2(weights_sink(a, h), 1.0f));
     // (a row that sees nothing: every score is dropped)
     a.ws_row[(int64_t)g * rows + row] = p.y == 0.0f ? make_float2(-kNegBig, 0.0f) : make_float2(p.x, 1.0f / p.y);
   }
@@ -682,7 +691,7 @@ __global__ __launch_bounds__(256) void weights_from_scores_kernel(WeightsArgs a)
     __syncthreads();
     if (tid < M) {
       for (int s = 1; s < 16; ++s) p = weights_join(p, sm[s][tid]);
-      if (a.sinks) p = weights_join(p, make_float2(a.sinks[g * a.group + tid % a.group] * kLog2e, 1.0f));
+      if (a.sinks) p = weights_join(p, make_float2(weights_sink(a, g * a.group + tid % a.group), 1.0f));
       sm_row[tid] = p.y == 0.0f ? make_float2(-kNegBig, 0.0f) : make_float2(p.x, 1.0f / p.y);
     }
     __syncthreads();
@@ -821,7 +830,7 @@ __global__ __launch_bounds__(kRowThreads) void weights_row_kernel(WeightsArgs a)
   if (g4 == 0) sm_wave[wave][m] = best;
   __syncthreads();
   if (tid < M) {  // the rows' largest, and their sinks' share of the sum
-    const float sink = a.sinks ? a.sinks[g * a.group + tid % a.group] * kLog2e : -INFINITY;
+    const float sink = a.sinks ? weights_sink(a, g * a.group + tid % a.group) : -INFINITY;
     float v = a.sinks ? sink : kNegBig;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) v = fmaxf(v, sm_wave[w][tid]);

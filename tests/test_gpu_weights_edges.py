@@ -121,3 +121,18 @@ def test_keys_whose_scores_are_minus_infinity(name, build):
     got = prefill(c)
     assert bool(torch.isfinite(got).all()) and bool((got[0, :, keys] == 0).all())
     check(c, got, want, reach, "beside them")
+
+
+@pytest.mark.parametrize("form,H,G,R,queries,keys", FORMS, ids=[f[0] for f in FORMS])
+def test_sinks_past_every_score(form, H, G, R, queries, keys):
+    """A sink that is infinite, or finite and infinite in the log2 domain, leaves its head's keys nothing; one of the lowest
+    value takes nothing."""
+    announce(f"sinks {form}")
+    c = few_rows(R, H, G, 64, 16, keys, queries, False, seed=6) if form in ("scores", "lds") else \
+        make(59, H, G, 64, 16, [keys, 50, 70][:R], [queries, 3, 70][:R], False)
+    sinks = torch.randn(H, generator=torch.Generator().manual_seed(2))
+    sinks[::4], sinks[1::8], sinks[2::8], sinks[3::8] = math.inf, 3.0e38, -math.inf, torch.finfo(torch.float32).min
+    _compare(c, c, sinks=sinks)
+    all_of = torch.full((H,), math.inf)
+    got = prefill(c, sinks=all_of.to(DEV))
+    assert bool((got == 0).all())
