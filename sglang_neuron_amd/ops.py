@@ -1101,7 +1101,8 @@ def select_tokens(weights: Tensor, seq_lens: Tensor, *, keep: int, first: int = 
     counts as N: tokens without a weight are not kept.
 
     ``weights_out`` [R, G, M >= keep] fp32, when given, receives the kept tokens' weights and zeros after them; it may be
-    ``weights`` itself, so that the tokens written next start at zero."""
+    ``weights`` itself, so that the tokens written next start at zero, and be wider or narrower than it (``weights=buf[..., :n],
+    weights_out=buf``)."""
     dev = _on_gpu(weights, seq_lens, weights_out)
     args, (kept, new_lens), _keep = _select_args(dev, weights, seq_lens, keep, first, recent, weights_out)
     if kept.shape[0] and kept.shape[1]:
@@ -1133,8 +1134,11 @@ def _select_args(dev, weights, seq_lens, keep, first, recent, weights_out):
         M = weights_out.shape[2]
         if M < keep:
             _need(False, f"weights_out of {M} columns for {keep} tokens")
-        same = weights_out.data_ptr() == weights.data_ptr() and (o_row, o_head) == (row, head)
-        if not same and _overlap(weights, weights_out):
+        same = weights_out.data_ptr() == weights.data_ptr() and _same_strides(weights, weights_out)
+        if same:  # (where there is one row or head its stride is the wider tensor's)
+            row = o_row = max(row, o_row)
+            head = o_head = max(head, o_head)
+        elif _overlap(weights, weights_out):
             _need(False, "weights_out overlaps weights without being it")
     kept = torch.empty(R, G, keep, dtype=torch.int32, device=dev)
     new_lens = torch.empty(R, dtype=torch.int32, device=dev)
@@ -1145,6 +1149,11 @@ def _select_args(dev, weights, seq_lens, keep, first, recent, weights_out):
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
     return (weights.data_ptr(), row, head, N, lens.data_ptr(), R, G, keep, first, recent, kept.data_ptr(),
             new_lens.data_ptr(), _ptr(weights_out), o_row, o_head, M, _ptr(ws), need), (kept, new_lens), (lens, ws)
+
+
+def _same_strides(a: Tensor, b: Tensor) -> bool:
+    """Whether the rows and heads of two [R, G, .] tensors are equally far apart, where there are several."""
+    return (a.shape[0] < 2 or a.stride(0) == b.stride(0)) and (a.shape[1] < 2 or a.stride(1) == b.stride(1))
 
 
 def _overlap(a: Tensor, b: Tensor) -> bool:
