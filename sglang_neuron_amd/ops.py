@@ -1157,13 +1157,27 @@ def _same_strides(a: Tensor, b: Tensor) -> bool:
 
 
 def _overlap(a: Tensor, b: Tensor) -> bool:
-    """Whether the address ranges of two tensors meet."""
+    """Whether two fp32 tensors [R, G, N] and [R, G, M], each of rows that do not overlap, share an element. Exact where their
+    rows and heads are equally far apart (views of one buffer); else whether their address ranges meet."""
     if a.numel() == 0 or b.numel() == 0:
         return False
 
     def end(t):
         return t.data_ptr() + (sum([(n - 1) * s for n, s in zip(t.shape, t.stride())]) + 1) * t.element_size()
-    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
+    if a.data_ptr() >= end(b) or b.data_ptr() >= end(a):
+        return False
+    R, G, N = a.shape
+    M, off = b.shape[2], b.data_ptr() - a.data_ptr()
+    if off % 4 or not _same_strides(a, b):
+        return True
+    # b's row (r + i, g + j) starts off / 4 + i * outer + j * inner elements behind a's (r, g): is that in (-M, N)?
+    (R, outer), (G, inner) = sorted(((R, a.stride(0) if R > 1 else 0), (G, a.stride(1) if G > 1 else 0)))
+    for i in range(1 - R, R):
+        at = off // 4 + i * outer
+        first = 1 - G if inner == 0 else max(1 - G, (-M - at) // inner + 1)  # the least j past the lower bound
+        if first < G and at + first * inner < N and at + first * inner > -M:
+            return True
+    return False
 
 
 def compact_tokens(k_cache: Tensor, v_cache: Tensor, block_table: Tensor, kept: Tensor, *,

@@ -57,3 +57,26 @@ def test_a_batch_that_shrinks_to_one_row_is_thinned_in_place():
         for g in range(G):
             rows = b[1:, g].reshape(-1, d)
             assert torch.equal(c[1:, g].reshape(-1, d)[:keep], rows[kept[0, g].long()])
+
+
+@pytest.mark.parametrize("N,keep", [(150, 40), (16500, 300)])
+def test_views_of_one_buffer_that_share_no_element(N, keep):
+    announce(f"disjoint views {N}")
+    R, G = 3, 2
+    w = _weights(N, R, G, N)
+    lens = [N, N - 7, keep - 1]
+    want, _, carried = _want(w, lens, keep, 1, 2)
+    dl = torch.tensor(lens, device=DEV)
+    for shape, src, dst in (((R, G, 2 * N), lambda b: b[..., :N], lambda b: b[..., N:]),
+                            ((R, G, 2 * N), lambda b: b[..., N:], lambda b: b[..., :N]),
+                            ((2 * R, G, N), lambda b: b[::2], lambda b: b[1::2]),
+                            ((R, 2 * G, N), lambda b: b[:, :G], lambda b: b[:, G:]),
+                            ((G, R, 2 * N), lambda b: b[..., :N].transpose(0, 1), lambda b: b[..., N:].transpose(0, 1))):
+        buf = torch.full(shape, 9.0, device=DEV)
+        src(buf).copy_(w)
+        kept, _ = ops.select_tokens(src(buf), dl, keep=keep, first=1, recent=2, weights_out=dst(buf))
+        assert torch.equal(kept.cpu(), want) and torch.equal(src(buf).cpu(), w)
+        assert torch.equal(dst(buf)[..., :keep].cpu(), carried) and bool((dst(buf)[..., keep:] == 0).all())
+    buf = torch.zeros(R, G, 2 * N, device=DEV)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.select_tokens(buf[..., :N], dl, keep=keep, weights_out=buf[..., N - 1:2 * N - 1])

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import array
+import random
 
 import numpy as np
 import pytest
@@ -42,3 +43,33 @@ def test_axes_are_read_element_by_element():
     for bad in ([0.0, 1.0], np.array([0.0, 1.0])):
         with pytest.raises(TypeError):
             ops._axis_bytes(bad)
+
+
+def test_overlap_of_views_of_one_buffer():
+    rng = random.Random(1)
+    buf = torch.zeros(600)
+    seen = {True: 0, False: 0}
+    for _ in range(4000):
+        R, G, N, M = rng.randint(1, 4), rng.randint(1, 4), rng.randint(0, 6), rng.randint(0, 6)
+        wide = max(N, M, 1)
+        inner = wide + rng.randint(0, 8)
+        outer = inner * G + rng.randint(0, 9)
+        strides = (outer, inner, 1) if rng.random() < 0.5 else (inner, inner * R + rng.randint(0, 9), 1)
+        at = [rng.randint(0, 90) for _ in range(2)]
+        a, b = (buf.as_strided((R, G, n), strides, o) for n, o in zip((N, M), at))
+        elements = [set(torch.arange(600).as_strided(t.shape, t.stride(), t.storage_offset()).flatten().tolist())
+                    for t in (a, b)]
+        want = bool(elements[0] & elements[1])
+        assert ops._overlap(a, b) == ops._overlap(b, a) == want, (R, G, N, M, strides, at)
+        seen[want] += 1
+    assert min(seen.values()) > 500
+    # strides that differ: never told to be apart where they meet
+    for _ in range(2000):
+        R, G, N = rng.randint(1, 3), rng.randint(1, 3), rng.randint(1, 5)
+        views = []
+        for _ in range(2):
+            inner = N + rng.randint(0, 5)
+            views.append(buf.as_strided((R, G, N), (inner * G + rng.randint(0, 5), inner, 1), rng.randint(0, 80)))
+        elements = [set(torch.arange(600).as_strided(t.shape, t.stride(), t.storage_offset()).flatten().tolist())
+                    for t in views]
+        assert ops._overlap(*views) or not elements[0] & elements[1]
