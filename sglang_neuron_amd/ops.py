@@ -240,7 +240,7 @@ def mrope_axes(sections: Sequence[int], interleaved: bool = False) -> tuple[int,
 def _axis_bytes(axes: Sequence[int]) -> bytes:
     """One byte a pair, element by element: bytes() of an array would be its memory. (ValueError outside [0, 256); the
     library refuses what else is no axis.)"""
-    return axes if type(axes) is bytes else bytes(list(axes))
+    return bytes(axes if type(axes) in (tuple, list, bytes) else list(axes))
 
 
 def qkv_norm_mrope_store(qkv: Tensor, *, positions: Tensor, inv_freq: Tensor, axes: Sequence[int], num_q_heads: int,
@@ -251,8 +251,8 @@ def qkv_norm_mrope_store(qkv: Tensor, *, positions: Tensor, inv_freq: Tensor, ax
     """The writer of qkv_norm_rope_store for rotary positions with several axes (images, video): pair i of a Q or K head
     (elements i and i + n, n = len(inv_freq)) is rotated by the angle ``positions[axes[i], t] * inv_freq[i]``, elements
     past 2 n stay. ``positions`` [A, T] int64 (A of 1 to 4), ``inv_freq`` [n] fp32 (n a multiple of 8, at most d / 2),
-    ``axes`` [n] host ints (mrope_axes). The other arguments are qkv_norm_rope_store's. Angles are formed in 64 bits, so
-    positions of any size serve; norm and rotation are fp32 and every output is rounded once. Returns Q [T, q, d] bf16; the
+    ``axes`` [n] host ints (mrope_axes). The other arguments are qkv_norm_rope_store's. Every angle keeps its fraction
+    of a turn to fp32, at positions of any size; norm and rotation are fp32 and every output is rounded once. Returns Q [T, q, d] bf16; the
     caches are written in place."""
     # (conditions are tested here and messages built by _need only where one fails: the checks of a small call cost as much
     # as its kernel)

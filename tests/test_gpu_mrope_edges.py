@@ -4,13 +4,16 @@ numbers, infinite elements that no rotation touches. Tolerance as in test_gpu_mr
 from __future__ import annotations
 
 import array
+import math
+from fractions import Fraction
 
 import numpy as np
 import pytest
 import torch
 
 from sglang_neuron_amd import ops
-from tests.test_gpu_mrope import _make, _run
+from tests.conftest import announce
+from tests.test_gpu_mrope import E, _make, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +31,42 @@ def test_axes_in_any_container():
     for bad in (np.full(64, 300), np.full(64, -1), np.full(64, 3)):
         with pytest.raises(ValueError):
             _run(qkv, pos, inv, bad, Hq, Hkv, d, k, v, slots, gam, sc)
+
+
+def _pi(bits=400):
+    """pi * 2^bits, by Machin's formula in whole numbers."""
+    def atan(n):
+        term = s = (1 << bits + 32) // n
+        i = 1
+        while term:
+            term //= n * n
+            i += 2
+            s += (-1 if i // 2 % 2 else 1) * (term // i)
+        return s
+    return 4 * (4 * atan(5) - atan(239)) >> 32
+
+
+@pytest.mark.parametrize("rot", [128, 32])
+@pytest.mark.parametrize("base", [0, -5, 2 ** 24 + 1, 2 ** 31 + 3, -2 ** 33 - 7, 2 ** 40 + 9, 2 ** 52 + 1, 2 ** 53 + 1,
+                                  2 ** 62 + 12345, 2 ** 63 - 8, -2 ** 63])
+def test_positions_of_any_size(base, rot):
+    """Each angle's fraction of a turn from whole numbers; the same tolerance at every position."""
+    announce(f"positions from {base} rot {rot}")
+    T, Hq, Hkv, d, P, n = 8, 2, 1, 128, 16, rot // 2
+    qkv, _, inv, gam, slots, k, v, sc = _make(33, T, Hq, Hkv, d, P, False, False, rot, 1, 0)
+    pos = torch.tensor([[base + t for t in range(T)]], dtype=torch.int64)
+    q, kc, _ = _run(qkv, pos, inv, [0] * n, Hq, Hkv, d, k, v, slots, gam, sc)
+    two_pi = Fraction(2 * _pi(), 1 << 400)
+    x = qkv.double().view(T, Hq + 2 * Hkv, d)[:, :Hq + Hkv]
+    want, size = x.clone(), x.abs().clone()
+    for t in range(T):
+        for i in range(n):
+            turns = int(pos[0, t]) * Fraction(float(inv[i])) / two_pi
+            angle = 2 * math.pi * float(turns - round(turns))
+            c, s = math.cos(angle), math.sin(angle)
+            a, b = x[t, :, i], x[t, :, i + n]
+            want[t, :, i], want[t, :, i + n] = a * c - b * s, b * c + a * s
+            size[t, :, i] = size[t, :, i + n] = a.abs() + b.abs()
+    got = torch.cat([q.double(), kc.double()[slots // P, :, slots % P]], 1)
+    tol = want.abs() * 2.0 ** -8 + size * E * (1 + 2.0 ** -8) + 2.0 ** -134
+    assert bool(((got - want).abs() <= tol).all()), f"off by {float(((got - want).abs() - tol).max()):.3e} past the tolerance"
