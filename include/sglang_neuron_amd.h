@@ -121,7 +121,8 @@ int sna_qkv_norm_rope_store(const void *qkv, int64_t qkv_stride, int64_t n_token
  *   positions  [n_axes, n_tokens] int64 (row stride pos_stride), any values; n_axes 1 to 4.
  *   inv_freq   [n_pairs] fp32; n_pairs a multiple of 8, at most head_dim / 2.
  *   axes       HOST array [n_pairs], each below n_axes.
- * Every position keeps its fraction of a turn to fp32; norm and rotation are fp32 and every output is rounded once (bf16, or e4m3fn(x / s)).
+ * Every angle keeps its fraction of a turn to fp32; norm and rotation are fp32 and every output is rounded once (bf16, or
+ * e4m3fn(x / s)).
  * cache_dtype SNA_DTYPE_BF16 or SNA_DTYPE_FP8_E4M3FN; head_dim 64 or 128.
  * This has no reference counterpart (its rope takes one position a token, ops/attention/qkv_paged.py:56-60). */
 int sna_qkv_norm_mrope_store(const void *qkv, int64_t qkv_stride, int64_t n_tokens, int32_t num_q_heads,

@@ -119,14 +119,14 @@ __global__ __launch_bounds__(256) void qkv_norm_mrope_store_kernel(MropeArgs a) 
   // the rotation partner of the lane's elements, half elements away; the lane's cosines and signed sines
   const bool rotated = FULL || 8 * sub < 2 * half, first = 8 * sub < half;
   const int partner = rotated ? lane + (first ? half / 8 : -(half / 8)) : lane;
-  const int pair0 = rotated ? (first ? 8 * sub : 8 * sub - half) : 0;
+  const int pair0 = rotated ? (first ? 8 * sub : 8 * sub - half) : 0;  // (one that is not rotated: any pair's, unused)
   float cs[U][8], sn[U][8];
 #pragma unroll
   for (int k = 0; k < U; ++k)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      cs[k][e] = rotated ? sm_cos[wave * U + k][pair0 + e] : 1.0f;
-      const float v = rotated ? sm_sin[wave * U + k][pair0 + e] : 0.0f;
+      const float v = sm_sin[wave * U + k][pair0 + e];
+      cs[k][e] = sm_cos[wave * U + k][pair0 + e];
       sn[k][e] = first ? -v : v;
     }
   for (int32_t grp = g0; grp < g1; ++grp) {  // uniform
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(256) void qkv_norm_mrope_store_kernel(MropeArgs a) 
           o = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x[e]), 0x128, 0xf, 0xf, true));  // row_ror:8
         else
           o = __shfl(x[e], partner, 64);
-        y[e] = roped ? fmaf(x[e], cs[k][e], o * sn[k][e]) : x[e];
+        y[e] = roped && rotated ? fmaf(x[e], cs[k][e], o * sn[k][e]) : x[e];  // (an infinite x * 0 would be NaN)
       }
       if (!head_ok) continue;
       const uint4 b16 = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),

@@ -70,3 +70,19 @@ def test_positions_of_any_size(base, rot):
     got = torch.cat([q.double(), kc.double()[slots // P, :, slots % P]], 1)
     tol = want.abs() * 2.0 ** -8 + size * E * (1 + 2.0 ** -8) + 2.0 ** -134
     assert bool(((got - want).abs() <= tol).all()), f"off by {float(((got - want).abs() - tol).max()):.3e} past the tolerance"
+
+
+@pytest.mark.parametrize("d,rot", [(128, 64), (64, 16)])
+def test_infinite_elements_that_are_not_rotated_stay(d, rot):
+    T, Hq, Hkv, P = 9, 3, 1, 16
+    qkv, pos, inv, gam, slots, k, v, sc = _make(35, T, Hq, Hkv, d, P, False, False, rot, 2, 10)
+    x = qkv.view(T, Hq + 2 * Hkv, d)
+    x[2, 0, rot], x[3, 1, d - 1], x[4, Hq, rot + 3], x[5, Hq + Hkv, 0] = math.inf, -math.inf, -math.inf, math.inf
+    x[6, 2, rot + 1], x[6, Hq, rot + 1] = -0.0, -0.0
+    q, kc, vc = _run(qkv, pos, inv, ops.mrope_axes([rot // 4, rot // 4]), Hq, Hkv, d, k, v, slots, gam, sc)
+    at = (slots // P, slice(None), slots % P)
+    bits = lambda t: t.contiguous().view(torch.int16)  # noqa: E731
+    assert torch.equal(bits(q[..., rot:]), bits(x[:, :Hq, rot:]))
+    assert torch.equal(bits(kc[at][..., rot:]), bits(x[:, Hq:Hq + Hkv, rot:]))
+    assert torch.equal(bits(vc[at]), bits(x[:, Hq + Hkv:]))
+    assert bool(torch.isfinite(q[..., :rot]).all())
