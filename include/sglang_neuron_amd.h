@@ -513,7 +513,8 @@ int sna_decode_attention_weights(const void *q, const void *k_cache, const float
  *             may be `weights` itself (same address and strides; wider or narrower), and overlaps it in no other way.
  *   workspace device, 16-byte aligned, at least sna_select_workspace_bytes bytes (in_place: weights_out is weights; 0 for
  *             rows of up to 16384 columns, and it may be NULL then), any contents; calls that share one on different
- *             streams race. */
+ *             streams race.
+ * width, keep and out_width are at most 2^30 - 2^15. */
 int64_t sna_select_workspace_bytes(int32_t R, int32_t num_kv_heads, int32_t width, int32_t keep, int32_t in_place);
 int sna_select_tokens(const float *weights, int64_t row_stride, int64_t head_stride, int32_t width,
                       const int32_t *seq_lens, int32_t R, int32_t num_kv_heads, int32_t keep, int32_t first,
@@ -526,7 +527,7 @@ int sna_select_tokens(const float *weights, int64_t row_stride, int64_t head_str
  * where kept must ascend, as sna_select_tokens writes it). Entries of -1 move nothing, nor does a token whose source or
  * target lies past its table or on an invalid page. Bytes move as they are (the scales are the head's). A page that two
  * rows share may be read through both, not written: evict such rows to pages of their own, and let dst_table name no page
- * that block_table names. head_dim 64 or 128; the caches as for sna_kv_store_mha. */
+ * that block_table names. head_dim 64 or 128, keep at most 2^30 - 2^15; the caches as for sna_kv_store_mha. */
 int sna_compact_tokens(void *k_cache, void *v_cache, int64_t num_blocks, int32_t num_kv_heads, int32_t page_size,
                        int32_t head_dim, int32_t cache_dtype, const int32_t *block_table, int64_t table_stride,
                        int32_t table_width, const int32_t *dst_table, int64_t dst_stride, int32_t dst_width,

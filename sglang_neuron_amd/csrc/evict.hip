@@ -420,6 +420,10 @@ using namespace sna;
 
 namespace {
 
+// The kernels number a row's places by 32 bits: a segment's start behind the first tokens, and a loop's place a step past its
+// end, stay below 2^31 with so many.
+constexpr int32_t kMostTokens = (1 << 30) - (1 << 15);
+
 // The workspace of a launch whose rows may be longer than one workgroup holds: histograms, counts and thresholds, and the
 // kept weights where rows are thinned in place.
 int64_t select_segments(int32_t width) { return ((int64_t)width + kSelectSegment - 1) / kSelectSegment; }
@@ -476,8 +480,9 @@ int plan_select(const char* what, const float* weights, int64_t row_stride, int6
   if (weights_out && (out_width < keep || out_row_stride < out_width || out_head_stride < out_width))
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: weights_out of %d columns (strides %lld / %lld) for %d tokens", what,
                 out_width, (long long)out_row_stride, (long long)out_head_stride, keep);
-  if (width > INT32_MAX - kSelectSegment || (weights_out && out_width > INT32_MAX - (1 << 20)))
-    return fail(SNA_ERR_UNSUPPORTED, "%s: %d columns, %d out (under 2^31)", what, width, out_width);
+  if (width > kMostTokens || keep > kMostTokens || (weights_out && out_width > kMostTokens))
+    return fail(SNA_ERR_UNSUPPORTED, "%s: %d columns, %d kept, %d out (at most %d)", what, width, keep, out_width,
+                kMostTokens);
   if (R == 0) return SNA_OK;
   if (!weights || !seq_lens || !kept || !new_lens)
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
@@ -552,6 +557,8 @@ int plan_compact(const char* what, void* k_cache, void* v_cache, int64_t num_blo
     return fail(SNA_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", what, head_dim);
   if (cache_dtype != SNA_DTYPE_BF16 && cache_dtype != SNA_DTYPE_FP8_E4M3FN && cache_dtype != SNA_DTYPE_FP8_E4M3FN_MUL)
     return fail(SNA_ERR_UNSUPPORTED, "%s: KV dtype %d (FP8 e4m3fn or bf16)", what, cache_dtype);
+  if (keep > kMostTokens)
+    return fail(SNA_ERR_UNSUPPORTED, "%s: %d kept tokens (at most %d)", what, keep, kMostTokens);
   if (R == 0) return SNA_OK;
   if (!k_cache || !v_cache || !block_table || !kept)
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: null pointer", what);

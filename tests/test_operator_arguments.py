@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from sglang_neuron_amd import ops
+from sglang_neuron_amd import _lib, ops
 
 
 @pytest.mark.parametrize("R,N", [(1, 1), (1, 5), (3, 1), (3, 5), (2, 0), (0, 4)])
@@ -73,3 +73,27 @@ def test_overlap_of_views_of_one_buffer():
         elements = [set(torch.arange(600).as_strided(t.shape, t.stride(), t.storage_offset()).flatten().tolist())
                     for t in views]
         assert ops._overlap(*views) or not elements[0] & elements[1]
+
+
+# The C ABI refuses on the host, before any launch: no pointer below is followed.
+A = 1 << 20
+MOST = 2 ** 30 - 2 ** 15
+
+
+@pytest.mark.parametrize("width,keep,out", [(MOST + 1, 5, 0), (2 ** 31 - 1 - 16384, 2 ** 30, 0), (8, MOST + 1, 0),
+                                            (8, 2 ** 31 - 1, 0), (8, 5, MOST + 1), (8, 5, 2 ** 31 - 1 - 2 ** 20)])
+def test_selections_that_32_bits_cannot_number_are_refused(width, keep, out):
+    """A place past 2^31 would wrap to a negative one: rows, kept tokens and columns stop before."""
+    lib = _lib.load()
+    args = (A, width, width, width, A, 1, 1, keep, 1, 1, A, A, A + 4096 if out else None, out, out, out, A, 1 << 60)
+    assert lib.sna_select_tokens(*args, None) == -4 and "at most" in _lib.last_error()
+    w, row, head, n, lens, R, _, *rest = args
+    caches = (A, A, 4, 1, 16, 64, 0, A, 2, 2, None, 2, 2)
+    assert lib.sna_evict_tokens(*caches, w, row, head, n, lens, R, *rest, None) == -4 and "at most" in _lib.last_error()
+
+
+@pytest.mark.parametrize("keep", [MOST + 1, 2 ** 31 - 1])
+@pytest.mark.parametrize("dst", [None, 2 * A])
+def test_compactions_that_32_bits_cannot_number_are_refused(keep, dst):
+    assert _lib.load().sna_compact_tokens(A, A, 4, 1, 16, 64, 0, A, 2, 2, dst, 2, 2, A, 1, keep, None) == -4
+    assert "at most" in _lib.last_error()
