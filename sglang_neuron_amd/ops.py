@@ -19,6 +19,7 @@ from torch import Tensor
 from . import _lib
 
 FP8 = torch.float8_e4m3fn
+_INT32_MAX = 2 ** 31 - 1
 _cu_count: dict[int, int] = {}
 
 
@@ -1039,12 +1040,15 @@ def _attention_weights(what, q, T, R, k_cache, block_table, q_start, lens, max_q
     if add:
         row, head = _weight_strides(weights, R, G, "weights")
         N = weights.shape[2]
+        if N > _INT32_MAX:
+            _need(False, f"weights of {N} columns (under 2^31)")
     else:
         N = W * P
         row, head = G * N, N
         weights = torch.empty(R, G, N, dtype=torch.float32, device=dev)
     lib = _lib.load()
-    window = int(window)
+    # (bounds: what is past the keys or the queries bounds as well as they do, and 32 bits cross the C boundary)
+    window, max_q_len = min(int(window), _INT32_MAX), min(max_q_len, T)
     need = _weights_workspace(T, R, max_q_len, H, G, d, P, W, N, code, window)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     if q_start is None:
@@ -1125,6 +1129,8 @@ def _select_args(dev, weights, seq_lens, keep, first, recent, weights_out):
     lens = _contig(_as(seq_lens if seq_lens.dim() == 1 else seq_lens.reshape(-1), torch.int32), "seq_lens")
     if lens.shape[0] != R:
         _need(False, f"{lens.shape[0]} seq_lens for {R} rows")
+    if N > _INT32_MAX or keep > _INT32_MAX:
+        _need(False, f"{N} columns, {keep} kept tokens (under 2^31)")
     if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
         _need(False, f"keep {keep} tokens of which {first} first and {recent} recent")
     o_row = o_head = M = 0
@@ -1132,8 +1138,8 @@ def _select_args(dev, weights, seq_lens, keep, first, recent, weights_out):
     if weights_out is not None:
         o_row, o_head = _weight_strides(weights_out, R, G, "weights_out")
         M = weights_out.shape[2]
-        if M < keep:
-            _need(False, f"weights_out of {M} columns for {keep} tokens")
+        if M < keep or M > _INT32_MAX:
+            _need(False, f"weights_out of {M} columns for {keep} tokens (under 2^31)")
         same = weights_out.data_ptr() == weights.data_ptr() and _same_strides(weights, weights_out)
         if same:  # (where there is one row or head its stride is the wider tensor's)
             row = o_row = max(row, o_row)

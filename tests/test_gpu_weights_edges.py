@@ -136,3 +136,19 @@ def test_sinks_past_every_score(form, H, G, R, queries, keys):
     all_of = torch.full((H,), math.inf)
     got = prefill(c, sinks=all_of.to(DEV))
     assert bool((got == 0).all())
+
+
+def test_bounds_past_32_bits():
+    """A window, or a longest query count, that 32 bits do not hold bounds nothing."""
+    c = make(61, 8, 2, 64, 16, [300, 40], [40, 3], False)
+    dev = [t.to(DEV) for t in (c.q, c.k, c.table)]
+    start, prior = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (c.start, c.prior))
+    want = ops.prefill_attention_weights(*dev, start, prior, max_q_len=40, sm_scale=c.scale)
+    check(c, want, *oracle(c, c.table.shape[1] * 16), "plain")
+    for most in (2 ** 31, 2 ** 32 + 3, 2 ** 63):
+        assert torch.equal(ops.prefill_attention_weights(*dev, start, prior, max_q_len=most, sm_scale=c.scale), want)
+    windowed = ops.prefill_attention_weights(*dev, start, prior, max_q_len=40, sm_scale=c.scale, window=2 ** 31 - 1)
+    for window in (2 ** 31, 2 ** 32 + 2, 2 ** 63):
+        got = ops.prefill_attention_weights(*dev, start, prior, max_q_len=40, sm_scale=c.scale, window=window)
+        assert torch.equal(got, windowed)
+        check(c, got, *oracle(c, c.table.shape[1] * 16), "no key is outside")

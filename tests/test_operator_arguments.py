@@ -97,3 +97,13 @@ def test_selections_that_32_bits_cannot_number_are_refused(width, keep, out):
 def test_compactions_that_32_bits_cannot_number_are_refused(keep, dst):
     assert _lib.load().sna_compact_tokens(A, A, 4, 1, 16, 64, 0, A, 2, 2, dst, 2, 2, A, 1, keep, None) == -4
     assert "at most" in _lib.last_error()
+
+
+@pytest.mark.parametrize("N,M,keep", [(2 ** 32 + 100, 0, 5), (2 ** 32 + 100, 2 ** 32 + 100, 5), (100, 2 ** 32 + 5, 5),
+                                      (100, 0, 2 ** 32 + 5)])
+def test_selections_whose_sizes_would_wrap_at_the_c_boundary(N, M, keep):
+    w = torch.empty(1, 1, N, device="meta")
+    out = torch.empty(1, 1, M, device="meta") if M else None
+    lens = torch.empty(1, dtype=torch.int32, device="meta")
+    with pytest.raises(ValueError, match="under 2"):
+        ops._select_args(w.device, w, lens, keep, 1, 1, out)
