@@ -973,9 +973,10 @@ WeightsPlan weights_plan(int64_t T, int64_t R, int64_t max_q, int32_t H, int32_t
 }
 
 // Up to so many rows (of all requests and KV heads) are merged 8 to a workgroup, a row's blocks by 32 threads, else 32 and by
-// 8: 2048 rows of 512 blocks take 6.1 us by 8 and 10.7 by 32, 4096 rows of 12 to 64 blocks 5.3 and 5.2, 262144 of 8 to 16
-// blocks 37 and 10.
-constexpr int64_t kMergeFewRows = 16384;
+// 8. In us by 8 / 32, rows of 512 blocks: 2048 rows 5.8 / 10.2, 4096 8.4 / 10.8, 6144 11.2 / 11.2, 8192 13.5 / 11.3, 16384
+// 23 / 15; of 64 blocks 4 to 5 both up to 6144 rows, 16384 6.1 / 5.2, 65536 13.7 / 7.4; of 8 blocks 4 to 5 both up to 16384,
+// 32768 6.9 / 5.2.
+constexpr int64_t kMergeFewRows = 6144;
 template <int D, int ESZ>
 void launch_weights(const WeightsArgs& a, uint32_t wgs, int32_t row_floats, hipStream_t s) {
   if (row_floats > 0) {
