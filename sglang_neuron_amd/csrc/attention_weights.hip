@@ -273,7 +273,6 @@ void weights_tile_kernel(WeightsArgs a) {
   using Geo = WeightsGeo<D, ESZ>;
   using Ring = WeightsRing<D, ESZ>;
   constexpr int NS = Geo::NS, CH = Geo::QCH, SLOTS = Ring::SLOTS, LD = Ring::LD;
-  constexpr int DMAS = LD + (PASS == kSum);  // that a wave issues for a tile
   __shared__ __attribute__((aligned(1024))) uint8_t sm[Ring::BYTES];
   __shared__ float2 sm_row[PASS == kSum ? SLOTS : 1][kWeightRows];  // the tiles' rows of ws_row
   __shared__ float sm_out[PASS == kSum ? kWeightKeys : 1];
