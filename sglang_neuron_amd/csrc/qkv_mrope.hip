@@ -57,6 +57,17 @@ __device__ __forceinline__ uint32_t mrope_fp8_pair(float x0, float x1, float s, 
   return b;
 }
 
+// 1 / sqrt(v), v >= eps, to 1 ulp. The instruction takes numbers below 2^-126 as 0, so where eps leaves room for them (a
+// uniform branch; for every row 8192 tokens took 41.6 us instead of 41.2) small ones are scaled.
+__device__ __forceinline__ float mrope_rsqrt(float v, float eps) {
+  float up = 1.0f;
+  if (__builtin_expect(eps < 0x1p-100f, 0)) {
+    asm volatile("");  // (a branch: selects would be paid for by every row)
+    if (v < 0x1p-100f) v *= 0x1p100f, up = 0x1p50f;
+  }
+  return __builtin_amdgcn_rsqf(v) * up;
+}
+
 // The angle position * inv_freq in half turns, in [-1, 1]. Up to 2^24 turns one double holds them: the constant's rounding, the
 // position's and those of two products are 2^-27 of a turn at most, and the fraction's rounding to fp32 is 2^-26. Farther ones take
 // 1 / (2 pi) as two doubles, its product with inv_freq as the rounded one (hi) and what is left of it (lo), and the position as
@@ -173,7 +184,7 @@ __global__ __launch_bounds__(256) void qkv_norm_mrope_store_kernel(MropeArgs a) 
           for (int off = LPH / 2; off > 0; off >>= 1) ss += __shfl_xor(ss, off, 64);
         }
         if (roped) {
-          const float inv = __builtin_amdgcn_rsqf(ss * (1.0f / D) + a.eps);  // (1 ulp)
+          const float inv = mrope_rsqrt(ss * (1.0f / D) + a.eps, a.eps);
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * gf[e];
         }

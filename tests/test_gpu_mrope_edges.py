@@ -11,6 +11,7 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import weights as ow
 from sglang_neuron_amd import ops
 from tests.conftest import announce
 from tests.test_gpu_mrope import E, _make, _run
@@ -86,3 +87,22 @@ def test_infinite_elements_that_are_not_rotated_stay(d, rot):
     assert torch.equal(bits(kc[at][..., rot:]), bits(x[:, Hq:Hq + Hkv, rot:]))
     assert torch.equal(bits(vc[at]), bits(x[:, Hq + Hkv:]))
     assert bool(torch.isfinite(q[..., :rot]).all())
+
+
+@pytest.mark.parametrize("d", [128, 64])
+@pytest.mark.parametrize("power", [-50, -62, -63, -64, -65])
+def test_norm_of_tiny_rows_without_an_eps(power, d):
+    """Down to mean squares that fp32 holds in fewer bits. (2^-130 in steps of 2^-149 is off by 2^-20 at most, and so is each of
+    its d squares, all of one sign: the norm by half of both, 2^-20.)"""
+    T, Hq, Hkv, P = 6, 2, 1, 16
+    qkv, pos, inv, gam, slots, k, v, sc = _make(37, T, Hq, Hkv, d, P, False, True, d, 1, 10)
+    qkv = (qkv.double() * 2.0 ** power).to(torch.bfloat16)
+    q, kc, _ = _run(qkv, pos, inv, [0] * (d // 2), Hq, Hkv, d, k, v, slots, gam, sc, norm_eps=0.0)
+    wq, wk, _, size = ow.mrope_rows(qkv, pos, inv, [0] * (d // 2), Hq, Hkv, d, gam[0], gam[1], 0.0)
+    got, want = torch.cat([q.double(), kc.double()[slots // P, :, slots % P]], 1), torch.cat([wq, wk], 1)
+    tol = want.abs() * 2.0 ** -8 + size * (E + 2.0 ** -20) * (1 + 2.0 ** -8)
+    assert bool(((got - want).abs() <= tol).all())
+    # a row of zeros has no direction: 0 / 0
+    qkv[2] = 0
+    q, _, _ = _run(qkv, pos, inv, [0] * (d // 2), Hq, Hkv, d, k, v, slots, gam, sc, norm_eps=0.0)
+    assert bool(q[2].isnan().all()) and bool(torch.isfinite(q[[0, 1, 3, 4, 5]]).all())
