@@ -510,7 +510,7 @@ int sna_decode_attention_weights(const void *q, const void *k_cache, const float
  *   kept      [R, num_kv_heads, keep] int32: the positions in ascending order, -1 past a short row's.
  *   new_lens  [R] int32: min(L, keep).
  *   weights_out [R, num_kv_heads, out_width] fp32 (out_width >= keep): the kept tokens' weights, then zeros; or NULL. It
- *             may be `weights` itself (same address and strides; wider or narrower), and overlaps it in no other way.
+ *             may be `weights` itself (same address and strides; out_width may differ), and overlaps it in no other way.
  *   workspace device, 16-byte aligned, at least sna_select_workspace_bytes bytes (in_place: weights_out is weights; 0 for
  *             rows of up to 16384 columns, and it may be NULL then), any contents; calls that share one on different
  *             streams race.

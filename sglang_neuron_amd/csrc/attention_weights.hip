@@ -19,14 +19,14 @@
 //     weights_row_kernel           a pair's scores in the LDS of one workgroup: one launch
 // Scores are fp32, exponentials in the log2 domain, every sum fp32; sums run in a fixed order, without atomics.
 //
-// Measured (us of kernels; heads 32/8 of 128, e4m3fn, pages of 16, where not said): 64 rows of 4096 keys 65.6, 273 MB of
-// keys at 4.2 TB/s (HBM: a plain copy reaches 4.8); 8 rows of 128-1024 bf16 keys, heads 16/8, 5.2 + 4.4 (two launches and
-// their chains of round trips); 128 rows of 2048-8192 keys, heads 8/1 of 64, 17 + 8 (the same, ragged); 32 queries over
-// each of 3001 to 16384 keys 22.8 + 5 + 26.8 (three launches' chains of loads) and 64 over 131071 bf16 keys 105 + 6 + 115
-// (products 28-31% and VALU 50-56% of the cycles, the keys read twice at 2.6 TB/s); 4 x 2048 queries after 2048 each 470-490
-// in all, the first pass a little over half: products take 37% (41% in the second pass) of a SIMD's cycles and VALU
-// instructions 61% (57%), which together is all of them: a wave's matrix instructions and the other waves' VALU hardly
-// overlap here.
+// Measured (us of kernels; heads 32/8 of 128, e4m3fn, pages of 16, where not said): 64 rows of 4096 keys 66, 273 MB of
+// keys at 4.2 TB/s (HBM: a plain copy reaches 4.8); 8 rows of 128-1024 bf16 keys, heads 16/8, 5.0 + 4.1 (two launches and
+// their chains of round trips); 128 rows of 2048-8192 keys, heads 8/1 of 64, 17 + 8 (the same, ragged, and 22 MB of scores
+// written and read beside 43 MB of keys); 32 queries over each of 3001 to 16384 keys 22 + 5 + 26 (three launches' chains of
+// loads) and 64 over 131071 bf16 keys 214 in all (products 28-31% and VALU 49-56% of the cycles, the keys read twice at 2.6
+// TB/s); 4 x 2048 queries after 2048 each 470 in all, the first pass a little over half: products take 36% (40% in the second
+// pass) of a SIMD's cycles and VALU instructions 59% (54%). These are two pipes that different waves could keep busy at once;
+// that their shares add up to 95% says that the three waves of a SIMD hardly overlap them here, not that they cannot.
 #include <float.h>
 
 #include <algorithm>

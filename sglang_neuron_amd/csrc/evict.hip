@@ -14,10 +14,11 @@
 //            independent, so several workgroups share a row by columns, and K and V are apart. To other pages nothing
 //            orders the tokens and the tiles go to workgroups of their own.
 // Both are bound by memory (latency for few rows): select reads 4 bytes a token and head, compact reads and writes the
-// kept rows. Measured (us, 8 KV heads): select of one row of 1000 tokens 7.4 (a chain of 3 histograms on one CU), of 32 rows
-// of up to 8192 12.7, of 4 rows of 50001 to 131072 7 + 9 + 10 + 14 (three passes and the writer, each one round trip and the
-// row's histograms); compact to other pages of 32 x 1024 e4m3fn tokens of 128 24, 5.6 TB/s read and written, of 4 x 8192 bf16
-// 62, 4.3 TB/s (a plain copy: 4.8), in place 26 and 94.
+// kept rows. Measured (us, 8 KV heads): select of one row of 1000 tokens 7.6 (a chain of 3 histograms on one CU), of 32 rows
+// of up to 8192 13-14, of 4 rows of 50001 to 131072 7 + 9 + 10 + 14 (three passes and the writer, each one round trip and the
+// row's histograms; in place 10 more for the weights' way back); compact to other pages of 32 x 1024 e4m3fn tokens of 128
+// 24-26, 5.2-5.6 TB/s read and written, of 4 x 8192 bf16 62, 4.3 TB/s (a plain copy: 4.8), in place 26-28 and 94-99 (a
+// workgroup reads a tile, waits, writes it, and only then asks for the next).
 #include <algorithm>
 
 #include "sna_device.h"

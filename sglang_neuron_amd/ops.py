@@ -252,9 +252,9 @@ def qkv_norm_mrope_store(qkv: Tensor, *, positions: Tensor, inv_freq: Tensor, ax
     """The writer of qkv_norm_rope_store for rotary positions with several axes (images, video): pair i of a Q or K head
     (elements i and i + n, n = len(inv_freq)) is rotated by the angle ``positions[axes[i], t] * inv_freq[i]``, elements
     past 2 n stay. ``positions`` [A, T] int64 (A of 1 to 4), ``inv_freq`` [n] fp32 (n a multiple of 8, at most d / 2),
-    ``axes`` [n] host ints (mrope_axes). The other arguments are qkv_norm_rope_store's. Every angle keeps its fraction
-    of a turn to fp32, at positions of any size; norm and rotation are fp32 and every output is rounded once. Returns Q [T, q, d] bf16; the
-    caches are written in place."""
+    ``axes`` [n] host ints (mrope_axes; any sequence or array of them). The other arguments are qkv_norm_rope_store's. Every
+    angle keeps its fraction of a turn to fp32, at positions of any size; norm and rotation are fp32 and every output is rounded
+    once. Returns Q [T, q, d] bf16; the caches are written in place."""
     # (conditions are tested here and messages built by _need only where one fails: the checks of a small call cost as much
     # as its kernel)
     dev = _on_gpu(qkv, positions, inv_freq, k_cache, v_cache, slot_mapping, q_norm, k_norm, k_scale, v_scale, q_out)
@@ -1073,7 +1073,12 @@ def prefill_attention_weights(q: Tensor, k_cache: Tensor, block_table: Tensor, q
 
     ``weights`` [R, G, N] fp32, when given, is added to and returned (keys past N get nothing, entries without a key stay
     as they are); without it a new tensor of N = table width * page is returned, zero where there is no key. The same call
-    gives the same bits."""
+    gives the same bits. A query or key that is NaN makes the keys that its rows see NaN, and no others.
+
+    More than 16 rows (queries * heads of a KV head) a request take a workspace of 8 bytes a token, query head and 256 columns
+    of the table (8192 tokens of 32 heads over a table of 131072 keys: 1.07 GB), whatever the rows' lengths: where that is too
+    much, pass the requests or the chunk's parts in turn and add (``weights``). ``max_q_len`` bounds the chunk lengths; queries
+    past it add nothing."""
     _need(q.dim() == 3, lambda: f"q must be [T, H, d], got {tuple(q.shape)}")
     T, R = q.shape[0], prior_lens.numel()
     _need(q_start.numel() == R + 1, lambda: f"q_start must be [{R + 1}]")
@@ -1105,8 +1110,8 @@ def select_tokens(weights: Tensor, seq_lens: Tensor, *, keep: int, first: int = 
     counts as N: tokens without a weight are not kept.
 
     ``weights_out`` [R, G, M >= keep] fp32, when given, receives the kept tokens' weights and zeros after them; it may be
-    ``weights`` itself, so that the tokens written next start at zero, and be wider or narrower than it (``weights=buf[..., :n],
-    weights_out=buf``)."""
+    ``weights`` itself, so that the tokens written next start at zero, wider or narrower than it included
+    (``weights=buf[..., :n], weights_out=buf``)."""
     dev = _on_gpu(weights, seq_lens, weights_out)
     args, (kept, new_lens), _keep = _select_args(dev, weights, seq_lens, keep, first, recent, weights_out)
     if kept.shape[0] and kept.shape[1]:
