@@ -23,8 +23,8 @@
 // keys at 4.2 TB/s (HBM: a plain copy reaches 4.8); 8 rows of 128-1024 bf16 keys, heads 16/8, 5.0 + 4.1 (two launches and
 // their chains of round trips); 128 rows of 2048-8192 keys, heads 8/1 of 64, 17 + 8 (the same, ragged, and 22 MB of scores
 // written and read beside 43 MB of keys); 32 queries over each of 3001 to 16384 keys 22 + 5 + 26 (three launches' chains of
-// loads) and 64 over 131071 bf16 keys 214 in all (products 28-31% and VALU 49-56% of the cycles, the keys read twice at 2.6
-// TB/s); 4 x 2048 queries after 2048 each 470 in all, the first pass a little over half: products take 36% (40% in the second
+// loads) and 64 over 131071 bf16 keys 214-224 in all (products 28-31% and VALU 49-56% of the cycles, the keys read twice at 2.6
+// TB/s); 4 x 2048 queries after 2048 each 470-490 in all, the first pass a little over half: products take 36% (40% in the second
 // pass) of a SIMD's cycles and VALU instructions 59% (54%). These are two pipes that different waves could keep busy at once;
 // that their shares add up to 95% says that the three waves of a SIMD hardly overlap them here, not that they cannot.
 #include <float.h>
