@@ -54,6 +54,7 @@ extern "C" {
 #define SNA_DTYPE_BF16 0
 #define SNA_DTYPE_FP8_E4M3FN 1
 #define SNA_DTYPE_FP8_E4M3FN_MUL 2
+#define SNA_DTYPE_INT8 3 /* int8 codes: only in a cache whose blocks of tokens carry scales */
 
 /* Library ABI version (major * 100 + minor). */
 int sna_version(void);
@@ -460,6 +461,73 @@ int sna_prefill_attention_split(const void *q, const void *k_cache, const void *
                                 int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
                                 int64_t num_blocks, int32_t kv_dtype, void *workspace, int64_t workspace_bytes,
                                 void *stream);
+
+/* =====================================================================================================
+ * A cache whose blocks of tokens carry scales: its writer, attention over it, and over the pages that a query selects
+ * ===================================================================================================== */
+
+/* One layer's caches [num_blocks, num_kv_heads, page_size, head_dim] of SNA_DTYPE_FP8_E4M3FN or SNA_DTYPE_INT8 codes with
+ * k_scale, v_scale [num_blocks, num_kv_heads, page_size / scale_tokens] fp32: a code is worth code * the scale of its block
+ * of scale_tokens tokens (a multiple of 16 that divides the page). Or bf16 elements (SNA_DTYPE_BF16) without scales, which
+ * are then ignored. Pages are found through block tables [rows, table_width] int32 (row stride table_stride), entries
+ * outside the pool being no page. head_dim 64 or 128, page_size a multiple of 16. */
+#define SNA_MAX_BLOCK_PAGE 4096 /* the largest page_size of these calls */
+
+/* Appends tokens to their requests' rows and keeps the scales up.
+ *   k, v         [n_tokens, num_kv_heads, head_dim] bf16, 16-byte aligned, their rows k_row_stride and v_row_stride
+ *                elements apart (multiples of 8, at least num_kv_heads * head_dim); request r's tokens are rows q_start[r] ..
+ *                q_start[r + 1] - 1, at positions prior_lens[r], + 1, ..; q_start NULL: row r is request r's one token.
+ *   max_q_len    bounds the requests' tokens (tokens past it are not stored).
+ *   scales       contiguous. For each block of a page, KV head and cache that the call writes, with
+ *                  fresh = max(max |x| / top, 2^-100), top 448 (FP8) or 127 (int8), over the call's tokens of the block
+ *                  (infinities not counted; a NaN makes it NaN),
+ *                the scale becomes fresh where the call writes the block's first token (it starts anew), else the larger of
+ *                fresh and what it was. New codes are x / scale, clamped to +-top, to nearest even; where the scale grew, the
+ *                block's earlier tokens are rounded again, code * old / new. Tokens behind the written ones stay as they are.
+ *   k_bounds     [num_blocks, num_kv_heads, 2, head_dim] bf16 or NULL: the least and the largest value of each dimension
+ *                over a page's keys (the k given, before any rounding), likewise started anew by a page's first token. A NaN
+ *                widens nothing.
+ * A token without a page (past the table, or an entry outside the pool) is not stored. No page may be written for two
+ * requests of a call. The same call gives the same bits. */
+int sna_kv_store_blocks(const void *k, const void *v, int64_t k_row_stride, int64_t v_row_stride, int32_t n_tokens,
+                        const int32_t *block_table, int64_t table_stride, int32_t table_width, const int32_t *q_start, const int32_t *prior_lens, int32_t R,
+                        int32_t max_q_len, void *k_cache, void *v_cache, float *k_scale, float *v_scale,
+                        int32_t scale_tokens, void *k_bounds, int64_t num_blocks, int32_t num_kv_heads, int32_t page_size,
+                        int32_t head_dim, int32_t cache_dtype, void *stream);
+
+/* Attention of T single queries over the pool:
+ *   q            [T, num_q_heads, head_dim] bf16, 16-byte aligned; query t sees the first seq_lens[t] keys of table row
+ *                rows[t] (rows NULL: row t; a row outside the table's table_rows has no keys): its own key is stored
+ *                already. window > 0: the last `window` of them.
+ *   blocks       NULL, or [T, num_kv_heads, n_blocks] int32 table columns: query t's heads of KV head g see only the keys on
+ *                the pages that blocks[t, g] names. Entries outside the table (-1) name none; a column named twice counts
+ *                twice. No window then.
+ *   scales       strides scale_page_stride and scale_head_stride (elements; 0: one scale for all), the blocks of a page and
+ *                head contiguous.
+ *   sinks        [num_q_heads] fp32 logits joining the softmax denominator, or NULL.
+ *   out          [T, num_q_heads, head_dim] bf16; a query that sees no key gives zeros.
+ *   workspace    device, 16-byte aligned, sna_block_decode_workspace_bytes bytes (n_blocks 0: no list), any contents; calls
+ *                that share one on different streams race.
+ * num_q_heads / num_kv_heads <= 16. The same call gives the same bits. */
+int64_t sna_block_decode_workspace_bytes(int32_t T, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                         int32_t page_size, int32_t table_width, int32_t window, int32_t n_blocks);
+int sna_paged_decode_blocks(const void *q, const void *k_cache, const void *v_cache, const float *k_scale,
+                            const float *v_scale, int64_t scale_page_stride, int64_t scale_head_stride,
+                            int32_t scale_tokens, const int32_t *block_table, int64_t table_stride, int32_t table_width,
+                            int32_t table_rows, const int32_t *rows, const int32_t *seq_lens, const int32_t *blocks,
+                            int32_t n_blocks, const float *sinks, int32_t window, float sm_scale, void *out, int32_t T,
+                            int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                            int64_t num_blocks, int32_t cache_dtype, void *workspace, int64_t workspace_bytes,
+                            void *stream);
+
+/* The score of each page of a query's row, from the pages' key bounds: scores[t, g, c] = max over KV head g's query heads of
+ * sum_d max(q_d lo_d, q_d hi_d), which no key of the page in column c exceeds; -inf past the row's pages and on invalid
+ * ones. scores [T, num_kv_heads, table_width] fp32; counts [T] int32: the rows' pages, ceil(seq_lens / page_size), for a
+ * selection by the scores (sna_select_tokens). The other arguments as above. */
+int sna_block_scores(const void *q, const void *k_bounds, const int32_t *block_table, int64_t table_stride,
+                     int32_t table_width, int32_t table_rows, const int32_t *rows, const int32_t *seq_lens, float *scores,
+                     int32_t *counts, int32_t T, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                     int32_t page_size, int64_t num_blocks, void *stream);
 
 /* =====================================================================================================
  * Attention weights of cached keys, and eviction by them

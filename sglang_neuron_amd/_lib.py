@@ -26,6 +26,9 @@ NOALLOC_SCRATCH_BYTES = 16 << 20  # SNA_NOALLOC_SCRATCH_BYTES
 DTYPE_BF16 = 0
 DTYPE_FP8_E4M3FN = 1
 DTYPE_FP8_E4M3FN_MUL = 2  # FP8 bytes; the scales are the GPT-OSS quantization multipliers (SNA_DTYPE_FP8_E4M3FN_MUL)
+DTYPE_INT8 = 3  # int8 codes of a cache whose blocks of tokens carry scales (SNA_DTYPE_INT8)
+
+MAX_BLOCK_PAGE = 4096  # SNA_MAX_BLOCK_PAGE
 
 MAX_CTAS = 256       # SNA_MAX_CTAS
 MAX_PLAN_ROWS = 256  # SNA_MAX_PLAN_ROWS
@@ -108,6 +111,12 @@ SIGNATURES = {
                                   _P]),
     "sna_evict_tokens": (_I32, [_P, _P, _I64, _I32, _I32, _I32, _I32, _P, _I64, _I32, _P, _I64, _I32, _P, _I64, _I64, _I32,
                                 _P, _I32, _I32, _I32, _I32, _P, _P, _P, _I64, _I64, _I32, _P, _I64, _P]),
+    "sna_kv_store_blocks": (_I32, [_P, _P, _I64, _I64, _I32, _P, _I64, _I32, _P, _P, _I32, _I32, _P, _P, _P, _P, _I32, _P, _I64, _I32,
+                                   _I32, _I32, _I32, _P]),
+    "sna_block_decode_workspace_bytes": (_I64, [_I32] * 8),
+    "sna_paged_decode_blocks": (_I32, [_P, _P, _P, _P, _P, _I64, _I64, _I32, _P, _I64, _I32, _I32, _P, _P, _P, _I32, _P,
+                                       _I32, _F32, _P, _I32, _I32, _I32, _I32, _I32, _I64, _I32, _P, _I64, _P]),
+    "sna_block_scores": (_I32, [_P, _P, _P, _I64, _I32, _I32, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I64, _P]),
     "sna_index_key_store": (_I32, [_P, _P, _I64, _I32, _P, _I64, _P]),
     "sna_indexer_scores": (_I32, [_P, _P, _P, _P, _I64, _I32, _P, _I32, _I32, _I32, _I32, _I64, _I32, _P, _I64, _P]),
     "sna_page_items_wire_bytes": (_I64, [_P, _I32, _I64]),

@@ -39,7 +39,8 @@ HIP_FLAGS = [
 # straight away: in VGPRs they need no read back from AGPRs (16 moves a tile; 57.1 -> 56.6 us on the benchmark).
 _MFMA_VGPR = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
 EXTRA_FLAGS = {"decode_mla.hip": _MFMA_VGPR, "decode_gqa.hip": _MFMA_VGPR, "prefill_gqa.hip": _MFMA_VGPR,
-               "indexer.hip": _MFMA_VGPR, "attention_weights.hip": _MFMA_VGPR}
+               "indexer.hip": _MFMA_VGPR, "attention_weights.hip": _MFMA_VGPR,
+               "block_decode.hip": _MFMA_VGPR}
 
 
 def hipcc() -> str:

@@ -1,0 +1,537 @@
+// Attention of single query tokens over a paged GQA cache whose blocks of tokens carry scales (e4m3fn or int8 codes; bf16
+// without scales): over all of a row's keys, or over the pages that a list names for each query and KV head.
+//
+//   out[t, h] = sum_j p_j v_j / (sum_j p_j + e^(sink_h - m)),  p_j = e^(sm_scale q[t, h] . k_j - m),
+// over the keys j < seq_lens[t] of table row rows[t] (inside the window; on the listed pages), with k_j = code * its
+// block's K scale and v_j = code * its block's V scale. A block's scales are the same for 16 keys at a time, so K's joins
+// the score's factor and V's the probability: codes go into the matrix products as they are, exact in bf16.
+//
+// Work: one workgroup per (query, split, KV head); the splits of a query divide its 32-key tiles evenly, and a second launch
+// merges them where there are several. A wave takes tiles round-robin, the next one's loads in flight while it computes one.
+// A tile is two half-tiles of 16 keys, each inside one page and one block. Lane roles (lane = 16 g4 + li):
+//   QK   S^T[key, head] = K[key, :] . Q[head, :], v_mfma_f32_16x16x32_bf16 with M = 16 keys, N = 16 heads (the group's,
+//        zero-padded): lane (g4, li) feeds key li's 16-byte chunks 4 c + g4 and head li's elements of the same dims, and
+//        gets S^T[4 g4 + r, li].
+//   PV   O^T[d, head] = V^T[d, keys] . P^T[keys, head] over the tile's 32 keys, lane (g4, *) supplying keys 4 g4 .. + 3 of
+//        both halves, which are the probabilities it holds: only V is transposed, in registers (lane (g4, li) loads D / 16
+//        contiguous elements from D / 16 * li of its 8 keys).
+//   acc  lane (g4, j), d-tile t, row r: O[head j, D / 16 * (4 g4 + r) + t].
+// The softmax state is (m, l, acc) in the log2 domain, m moved only when a tile's maximum passes it by more than 8.
+#include <algorithm>
+
+#include "sna_device.h"
+#include "sna_host.h"
+
+namespace sna {
+
+struct BlockDecodeArgs {
+  const uint16_t* q;  // [T, H, D] bf16
+  const uint8_t* k_cache;
+  const uint8_t* v_cache;
+  const float* k_scale;  // [num_blocks, G, P / bt], page and head strides below
+  const float* v_scale;
+  int64_t scale_page, scale_head;
+  int32_t sub_magic;  // ceil(2^16 / (bt / 16)): a 16-key half's block in its page (0: one block a page)
+  const int32_t* table;
+  int64_t table_stride;
+  int32_t table_width, table_rows;
+  const int32_t* rows;      // [T] each query's table row, or null: query t's is t
+  const int32_t* seq_lens;  // [T]
+  const int32_t* blocks;    // SEL: [T, G, n_blocks] table columns
+  int32_t n_blocks;
+  const float* sinks;  // [H] or null
+  int32_t T, H, G, group, P, halves;  // halves: 16-key halves a page
+  int64_t num_blocks;
+  int32_t window;
+  float sm_scale;
+  int32_t splits;
+  float* ws_o;   // [T, splits, H, D] unnormalized partials
+  float* ws_ml;  // [T, splits, H, 2] reference max (log2 domain) and softmax sum
+  uint16_t* out;
+};
+
+constexpr float kBlockRescaleSlack = 8.0f;
+
+template <int NB>
+__device__ __forceinline__ void load_run(const uint8_t* p, uint32_t (&dst)[NB / 4]) {
+  if constexpr (NB % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < NB / 16; ++i) {
+      const uint4 w = ld16_stream(p + 16 * i);
+      dst[4 * i] = w.x, dst[4 * i + 1] = w.y, dst[4 * i + 2] = w.z, dst[4 * i + 3] = w.w;
+    }
+  } else if constexpr (NB == 8) {
+    const uint2 w = ld8_stream(p);
+    dst[0] = w.x, dst[1] = w.y;
+  } else {
+    static_assert(NB == 4, "4, 8 or a multiple of 16 bytes");
+    dst[0] = ld4_stream(p);
+  }
+}
+
+// Four codes of a dword to four bf16 values.
+template <int FMT>
+__device__ __forceinline__ void codes_to_bf16x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FMT == kBlockFp8) fp8x4_to_bf16x4(w, lo, hi);
+  else int8x4_to_bf16x4(w, lo, hi);
+}
+
+template <int D, int FMT>
+struct BlockTile {
+  static constexpr int ESZ = FMT == kBlockBf16 ? 2 : 1;
+  static constexpr int KB = D / 4 * ESZ;   // K bytes per lane and key
+  static constexpr int VB = D / 16 * ESZ;  // V bytes per lane and key
+  uint32_t k[2][KB / 4];
+  uint32_t v[8][VB / 4];
+  float scale;     // lane group 0: K's of half 0, 1: K's of half 1, 2 and 3: V's
+  int32_t pos[2];  // the halves' first positions
+  bool valid[2];   // on a page of the pool, below the table's width
+};
+
+template <int D, int FMT, bool SEL, bool FINAL, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2)))
+void block_decode_kernel(BlockDecodeArgs a) {
+  using Tile = BlockTile<D, FMT>;
+  constexpr int ESZ = Tile::ESZ, KB = Tile::KB, VB = Tile::VB;
+  constexpr int STEPS = D / 32;  // QK products of a half-tile
+  constexpr int VE = D / 16;     // V elements per lane and key
+  constexpr int DT = D / 16;     // d-tiles
+  constexpr int CE = 16 / ESZ;   // elements of a 16-byte chunk
+  const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, li = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int32_t g = blockIdx.y;
+  const int32_t t = (int32_t)(blockIdx.x / (uint32_t)a.splits), split = (int32_t)blockIdx.x - t * a.splits;
+  const int32_t row_v = a.rows ? a.rows[t] : t, len_v = a.seq_lens[t];
+
+  // query operand: step s, lane (g4, li): head li's 8 elements from dim CE (4 c + g4) + w, 8 s = CE c + w
+  uint32_t qv[STEPS][4];
+  {
+    const uint16_t* qp = a.q + ((int64_t)t * a.H + g * a.group + min(li, a.group - 1)) * D;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const uint4 w = ld16(qp + CE * (4 * (8 * s / CE) + g4) + (8 * s) % CE);
+      const bool live = li < a.group;
+      qv[s][0] = live ? w.x : 0u, qv[s][1] = live ? w.y : 0u, qv[s][2] = live ? w.z : 0u, qv[s][3] = live ? w.w : 0u;
+    }
+  }
+  const float sink_pre = FINAL && a.sinks && tid < a.group ? a.sinks[g * a.group + tid] : 0.0f;
+
+  const int32_t row = __builtin_amdgcn_readfirstlane(row_v);
+  const bool row_ok = row >= 0 && row < a.table_rows;
+  // (keys past the table have no page)
+  const int64_t table_keys = (int64_t)a.table_width * a.P;
+  const int32_t L = row_ok ? (int32_t)min((int64_t)max(__builtin_amdgcn_readfirstlane(len_v), 0), table_keys) : 0;
+  const int32_t lo = a.window > 0 ? max(0, L - a.window) : 0;  // visible: [lo, L)
+  const int32_t* trow = a.table + (int64_t)(row_ok ? row : 0) * a.table_stride;
+  const int32_t* list = SEL ? a.blocks + ((int64_t)t * a.G + g) * a.n_blocks : nullptr;
+  // The tiles of this split. Dense: tile i is positions 32 i ..; SEL: the listed pages' halves, two by two.
+  int32_t t_first, t_last;
+  {
+    const int32_t all0 = SEL ? 0 : lo / 32;
+    const int32_t all1 = SEL ? (L > 0 ? (a.n_blocks * a.halves + 1) / 2 : 0) : (int32_t)(((int64_t)L + 31) / 32);
+    const int32_t n = max(all1 - all0, 0), per = n / a.splits, extra = n - per * a.splits;
+    t_first = all0 + split * per + min(split, extra);
+    t_last = t_first + per + (split < extra ? 1 : 0);
+  }
+
+  const int32_t ncol = SEL ? a.n_blocks : a.table_width;
+  const bool pow2 = (a.P & (a.P - 1)) == 0;
+  const int p_shift = __builtin_ctz((uint32_t)a.P);
+  // entry (table column, or place in the list) of a half, and its place in the page
+  auto entry_of = [&](int32_t half) -> int32_t { return pow2 ? half >> (p_shift - 4) : half / a.halves; };
+  // The pages of 256 entries from col0 on, entry col0 + 64 i + lane in pg[i] (-1: none); SEL: their table columns in bk.
+  // A wave's entries ascend: it loads the next 256 when it gets there.
+  int32_t col0 = 0, pg[4], bk[4];
+  auto stage = [&](int32_t c0) {
+    col0 = c0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int32_t c = c0 + 64 * i + lane;
+      int32_t b = c;
+      if (SEL) b = c < ncol ? list[c] : -1;
+      pg[i] = b >= 0 && b < a.table_width && c < ncol ? trow[b] : -1;
+      if (pg[i] >= a.num_blocks) pg[i] = -1;
+      bk[i] = pg[i] >= 0 ? b : 0;
+    }
+  };
+  auto pick = [&](const int32_t (&v)[4], int32_t c) -> int32_t {
+    return __builtin_amdgcn_readlane(c < 64 ? v[0] : (c < 128 ? v[1] : (c < 192 ? v[2] : v[3])), c & 63);
+  };
+
+  const int64_t head_bytes = (int64_t)a.P * D * ESZ;
+  const float* scale_base = FMT == kBlockBf16 ? nullptr : (g4 < 2 ? a.k_scale : a.v_scale) + g * a.scale_head;
+  auto load_tile = [&](Tile& T, int32_t tile) {
+    int32_t page[2], sub[2];
+    const int32_t half0 = __builtin_amdgcn_readfirstlane(2 * tile);
+    if (entry_of(half0 + 1) - col0 >= 256) stage(entry_of(half0));
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int32_t half = half0 + hf, e = entry_of(half), in16 = half - e * a.halves;  // the half's place in its page
+      const bool inside = e < ncol;
+      const int32_t c = inside ? e - col0 : 0;
+      const int32_t p = pick(pg, c);
+      const int32_t b = SEL ? pick(bk, c) : e;
+      T.pos[hf] = b * a.P + 16 * in16;
+      T.valid[hf] = inside && p >= 0 && T.pos[hf] < L;
+      page[hf] = T.valid[hf] ? p : 0;
+      sub[hf] = T.valid[hf] ? (int32_t)((uint32_t)in16 * (uint32_t)a.sub_magic >> 16) : 0;
+      const int64_t blk = ((int64_t)page[hf] * a.G + g) * head_bytes + (int64_t)(16 * in16) * D * ESZ;
+      const uint8_t* kp = a.k_cache + blk + (int64_t)li * D * ESZ + 16 * g4;
+#pragma unroll
+      for (int c4 = 0; c4 < KB / 16; ++c4)
+        load_run<16>(kp + 64 * c4, *reinterpret_cast<uint32_t(*)[4]>(&T.k[hf][4 * c4]));
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4)
+        load_run<VB>(a.v_cache + blk + (int64_t)(4 * g4 + e4) * D * ESZ + VB * li, T.v[4 * hf + e4]);
+    }
+    if constexpr (FMT != kBlockBf16) {
+      const bool second = g4 & 1;
+      T.scale = scale_base[(int64_t)(second ? page[1] : page[0]) * a.scale_page + (second ? sub[1] : sub[0])];
+    }
+  };
+
+  float m_ref = kNegBig, l_run = 0.0f;
+  f32x4_t acc[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const float qk_scale = a.sm_scale * kLog2e;
+
+  auto compute_tile = [&](Tile& T) {
+    float ks[2] = {qk_scale, qk_scale}, vs[2] = {1.0f, 1.0f};
+    if constexpr (FMT != kBlockBf16) {
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        ks[hf] = qk_scale * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(T.scale), 16 * hf));
+        vs[hf] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(T.scale), 32 + 16 * hf));
+      }
+    }
+    float x[8];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st) {
+        uint32_t op[4];
+        if constexpr (FMT == kBlockBf16) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) op[i] = T.k[hf][4 * st + i];
+        } else {
+          codes_to_bf16x4<FMT>(T.k[hf][2 * st], op[0], op[1]);
+          codes_to_bf16x4<FMT>(T.k[hf][2 * st + 1], op[2], op[3]);
+        }
+        s = mfma_16x16x32_bf16(op, qv[st], s);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[4 * hf + r] = s[r] * ks[hf];
+    }
+    // a tile that is not wholly visible: hidden keys score -inf and their V (which may be anything) is zero
+    const bool full = T.valid[0] && T.valid[1] && T.pos[0] >= lo && T.pos[1] >= lo && T.pos[0] + 16 <= L && T.pos[1] + 16 <= L;
+    if (!full) {
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        bool any = false;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int32_t pos = T.pos[hf] + 4 * g4 + r;
+          const bool ok = T.valid[hf] && pos >= lo && pos < L;
+          any |= ok;
+          x[4 * hf + r] = ok ? x[4 * hf + r] : -INFINITY;
+#pragma unroll
+          for (int i = 0; i < VB / 4; ++i) T.v[4 * hf + r][i] = ok ? T.v[4 * hf + r][i] : 0u;
+        }
+        vs[hf] = any ? vs[hf] : 0.0f;  // (a block with no visible key here: its scale may be anything)
+      }
+    }
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) tmax = fmaxf(tmax, x[i]);
+    tmax = max_across_groups(tmax);
+    const bool bump = tmax > m_ref + kBlockRescaleSlack;
+    if (__any(bump)) {
+      const float m_new = bump ? tmax : m_ref;
+      const float alpha = __builtin_amdgcn_exp2f(m_ref - m_new);
+      m_ref = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int i = 0; i < DT; ++i) acc[i] *= alpha;
+    }
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(x[i] - m_ref);
+      l_run += p[i];
+      if constexpr (FMT != kBlockBf16) p[i] *= vs[i >> 2];
+    }
+    // the probabilities (times V's scale) go into the product as bf16, off by at most 2^-9 of themselves
+    const uint32_t pop[4] = {pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]),
+                             pack_bf16x2(p[6], p[7])};
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      uint32_t op[4];
+      if constexpr (FMT == kBlockBf16) {
+#pragma unroll
+        for (int pr = 0; pr < 4; ++pr) {
+          const uint32_t e0 = (T.v[2 * pr][dt >> 1] >> (16 * (dt & 1))) & 0xffffu;
+          const uint32_t e1 = (T.v[2 * pr + 1][dt >> 1] >> (16 * (dt & 1))) & 0xffffu;
+          op[pr] = e0 | (e1 << 16);
+        }
+      } else {
+        uint32_t c0 = 0, c1 = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          c0 |= ((T.v[e][dt >> 2] >> (8 * (dt & 3))) & 0xffu) << (8 * e);
+          c1 |= ((T.v[e + 4][dt >> 2] >> (8 * (dt & 3))) & 0xffu) << (8 * e);
+        }
+        codes_to_bf16x4<FMT>(c0, op[0], op[1]);
+        codes_to_bf16x4<FMT>(c1, op[2], op[3]);
+      }
+      acc[dt] = mfma_16x16x32_bf16(op, pop, acc[dt]);
+    }
+  };
+
+  // ---- the tile loop: two register tiles, one in flight ----
+  {
+    Tile ring[2];
+    const int32_t first = t_first + wave;
+    if (first < t_last) {
+      stage(entry_of(2 * first));
+      load_tile(ring[0], first);
+    }
+    for (int32_t cur = first; cur < t_last;) {
+      if (cur + WAVES < t_last) load_tile(ring[1], cur + WAVES);
+      compute_tile(ring[0]);
+      cur += WAVES;
+      if (cur >= t_last) break;
+      if (cur + WAVES < t_last) load_tile(ring[0], cur + WAVES);
+      compute_tile(ring[1]);
+      cur += WAVES;
+    }
+  }
+
+  // ---- merge the waves in LDS; write the output, or this split's partial ----
+  __shared__ float sm_o[WAVES][16][D + 1];
+  __shared__ float sm_m[WAVES][16], sm_l[WAVES][16], sm_sink[16];
+  if (FINAL && tid < a.group) sm_sink[tid] = sink_pre;
+  const float l_tot = sum_across_groups(l_run);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sm_o[wave][li][VE * (4 * g4 + r) + dt] = acc[dt][r];
+  if (g4 == 0) sm_m[wave][li] = m_ref, sm_l[wave][li] = l_tot;
+  __syncthreads();
+  for (int32_t idx = tid; idx < a.group * D; idx += 64 * WAVES) {
+    const int32_t j = idx / D, d = idx % D, h = g * a.group + j;
+    float M = kNegBig;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) M = fmaxf(M, sm_m[w][j]);
+    float o = 0.0f, l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float e = __builtin_amdgcn_exp2f(sm_m[w][j] - M);
+      o += e * sm_o[w][j][d];
+      l += e * sm_l[w][j];
+    }
+    if constexpr (FINAL) {
+      if (a.sinks) l += __builtin_amdgcn_exp2f(sm_sink[j] * kLog2e - M);
+      a.out[((int64_t)t * a.H + h) * D + d] = (uint16_t)f32_to_bf16_bits(l == 0.0f ? 0.0f : o / l);
+    } else {
+      const int64_t at = ((int64_t)t * a.splits + split) * a.H + h;
+      a.ws_o[at * D + d] = o;
+      if (d == 0) *reinterpret_cast<float2*>(a.ws_ml + 2 * at) = make_float2(M, l);
+    }
+  }
+}
+
+// Merge of a query's splits, one wave per (query, head): out = sum_s e_s o_s / (sum_s e_s l_s + e_sink), e_s = exp2(m_s -
+// M). Lane s of round i holds split 64 i + s's weight; lane i the dims D / 64 * i ... The partials stream 16 at a time.
+constexpr int kBlockMaxSplits = 256;
+template <int D>
+__global__ __launch_bounds__(64) void block_combine_kernel(BlockDecodeArgs a) {
+  constexpr int V = D / 64, CH = 16, N = kBlockMaxSplits / 64;
+  const int32_t t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, S = a.splits;
+  const int64_t at0 = (int64_t)t * S * a.H + h;
+  const float* ob = a.ws_o + at0 * D + V * lane;
+  const int64_t step = (int64_t)a.H * D;
+  float2 ml[N];
+  float M = kNegBig;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int32_t s = 64 * i + lane;
+    ml[i] = s < S ? *reinterpret_cast<const float2*>(a.ws_ml + 2 * (at0 + (int64_t)s * a.H)) : make_float2(kNegBig, 0.0f);
+    M = fmaxf(M, ml[i].x);
+  }
+  M = wave_max(M);
+  float den = 0.0f, e[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    e[i] = __builtin_amdgcn_exp2f(ml[i].x - M);
+    den += e[i] * ml[i].y;
+  }
+  den = wave_sum(den);
+  if (a.sinks) den += __builtin_amdgcn_exp2f(a.sinks[h] * kLog2e - M);
+  float o[V] = {};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (64 * i >= S) break;
+    for (int32_t s0 = 64 * i; s0 < min(S, 64 * i + 64); s0 += CH) {
+      float x[CH][V];
+#pragma unroll
+      for (int k = 0; k < CH; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[k][v] = ob[min(s0 + k, S - 1) * step + v];
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(e[i]), (s0 + k) & 63));
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] += s0 + k < S ? w * x[k][v] : 0.0f;
+      }
+    }
+  }
+  uint16_t* dst = a.out + ((int64_t)t * a.H + h) * D + V * lane;
+#pragma unroll
+  for (int v = 0; v < V; ++v) dst[v] = (uint16_t)f32_to_bf16_bits(den == 0.0f ? 0.0f : o[v] / den);
+}
+
+template <int D, int FMT, bool SEL>
+static void launch_block_decode(const BlockDecodeArgs& a, hipStream_t s) {
+  const dim3 grid((uint32_t)(a.T * a.splits), a.G);
+  if (a.splits == 1) {
+    hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, true, 4>), grid, dim3(256), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, false, 4>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((block_combine_kernel<D>), dim3(a.T, a.H), dim3(64), 0, s, a);
+  }
+}
+
+template <int D, bool SEL>
+static void launch_block_decode_format(const BlockDecodeArgs& a, int32_t dtype, hipStream_t s) {
+  if (dtype == SNA_DTYPE_BF16) launch_block_decode<D, kBlockBf16, SEL>(a, s);
+  else if (dtype == SNA_DTYPE_INT8) launch_block_decode<D, kBlockInt8, SEL>(a, s);
+  else launch_block_decode<D, kBlockFp8, SEL>(a, s);
+}
+
+// The splits of a query: enough workgroups for two a CU, none under 4 tiles.
+static int32_t block_splits(int32_t T, int32_t G, int64_t tiles) {
+  const int64_t base = (int64_t)T * G;
+  const int64_t want = (512 + base - 1) / base, most = std::max<int64_t>(1, tiles / 4);
+  return (int32_t)std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)kBlockMaxSplits}));
+}
+// The 32-key tiles that a query's keys can span.
+static int64_t block_tiles(int32_t page_size, int32_t table_width, int32_t window, int32_t n_blocks) {
+  const int64_t keys = (int64_t)(n_blocks > 0 ? n_blocks : table_width) * page_size;
+  return ((window > 0 ? std::min<int64_t>(keys, (int64_t)window + 31) : keys) + 31) / 32;
+}
+
+}  // namespace sna
+
+using namespace sna;
+
+extern "C" int64_t sna_block_decode_workspace_bytes(int32_t T, int32_t num_q_heads, int32_t num_kv_heads,
+                                                    int32_t head_dim, int32_t page_size, int32_t table_width,
+                                                    int32_t window, int32_t n_blocks) {
+  if (T < 1 || num_q_heads < 1 || num_kv_heads < 1 || head_dim < 1 || page_size < 1 || table_width < 1 || window < 0 ||
+      n_blocks < 0)
+    return 0;
+  const int32_t s = block_splits(T, num_kv_heads, block_tiles(page_size, table_width, window, n_blocks));
+  return s > 1 ? (int64_t)T * s * num_q_heads * (head_dim + 2) * (int64_t)sizeof(float) : 0;
+}
+
+extern "C" int sna_paged_decode_blocks(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                                       const float* v_scale, int64_t scale_page_stride, int64_t scale_head_stride,
+                                       int32_t scale_tokens, const int32_t* block_table, int64_t table_stride,
+                                       int32_t table_width, int32_t table_rows, const int32_t* rows,
+                                       const int32_t* seq_lens, const int32_t* blocks, int32_t n_blocks,
+                                       const float* sinks, int32_t window, float sm_scale, void* out, int32_t T,
+                                       int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                                       int64_t num_blocks, int32_t cache_dtype, void* workspace,
+                                       int64_t workspace_bytes, void* stream) {
+  ApiGuard guard;
+  const char* what = blocks ? "paged_decode_selected" : "paged_decode_blocks";
+  if (T < 0 || num_q_heads < 1 || num_kv_heads < 1 || num_q_heads % num_kv_heads || window < 0 || num_blocks < 1 ||
+      table_width < 1 || table_rows < 0 || table_stride < table_width || n_blocks < 0 || !(sm_scale > 0.0f))
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: bad sizes (T %d, heads %d / %d, window %d, blocks %lld, table %d x %d, "
+                "stride %lld, list %d) or scale %g", what, T, num_q_heads, num_kv_heads, window, (long long)num_blocks,
+                table_rows, table_width, (long long)table_stride, n_blocks, (double)sm_scale);
+  const int32_t group = num_q_heads / num_kv_heads;
+  if (group > 16) return fail(SNA_ERR_UNSUPPORTED, "%s: GQA group %d > 16 (a workgroup covers 16 query heads)", what, group);
+  if (head_dim != 64 && head_dim != 128)
+    return fail(SNA_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", what, head_dim);
+  if (page_size < 16 || page_size % 16 || page_size > SNA_MAX_BLOCK_PAGE)
+    return fail(SNA_ERR_UNSUPPORTED, "%s: page_size %d (a multiple of 16, at most %d)", what, page_size,
+                SNA_MAX_BLOCK_PAGE);
+  if (cache_dtype != SNA_DTYPE_BF16 && cache_dtype != SNA_DTYPE_FP8_E4M3FN && cache_dtype != SNA_DTYPE_INT8)
+    return fail(SNA_ERR_UNSUPPORTED, "%s: cache dtype %d (bf16, FP8 e4m3fn or int8)", what, cache_dtype);
+  const bool scaled = cache_dtype != SNA_DTYPE_BF16;
+  if (scaled && (scale_tokens < 16 || scale_tokens % 16 || page_size % scale_tokens || scale_page_stride < 0 ||
+                 scale_head_stride < 0))
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: a scale for every %d tokens (a multiple of 16 that divides the page of "
+                "%d), strides %lld and %lld", what, scale_tokens, page_size, (long long)scale_page_stride,
+                (long long)scale_head_stride);
+  if (blocks && (n_blocks < 1 || window > 0))
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: a list of %d pages, window %d (none)", what, n_blocks, window);
+  const int64_t keys = (int64_t)(blocks ? n_blocks : table_width) * page_size;
+  if (keys > INT32_MAX - 4096 || (int64_t)table_width * page_size > INT32_MAX - 4096)
+    return fail(SNA_ERR_UNSUPPORTED, "%s: %lld keys of a query, a table of %lld (positions are 32 bits)", what,
+                (long long)keys, (long long)table_width * page_size);
+  if (T == 0) return SNA_OK;
+  if (!q || !k_cache || !v_cache || !block_table || !seq_lens || !out || (scaled && (!k_scale || !v_scale)))
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16))
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: q and the caches must be 16-byte aligned", what);
+  if (!rows && table_rows < T)
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %d queries over a table of %d rows", what, T, table_rows);
+  if (num_q_heads > 65535) return fail(SNA_ERR_INVALID_ARGUMENT, "%s: grid too large", what);
+
+  BlockDecodeArgs a;
+  a.q = (const uint16_t*)q;
+  a.k_cache = (const uint8_t*)k_cache;
+  a.v_cache = (const uint8_t*)v_cache;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.scale_page = scale_page_stride;
+  a.scale_head = scale_head_stride;
+  const int32_t per = scaled ? scale_tokens / 16 : page_size / 16;
+  a.sub_magic = scaled && scale_tokens < page_size ? (65536 + per - 1) / per : 0;
+  a.table = block_table;
+  a.table_stride = table_stride;
+  a.table_width = table_width;
+  a.table_rows = table_rows;
+  a.rows = rows;
+  a.seq_lens = seq_lens;
+  a.blocks = blocks;
+  a.n_blocks = blocks ? n_blocks : 0;
+  a.sinks = sinks;
+  a.T = T;
+  a.H = num_q_heads;
+  a.G = num_kv_heads;
+  a.group = group;
+  a.P = page_size;
+  a.halves = page_size / 16;
+  a.num_blocks = num_blocks;
+  a.window = window;
+  a.sm_scale = sm_scale;
+  a.splits = block_splits(T, num_kv_heads, block_tiles(page_size, table_width, window, a.n_blocks));
+  a.ws_o = a.ws_ml = nullptr;
+  if (a.splits > 1) {
+    const int64_t rows_n = (int64_t)T * a.splits * num_q_heads, need = rows_n * (head_dim + 2) * (int64_t)sizeof(float);
+    if (!workspace || workspace_bytes < need)
+      return fail(SNA_ERR_WORKSPACE, "%s: workspace of %lld bytes, the splits need %lld", what,
+                  (long long)(workspace ? workspace_bytes : 0), (long long)need);
+    if (!aligned(workspace, 16))
+      return fail(SNA_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", what);
+    a.ws_o = (float*)workspace;
+    a.ws_ml = a.ws_o + rows_n * head_dim;
+  }
+  if ((int64_t)T * a.splits >= 1 << 24)  // (a grid has under 2^32 threads)
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %d queries exceed the grid", what, T);
+  a.out = (uint16_t*)out;
+  const hipStream_t s = (hipStream_t)stream;
+  if (head_dim == 128) {
+    if (blocks) launch_block_decode_format<128, true>(a, cache_dtype, s);
+    else launch_block_decode_format<128, false>(a, cache_dtype, s);
+  } else {
+    if (blocks) launch_block_decode_format<64, true>(a, cache_dtype, s);
+    else launch_block_decode_format<64, false>(a, cache_dtype, s);
+  }
+  return check_launch(what);
+}

@@ -120,8 +120,8 @@ __device__ __forceinline__ void split_q(float v, float& hi, float& lo) {
 }
 // Four floats in the e4m3fn range to e4m3fn bytes 0..3 (round to nearest even; an exactly representable value is
 // unchanged).
+typedef short s16x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack_e4m3fn_x4(float a, float b, float c, float d) {
-  typedef short s16x2_t __attribute__((ext_vector_type(2)));
   s16x2_t w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32((s16x2_t){0, 0}, a, b, 1.0f, false);
   w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, c, d, 1.0f, true);
   return (uint32_t)(uint16_t)w[0] | ((uint32_t)(uint16_t)w[1] << 16);
@@ -202,6 +202,21 @@ __device__ __forceinline__ void fp8x4_to_bf16x4(uint32_t w, uint32_t& lo, uint32
   lo = __builtin_bit_cast(uint32_t, a);
   hi = __builtin_bit_cast(uint32_t, b);
 }
+
+// Four int8 codes of a dword to four bf16 values in order. Exact: a bf16 value has 8 significant bits.
+__device__ __forceinline__ void int8x4_to_bf16x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  bf16x2_t a = {(__bf16)(float)(int8_t)w, (__bf16)(float)(int8_t)(w >> 8)};
+  bf16x2_t b = {(__bf16)(float)(int8_t)(w >> 16), (__bf16)(float)(int8_t)(w >> 24)};
+  lo = __builtin_bit_cast(uint32_t, a);
+  hi = __builtin_bit_cast(uint32_t, b);
+}
+
+// A cache whose blocks of tokens carry scales: the elements' formats, as kernel template arguments (the C ABI's dtypes).
+enum BlockFormat { kBlockBf16 = 0, kBlockFp8 = 1, kBlockInt8 = 3 };
+// The largest code of a format, and the least scale of a block: small enough to lose nothing that a bf16 model holds, large
+// enough that the scale, its reciprocal and a code times it are normal numbers.
+constexpr float kInt8Max = 127.0f;
+constexpr float kLeastBlockScale = 0x1p-100f;
 
 // ds_read_b64_tr_b8: in each 16-lane group the lanes' 8-byte chunks (8-byte aligned) form 8 rows of 16 bytes, row k
 // being the chunks of lanes 2 k and 2 k + 1; lane j receives column j, so byte k of its result is byte j of row k.

@@ -1258,6 +1258,221 @@ def evict_tokens(k_cache: Tensor, v_cache: Tensor, block_table: Tensor, seq_lens
 
 
 # ------------------------------------------------------------------------------------------------------------------
+# a cache whose blocks of tokens carry scales, and attention over it
+# ------------------------------------------------------------------------------------------------------------------
+
+_BLOCK_CODES = {torch.bfloat16: _lib.DTYPE_BF16, FP8: _lib.DTYPE_FP8_E4M3FN, torch.int8: _lib.DTYPE_INT8}
+
+
+def _block_cache(k_cache: Tensor, v_cache: Tensor, k_scale: Optional[Tensor], v_scale: Optional[Tensor]):
+    """(dtype code, shape, k_scale, v_scale, their page and head strides, tokens that share a scale) of a layer's caches
+    [blocks, G, page, d]: bf16, or FP8 or int8 codes with scales [blocks, G, page / tokens] fp32."""
+    shape = k_cache.shape
+    code = _BLOCK_CODES.get(k_cache.dtype)
+    if code is None:
+        _need(False, f"unsupported cache dtype {k_cache.dtype} (bfloat16, float8_e4m3fn or int8)")
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != k_cache.dtype:
+        _need(False, f"caches must be [blocks, kv_heads, page, d] of one type, got {tuple(shape)} {k_cache.dtype} and "
+              f"{tuple(v_cache.shape)} {v_cache.dtype}")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        _need(False, "caches must be contiguous")
+    if shape[0] < 1 or shape[1] < 1 or shape[2] < 1:
+        _need(False, f"caches of shape {tuple(shape)}")
+    if code == _lib.DTYPE_BF16:
+        return code, shape, None, None, 0, 0, shape[2]
+    if k_scale is None or v_scale is None:
+        _need(False, "a cache of 8-bit codes needs k_scale and v_scale")
+    nb, G, P, _ = shape
+    n = k_scale.shape[-1] if k_scale.dim() == 3 else 0
+    if (n < 1 or k_scale.shape != (nb, G, n) or v_scale.shape != k_scale.shape or P % n or (P // n) % 16 or
+            k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32):
+        _need(False, f"scales must be [{nb}, {G}, n] fp32, each for {P} / n tokens (a multiple of 16), got "
+              f"{tuple(k_scale.shape)} {k_scale.dtype} and {tuple(v_scale.shape)} {v_scale.dtype}")
+    page, head, one = k_scale.stride()
+    if k_scale.stride() != v_scale.stride() or (n > 1 and one != 1):
+        k_scale, v_scale = k_scale.contiguous(), v_scale.contiguous()
+        page, head = G * n, n
+    return code, shape, k_scale, v_scale, page, head, P // n
+
+
+def kv_store_blocks(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, prior_lens: Tensor, *,
+                    q_start: Optional[Tensor] = None, max_q_len: int = 1, k_scale: Optional[Tensor] = None,
+                    v_scale: Optional[Tensor] = None, k_bounds: Optional[Tensor] = None, host_q_start=None) -> None:
+    """Append tokens k, v [T, G, d] bf16 to their requests' rows of a layer's caches [blocks, G, page, d] whose blocks of
+    tokens carry a scale each: request r's tokens are rows q_start[r] .. q_start[r + 1] (without ``q_start``: row r, one a
+    request) and go to positions prior_lens[r], + 1, .. of its pages in ``block_table`` [R, width].
+
+    The caches hold float8_e4m3fn or int8 codes, with k_scale, v_scale [blocks, G, page / tokens] fp32 that the call keeps up:
+    a code is worth code * the scale of its block of ``tokens`` tokens and KV head. A block's scale is its largest magnitude
+    over 448 or 127 (at least 2^-100): it starts anew with the block's first token and grows when a larger token comes, and the
+    block's earlier tokens are then rounded again. (Infinities are clamped and do not count; a NaN makes the scale, so the
+    block, NaN.) bf16 caches have no scales. ``k_bounds`` [blocks, G, 2, d] bf16, when given, is kept up as well: the least and
+    the largest value of each dimension over a page's keys (block_scores reads it).
+
+    ``max_q_len`` bounds the chunk lengths (a host int); ``host_q_start``: a host copy of q_start, checked before the launch.
+    Tokens without a page are not stored. No page may be written for two requests of a call (a cached prefix is shared by whole
+    pages only)."""
+    dev = _on_gpu(k, v, k_cache, v_cache, block_table, prior_lens, q_start, k_scale, v_scale, k_bounds)
+    code, (nb, G, P, d), ks, vs, _, _, tokens = _block_cache(k_cache, v_cache, k_scale, v_scale)
+    if k.dim() != 3 or k.shape[1:] != (G, d) or v.shape != k.shape or k.dtype != torch.bfloat16 or v.dtype != k.dtype:
+        _need(False, f"k and v must be [T, {G}, {d}] bf16, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+    if code != _lib.DTYPE_BF16 and not (k_scale.is_contiguous() and v_scale.is_contiguous()):
+        _need(False, "scales that are written must be contiguous")
+    if k_bounds is not None and (k_bounds.shape != (nb, G, 2, d) or k_bounds.dtype != torch.bfloat16 or
+                                 not k_bounds.is_contiguous()):
+        _need(False, f"k_bounds must be contiguous [{nb}, {G}, 2, {d}] bf16, got {tuple(k_bounds.shape)} {k_bounds.dtype}")
+    if abs(k_cache.data_ptr() - v_cache.data_ptr()) < k_cache.numel() * k_cache.element_size():
+        _need(False, "K and V are one tensor, or overlap")
+    if ks is not None and abs(ks.data_ptr() - vs.data_ptr()) < 4 * ks.numel():
+        _need(False, "k_scale and v_scale are one tensor, or overlap")
+    T, R = k.shape[0], prior_lens.numel()
+    k, v = _head_rows(k), _head_rows(v)
+    if block_table.dim() != 2 or block_table.shape[0] < R or block_table.shape[1] < 1:
+        _need(False, f"block_table must be [{R}, width], got {tuple(block_table.shape)}")
+    table, stride = _strided_rows(_as(block_table, torch.int32))
+    prior = _contig(_as(prior_lens.reshape(-1), torch.int32), "prior_lens")
+    if q_start is None:
+        if T != R or max_q_len != 1:
+            _need(False, f"{T} tokens of {R} requests, max_q_len {max_q_len}, and no q_start")
+    else:
+        if q_start.numel() != R + 1:
+            _need(False, f"q_start must be [{R + 1}]")
+        if host_q_start is not None:
+            _check_q_start(host_q_start, R, T, max_q_len)
+        q_start = _contig(_as(q_start.reshape(-1), torch.int32), "q_start")
+    if T == 0 or R == 0:
+        return
+    _launch(dev, _lib.load().sna_kv_store_blocks, "kv_store_blocks", k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), T,
+            table.data_ptr(), stride, table.shape[1], _ptr(q_start), prior.data_ptr(), R, min(int(max_q_len), T),
+            k_cache.data_ptr(), v_cache.data_ptr(), _ptr(ks), _ptr(vs), tokens, _ptr(k_bounds), nb, G, P, d, code)
+
+
+def _head_rows(x: Tensor) -> Tensor:
+    """x [T, G, d] (a slice of a projection's rows, say) or its copy, each row's heads together and on 16 bytes."""
+    T, G, d = x.shape
+    row, head, one = x.stride()
+    if (one == 1 or d < 2) and (head == d or G < 2) and row % 8 == 0 and row >= G * d and x.data_ptr() % 16 == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+@functools.lru_cache(maxsize=1024)
+def _block_workspace(*sizes: int) -> int:
+    """sna_block_decode_workspace_bytes, a function of sizes alone."""
+    return _lib.load().sna_block_decode_workspace_bytes(*sizes)
+
+
+def _query_rows(q: Tensor, block_table: Tensor, seq_lens: Tensor, rows: Optional[Tensor]):
+    """(q, table, its row stride, seq_lens, rows) of a call of single queries, checked."""
+    if q.dim() != 3 or q.dtype != torch.bfloat16 or seq_lens.numel() != q.shape[0]:
+        _need(False, f"q must be [T, H, d] bf16 with one of seq_lens a query, got {tuple(q.shape)} {q.dtype} and "
+              f"{tuple(seq_lens.shape)}")
+    T = q.shape[0]
+    if rows is None:
+        if block_table.dim() != 2 or block_table.shape[0] < T or block_table.shape[1] < 1:
+            _need(False, f"block_table must be [{T}, width], got {tuple(block_table.shape)}")
+    else:
+        if rows.numel() != T or block_table.dim() != 2 or block_table.shape[1] < 1:
+            _need(False, f"rows must be [{T}] over a block_table [R, width], got {tuple(rows.shape)} and "
+                  f"{tuple(block_table.shape)}")
+        rows = _contig(_as(rows.reshape(-1), torch.int32), "rows")
+    table, stride = _strided_rows(_as(block_table, torch.int32))
+    q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
+    return q, table, stride, _contig(_as(seq_lens.reshape(-1), torch.int32), "seq_lens"), rows
+
+
+def _block_attention(what, q, k_cache, v_cache, block_table, seq_lens, blocks, sm_scale, k_scale, v_scale, sinks, window, rows,
+                     out) -> Tensor:
+    dev = _on_gpu(q, k_cache, v_cache, block_table, seq_lens, blocks, k_scale, v_scale, sinks, rows, out)
+    code, (nb, G, P, dk), ks, vs, page, head, tokens = _block_cache(k_cache, v_cache, k_scale, v_scale)
+    q, table, stride, lens, rows = _query_rows(q, block_table, seq_lens, rows)
+    T, H, d = q.shape
+    if d != dk or H % G:
+        _need(False, f"queries {tuple(q.shape)} over caches {tuple(k_cache.shape)}")
+    n = 0
+    if blocks is not None:
+        if blocks.dim() != 3 or blocks.shape[:2] != (T, G) or blocks.shape[2] < 1:
+            _need(False, f"blocks must be [{T}, {G}, n], got {tuple(blocks.shape)}")
+        blocks = _contig(_as(blocks, torch.int32), "blocks")
+        n = blocks.shape[2]
+    if sinks is not None:
+        sinks = _contig(_as(sinks.reshape(-1), torch.float32), "sinks")
+        if sinks.shape[0] != H:
+            _need(False, f"{sinks.shape[0]} sinks for {H} heads")
+    if out is None:
+        out = torch.empty(T, H, d, dtype=torch.bfloat16, device=dev)
+    elif out.shape != (T, H, d) or out.dtype != torch.bfloat16 or not out.is_contiguous():
+        _need(False, f"out must be contiguous [{T}, {H}, {d}] bf16, got {tuple(out.shape)} {out.dtype}")
+    if T == 0:
+        return out
+    W, window = table.shape[1], min(int(window), _INT32_MAX)
+    need = _block_workspace(T, H, G, d, P, W, window, n)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    _launch(dev, _lib.load().sna_paged_decode_blocks, what, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(ks),
+            _ptr(vs), page, head, tokens, table.data_ptr(), stride, W, table.shape[0], _ptr(rows), lens.data_ptr(),
+            _ptr(blocks), n, _ptr(sinks), window, sm_scale, out.data_ptr(), T, H, G, d, P, nb, code, _ptr(ws), need)
+    return out
+
+
+def paged_decode_blocks(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, seq_lens: Tensor, *,
+                        sm_scale: float, k_scale: Optional[Tensor] = None, v_scale: Optional[Tensor] = None,
+                        sinks: Optional[Tensor] = None, window: int = 0, rows: Optional[Tensor] = None,
+                        out: Optional[Tensor] = None) -> Tensor:
+    """Attention of single queries q [T, H, d] bf16 over caches whose blocks of tokens carry scales (kv_store_blocks; bf16
+    caches without scales too): query t sees the first seq_lens[t] keys of row t of ``block_table`` [R, width], its own
+    token's, stored already, the last of them. With ``rows`` [T] it is row rows[t] instead: several tokens of a row, each at
+    a length of its own (a verify step). ``window``: the last so many keys only; ``sinks`` [H] join the softmax
+    denominators. Scales may be expanded (one for all pages, say). A query that sees no key gives zeros. Returns [T, H, d]
+    bf16."""
+    return _block_attention("paged_decode_blocks", q, k_cache, v_cache, block_table, seq_lens, None, sm_scale, k_scale,
+                            v_scale, sinks, window, rows, out)
+
+
+def paged_decode_selected(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, seq_lens: Tensor, blocks: Tensor,
+                          *, sm_scale: float, k_scale: Optional[Tensor] = None, v_scale: Optional[Tensor] = None,
+                          sinks: Optional[Tensor] = None, rows: Optional[Tensor] = None,
+                          out: Optional[Tensor] = None) -> Tensor:
+    """paged_decode_blocks over some of the row's pages: query t's heads of KV head g see the keys below seq_lens[t] on the
+    pages in the table columns ``blocks[t, g]`` ([T, G, n] int32, as select_blocks returns them; -1 names none, a column named
+    twice counts twice). A prompt's queries, each with pages of its own, are given row by row (``rows``)."""
+    return _block_attention("paged_decode_selected", q, k_cache, v_cache, block_table, seq_lens, blocks, sm_scale, k_scale,
+                            v_scale, sinks, 0, rows, out)
+
+
+def block_scores(q: Tensor, k_bounds: Tensor, block_table: Tensor, seq_lens: Tensor, *, page_size: int,
+                 rows: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
+    """What a page can give a query at the most: (scores [T, G, width] fp32, counts [T] int32), scores[t, g, c] the largest,
+    over the query heads of KV head g, of sum_d max(q_d lo_d, q_d hi_d) with the bounds ``k_bounds`` [blocks, G, 2, d] bf16
+    (kv_store_blocks) of the page in column c of query t's table row; -inf past the row's ceil(seq_lens / page_size) = counts
+    pages and where the table names no page. The other arguments are paged_decode_blocks'."""
+    dev = _on_gpu(q, k_bounds, block_table, seq_lens, rows)
+    q, table, stride, lens, rows = _query_rows(q, block_table, seq_lens, rows)
+    T, H, d = q.shape
+    if k_bounds.dim() != 4 or k_bounds.shape[2:] != (2, d) or k_bounds.dtype != torch.bfloat16 or \
+            not k_bounds.is_contiguous() or k_bounds.shape[0] < 1 or k_bounds.shape[1] < 1 or H % k_bounds.shape[1]:
+        _need(False, f"k_bounds must be contiguous [blocks, kv_heads, 2, {d}] bf16 with kv_heads dividing {H}, got "
+              f"{tuple(k_bounds.shape)} {k_bounds.dtype}")
+    nb, G = k_bounds.shape[:2]
+    W = table.shape[1]
+    scores = torch.empty(T, G, W, dtype=torch.float32, device=dev)
+    counts = torch.empty(T, dtype=torch.int32, device=dev)
+    if T:
+        _launch(dev, _lib.load().sna_block_scores, "block_scores", q.data_ptr(), k_bounds.data_ptr(), table.data_ptr(), stride,
+                W, table.shape[0], _ptr(rows), lens.data_ptr(), scores.data_ptr(), counts.data_ptr(), T, H, G, d,
+                int(page_size), nb)
+    return scores, counts
+
+
+def select_blocks(q: Tensor, k_bounds: Tensor, block_table: Tensor, seq_lens: Tensor, *, keep: int, page_size: int,
+                  first: int = 1, recent: int = 1, rows: Optional[Tensor] = None) -> Tensor:
+    """The pages that each query and KV head attends to: [T, G, keep] int32 table columns in ascending order, -1 past a short
+    row's, for paged_decode_selected. A row of at most ``keep`` pages keeps them all, a longer one its ``first`` first and
+    ``recent`` last ones and those of the largest block_scores (select_tokens)."""
+    scores, counts = block_scores(q, k_bounds, block_table, seq_lens, page_size=page_size, rows=rows)
+    return select_tokens(scores, counts, keep=keep, first=first, recent=recent)[0]
+
+
+# ------------------------------------------------------------------------------------------------------------------
 # DSA indexer
 # ------------------------------------------------------------------------------------------------------------------
 
