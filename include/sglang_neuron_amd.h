@@ -520,6 +520,18 @@ int sna_paged_decode_blocks(const void *q, const void *k_cache, const void *v_ca
                             int64_t num_blocks, int32_t cache_dtype, void *workspace, int64_t workspace_bytes,
                             void *stream);
 
+/* sna_prefill_attention_split over such a pool: a batch of chunks, causal. Scales as in sna_paged_decode_blocks, the rest,
+ * the workspace (sna_prefill_workspace_bytes) included, as in sna_prefill_attention_split. A query that sees no key gives zeros.
+ * With int8 codes a query element is taken to within 2^-16 of its row's largest. */
+int sna_prefill_attention_blocks(const void *q, const void *k_cache, const void *v_cache, const float *k_scale,
+                                 const float *v_scale, int64_t scale_page_stride, int64_t scale_head_stride,
+                                 int32_t scale_tokens, const int32_t *block_table, int64_t table_stride,
+                                 int32_t table_width, const int32_t *q_start, const int32_t *prior_lens, int32_t R,
+                                 int32_t max_q_len, const float *sinks, float sm_scale, int32_t window, void *out,
+                                 int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                                 int64_t num_blocks, int32_t cache_dtype, void *workspace, int64_t workspace_bytes,
+                                 void *stream);
+
 /* The score of each page of a query's row, from the pages' key bounds: scores[t, g, c] = max over KV head g's query heads of
  * sum_d max(q_d lo_d, q_d hi_d), which no key of the page in column c exceeds; -inf past the row's pages and on invalid
  * ones. scores [T, num_kv_heads, table_width] fp32; counts [T] int32: the rows' pages, ceil(seq_lens / page_size), for a

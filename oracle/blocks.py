@@ -80,10 +80,11 @@ def rows_of(cache: Tensor, scale: Optional[Tensor], pages: Sequence[int], g: int
     return x.reshape(-1, d)
 
 
-def attend(q: Tensor, k: Tensor, v: Tensor, sm_scale: float, sinks: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+def attend(q: Tensor, k: Tensor, v: Tensor, sm_scale: float, sinks: Optional[Tensor],
+           q_off: float = 0.0) -> tuple[Tensor, Tensor]:
     """(out [grp, d], its error bound [grp, d]) of one query's heads q [grp, d] over keys k, v [n, d] (float64) with sinks
     [grp]. The bound is for a kernel that holds scores, statistics and sums in 32 bits and rounds probabilities and the
-    output to bf16, each by at most 2^-8 of itself."""
+    output to bf16, each by at most 2^-8 of itself, and takes a query element to within q_off of its row's largest."""
     grp, d = q.shape
     if k.shape[0] == 0:
         return torch.zeros(grp, d, dtype=torch.float64), torch.zeros(grp, d, dtype=torch.float64)
@@ -96,13 +97,15 @@ def attend(q: Tensor, k: Tensor, v: Tensor, sm_scale: float, sinks: Optional[Ten
     reach = (q.double().abs() @ k.abs().t()).amax(-1, keepdim=True) * sm_scale
     # a score is off by at most (d + 4) 2^-24 reach and the exponential by 2^-20 (its argument's rounding among it, under
     # reach 2^-22), so a weight, over its sum, by twice that; the sums by n 2^-24
-    rel = 2.0 ** -8 + 2 * ((d + 8) * 2.0 ** -24 * reach + 2.0 ** -20) + k.shape[0] * 2.0 ** -23
+    q_err = q_off * q.double().abs().amax(-1, keepdim=True) * k.abs().sum(-1).amax() * sm_scale
+    rel = 2.0 ** -8 + torch.expm1(2 * q_err) + 2 * ((d + 8) * 2.0 ** -24 * reach + 2.0 ** -20) + k.shape[0] * 2.0 ** -23
     return out, 2.0 ** -8 * out.abs() + rel * (p @ v.abs())
 
 
 def decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, lens: Sequence[int], *, sm_scale: float,
            k_scale: Optional[Tensor] = None, v_scale: Optional[Tensor] = None, sinks: Optional[Tensor] = None, window: int = 0,
-           rows: Optional[Sequence[int]] = None, blocks: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
+           rows: Optional[Sequence[int]] = None, blocks: Optional[Tensor] = None,
+           q_off: float = 0.0) -> tuple[Tensor, Tensor]:
     """([T, H, d] float64, its error bound) of single queries over their rows, or over the columns that blocks [T, G, n]
     names."""
     T, H, d = q.shape
@@ -124,7 +127,8 @@ def decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, lens: Seq
             pages = [int(table[r, c]) for c in cols]
             k, v = rows_of(k_cache, k_scale, pages, g)[seen], rows_of(v_cache, v_scale, pages, g)[seen]
             h = slice(g * grp, (g + 1) * grp)
-            out[t, h], off[t, h] = attend(q[t, h], k, v, sm_scale, None if sinks is None else sinks[h])
+            out[t, h], off[t, h] = attend(q[t, h], k, v, sm_scale, None if sinks is None else sinks[h],
+                                           q_off)
     return out, off
 
 

@@ -66,6 +66,7 @@ struct PrefillArgs {
   int64_t num_blocks;
   float sm_scale;
   int32_t window;
+  bool empty_zero;  // a row that sees no key gives zeros (else what 0 / 0 gives)
   // a launch that splits the keys (SPLIT): see prefill_item
   int32_t qblocks;   // query blocks of the longest chunk (max_q_len)
   int32_t slots;     // workgroups of the launch: the items it may run
@@ -74,6 +75,16 @@ struct PrefillArgs {
   float* ws_ml;      // [slots, 128, 2] reference max (log2 domain) and softmax sum
   int2* ws_item;     // [G, R, qblocks] a query block's first item and its split count
 };
+
+// A pool whose blocks of tokens carry scales (kBlockFp8, kBlockInt8): k_scale and v_scale are [num_blocks, G, P / bt].
+struct PrefillBlockArgs : PrefillArgs {
+  int64_t scale_page, scale_head;  // strides
+  int32_t sub_magic;               // ceil(2^16 / (bt / 16)): a 16-key group's block in its page (0: one block a page)
+};
+// SCALES: a BlockFormat of such a pool, or kBlockBf16 for none
+template <int SCALES>
+using PrefillArgsOf = std::conditional_t<SCALES != kBlockBf16, PrefillBlockArgs, PrefillArgs>;
+constexpr int kPrefillScaleTiles = 256;  // tiles whose blocks' scales are staged in LDS at a time
 
 constexpr int kPrefillTile = 64;   // keys per tile
 constexpr int kPrefillRows = 128;  // query rows of a workgroup
@@ -238,21 +249,25 @@ __device__ bool prefill_item(const PrefillArgs& a, int32_t& w, int32_t& g, int32
 // second sub-tile are left out (32 / 8 heads of 128, FP8 / bf16, us: 16 tokens 8.2 / 7.6 through the loop, 6.9 / 6.2 so;
 // 60 tokens 9.0 / 8.4 and 8.7 / 8.0; as runtime branches of one kernel 7.8 / 7.4 and 9.1 / 9.0).
 enum PrefillMode { kWhole, kSplit, kOneTile, kHalfTile };
-template <int D, int ESZ, PrefillMode MODE>
+template <int D, int ESZ, PrefillMode MODE, int SCALES = kBlockBf16>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
-void prefill_gqa_kernel(PrefillArgs a) {
+void prefill_gqa_kernel(PrefillArgsOf<SCALES> a) {
   using Geo = PrefillGeo<D, ESZ>;
   constexpr int ROWB = Geo::ROWB, CH = Geo::CH, HALF = Geo::HALF, SLOT = Geo::SLOT;
   constexpr bool ONE = MODE == kOneTile || MODE == kHalfTile;
   constexpr int TK = MODE == kHalfTile ? Geo::TK / 2 : Geo::TK, NSUB = TK / 32;
   constexpr int MW = Geo::MW, RPD = Geo::RPD;
   constexpr bool FP8 = ESZ == 1, SPLIT = MODE == kSplit;
+  constexpr bool BLK = SCALES != kBlockBf16, INT8 = SCALES == kBlockInt8;  // FP8 too: one-byte elements
+  constexpr int TG = TK / 16;  // 16-key groups of a tile
   constexpr int NS = FP8 ? D / 64 : D / 16;  // QK steps
   constexpr int NC = D / 32;                 // PV dim tiles
   typedef __attribute__((address_space(3))) void lds_void;
   typedef __attribute__((address_space(3))) uint8_t lds_u8;
   __shared__ __attribute__((aligned(1024))) uint8_t sm_ring[2 * SLOT];
   __shared__ int32_t sm_pages[Geo::PAGES];
+  // BLK: the staged tiles' scales of K and of V, group by group (and room for the tile behind the last)
+  __shared__ __attribute__((aligned(16))) float sm_scale[2][BLK ? (kPrefillScaleTiles + 1) * TG : 1];
 
   const int tid = threadIdx.x, lane = tid & 63, g2 = lane >> 5, i32 = lane & 31, li = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -300,6 +315,8 @@ void prefill_gqa_kernel(PrefillArgs a) {
       const uint4 w = ld16(qrow + 16 * s + 8 * g2);
       qf[s][0] = w.x, qf[s][1] = w.y, qf[s][2] = w.z, qf[s][3] = w.w;
     }
+  } else if constexpr (INT8) {
+    // (below)
   } else {
     float v[NS][32];
     float amax = 0.0f;
@@ -338,9 +355,55 @@ void prefill_gqa_kernel(PrefillArgs a) {
         qlo[s][k] = pack_e4m3fn_x4(l4[0], l4[1], l4[2], l4[3]);
       }
   }
-  const float k_deq = FP8 ? (a.mul_scale ? 1.0f / a.k_scale[g] : a.k_scale[g]) : 1.0f;
-  const float qk_scale = a.sm_scale * kLog2e * k_deq;
-  const float v_scale = FP8 ? (a.mul_scale ? 1.0f / a.v_scale[g] : a.v_scale[g]) : 1.0f;
+  // int8 codes take the query as whole numbers too, on v_mfma_i32_32x32x32_i8: the row times 32600 / its absolute maximum,
+  // to nearest (an element is off by at most 2^-16 of that maximum), as 256 hi + lo with hi and lo int8. The dot product
+  // with the codes is then exact: |256 sum hi k + sum lo k| < 2^30. An element that is no number makes the row NaN.
+  float q_unit = 1.0f;
+  if constexpr (INT8) {
+    uint32_t most = 0;  // the bits of the largest magnitude: as whole numbers NaN's are above infinity's
+    float v[NS][32];
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint4 w = ld16(qrow + 64 * s + 32 * g2 + 8 * c);
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[s][8 * c + 2 * e] = bf16_bits_to_f32(ww[e] & 0xffffu);
+          v[s][8 * c + 2 * e + 1] = bf16_bits_to_f32(ww[e] >> 16);
+        }
+      }
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int e = 0; e < 32; ++e) most = max(most, __float_as_uint(v[s][e]) & 0x7fffffffu);
+    const auto both = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+    most = max((uint32_t)both[0], (uint32_t)both[1]);
+    const bool number = most < 0x7f800000u;
+    // (an amplitude under 2^-100 is taken for that: nothing of it survives the softmax scale)
+    const float amp = fmaxf(__uint_as_float(most), 0x1p-100f);
+    const float per = number ? 32600.0f / amp : 0.0f;
+    q_unit = number ? amp / 32600.0f : __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        uint32_t h = 0, l = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int32_t n = number ? (int32_t)__builtin_rintf(v[s][4 * k + e] * per) : 0;
+          const int32_t top = (n + 128) >> 8;
+          h |= ((uint32_t)top & 0xffu) << (8 * e);
+          l |= ((uint32_t)(n - 256 * top) & 0xffu) << (8 * e);
+        }
+        qhi[s][k] = h;
+        qlo[s][k] = l;
+      }
+  }
+  const float k_deq = FP8 && !BLK ? (a.mul_scale ? 1.0f / a.k_scale[g] : a.k_scale[g]) : 1.0f;
+  const float qk_scale = a.sm_scale * kLog2e * (INT8 ? q_unit : k_deq);
+  const float v_scale = FP8 && !BLK ? (a.mul_scale ? 1.0f / a.v_scale[g] : a.v_scale[g]) : 1.0f;
 
   float m_ref = 0.0f, l_run = 0.0f;
   f32x16_t acc[NC];
@@ -410,6 +473,35 @@ void prefill_gqa_kernel(PrefillArgs a) {
           const uint32_t kop[4] = {w.x, w.y, w.z, w.w};
           st[u] = mfma_32x32x16_bf16(kop, qf[s], st[u]);
         }
+    } else if constexpr (INT8) {
+      i32x16_t n[NSUB];
+#pragma unroll
+      for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) n[u][e] = 0;
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        if (part == 1) {
+#pragma unroll
+          for (int u = 0; u < NSUB; ++u) n[u] <<= 8;
+        }
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int u = 0; u < NSUB; ++u) {
+              const uint4 w = *reinterpret_cast<const uint4*>(S0 + 32 * u * ROWB + (k_at ^ (64 * s + 16 * c)));
+              const uint32_t kop[4] = {w.x, w.y, w.z, w.w};
+              const uint32_t(&qp)[8] = part == 0 ? qhi[s] : qlo[s];
+              const uint32_t qop[4] = {qp[4 * c], qp[4 * c + 1], qp[4 * c + 2], qp[4 * c + 3]};
+              n[u] = mfma_32x32x32_i8(kop, qop, n[u]);
+            }
+      }
+#pragma unroll
+      for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) st[u][e] = (float)n[u][e];
     } else {
       // the K bytes of the lane's key and dims straight from LDS (e4m3fn, no conversion)
 #pragma unroll
@@ -432,13 +524,18 @@ void prefill_gqa_kernel(PrefillArgs a) {
   // The exponents of a tile's raw scores relative to the row's reference maximum (log2 domain), in place, and the lane's
   // largest.
   float mx = -INFINITY;
-  auto exponents = [&](f32x16_t (&y)[NSUB]) {
+  float v_grp[TG];  // BLK: the V scales of the tile's groups, for this lane's row
+  // (i: the tile's place among the staged ones)
+  auto exponents = [&](f32x16_t (&y)[NSUB], int32_t i) {
+    float k_grp[TG];
+#pragma unroll
+    for (int u = 0; u < TG; ++u) k_grp[u] = BLK ? qk_scale * sm_scale[0][i * TG + u] : qk_scale;
     mx = -INFINITY;
 #pragma unroll
     for (int u = 0; u < NSUB; ++u)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        y[u][e] = fmaf(y[u][e], qk_scale, -m_ref);
+        y[u][e] = fmaf(y[u][e], k_grp[2 * u + e / 8], -m_ref);
         mx = fmaxf(mx, y[u][e]);
       }
   };
@@ -455,6 +552,12 @@ void prefill_gqa_kernel(PrefillArgs a) {
         y[u][e] = (page_ok & (key <= last) & (key >= first)) ? y[u][e] : -INFINITY;
         mx = fmaxf(mx, y[u][e]);
       }
+    if constexpr (BLK) {
+      // a group of keys that the row does not see has no scale for it (a later token's may be NaN)
+#pragma unroll
+      for (int u = 0; u < TG; ++u)
+        if (k0 + 16 * u > qpos || (a.window > 0 && k0 + 16 * u + 15 < qpos - a.window + 1)) v_grp[u] = 0.0f;
+    }
   };
   // The reference moves to the row's maximum when that passes it by the slack; a row that has seen no key yet (its
   // reference 0 stands for none) takes its first maximum, whatever it is.
@@ -482,6 +585,13 @@ void prefill_gqa_kernel(PrefillArgs a) {
     for (int u = 0; u < NSUB; ++u)
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
+        if constexpr (BLK) {
+          // (the sum is of the probabilities alone)
+          const float p0 = __builtin_amdgcn_exp2f(y[u][2 * k]), p1 = __builtin_amdgcn_exp2f(y[u][2 * k + 1]);
+          l_run += p0 + p1;
+          pop[u][k / 4][k % 4] = pack_bf16x2(p0 * v_grp[2 * u + k / 4], p1 * v_grp[2 * u + k / 4]);
+          continue;
+        }
         const uint32_t w = pack_bf16x2(__builtin_amdgcn_exp2f(y[u][2 * k]), __builtin_amdgcn_exp2f(y[u][2 * k + 1]));
         pop[u][k / 4][k % 4] = w;
         l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w),
@@ -499,8 +609,13 @@ void prefill_gqa_kernel(PrefillArgs a) {
           uint32_t vop[4];
           if constexpr (FP8) {
             const uint2 w = lds_read_tr8(V0 + (v_at[0] ^ (32 * c)));
-            fp8x4_to_bf16x4(w.x, vop[0], vop[1]);
-            fp8x4_to_bf16x4(w.y, vop[2], vop[3]);
+            if constexpr (INT8) {
+              int8x4_to_bf16x4(w.x, vop[0], vop[1]);
+              int8x4_to_bf16x4(w.y, vop[2], vop[3]);
+            } else {
+              fp8x4_to_bf16x4(w.x, vop[0], vop[1]);
+              fp8x4_to_bf16x4(w.y, vop[2], vop[3]);
+            }
           } else {
             const uint2 w0 = lds_read_tr16(V0 + (v_at[0] ^ (64 * c)));
             const uint2 w1 = lds_read_tr16(V0 + (v_at[FP8 ? 0 : 1] ^ (64 * c)));
@@ -517,7 +632,8 @@ void prefill_gqa_kernel(PrefillArgs a) {
   const int32_t t_first = blk.t0 + (SPLIT ? split * split_tiles : 0);
   // (ONE: a length past the table has only invalid keys in its other tiles)
   const int32_t t_end = SPLIT ? min(blk.t1, t_first + split_tiles) : ONE ? min(blk.t1, t_first + 1) : blk.t1;
-  const int32_t chunk_tiles = (Geo::PAGES - 1) * a.P / TK;  // (a chunk may start mid-page: PAGES - 1 whole pages)
+  // (a chunk may start mid-page: PAGES - 1 whole pages)
+  const int32_t chunk_tiles = BLK ? min((Geo::PAGES - 1) * a.P / TK, kPrefillScaleTiles) : (Geo::PAGES - 1) * a.P / TK;
   for (int32_t c0 = t_first; c0 < t_end; c0 += chunk_tiles) {
     const int32_t c1 = min(c0 + chunk_tiles, t_end);
     // stage the table entries of pages [p0, p1) (ring and pages are free: the previous chunk drained)
@@ -532,6 +648,17 @@ void prefill_gqa_kernel(PrefillArgs a) {
     }
     __syncthreads();
     const int32_t n = c1 - c0;
+    if constexpr (BLK) {
+      // the scales of the chunk's 16-key groups (read behind the barrier below); none past the block's keys, where a
+      // block of tokens may never have been written
+      for (int32_t i = tid; i < 2 * n * TG; i += 256) {
+        const int32_t kv = i >= n * TG ? 1 : 0, u = i - kv * n * TG, key = TK * c0 + 16 * u, col = column(key);
+        const int32_t page = sm_pages[col - p0], sub = (int32_t)((uint32_t)((key - col * a.P) / 16) * (uint32_t)a.sub_magic >> 16);
+        float sc = 0.0f;
+        if (page >= 0 && key < hi) sc = (kv ? a.v_scale : a.k_scale)[page * a.scale_page + g * a.scale_head + sub];
+        sm_scale[kv][u] = sc;
+      }
+    }
     // The loop over tiles holds tile i's scores and computes tile i + 1's beside tile i's probabilities (the matrix
     // products of one, the vector work of the other, in one stretch of code), so K runs a tile ahead of V in the ring:
     // K of tile i + 2 loads into tile i's slot, V of tile i + 1 into its own, while tile i computes.
@@ -551,11 +678,15 @@ void prefill_gqa_kernel(PrefillArgs a) {
     __syncthreads();
     f32x16_t sa[NSUB], sb[NSUB];
     qk(&sm_ring[0], sa);
-    exponents(sa);
+    exponents(sa, 0);
     // tile i (in ring slot P) up to its exponents under the reference maximum: V cleaned, scores masked
     auto settle = [&](int32_t i, int P, f32x16_t (&cur)[NSUB]) {
       const int32_t k0 = TK * (c0 + i);
       const bool valid = ok_cur == (1u << (TK / 16)) - 1;
+      if constexpr (BLK) {
+#pragma unroll
+        for (int u = 0; u < TG; ++u) v_grp[u] = sm_scale[1][i * TG + u];
+      }
       if (!valid || k0 + TK > hi) {
         // keys no row of the block may see (past the chunk, or on an invalid page): their V rows are zeroed, so that
         // stale pool bytes (a NaN among them) cannot reach the output through p = 0
@@ -591,7 +722,7 @@ void prefill_gqa_kernel(PrefillArgs a) {
         qk(&sm_ring[(1 - P) * SLOT], next);  // (past the last tile: whatever the slot holds, not used)
         probabilities(cur);
         pv(&sm_ring[P * SLOT]);
-        exponents(next);
+        exponents(next, i + 1);
         // (a use here, so the compiler does not move the next tile's products past the loop's exit test)
         asm volatile("" : "+v"(mx), "+v"(next[0]), "+v"(next[1]));
         ok_cur = ok_next;
@@ -637,7 +768,7 @@ void prefill_gqa_kernel(PrefillArgs a) {
   }
   // ---- epilogue: normalize (sinks join the denominator), scale by v_scale, write the valid rows ----
   if (a.sinks) L += __builtin_amdgcn_exp2f(a.sinks[head_of(row)] * kLog2e - m_ref);
-  const float inv = v_scale / L;
+  const float inv = a.empty_zero && L == 0.0f ? 0.0f : v_scale / L;
   if (!row_ok) return;
   uint16_t* dst = a.out + q_offset(row) + 4 * g2;
 #pragma unroll
@@ -690,7 +821,7 @@ __global__ __launch_bounds__(256) void prefill_combine_kernel(PrefillArgs a, boo
       o += e * x[k];
     }
   }
-  const float inv = v_scale / den;
+  const float inv = a.empty_zero && den == 0.0f ? 0.0f : v_scale / den;
   uint16_t* dst = a.out + ((int64_t)(qa + blk.q0 + t) * a.H + head) * D + col;
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
 }
@@ -734,24 +865,30 @@ int64_t split_workspace_bytes(int32_t slots, int32_t R, int32_t max_q_len, int32
          qblocks * R * num_kv_heads * (int64_t)sizeof(int2);
 }
 
-template <int D, int ESZ>
-void launch_prefill(const PrefillArgs& a, hipStream_t s) {
+template <int D, int ESZ, int SCALES = kBlockBf16>
+void launch_prefill(const PrefillArgsOf<SCALES>& a, hipStream_t s) {
   if (a.slots > 0) {
-    hipLaunchKernelGGL((prefill_gqa_kernel<D, ESZ, kSplit>), dim3(a.slots), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((prefill_gqa_kernel<D, ESZ, kSplit, SCALES>), dim3(a.slots), dim3(256), 0, s, a);
     hipLaunchKernelGGL((prefill_combine_kernel<D>), dim3(kPrefillRows * D / 1024 * a.qblocks, a.R, a.G),
-                       dim3(256), 0, s, a, ESZ == 1);
+                       dim3(256), 0, s, a, ESZ == 1 && SCALES == kBlockBf16);
   } else if ((int64_t)a.table_width * a.P <= kPrefillTile / 2) {
-    hipLaunchKernelGGL((prefill_gqa_kernel<D, ESZ, kHalfTile>), dim3(a.qblocks, a.R, a.G), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((prefill_gqa_kernel<D, ESZ, kHalfTile, SCALES>), dim3(a.qblocks, a.R, a.G), dim3(256), 0, s, a);
   } else if ((int64_t)a.table_width * a.P <= kPrefillTile) {
-    hipLaunchKernelGGL((prefill_gqa_kernel<D, ESZ, kOneTile>), dim3(a.qblocks, a.R, a.G), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((prefill_gqa_kernel<D, ESZ, kOneTile, SCALES>), dim3(a.qblocks, a.R, a.G), dim3(256), 0, s, a);
   } else {
-    hipLaunchKernelGGL((prefill_gqa_kernel<D, ESZ, kWhole>), dim3(a.qblocks, a.R, a.G), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((prefill_gqa_kernel<D, ESZ, kWhole, SCALES>), dim3(a.qblocks, a.R, a.G), dim3(256), 0, s, a);
   }
 }
 
 }  // namespace
 
-static int prefill_attention(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+// The scales of a pool whose blocks of tokens carry them.
+struct PrefillScales {
+  int64_t page_stride, head_stride;
+  int32_t tokens;
+};
+
+static int prefill_attention(const char* what, const PrefillScales* scales, bool empty_zero, const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
                                      const float* v_scale, const int32_t* block_table, int64_t table_stride,
                                      int32_t table_width, const int32_t* q_start, const int32_t* prior_lens,
                                      int32_t R, int32_t max_q_len, const float* sinks, float sm_scale, int32_t window,
@@ -761,28 +898,34 @@ static int prefill_attention(const void* q, const void* k_cache, const void* v_c
   if (R < 0 || max_q_len < 0 || num_q_heads < 1 || num_kv_heads < 1 || num_q_heads % num_kv_heads != 0 ||
       window < 0 || num_blocks < 1 || table_width < 1 || table_stride < table_width)
     return fail(SNA_ERR_INVALID_ARGUMENT,
-                "prefill_attention: bad sizes (R %d, max_q_len %d, heads %d / %d, window %d, blocks %lld, table %d "
-                "wide, stride %lld)",
+                "%s: bad sizes (R %d, max_q_len %d, heads %d / %d, window %d, blocks %lld, table %d "
+                "wide, stride %lld)", what,
                 R, max_q_len, num_q_heads, num_kv_heads, window, (long long)num_blocks, table_width,
                 (long long)table_stride);
   const int32_t group = num_q_heads / num_kv_heads;
-  if (group > 128) return fail(SNA_ERR_UNSUPPORTED, "prefill_attention: %d query heads per KV head (at most 128)", group);
+  if (group > 128) return fail(SNA_ERR_UNSUPPORTED, "%s: %d query heads per KV head (at most 128)", what, group);
   if (head_dim != 64 && head_dim != 128)
-    return fail(SNA_ERR_UNSUPPORTED, "prefill_attention: head_dim %d (64 or 128)", head_dim);
+    return fail(SNA_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", what, head_dim);
   if (page_size < 16 || page_size % 16 != 0)
-    return fail(SNA_ERR_UNSUPPORTED, "prefill_attention: page_size %d (a multiple of 16)", page_size);
-  if (kv_dtype != SNA_DTYPE_FP8_E4M3FN && kv_dtype != SNA_DTYPE_FP8_E4M3FN_MUL && kv_dtype != SNA_DTYPE_BF16)
-    return fail(SNA_ERR_UNSUPPORTED, "prefill_attention: KV dtype %d (FP8 e4m3fn or bf16)", kv_dtype);
+    return fail(SNA_ERR_UNSUPPORTED, "%s: page_size %d (a multiple of 16)", what, page_size);
+  if (scales && (page_size > SNA_MAX_BLOCK_PAGE || scales->tokens < 16 || scales->tokens % 16 ||
+                 page_size % scales->tokens || scales->page_stride < 0 || scales->head_stride < 0))
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: a scale for every %d tokens (a multiple of 16 that divides the page of %d, at "
+                "most %d), strides %lld and %lld", what, scales->tokens, page_size, SNA_MAX_BLOCK_PAGE,
+                (long long)scales->page_stride, (long long)scales->head_stride);
+  if (scales ? kv_dtype != SNA_DTYPE_FP8_E4M3FN && kv_dtype != SNA_DTYPE_INT8
+             : kv_dtype != SNA_DTYPE_FP8_E4M3FN && kv_dtype != SNA_DTYPE_FP8_E4M3FN_MUL && kv_dtype != SNA_DTYPE_BF16)
+    return fail(SNA_ERR_UNSUPPORTED, "%s: KV dtype %d (FP8 e4m3fn or bf16)", what, kv_dtype);
   if (R == 0 || max_q_len == 0) return SNA_OK;
   if (!q || !k_cache || !v_cache || (kv_dtype != SNA_DTYPE_BF16 && (!k_scale || !v_scale)) || !block_table ||
       !q_start || !prior_lens || !out)
-    return fail(SNA_ERR_INVALID_ARGUMENT, "prefill_attention: null pointer");
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16))
-    return fail(SNA_ERR_INVALID_ARGUMENT, "prefill_attention: q, out and the caches must be 16-byte aligned");
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: q, out and the caches must be 16-byte aligned", what);
   if (R > 65535 || num_kv_heads > 65535)
-    return fail(SNA_ERR_INVALID_ARGUMENT, "prefill_attention: %d requests x %d KV heads exceed the grid", R,
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %d requests x %d KV heads exceed the grid", what, R,
                 num_kv_heads);
-  PrefillArgs a;
+  PrefillBlockArgs a;
   a.q = (const uint16_t*)q;
   a.k_cache = (const uint8_t*)k_cache;
   a.v_cache = (const uint8_t*)v_cache;
@@ -806,10 +949,11 @@ static int prefill_attention(const void* q, const void* k_cache, const void* v_c
   a.num_blocks = num_blocks;
   a.sm_scale = sm_scale;
   a.window = window;
+  a.empty_zero = empty_zero;
   const int64_t qblocks = ((int64_t)max_q_len + a.bq - 1) / a.bq;
   if (qblocks * R * num_kv_heads > (int64_t)UINT32_MAX)  // the kernel's XCD-aware order numbers them in 32 bits
-    return fail(SNA_ERR_INVALID_ARGUMENT, "prefill_attention: %lld query blocks x %d requests x %d KV heads exceed "
-                "the grid (split the batch)", (long long)qblocks, R, num_kv_heads);
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %lld query blocks x %d requests x %d KV heads exceed "
+                "the grid (split the batch)", what, (long long)qblocks, R, num_kv_heads);
   a.qblocks = (int32_t)qblocks;
   a.min_tiles = kPrefillMinSplit;
   a.slots = 0;
@@ -820,22 +964,32 @@ static int prefill_attention(const void* q, const void* k_cache, const void* v_c
   if (slots > 0) {
     const int64_t need = split_workspace_bytes(slots, R, max_q_len, num_q_heads, num_kv_heads, head_dim);
     if (workspace_bytes < need)
-      return fail(SNA_ERR_WORKSPACE, "prefill_attention: workspace of %lld bytes, the split needs %lld",
+      return fail(SNA_ERR_WORKSPACE, "%s: workspace of %lld bytes, the split needs %lld", what,
                   (long long)workspace_bytes, (long long)need);
     if (!aligned(workspace, 16))
-      return fail(SNA_ERR_INVALID_ARGUMENT, "prefill_attention: the workspace must be 16-byte aligned");
+      return fail(SNA_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", what);
     a.slots = slots;
     a.ws_o = (float*)workspace;
     a.ws_ml = a.ws_o + (int64_t)slots * kPrefillRows * head_dim;
     a.ws_item = (int2*)(a.ws_ml + (int64_t)slots * kPrefillRows * 2);
   }
   const hipStream_t s = (hipStream_t)stream;
-  if (kv_dtype != SNA_DTYPE_BF16) {
+  if (scales) {
+    a.scale_page = scales->page_stride;
+    a.scale_head = scales->head_stride;
+    const int32_t per = scales->tokens / 16;
+    a.sub_magic = scales->tokens < page_size ? (65536 + per - 1) / per : 0;
+    if (kv_dtype == SNA_DTYPE_INT8) {
+      if (head_dim == 128) launch_prefill<128, 1, kBlockInt8>(a, s); else launch_prefill<64, 1, kBlockInt8>(a, s);
+    } else {
+      if (head_dim == 128) launch_prefill<128, 1, kBlockFp8>(a, s); else launch_prefill<64, 1, kBlockFp8>(a, s);
+    }
+  } else if (kv_dtype != SNA_DTYPE_BF16) {
     if (head_dim == 128) launch_prefill<128, 1>(a, s); else launch_prefill<64, 1>(a, s);
   } else {
     if (head_dim == 128) launch_prefill<128, 2>(a, s); else launch_prefill<64, 2>(a, s);
   }
-  return check_launch("prefill_attention");
+  return check_launch(what);
 }
 
 extern "C" int sna_prefill_attention(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
@@ -845,7 +999,7 @@ extern "C" int sna_prefill_attention(const void* q, const void* k_cache, const v
                                      void* out, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                                      int32_t page_size, int64_t num_blocks, int32_t kv_dtype, void* stream) {
   ApiGuard guard;
-  return prefill_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, table_stride, table_width, q_start,
+  return prefill_attention("prefill_attention", nullptr, false, q, k_cache, v_cache, k_scale, v_scale, block_table, table_stride, table_width, q_start,
                            prior_lens, R, max_q_len, sinks, sm_scale, window, out, num_q_heads, num_kv_heads, head_dim,
                            page_size, num_blocks, kv_dtype, nullptr, 0, stream);
 }
@@ -869,7 +1023,23 @@ extern "C" int sna_prefill_attention_split(const void* q, const void* k_cache, c
                                            int64_t num_blocks, int32_t kv_dtype, void* workspace,
                                            int64_t workspace_bytes, void* stream) {
   ApiGuard guard;
-  return prefill_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, table_stride, table_width, q_start,
+  return prefill_attention("prefill_attention", nullptr, false, q, k_cache, v_cache, k_scale, v_scale, block_table, table_stride, table_width, q_start,
                            prior_lens, R, max_q_len, sinks, sm_scale, window, out, num_q_heads, num_kv_heads, head_dim,
                            page_size, num_blocks, kv_dtype, workspace, workspace_bytes, stream);
+}
+
+extern "C" int sna_prefill_attention_blocks(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                                            const float* v_scale, int64_t scale_page_stride, int64_t scale_head_stride,
+                                            int32_t scale_tokens, const int32_t* block_table, int64_t table_stride,
+                                            int32_t table_width, const int32_t* q_start, const int32_t* prior_lens,
+                                            int32_t R, int32_t max_q_len, const float* sinks, float sm_scale,
+                                            int32_t window, void* out, int32_t num_q_heads, int32_t num_kv_heads,
+                                            int32_t head_dim, int32_t page_size, int64_t num_blocks, int32_t cache_dtype,
+                                            void* workspace, int64_t workspace_bytes, void* stream) {
+  ApiGuard guard;
+  const PrefillScales scales = {scale_page_stride, scale_head_stride, scale_tokens};
+  return prefill_attention("prefill_attention_blocks", cache_dtype == SNA_DTYPE_BF16 ? nullptr : &scales, true, q, k_cache,
+                           v_cache, k_scale, v_scale, block_table, table_stride, table_width, q_start, prior_lens, R, max_q_len,
+                           sinks, sm_scale, window, out, num_q_heads, num_kv_heads, head_dim, page_size, num_blocks,
+                           cache_dtype, workspace, workspace_bytes, stream);
 }

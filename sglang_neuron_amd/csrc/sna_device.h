@@ -333,6 +333,14 @@ __device__ __forceinline__ f32x16_t mfma_32x32x16_bf16(const uint32_t (&a)[4], c
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), __builtin_bit_cast(bf16x8_t, bv),
                                                   c, 0, 0, 0);
 }
+// int8 A and B, K = 32: 16 bytes of K a lane at the same positions in A and B.
+typedef int32_t i32x16_t __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ i32x16_t mfma_32x32x32_i8(const uint32_t (&a)[4], const uint32_t (&b)[4], i32x16_t c) {
+  typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
+  i32x4_t av = {(int32_t)a[0], (int32_t)a[1], (int32_t)a[2], (int32_t)a[3]};
+  i32x4_t bv = {(int32_t)b[0], (int32_t)b[1], (int32_t)b[2], (int32_t)b[3]};
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(av, bv, c, 0, 0, 0);
+}
 __device__ __forceinline__ f32x16_t mfma_32x32x64_fp8(const uint32_t (&a)[8], const uint32_t (&b)[8], f32x16_t c,
                                                       int32_t scale_b) {
   i32x8_t av, bv;

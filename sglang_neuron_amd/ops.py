@@ -1439,6 +1439,57 @@ def paged_decode_selected(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tab
                             v_scale, sinks, 0, rows, out)
 
 
+@functools.lru_cache(maxsize=1024)
+def _prefill_workspace(*sizes: int) -> int:
+    """sna_prefill_workspace_bytes, a function of sizes alone."""
+    return _lib.load().sna_prefill_workspace_bytes(*sizes)
+
+
+def prefill_attention_blocks(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, q_start: Tensor,
+                             prior_lens: Tensor, *, max_q_len: int, sm_scale: float, k_scale: Optional[Tensor] = None,
+                             v_scale: Optional[Tensor] = None, sinks: Optional[Tensor] = None, window: int = 0,
+                             out: Optional[Tensor] = None, host_q_start=None) -> Tensor:
+    """prefill_attention over caches whose blocks of tokens carry scales (kv_store_blocks, the chunk's tokens stored first;
+    bf16 caches without scales too): q [T, H, d] bf16, request r's rows q_start[r] .. q_start[r + 1] at positions
+    prior_lens[r] + i, causal, optionally windowed and with sinks [H]. ``max_q_len`` bounds the chunk lengths;
+    ``host_q_start``: a host copy of q_start, checked before the launch. A query that sees no key gives zeros. Over int8
+    codes a query element is taken to within 2^-16 of its row's largest. Returns [T, H, d] bf16."""
+    dev = _on_gpu(q, k_cache, v_cache, block_table, q_start, prior_lens, k_scale, v_scale, sinks, out)
+    code, (nb, G, P, dk), ks, vs, page, head, tokens = _block_cache(k_cache, v_cache, k_scale, v_scale)
+    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.shape[2] != dk or q.shape[1] % G:
+        _need(False, f"q must be [T, H, {dk}] bf16 with {G} KV heads dividing H, got {tuple(q.shape)} {q.dtype}")
+    T, H, d = q.shape
+    R = prior_lens.numel()
+    if q_start.numel() != R + 1:
+        _need(False, f"q_start must be [{R + 1}]")
+    if host_q_start is not None:
+        _check_q_start(host_q_start, R, T, max_q_len)
+    if block_table.dim() != 2 or block_table.shape[0] < R or block_table.shape[1] < 1:
+        _need(False, f"block_table must be [{R}, width], got {tuple(block_table.shape)}")
+    table, stride = _strided_rows(_as(block_table, torch.int32))
+    q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
+    q_start = _contig(_as(q_start.reshape(-1), torch.int32), "q_start")
+    prior = _contig(_as(prior_lens.reshape(-1), torch.int32), "prior_lens")
+    if sinks is not None:
+        sinks = _contig(_as(sinks.reshape(-1), torch.float32), "sinks")
+        if sinks.shape[0] != H:
+            _need(False, f"{sinks.shape[0]} sinks for {H} heads")
+    if out is None:
+        out = torch.empty(T, H, d, dtype=torch.bfloat16, device=dev)
+    elif out.shape != (T, H, d) or out.dtype != torch.bfloat16 or not out.is_contiguous():
+        _need(False, f"out must be contiguous [{T}, {H}, {d}] bf16, got {tuple(out.shape)} {out.dtype}")
+    if T == 0 or R == 0:
+        return out
+    W, max_q_len, window = table.shape[1], min(int(max_q_len), T), min(int(window), _INT32_MAX)
+    need = _prefill_workspace(R, max_q_len, H, G, d, P, W, window)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    _launch(dev, _lib.load().sna_prefill_attention_blocks, "prefill_attention_blocks", q.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), _ptr(ks), _ptr(vs), page, head, tokens, table.data_ptr(), stride, W, q_start.data_ptr(),
+            prior.data_ptr(), R, max_q_len, _ptr(sinks), sm_scale, window, out.data_ptr(), H, G, d, P, nb, code, _ptr(ws),
+            need)
+    return out
+
+
 def block_scores(q: Tensor, k_bounds: Tensor, block_table: Tensor, seq_lens: Tensor, *, page_size: int,
                  rows: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
     """What a page can give a query at the most: (scores [T, G, width] fp32, counts [T] int32), scores[t, g, c] the largest,
