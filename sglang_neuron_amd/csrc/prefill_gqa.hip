@@ -266,8 +266,8 @@ void prefill_gqa_kernel(PrefillArgsOf<SCALES> a) {
   typedef __attribute__((address_space(3))) uint8_t lds_u8;
   __shared__ __attribute__((aligned(1024))) uint8_t sm_ring[2 * SLOT];
   __shared__ int32_t sm_pages[Geo::PAGES];
-  // BLK: the staged tiles' scales of K and of V, group by group (and room for the tile behind the last)
-  __shared__ __attribute__((aligned(16))) float sm_scale[2][BLK ? (kPrefillScaleTiles + 1) * TG : 1];
+  // BLK: for the staged tiles' groups K's scale, log2 of V's and 1 / V's (and room for the tile behind the last)
+  __shared__ __attribute__((aligned(16))) float sm_scale[3][BLK ? (kPrefillScaleTiles + 1) * TG : 1];
 
   const int tid = threadIdx.x, lane = tid & 63, g2 = lane >> 5, i32 = lane & 31, li = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -522,27 +522,44 @@ void prefill_gqa_kernel(PrefillArgsOf<SCALES> a) {
     }
   };
   // The exponents of a tile's raw scores relative to the row's reference maximum (log2 domain), in place, and the lane's
-  // largest.
+  // largest. BLK: log2 of the group's V scale is in them, so that the probabilities come out times it, without a product
+  // each (24 / 4 heads of 64, int8, 3 chunks of up to 635 tokens: 41.3 -> 39.7 us; 32 / 8 heads of 128, FP8, 4 x 2048 after
+  // 2048: 416 -> 413); the largest is without it.
   float mx = -INFINITY;
-  float v_grp[TG];  // BLK: the V scales of the tile's groups, for this lane's row
+  float v_inv[TG];  // BLK: 1 / the V scales of the tile's groups, 0 for a group that this lane's row does not see
   // (i: the tile's place among the staged ones)
   auto exponents = [&](f32x16_t (&y)[NSUB], int32_t i) {
-    float k_grp[TG];
-#pragma unroll
-    for (int u = 0; u < TG; ++u) k_grp[u] = BLK ? qk_scale * sm_scale[0][i * TG + u] : qk_scale;
     mx = -INFINITY;
+    if constexpr (BLK) {
 #pragma unroll
-    for (int u = 0; u < NSUB; ++u)
+      for (int u = 0; u < TG; ++u) {
+        const float k_grp = qk_scale * sm_scale[0][i * TG + u], lv = sm_scale[1][i * TG + u], off = lv - m_ref;
+        float m = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        y[u][e] = fmaf(y[u][e], k_grp[2 * u + e / 8], -m_ref);
-        mx = fmaxf(mx, y[u][e]);
+        for (int e = 0; e < 8; ++e) {
+          const float z = fmaf(y[u / 2][8 * (u & 1) + e], k_grp, off);
+          y[u / 2][8 * (u & 1) + e] = z;
+          m = fmaxf(m, z);
+        }
+        mx = fmaxf(mx, m - lv);
       }
+    } else {
+#pragma unroll
+      for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          y[u][e] = fmaf(y[u][e], qk_scale, -m_ref);
+          mx = fmaxf(mx, y[u][e]);
+        }
+    }
   };
-  auto mask = [&](int32_t k0, uint32_t pg_ok, f32x16_t (&y)[NSUB]) {
+  auto mask = [&](int32_t k0, uint32_t pg_ok, f32x16_t (&y)[NSUB], int32_t i) {
     // (no position is below 0, so neither is a window's first key: `first` does not leave 32 bits for any window)
     const int32_t last = qpos - 8 * g2, first = a.window > 0 ? max(qpos - a.window + 1, 0) - 8 * g2 : INT32_MIN;
     mx = -INFINITY;
+    float m[TG];
+#pragma unroll
+    for (int u = 0; u < TG; ++u) m[u] = -INFINITY;
 #pragma unroll
     for (int u = 0; u < NSUB; ++u)
 #pragma unroll
@@ -550,13 +567,16 @@ void prefill_gqa_kernel(PrefillArgsOf<SCALES> a) {
         const bool page_ok = (pg_ok >> (2 * u + e / 8)) & 1u;  // uniform
         const int32_t key = k0 + 32 * u + 16 * (e / 8) + e % 8;  // less 8 g2
         y[u][e] = (page_ok & (key <= last) & (key >= first)) ? y[u][e] : -INFINITY;
-        mx = fmaxf(mx, y[u][e]);
+        if constexpr (BLK) m[2 * u + e / 8] = fmaxf(m[2 * u + e / 8], y[u][e]);
+        else mx = fmaxf(mx, y[u][e]);
       }
     if constexpr (BLK) {
-      // a group of keys that the row does not see has no scale for it (a later token's may be NaN)
 #pragma unroll
-      for (int u = 0; u < TG; ++u)
-        if (k0 + 16 * u > qpos || (a.window > 0 && k0 + 16 * u + 15 < qpos - a.window + 1)) v_grp[u] = 0.0f;
+      for (int u = 0; u < TG; ++u) {
+        mx = fmaxf(mx, m[u] - sm_scale[1][i * TG + u]);
+        // a group of keys that the row does not see has no scale for it (a later token's may be NaN)
+        if (k0 + 16 * u > qpos || (a.window > 0 && k0 + 16 * u + 15 < qpos - a.window + 1)) v_inv[u] = 0.0f;
+      }
     }
   };
   // The reference moves to the row's maximum when that passes it by the slack; a row that has seen no key yet (its
@@ -584,18 +604,18 @@ void prefill_gqa_kernel(PrefillArgsOf<SCALES> a) {
 #pragma unroll
     for (int u = 0; u < NSUB; ++u)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if constexpr (BLK) {
-          // (the sum is of the probabilities alone)
-          const float p0 = __builtin_amdgcn_exp2f(y[u][2 * k]), p1 = __builtin_amdgcn_exp2f(y[u][2 * k + 1]);
-          l_run += p0 + p1;
-          pop[u][k / 4][k % 4] = pack_bf16x2(p0 * v_grp[2 * u + k / 4], p1 * v_grp[2 * u + k / 4]);
-          continue;
+      for (int h = 0; h < 2; ++h) {
+        float part = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int e = 8 * h + 2 * k;
+          const uint32_t w = pack_bf16x2(__builtin_amdgcn_exp2f(y[u][e]), __builtin_amdgcn_exp2f(y[u][e + 1]));
+          pop[u][h][k] = w;
+          float& sum = BLK ? part : l_run;
+          sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), __builtin_bit_cast(bf16x2_t, 0x3f803f80u),
+                                                sum, false);
         }
-        const uint32_t w = pack_bf16x2(__builtin_amdgcn_exp2f(y[u][2 * k]), __builtin_amdgcn_exp2f(y[u][2 * k + 1]));
-        pop[u][k / 4][k % 4] = w;
-        l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w),
-                                                __builtin_bit_cast(bf16x2_t, 0x3f803f80u), l_run, false);
+        if constexpr (BLK) l_run = fmaf(part, v_inv[2 * u + h], l_run);
       }
   };
   auto pv = [&](const uint8_t* S0) {
@@ -649,14 +669,22 @@ void prefill_gqa_kernel(PrefillArgsOf<SCALES> a) {
     __syncthreads();
     const int32_t n = c1 - c0;
     if constexpr (BLK) {
-      // the scales of the chunk's 16-key groups (read behind the barrier below); none past the block's keys, where a
-      // block of tokens may never have been written
+      // the scales of the chunk's 16-key groups (read behind the barrier below); 1 past the block's keys, where a block of
+      // tokens may never have been written
       for (int32_t i = tid; i < 2 * n * TG; i += 256) {
         const int32_t kv = i >= n * TG ? 1 : 0, u = i - kv * n * TG, key = TK * c0 + 16 * u, col = column(key);
         const int32_t page = sm_pages[col - p0], sub = (int32_t)((uint32_t)((key - col * a.P) / 16) * (uint32_t)a.sub_magic >> 16);
-        float sc = 0.0f;
+        float sc = 1.0f;
         if (page >= 0 && key < hi) sc = (kv ? a.v_scale : a.k_scale)[page * a.scale_page + g * a.scale_head + sub];
-        sm_scale[kv][u] = sc;
+        if (kv) {
+          // at least the least scale of a block: a key whose weight is 2^-26 of the row's largest, times it, is the least
+          // that the exponentials hold
+          const float v = sc < kLeastBlockScale ? kLeastBlockScale : sc;
+          sm_scale[1][u] = log2f(v);
+          sm_scale[2][u] = 1.0f / v;
+        } else {
+          sm_scale[0][u] = sc;
+        }
       }
     }
     // The loop over tiles holds tile i's scores and computes tile i + 1's beside tile i's probabilities (the matrix
@@ -685,7 +713,7 @@ void prefill_gqa_kernel(PrefillArgsOf<SCALES> a) {
       const bool valid = ok_cur == (1u << (TK / 16)) - 1;
       if constexpr (BLK) {
 #pragma unroll
-        for (int u = 0; u < TG; ++u) v_grp[u] = sm_scale[1][i * TG + u];
+        for (int u = 0; u < TG; ++u) v_inv[u] = sm_scale[2][i * TG + u];
       }
       if (!valid || k0 + TK > hi) {
         // keys no row of the block may see (past the chunk, or on an invalid page): their V rows are zeroed, so that
@@ -698,7 +726,7 @@ void prefill_gqa_kernel(PrefillArgsOf<SCALES> a) {
         __syncthreads();
       }
       // a tile that is not full (a key invalid or not visible to every row of the block) masks its scores
-      if (!valid || k0 + TK - 1 > pos0 || (a.window != 0 && k0 <= hi - 1 - a.window)) mask(k0, ok_cur, cur);
+      if (!valid || k0 + TK - 1 > pos0 || (a.window != 0 && k0 <= hi - 1 - a.window)) mask(k0, ok_cur, cur, i);
       if (any_unset || __any(mx > kPrefillRescaleSlack)) move_reference(cur);
     };
     if constexpr (ONE) {

@@ -47,7 +47,7 @@ def _check(args, priors, fmt, rows=None, **kw):
     got = _run(*args, priors, **kw).cpu().double()
     assert bool(torch.isfinite(got).all())
     okw = dict(sm_scale=kw["sm_scale"], k_scale=ks, v_scale=vs, sinks=kw.get("sinks"), window=kw.get("window", 0),
-               q_off=2.0 ** -16 if fmt == "int8" else 0.0)
+               q_off=2.0 ** -16 if fmt == "int8" else 0.0, rounded_sum=True)
     at = [(r, i) for r in range(len(priors)) for i in range(start[r + 1] - start[r])]
     pick = range(len(at)) if rows is None else rows
     want, off = ob.decode(q[list(pick)], kc, vc, table, [priors[at[t][0]] + at[t][1] + 1 for t in pick],
@@ -114,7 +114,7 @@ def test_restaged_scales(fmt):
         _lib.check(rc, "prefill_attention_blocks")
         some = [0, 150, 299]
         want, off = ob.decode(q[some], kc, vc, table, [n - 300 + t + 1 for t in some], rows=[0] * 3, sm_scale=0.125, k_scale=ks,
-                              v_scale=vs, window=window, q_off=2.0 ** -16 if fmt == "int8" else 0.0)
+                              v_scale=vs, window=window, q_off=2.0 ** -16 if fmt == "int8" else 0.0, rounded_sum=True)
         assert float(((out[some].cpu().double() - want).abs() - off).max()) <= 0
 
 
