@@ -6,8 +6,8 @@
 // block's K scale and v_j = code * its block's V scale. A block's scales are the same for 16 keys at a time, so K's joins
 // the score's factor and V's the probability: codes go into the matrix products as they are, exact in bf16.
 //
-// Work: one workgroup per (query, split, KV head); the splits of a query divide its 32-key tiles evenly, and a second launch
-// merges them where there are several. A wave takes tiles round-robin, the next one's loads in flight while it computes one.
+// Work: one workgroup per (query, KV head), or, where those do not fill the card, per (split of a query, KV head): a
+// query's splits divide its tiles evenly, and a second launch merges them. A wave takes tiles round-robin, the next one's loads in flight while it computes one.
 // A tile is two half-tiles of 16 keys, each inside one page and one block. Lane roles (lane = 16 g4 + li):
 //   QK   S^T[key, head] = K[key, :] . Q[head, :], v_mfma_f32_16x16x32_bf16 with M = 16 keys, N = 16 heads (the group's,
 //        zero-padded): lane (g4, li) feeds key li's 16-byte chunks 4 c + g4 and head li's elements of the same dims, and
@@ -44,11 +44,25 @@ struct BlockDecodeArgs {
   int64_t num_blocks;
   int32_t window;
   float sm_scale;
-  int32_t splits;
-  float* ws_o;   // [T, splits, H, D] unnormalized partials
-  float* ws_ml;  // [T, splits, H, 2] reference max (log2 domain) and softmax sum
+  bool head_fast;  // the launch's order: KV head fastest
+  int32_t splits;  // of a query's tiles
+  float* ws_o;     // [T, splits, H, D] unnormalized partials
+  float* ws_ml;    // [T, splits, H, 2] reference max (log2 domain) and softmax sum
   uint16_t* out;
 };
+
+// The 32-key tiles of a query of L keys: [first, first + n). Dense: tile i is positions 32 i ..; SEL: the listed pages'
+// halves two by two, whatever they name.
+template <bool SEL>
+__device__ __forceinline__ void block_tiles_of(const BlockDecodeArgs& a, int32_t L, int32_t& first, int32_t& n) {
+  const int32_t lo = a.window > 0 ? max(0, L - a.window) : 0;
+  first = SEL ? 0 : lo / 32;
+  n = L <= 0 ? 0 : SEL ? (a.n_blocks * a.halves + 1) / 2 : (int32_t)(((int64_t)L + 31) / 32) - first;
+}
+// (keys past the table have no page)
+__device__ __forceinline__ int32_t block_len(const BlockDecodeArgs& a, int32_t len) {
+  return (int32_t)min((int64_t)max(len, 0), (int64_t)a.table_width * a.P);
+}
 
 constexpr float kBlockRescaleSlack = 8.0f;
 
@@ -88,7 +102,7 @@ struct BlockTile {
   bool valid[2];   // on a page of the pool, below the table's width
 };
 
-template <int D, int FMT, bool SEL, bool FINAL, int WAVES>
+template <int D, int FMT, bool SEL, bool SPLIT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2)))
 void block_decode_kernel(BlockDecodeArgs a) {
   using Tile = BlockTile<D, FMT>;
@@ -99,9 +113,12 @@ void block_decode_kernel(BlockDecodeArgs a) {
   constexpr int CE = 16 / ESZ;   // elements of a 16-byte chunk
   const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, li = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int32_t g = blockIdx.y;
-  const int32_t t = (int32_t)(blockIdx.x / (uint32_t)a.splits), split = (int32_t)blockIdx.x - t * a.splits;
-  const int32_t row_v = a.rows ? a.rows[t] : t, len_v = a.seq_lens[t];
+  const uint32_t items = (uint32_t)(SPLIT ? a.T * a.splits : a.T);  // of a KV head
+  const uint32_t v = a.head_fast ? blockIdx.x / (uint32_t)a.G : blockIdx.x % items;
+  const int32_t g = (int32_t)(a.head_fast ? blockIdx.x - v * a.G : blockIdx.x / items);
+  const int32_t t = (int32_t)(SPLIT ? v / (uint32_t)a.splits : v), split = SPLIT ? (int32_t)v - t * a.splits : 0;
+  const int32_t len_v = a.seq_lens[t];
+  const int32_t row_v = a.rows ? a.rows[t] : t;
 
   // query operand: step s, lane (g4, li): head li's 8 elements from dim CE (4 c + g4) + w, 8 s = CE c + w
   uint32_t qv[STEPS][4];
@@ -114,23 +131,20 @@ void block_decode_kernel(BlockDecodeArgs a) {
       qv[s][0] = live ? w.x : 0u, qv[s][1] = live ? w.y : 0u, qv[s][2] = live ? w.z : 0u, qv[s][3] = live ? w.w : 0u;
     }
   }
-  const float sink_pre = FINAL && a.sinks && tid < a.group ? a.sinks[g * a.group + tid] : 0.0f;
+  const float sink_pre = a.sinks && tid < a.group ? a.sinks[g * a.group + tid] : 0.0f;
 
   const int32_t row = __builtin_amdgcn_readfirstlane(row_v);
   const bool row_ok = row >= 0 && row < a.table_rows;
-  // (keys past the table have no page)
-  const int64_t table_keys = (int64_t)a.table_width * a.P;
-  const int32_t L = row_ok ? (int32_t)min((int64_t)max(__builtin_amdgcn_readfirstlane(len_v), 0), table_keys) : 0;
+  const int32_t L = row_ok ? block_len(a, __builtin_amdgcn_readfirstlane(len_v)) : 0;
   const int32_t lo = a.window > 0 ? max(0, L - a.window) : 0;  // visible: [lo, L)
   const int32_t* trow = a.table + (int64_t)(row_ok ? row : 0) * a.table_stride;
   const int32_t* list = SEL ? a.blocks + ((int64_t)t * a.G + g) * a.n_blocks : nullptr;
-  // The tiles of this split. Dense: tile i is positions 32 i ..; SEL: the listed pages' halves, two by two.
   int32_t t_first, t_last;
-  {
-    const int32_t all0 = SEL ? 0 : lo / 32;
-    const int32_t all1 = SEL ? (L > 0 ? (a.n_blocks * a.halves + 1) / 2 : 0) : (int32_t)(((int64_t)L + 31) / 32);
-    const int32_t n = max(all1 - all0, 0), per = n / a.splits, extra = n - per * a.splits;
-    t_first = all0 + split * per + min(split, extra);
+  block_tiles_of<SEL>(a, L, t_first, t_last);
+  t_last += t_first;
+  if constexpr (SPLIT) {
+    const int32_t n = t_last - t_first, per = n / a.splits, extra = n - per * a.splits;
+    t_first += split * per + min(split, extra);
     t_last = t_first + per + (split < extra ? 1 : 0);
   }
 
@@ -172,7 +186,7 @@ void block_decode_kernel(BlockDecodeArgs a) {
       const int32_t p = pick(pg, c);
       const int32_t b = SEL ? pick(bk, c) : e;
       T.pos[hf] = b * a.P + 16 * in16;
-      T.valid[hf] = inside && p >= 0 && T.pos[hf] < L;
+      T.valid[hf] = inside && p >= 0 && T.pos[hf] < L && T.pos[hf] + 16 > lo;
       page[hf] = T.valid[hf] ? p : 0;
       sub[hf] = T.valid[hf] ? (int32_t)((uint32_t)in16 * (uint32_t)a.sub_magic >> 16) : 0;
       const int64_t blk = ((int64_t)page[hf] * a.G + g) * head_bytes + (int64_t)(16 * in16) * D * ESZ;
@@ -311,7 +325,7 @@ void block_decode_kernel(BlockDecodeArgs a) {
   // ---- merge the waves in LDS; write the output, or this split's partial ----
   __shared__ float sm_o[WAVES][16][D + 1];
   __shared__ float sm_m[WAVES][16], sm_l[WAVES][16], sm_sink[16];
-  if (FINAL && tid < a.group) sm_sink[tid] = sink_pre;
+  if (tid < a.group) sm_sink[tid] = sink_pre;
   const float l_tot = sum_across_groups(l_run);
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -320,7 +334,7 @@ void block_decode_kernel(BlockDecodeArgs a) {
   if (g4 == 0) sm_m[wave][li] = m_ref, sm_l[wave][li] = l_tot;
   __syncthreads();
   for (int32_t idx = tid; idx < a.group * D; idx += 64 * WAVES) {
-    const int32_t j = idx / D, d = idx % D, h = g * a.group + j;
+    const int32_t j = idx / D, d = idx % D;
     float M = kNegBig;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) M = fmaxf(M, sm_m[w][j]);
@@ -331,95 +345,116 @@ void block_decode_kernel(BlockDecodeArgs a) {
       o += e * sm_o[w][j][d];
       l += e * sm_l[w][j];
     }
-    if constexpr (FINAL) {
-      if (a.sinks) l += __builtin_amdgcn_exp2f(sm_sink[j] * kLog2e - M);
-      a.out[((int64_t)t * a.H + h) * D + d] = (uint16_t)f32_to_bf16_bits(l == 0.0f ? 0.0f : o / l);
-    } else {
-      const int64_t at = ((int64_t)t * a.splits + split) * a.H + h;
+    if constexpr (SPLIT) {
+      const int64_t at = (int64_t)v * a.H + g * a.group + j;
       a.ws_o[at * D + d] = o;
       if (d == 0) *reinterpret_cast<float2*>(a.ws_ml + 2 * at) = make_float2(M, l);
+    } else {
+      if (a.sinks) l += __builtin_amdgcn_exp2f(sm_sink[j] * kLog2e - M);
+      a.out[((int64_t)t * a.H + g * a.group + j) * D + d] = (uint16_t)f32_to_bf16_bits(l == 0.0f ? 0.0f : o / l);
     }
   }
 }
 
-// Merge of a query's splits, one wave per (query, head): out = sum_s e_s o_s / (sum_s e_s l_s + e_sink), e_s = exp2(m_s -
-// M). Lane s of round i holds split 64 i + s's weight; lane i the dims D / 64 * i ... The partials stream 16 at a time.
-constexpr int kBlockMaxSplits = 256;
+// Merge of a query's splits, one workgroup per (query, head): out = sum_s e_s o_s / (sum_s e_s l_s + e_sink), e_s =
+// exp2(m_s - M). D / 4 lanes take a split's row in 16-byte pieces, 1024 / D splits at a time, each such group of lanes with a
+// running (M, l, o) of its own; the groups are merged in LDS.
 template <int D>
-__global__ __launch_bounds__(64) void block_combine_kernel(BlockDecodeArgs a) {
-  constexpr int V = D / 64, CH = 16, N = kBlockMaxSplits / 64;
-  const int32_t t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, S = a.splits;
-  const int64_t at0 = (int64_t)t * S * a.H + h;
-  const float* ob = a.ws_o + at0 * D + V * lane;
-  const int64_t step = (int64_t)a.H * D;
-  float2 ml[N];
-  float M = kNegBig;
+__global__ __launch_bounds__(256) void block_combine_kernel(BlockDecodeArgs a) {
+  constexpr int LR = D / 4, NG = 256 / LR, CH = 4;
+  const int32_t t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, gi = tid / LR, d = 4 * (tid % LR);
+  const int32_t ns = a.splits;
+  const int64_t at0 = (int64_t)t * ns * a.H + h;
+  const float* wo = a.ws_o + at0 * D + d;
+  const float* ml = a.ws_ml + 2 * at0;
+  float M = kNegBig, l = 0.0f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (int32_t s0 = gi; s0 < ns; s0 += NG * CH) {
+    f32x4_t x[CH];
+    float2 w[CH];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int32_t s = 64 * i + lane;
-    ml[i] = s < S ? *reinterpret_cast<const float2*>(a.ws_ml + 2 * (at0 + (int64_t)s * a.H)) : make_float2(kNegBig, 0.0f);
-    M = fmaxf(M, ml[i].x);
-  }
-  M = wave_max(M);
-  float den = 0.0f, e[N];
+    for (int k = 0; k < CH; ++k) {
+      const int64_t s = (int64_t)min(s0 + NG * k, ns - 1) * a.H;
+      x[k] = *reinterpret_cast<const f32x4_t*>(wo + s * D);
+      w[k] = *reinterpret_cast<const float2*>(ml + 2 * s);
+    }
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    e[i] = __builtin_amdgcn_exp2f(ml[i].x - M);
-    den += e[i] * ml[i].y;
-  }
-  den = wave_sum(den);
-  if (a.sinks) den += __builtin_amdgcn_exp2f(a.sinks[h] * kLog2e - M);
-  float o[V] = {};
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if (64 * i >= S) break;
-    for (int32_t s0 = 64 * i; s0 < min(S, 64 * i + 64); s0 += CH) {
-      float x[CH][V];
-#pragma unroll
-      for (int k = 0; k < CH; ++k)
-#pragma unroll
-        for (int v = 0; v < V; ++v) x[k][v] = ob[min(s0 + k, S - 1) * step + v];
-#pragma unroll
-      for (int k = 0; k < CH; ++k) {
-        const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(e[i]), (s0 + k) & 63));
-#pragma unroll
-        for (int v = 0; v < V; ++v) o[v] += s0 + k < S ? w * x[k][v] : 0.0f;
+    for (int k = 0; k < CH; ++k) {
+      if (s0 + NG * k < ns) {
+        const float m = fmaxf(M, w[k].x), e0 = __builtin_amdgcn_exp2f(M - m), e1 = __builtin_amdgcn_exp2f(w[k].x - m);
+        l = l * e0 + w[k].y * e1;
+        o = o * e0 + x[k] * e1;
+        M = m;
       }
     }
   }
-  uint16_t* dst = a.out + ((int64_t)t * a.H + h) * D + V * lane;
+  __shared__ __attribute__((aligned(16))) float sm_o[NG][D];
+  __shared__ float sm_m[NG], sm_l[NG];
+  *reinterpret_cast<f32x4_t*>(&sm_o[gi][d]) = o;
+  if (tid % LR == 0) sm_m[gi] = M, sm_l[gi] = l;
+  __syncthreads();
+  if (tid >= D / 2) return;
+  float T = kNegBig, den = 0.0f, a0 = 0.0f, a1 = 0.0f;
 #pragma unroll
-  for (int v = 0; v < V; ++v) dst[v] = (uint16_t)f32_to_bf16_bits(den == 0.0f ? 0.0f : o[v] / den);
+  for (int k = 0; k < NG; ++k) T = fmaxf(T, sm_m[k]);
+#pragma unroll
+  for (int k = 0; k < NG; ++k) {
+    const float e = __builtin_amdgcn_exp2f(sm_m[k] - T);
+    den += e * sm_l[k];
+    a0 += e * sm_o[k][2 * tid], a1 += e * sm_o[k][2 * tid + 1];
+  }
+  if (a.sinks) den += __builtin_amdgcn_exp2f(a.sinks[h] * kLog2e - T);
+  const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+  reinterpret_cast<uint32_t*>(a.out + ((int64_t)t * a.H + h) * D)[tid] =
+      f32_to_bf16_bits(a0 * inv) | f32_to_bf16_bits(a1 * inv) << 16;
 }
 
 template <int D, int FMT, bool SEL>
-static void launch_block_decode(const BlockDecodeArgs& a, hipStream_t s) {
-  const dim3 grid((uint32_t)(a.T * a.splits), a.G);
-  if (a.splits == 1) {
-    hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, true, 4>), grid, dim3(256), 0, s, a);
+static void launch_block_decode(const BlockDecodeArgs& a, int32_t waves, hipStream_t s) {
+  const dim3 grid((uint32_t)(a.T * a.splits * a.G));
+  if (a.splits > 1) {
+    if (waves == 4) hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, true, 4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, true, 8>), grid, dim3(512), 0, s, a);
+    hipLaunchKernelGGL((block_combine_kernel<D>), dim3(a.T, a.H), dim3(256), 0, s, a);
   } else {
-    hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, false, 4>), grid, dim3(256), 0, s, a);
-    hipLaunchKernelGGL((block_combine_kernel<D>), dim3(a.T, a.H), dim3(64), 0, s, a);
+    if (waves == 4) hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, false, 4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, false, 8>), grid, dim3(512), 0, s, a);
   }
 }
 
 template <int D, bool SEL>
-static void launch_block_decode_format(const BlockDecodeArgs& a, int32_t dtype, hipStream_t s) {
-  if (dtype == SNA_DTYPE_BF16) launch_block_decode<D, kBlockBf16, SEL>(a, s);
-  else if (dtype == SNA_DTYPE_INT8) launch_block_decode<D, kBlockInt8, SEL>(a, s);
-  else launch_block_decode<D, kBlockFp8, SEL>(a, s);
+static void launch_block_decode_format(const BlockDecodeArgs& a, int32_t dtype, int32_t waves, hipStream_t s) {
+  if (dtype == SNA_DTYPE_BF16) launch_block_decode<D, kBlockBf16, SEL>(a, waves, s);
+  else if (dtype == SNA_DTYPE_INT8) launch_block_decode<D, kBlockInt8, SEL>(a, waves, s);
+  else launch_block_decode<D, kBlockFp8, SEL>(a, waves, s);
 }
 
-// The splits of a query: enough workgroups for two a CU, none under 4 tiles.
-static int32_t block_splits(int32_t T, int32_t G, int64_t tiles) {
-  const int64_t base = (int64_t)T * G;
-  const int64_t want = (512 + base - 1) / base, most = std::max<int64_t>(1, tiles / 4);
-  return (int32_t)std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)kBlockMaxSplits}));
-}
-// The 32-key tiles that a query's keys can span.
-static int64_t block_tiles(int32_t page_size, int32_t table_width, int32_t window, int32_t n_blocks) {
+// How a launch shares its keys out: waves a workgroup, and the splits of a query, each an even share of its own tiles (the
+// table's width says little about them: it is what a graph is captured for).
+//   Queries of equal work (lists of one length; a single query): 8 waves and one round of workgroups, so the fewest partials
+//   (32 queries of 2048 selected FP8 keys, 32 / 8 heads of 128: whole rows on 8 waves 27.0 us, two splits on 4 waves 32.3, on
+//   8 32.3; one row of 131071 int8 keys: 32 splits on 8 waves 48.6, 64 on 4 50.0, 32 on 4 60.0).
+//   Rows of unequal lengths: 4 waves, some 1024 workgroups, so that the short ones even the long ones out (24 rows of 1000 to
+//   4096 keys: 2, 4 and 8 splits on 4 waves 40.5, 33.3, 34.6 us, on 8 waves 43.2, 40.4, 47.7; 40 of 200 to 8000: whole 128, 3
+//   splits 85, 6 78; 16 of 4096: 2, 4, 8, 16 splits 31.6, 28.5, 28.9, 33.5). Where whole rows fill the card they stay whole (64
+//   rows of 4096: 89.5, two splits 93.7), above that up to three rounds of them are halved (70 of 100 to 6000: 131 and 103; 100
+//   of 500 to 2000: 61.8 and 60.8).
+// The card holds 512 workgroups of 4 waves at head dim 128 (FP8 768), 1024 at 64. A split has 4 tiles at the least.
+struct BlockShape {
+  int32_t waves, splits;
+};
+static BlockShape block_shape(int32_t T, int32_t G, int32_t head_dim, int32_t page_size, int32_t table_width, int32_t window,
+                              int32_t n_blocks) {
   const int64_t keys = (int64_t)(n_blocks > 0 ? n_blocks : table_width) * page_size;
-  return ((window > 0 ? std::min<int64_t>(keys, (int64_t)window + 31) : keys) + 31) / 32;
+  const int64_t tiles = ((window > 0 ? std::min<int64_t>(keys, (int64_t)window + 31) : keys) + 31) / 32;
+  const int64_t base = (int64_t)T * G, slots = head_dim == 64 ? 1024 : 512;
+  const bool even = n_blocks > 0 || T == 1, full = base >= slots * 7 / 8;
+  int64_t n = 1;
+  if (even) n = slots / 2 / base;
+  else if (!full) n = 1024 / base;
+  else if (base > slots && base < 3 * slots) n = 2;
+  n = std::max<int64_t>(1, std::min<int64_t>({n, tiles / 4, (int64_t)256}));
+  return {even && !full ? 8 : 4, (int32_t)n};
 }
 
 }  // namespace sna
@@ -432,8 +467,8 @@ extern "C" int64_t sna_block_decode_workspace_bytes(int32_t T, int32_t num_q_hea
   if (T < 1 || num_q_heads < 1 || num_kv_heads < 1 || head_dim < 1 || page_size < 1 || table_width < 1 || window < 0 ||
       n_blocks < 0)
     return 0;
-  const int32_t s = block_splits(T, num_kv_heads, block_tiles(page_size, table_width, window, n_blocks));
-  return s > 1 ? (int64_t)T * s * num_q_heads * (head_dim + 2) * (int64_t)sizeof(float) : 0;
+  const BlockShape b = block_shape(T, num_kv_heads, head_dim, page_size, table_width, window, n_blocks);
+  return b.splits > 1 ? (int64_t)T * b.splits * num_q_heads * (head_dim + 2) * (int64_t)sizeof(float) : 0;
 }
 
 extern "C" int sna_paged_decode_blocks(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
@@ -510,7 +545,12 @@ extern "C" int sna_paged_decode_blocks(const void* q, const void* k_cache, const
   a.num_blocks = num_blocks;
   a.window = window;
   a.sm_scale = sm_scale;
-  a.splits = block_splits(T, num_kv_heads, block_tiles(page_size, table_width, window, a.n_blocks));
+  const BlockShape shape = block_shape(T, num_kv_heads, head_dim, page_size, table_width, window, a.n_blocks);
+  a.splits = shape.splits;
+  // queries of one row read the same pages: with the KV head fastest a head's are found in one L2 (2 x 256 queries of 1024
+  // selected keys, bf16: 290 -> 247 us). Rows of their own gain nothing by it and lose where a head's rows of a page are
+  // a few KB, which one head alone reads through a part of its L2's channels (64 rows of 4096 FP8 keys: 90 -> 101 us).
+  a.head_fast = rows != nullptr;
   a.ws_o = a.ws_ml = nullptr;
   if (a.splits > 1) {
     const int64_t rows_n = (int64_t)T * a.splits * num_q_heads, need = rows_n * (head_dim + 2) * (int64_t)sizeof(float);
@@ -522,16 +562,16 @@ extern "C" int sna_paged_decode_blocks(const void* q, const void* k_cache, const
     a.ws_o = (float*)workspace;
     a.ws_ml = a.ws_o + rows_n * head_dim;
   }
-  if ((int64_t)T * a.splits >= 1 << 24)  // (a grid has under 2^32 threads)
+  if ((int64_t)T * a.splits * num_kv_heads >= 1 << 23)  // (a grid has under 2^32 threads)
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %d queries exceed the grid", what, T);
   a.out = (uint16_t*)out;
   const hipStream_t s = (hipStream_t)stream;
   if (head_dim == 128) {
-    if (blocks) launch_block_decode_format<128, true>(a, cache_dtype, s);
-    else launch_block_decode_format<128, false>(a, cache_dtype, s);
+    if (blocks) launch_block_decode_format<128, true>(a, cache_dtype, shape.waves, s);
+    else launch_block_decode_format<128, false>(a, cache_dtype, shape.waves, s);
   } else {
-    if (blocks) launch_block_decode_format<64, true>(a, cache_dtype, s);
-    else launch_block_decode_format<64, false>(a, cache_dtype, s);
+    if (blocks) launch_block_decode_format<64, true>(a, cache_dtype, shape.waves, s);
+    else launch_block_decode_format<64, false>(a, cache_dtype, shape.waves, s);
   }
   return check_launch(what);
 }
