@@ -44,7 +44,6 @@ struct BlockDecodeArgs {
   int64_t num_blocks;
   int32_t window;
   float sm_scale;
-  bool head_fast;  // the launch's order: KV head fastest
   int32_t splits;  // of a query's tiles
   float* ws_o;     // [T, splits, H, D] unnormalized partials
   float* ws_ml;    // [T, splits, H, 2] reference max (log2 domain) and softmax sum
@@ -66,20 +65,21 @@ __device__ __forceinline__ int32_t block_len(const BlockDecodeArgs& a, int32_t l
 
 constexpr float kBlockRescaleSlack = 8.0f;
 
-template <int NB>
+// NB bytes of a V row; STREAM: non-temporal (see below).
+template <int NB, bool STREAM>
 __device__ __forceinline__ void load_run(const uint8_t* p, uint32_t (&dst)[NB / 4]) {
   if constexpr (NB % 16 == 0) {
 #pragma unroll
     for (int i = 0; i < NB / 16; ++i) {
-      const uint4 w = ld16_stream(p + 16 * i);
+      const uint4 w = STREAM ? ld16_stream(p + 16 * i) : ld16(p + 16 * i);
       dst[4 * i] = w.x, dst[4 * i + 1] = w.y, dst[4 * i + 2] = w.z, dst[4 * i + 3] = w.w;
     }
   } else if constexpr (NB == 8) {
-    const uint2 w = ld8_stream(p);
+    const uint2 w = STREAM ? ld8_stream(p) : ld8(p);
     dst[0] = w.x, dst[1] = w.y;
   } else {
     static_assert(NB == 4, "4, 8 or a multiple of 16 bytes");
-    dst[0] = ld4_stream(p);
+    dst[0] = STREAM ? ld4_stream(p) : *reinterpret_cast<const uint32_t*>(p);
   }
 }
 
@@ -102,7 +102,10 @@ struct BlockTile {
   bool valid[2];   // on a page of the pool, below the table's width
 };
 
-template <int D, int FMT, bool SEL, bool SPLIT, int WAVES>
+// SHARED: queries of one row, which read the same pages, may be among the call's (`rows`). V then stays in the L2 (2 x 256
+// queries of 1024 selected keys, bf16: 178 -> 152 us); else it is read once, past it (64 rows of 4096 FP8 keys 87.5 us, through
+// the L2 97). K, two loads a 128-byte line, always goes through it (past it 90; the 2 x 256 queries 244).
+template <int D, int FMT, bool SEL, bool SPLIT, int WAVES, bool SHARED>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2)))
 void block_decode_kernel(BlockDecodeArgs a) {
   using Tile = BlockTile<D, FMT>;
@@ -114,8 +117,11 @@ void block_decode_kernel(BlockDecodeArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, li = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t items = (uint32_t)(SPLIT ? a.T * a.splits : a.T);  // of a KV head
-  const uint32_t v = a.head_fast ? blockIdx.x / (uint32_t)a.G : blockIdx.x % items;
-  const int32_t g = (int32_t)(a.head_fast ? blockIdx.x - v * a.G : blockIdx.x / items);
+  // Queries of one row with the KV head fastest: a head's are found in one L2 (the 2 x 256: 290 -> 244 us, non-temporal then).
+  // Rows of their own gain nothing by that and lose where a head's rows of a page are a few KB, which one head alone reads
+  // through a part of its L2's channels (64 rows of 4096 FP8 keys: 90 -> 101 us).
+  const uint32_t v = SHARED ? blockIdx.x / (uint32_t)a.G : blockIdx.x % items;
+  const int32_t g = (int32_t)(SHARED ? blockIdx.x - v * a.G : blockIdx.x / items);
   const int32_t t = (int32_t)(SPLIT ? v / (uint32_t)a.splits : v), split = SPLIT ? (int32_t)v - t * a.splits : 0;
   const int32_t len_v = a.seq_lens[t];
   const int32_t row_v = a.rows ? a.rows[t] : t;
@@ -174,6 +180,7 @@ void block_decode_kernel(BlockDecodeArgs a) {
 
   const int64_t head_bytes = (int64_t)a.P * D * ESZ;
   const float* scale_base = FMT == kBlockBf16 ? nullptr : (g4 < 2 ? a.k_scale : a.v_scale) + g * a.scale_head;
+  const uint32_t k_off = (uint32_t)(li * D * ESZ + 16 * g4), v_off = (uint32_t)(4 * g4 * D * ESZ + VB * li);
   auto load_tile = [&](Tile& T, int32_t tile) {
     int32_t page[2], sub[2];
     const int32_t half0 = __builtin_amdgcn_readfirstlane(2 * tile);
@@ -189,14 +196,18 @@ void block_decode_kernel(BlockDecodeArgs a) {
       T.valid[hf] = inside && p >= 0 && T.pos[hf] < L && T.pos[hf] + 16 > lo;
       page[hf] = T.valid[hf] ? p : 0;
       sub[hf] = T.valid[hf] ? (int32_t)((uint32_t)in16 * (uint32_t)a.sub_magic >> 16) : 0;
+      // (uniform bases and 32-bit offsets of the lane: addresses take no vector arithmetic)
       const int64_t blk = ((int64_t)page[hf] * a.G + g) * head_bytes + (int64_t)(16 * in16) * D * ESZ;
-      const uint8_t* kp = a.k_cache + blk + (int64_t)li * D * ESZ + 16 * g4;
+      const uint8_t* kp = a.k_cache + blk;
+      const uint8_t* vp = a.v_cache + blk;
 #pragma unroll
-      for (int c4 = 0; c4 < KB / 16; ++c4)
-        load_run<16>(kp + 64 * c4, *reinterpret_cast<uint32_t(*)[4]>(&T.k[hf][4 * c4]));
+      for (int c4 = 0; c4 < KB / 16; ++c4) {
+        const uint4 w = ld16(kp + k_off + 64 * c4);
+        T.k[hf][4 * c4] = w.x, T.k[hf][4 * c4 + 1] = w.y, T.k[hf][4 * c4 + 2] = w.z, T.k[hf][4 * c4 + 3] = w.w;
+      }
 #pragma unroll
       for (int e4 = 0; e4 < 4; ++e4)
-        load_run<VB>(a.v_cache + blk + (int64_t)(4 * g4 + e4) * D * ESZ + VB * li, T.v[4 * hf + e4]);
+        load_run<VB, !SHARED>(vp + v_off + e4 * D * ESZ, T.v[4 * hf + e4]);
     }
     if constexpr (FMT != kBlockBf16) {
       const bool second = g4 & 1;
@@ -409,24 +420,35 @@ __global__ __launch_bounds__(256) void block_combine_kernel(BlockDecodeArgs a) {
       f32_to_bf16_bits(a0 * inv) | f32_to_bf16_bits(a1 * inv) << 16;
 }
 
-template <int D, int FMT, bool SEL>
+template <int D, int FMT, bool SEL, bool SHARED>
 static void launch_block_decode(const BlockDecodeArgs& a, int32_t waves, hipStream_t s) {
   const dim3 grid((uint32_t)(a.T * a.splits * a.G));
   if (a.splits > 1) {
-    if (waves == 4) hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, true, 4>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, true, 8>), grid, dim3(512), 0, s, a);
+    if (waves == 4) hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, true, 4, SHARED>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, true, 8, SHARED>), grid, dim3(512), 0, s, a);
     hipLaunchKernelGGL((block_combine_kernel<D>), dim3(a.T, a.H), dim3(256), 0, s, a);
   } else {
-    if (waves == 4) hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, false, 4>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, false, 8>), grid, dim3(512), 0, s, a);
+    if (waves == 4) hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, false, 4, SHARED>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, false, 8, SHARED>), grid, dim3(512), 0, s, a);
   }
 }
 
-template <int D, bool SEL>
+template <int D, int FMT>
+static void launch_block_decode_form(const BlockDecodeArgs& a, int32_t waves, hipStream_t s) {
+  if (a.rows) {
+    if (a.blocks) launch_block_decode<D, FMT, true, true>(a, waves, s);
+    else launch_block_decode<D, FMT, false, true>(a, waves, s);
+  } else {
+    if (a.blocks) launch_block_decode<D, FMT, true, false>(a, waves, s);
+    else launch_block_decode<D, FMT, false, false>(a, waves, s);
+  }
+}
+
+template <int D>
 static void launch_block_decode_format(const BlockDecodeArgs& a, int32_t dtype, int32_t waves, hipStream_t s) {
-  if (dtype == SNA_DTYPE_BF16) launch_block_decode<D, kBlockBf16, SEL>(a, waves, s);
-  else if (dtype == SNA_DTYPE_INT8) launch_block_decode<D, kBlockInt8, SEL>(a, waves, s);
-  else launch_block_decode<D, kBlockFp8, SEL>(a, waves, s);
+  if (dtype == SNA_DTYPE_BF16) launch_block_decode_form<D, kBlockBf16>(a, waves, s);
+  else if (dtype == SNA_DTYPE_INT8) launch_block_decode_form<D, kBlockInt8>(a, waves, s);
+  else launch_block_decode_form<D, kBlockFp8>(a, waves, s);
 }
 
 // How a launch shares its keys out: waves a workgroup, and the splits of a query, each an even share of its own tiles (the
@@ -547,10 +569,6 @@ extern "C" int sna_paged_decode_blocks(const void* q, const void* k_cache, const
   a.sm_scale = sm_scale;
   const BlockShape shape = block_shape(T, num_kv_heads, head_dim, page_size, table_width, window, a.n_blocks);
   a.splits = shape.splits;
-  // queries of one row read the same pages: with the KV head fastest a head's are found in one L2 (2 x 256 queries of 1024
-  // selected keys, bf16: 290 -> 247 us). Rows of their own gain nothing by it and lose where a head's rows of a page are
-  // a few KB, which one head alone reads through a part of its L2's channels (64 rows of 4096 FP8 keys: 90 -> 101 us).
-  a.head_fast = rows != nullptr;
   a.ws_o = a.ws_ml = nullptr;
   if (a.splits > 1) {
     const int64_t rows_n = (int64_t)T * a.splits * num_q_heads, need = rows_n * (head_dim + 2) * (int64_t)sizeof(float);
@@ -566,12 +584,7 @@ extern "C" int sna_paged_decode_blocks(const void* q, const void* k_cache, const
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %d queries exceed the grid", what, T);
   a.out = (uint16_t*)out;
   const hipStream_t s = (hipStream_t)stream;
-  if (head_dim == 128) {
-    if (blocks) launch_block_decode_format<128, true>(a, cache_dtype, shape.waves, s);
-    else launch_block_decode_format<128, false>(a, cache_dtype, shape.waves, s);
-  } else {
-    if (blocks) launch_block_decode_format<64, true>(a, cache_dtype, shape.waves, s);
-    else launch_block_decode_format<64, false>(a, cache_dtype, shape.waves, s);
-  }
+  if (head_dim == 128) launch_block_decode_format<128>(a, cache_dtype, shape.waves, s);
+  else launch_block_decode_format<64>(a, cache_dtype, shape.waves, s);
   return check_launch(what);
 }

@@ -22,63 +22,90 @@ struct BlockScoreArgs {
   const int32_t* seq_lens;  // [T]
   float* scores;            // [T, G, table_width]
   int32_t* counts;          // [T]
-  int32_t H, G, group, P;
+  int32_t T, H, G, group, P;
+  int32_t runs;  // workgroups of a (query, KV head)
   int64_t num_blocks;
 };
 
-template <int D>
+template <int D, int GROUPS>
 __global__ __launch_bounds__(256) void block_scores_kernel(BlockScoreArgs a) {
   constexpr int HS = D / 32, STEPS = 2 * HS;  // steps of the lower bounds, then as many of the upper ones
   const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, li = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int32_t t = blockIdx.y, g = blockIdx.z;
-  const int32_t c0 = (int32_t)blockIdx.x * 64 + 16 * wave;  // this wave's first column
+  // eight (query, run of columns) items' first heads, then their second ones, ..: an item's heads run on one XCD at about one
+  // time. Their bounds lie side by side, so that the reads in flight fall on every memory channel
+  const uint32_t run = 8u * (uint32_t)a.G, in = blockIdx.x % run, item = blockIdx.x / run * 8 + in % 8;
+  const int32_t g = (int32_t)(in / 8), t = (int32_t)(item / (uint32_t)a.runs);
+  if (t >= a.T) return;
+  const int32_t cx = (int32_t)(item - (uint32_t)t * (uint32_t)a.runs);
+  const int32_t c0 = (cx * 4 + wave) * 16 * GROUPS;  // this wave's first column
   const int32_t row = a.rows ? a.rows[t] : t;
-  const int32_t len = a.seq_lens[t], L = max(len, 0);
-  const int32_t count = (int32_t)(((int64_t)L + a.P - 1) / a.P);
-  if (blockIdx.x == 0 && g == 0 && tid == 0) a.counts[t] = count;
-  if (c0 >= a.table_width) return;
-  const bool row_ok = row >= 0 && row < a.table_rows;
-  const int32_t col = c0 + li;
-  int32_t page = row_ok && col < count && col < a.table_width ? a.table[(int64_t)row * a.table_stride + col] : -1;
-  const bool ok = page >= 0 && (int64_t)page < a.num_blocks;
-  float* dst = a.scores + ((int64_t)t * a.G + g) * a.table_width + c0;
-  if (!__any(ok)) {
-    if (lane < 16 && col < a.table_width) dst[li] = -INFINITY;
+  const int32_t len = a.seq_lens[t];
+  const uint16_t* qp = a.q + ((int64_t)t * a.H + g * a.group + min(li, a.group - 1)) * D + 8 * g4;
+  uint4 qw[HS];
+#pragma unroll
+  for (int s = 0; s < HS; ++s) qw[s] = ld16(qp + 32 * s);
+  if (c0 >= a.table_width) {
+    if (cx == 0 && g == 0 && tid == 0) a.counts[t] = (int32_t)(((int64_t)max(len, 0) + a.P - 1) / a.P);
     return;
   }
-  const uint16_t* b = a.bounds + ((int64_t)(ok ? page : 0) * a.G + g) * 2 * D + 8 * g4;
-  uint32_t bv[STEPS][4];
+  const bool row_ok = row >= 0 && row < a.table_rows;
+  const int32_t* trow = a.table + (int64_t)(row_ok ? row : 0) * a.table_stride;
+  int32_t page[GROUPS];
 #pragma unroll
-  for (int s = 0; s < STEPS; ++s) {
-    const uint4 w = ld16_stream(b + 32 * s);
-    bv[s][0] = w.x, bv[s][1] = w.y, bv[s][2] = w.z, bv[s][3] = w.w;
+  for (int i = 0; i < GROUPS; ++i) page[i] = trow[min(c0 + 16 * i + li, a.table_width - 1)];
+  const int32_t count = (int32_t)(((int64_t)max(len, 0) + a.P - 1) / a.P);
+  if (cx == 0 && g == 0 && tid == 0) a.counts[t] = count;
+  float* dst = a.scores + ((int64_t)t * a.G + g) * a.table_width;
+  uint32_t ok = 0;  // bit i: this lane's column of group i has a page
+  uint32_t bv[GROUPS][STEPS][4];
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) {
+    const int32_t col = c0 + 16 * i + li;
+    const bool good = row_ok && col < count && col < a.table_width && page[i] >= 0 && (int64_t)page[i] < a.num_blocks;
+    ok |= (uint32_t)good << i;
+    const uint16_t* b = a.bounds + ((int64_t)(good ? page[i] : 0) * a.G + g) * 2 * D + 8 * g4;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const uint4 w = ld16(b + 32 * s);  // (two loads a 128-byte line: non-temporal ones 17.2 us where these take 13.9)
+      bv[i][s][0] = w.x, bv[i][s][1] = w.y, bv[i][s][2] = w.z, bv[i][s][3] = w.w;
+    }
   }
-  const uint16_t* qp = a.q + ((int64_t)t * a.H + g * a.group + min(li, a.group - 1)) * D + 8 * g4;
-  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+  uint32_t neg[HS][4], pos[HS][4];
 #pragma unroll
   for (int s = 0; s < HS; ++s) {
-    const uint4 w = ld16(qp + 32 * s);
-    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-    uint32_t neg[4], pos[4];
+    const uint32_t ww[4] = {qw[s].x, qw[s].y, qw[s].z, qw[s].w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       // as 16-bit integers bf16 values have their sign
       const s16x2_t z = {0, 0}, v = __builtin_bit_cast(s16x2_t, ww[i]);
-      neg[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(v, z));
-      pos[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(v, z));
+      neg[s][i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(v, z));
+      pos[s][i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(v, z));
     }
-    acc = mfma_16x16x32_bf16(bv[s], neg, acc);
-    acc = mfma_16x16x32_bf16(bv[HS + s], pos, acc);
   }
-  // (a lane past the group repeats its last head)
-  float best[4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) best[r] = row16_max(acc[r]);
-  const float mine = li == 0 ? best[0] : (li == 1 ? best[1] : (li == 2 ? best[2] : best[3]));
-  const uint64_t okm = __ballot(ok);  // (bit li of each 16: column c0 + li)
-  const int32_t at = 4 * g4 + li;
-  if (li < 4 && c0 + at < a.table_width) dst[at] = (okm >> at) & 1 ? mine : -INFINITY;
+  for (int i = 0; i < GROUPS; ++i) {
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < HS; ++s) {
+      acc = mfma_16x16x32_bf16(bv[i][s], neg[s], acc);
+      acc = mfma_16x16x32_bf16(bv[i][HS + s], pos[s], acc);
+    }
+    // (a lane past the group repeats its last head)
+    float best[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) best[r] = row16_max(acc[r]);
+    const float mine = li == 0 ? best[0] : (li == 1 ? best[1] : (li == 2 ? best[2] : best[3]));
+    const uint64_t okm = __ballot((ok >> i) & 1u);  // (bit li of each 16: column c0 + 16 i + li)
+    const int32_t at = 4 * g4 + li, col = c0 + 16 * i + at;
+    if (li < 4 && col < a.table_width) dst[col] = (okm >> at) & 1 ? mine : -INFINITY;
+  }
+}
+
+template <int D>
+static void launch_block_scores(const BlockScoreArgs& a, hipStream_t s) {
+  const uint32_t items = (uint32_t)(a.T * a.runs);
+  hipLaunchKernelGGL((block_scores_kernel<D, 1>), dim3((items + 7) / 8 * 8 * a.G), dim3(256), 0, s, a);
 }
 
 }  // namespace sna
@@ -107,8 +134,6 @@ extern "C" int sna_block_scores(const void* q, const void* k_bounds, const int32
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: q and k_bounds must be 16-byte aligned", what);
   if (!rows && table_rows < T)
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %d queries over a table of %d rows", what, T, table_rows);
-  if (T > 65535 || num_kv_heads > 65535)
-    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %d queries x %d KV heads exceed the grid", what, T, num_kv_heads);
   BlockScoreArgs a;
   a.q = (const uint16_t*)q;
   a.bounds = (const uint16_t*)k_bounds;
@@ -125,9 +150,12 @@ extern "C" int sna_block_scores(const void* q, const void* k_bounds, const int32
   a.group = group;
   a.P = page_size;
   a.num_blocks = num_blocks;
-  const dim3 grid((uint32_t)(table_width / 64 + (table_width % 64 ? 1 : 0)), T, num_kv_heads);
-  if (grid.x >= 1u << 24) return fail(SNA_ERR_INVALID_ARGUMENT, "%s: a table of %d columns exceeds the grid", what, table_width);
-  if (head_dim == 128) hipLaunchKernelGGL((block_scores_kernel<128>), grid, dim3(256), 0, (hipStream_t)stream, a);
-  else hipLaunchKernelGGL((block_scores_kernel<64>), grid, dim3(256), 0, (hipStream_t)stream, a);
+  a.T = T;
+  a.runs = (int32_t)(((int64_t)table_width + 63) / 64);
+  if (((int64_t)T * a.runs + 8) * num_kv_heads >= 1 << 24)  // (a grid has under 2^32 threads)
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %d queries over %d columns, %d KV heads exceed the grid", what, T, table_width,
+                num_kv_heads);
+  if (head_dim == 128) launch_block_scores<128>(a, (hipStream_t)stream);
+  else launch_block_scores<64>(a, (hipStream_t)stream);
   return check_launch(what);
 }
