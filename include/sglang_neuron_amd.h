@@ -505,7 +505,7 @@ int sna_kv_store_blocks(const void *k, const void *v, int64_t k_row_stride, int6
  *   scales       strides scale_page_stride and scale_head_stride (elements; 0: one scale for all), the blocks of a page and
  *                head contiguous.
  *   sinks        [num_q_heads] fp32 logits joining the softmax denominator, or NULL.
- *   out          [T, num_q_heads, head_dim] bf16; a query that sees no key gives zeros.
+ *   out          [T, num_q_heads, head_dim] bf16, 4-byte aligned; a query that sees no key gives zeros.
  *   workspace    device, 16-byte aligned, sna_block_decode_workspace_bytes bytes (n_blocks 0: no list), any contents; calls
  *                that share one on different streams race.
  * num_q_heads / num_kv_heads <= 16. The same call gives the same bits. */
@@ -522,12 +522,12 @@ int sna_paged_decode_blocks(const void *q, const void *k_cache, const void *v_ca
 
 /* sna_prefill_attention_split over such a pool: a batch of chunks, causal. Scales as in sna_paged_decode_blocks, the rest,
  * the workspace (sna_prefill_workspace_bytes) included, as in sna_prefill_attention_split. A query that sees no key gives zeros.
- * With int8 codes a query element is taken to within 2^-16 of its row's largest. */
+ * With int8 codes a query element is taken to within 2^-16 of its row's largest. n_queries: q's rows (q_start[R]). */
 int sna_prefill_attention_blocks(const void *q, const void *k_cache, const void *v_cache, const float *k_scale,
                                  const float *v_scale, int64_t scale_page_stride, int64_t scale_head_stride,
                                  int32_t scale_tokens, const int32_t *block_table, int64_t table_stride,
-                                 int32_t table_width, const int32_t *q_start, const int32_t *prior_lens, int32_t R,
-                                 int32_t max_q_len, const float *sinks, float sm_scale, int32_t window, void *out,
+                                 int32_t table_width, const int32_t *q_start, const int32_t *prior_lens,
+                                 int32_t n_queries, int32_t R, int32_t max_q_len, const float *sinks, float sm_scale, int32_t window, void *out,
                                  int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
                                  int64_t num_blocks, int32_t cache_dtype, void *workspace, int64_t workspace_bytes,
                                  void *stream);

@@ -28,5 +28,7 @@ How each function is pinned (tests/test_oracle_*.py):
            its closed form; the writes against the pinned MHA store.
   weights  (no reference counterpart) closed forms of equal keys with a window and a sink; selection of hand-made rows;
            compaction of a hand-made table; the rotation against complex multiplication.
+  blocks   (no reference counterpart) hand-made blocks that start, grow and start anew; attention of equal keys, with a
+           window, sinks and lists; scores against every key inside the bounds.
 Nothing here is "parity unpinned"; see the tests for the pin of each function.
 """

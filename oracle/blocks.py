@@ -81,11 +81,11 @@ def rows_of(cache: Tensor, scale: Optional[Tensor], pages: Sequence[int], g: int
 
 
 def attend(q: Tensor, k: Tensor, v: Tensor, sm_scale: float, sinks: Optional[Tensor],
-           q_off: float = 0.0, rounded_sum: bool = False) -> tuple[Tensor, Tensor]:
+           q_off: float = 0.0) -> tuple[Tensor, Tensor]:
     """(out [grp, d], its error bound [grp, d]) of one query's heads q [grp, d] over keys k, v [n, d] (float64) with sinks
-    [grp]. The bound is for a kernel that holds scores, statistics and sums in 32 bits and rounds probabilities and the
-    output to bf16, each by at most 2^-8 of itself, takes a query element to within q_off of its row's largest, and (rounded_sum) sums the
-    probabilities as it rounded them."""
+    [grp]. The bound is for a kernel that holds scores, statistics and sums in 32 bits, rounds probabilities and the output to
+    bf16, each by at most 2^-8 of itself, sums the probabilities as it rounded them, and takes a query element to within q_off
+    of its row's largest."""
     grp, d = q.shape
     if k.shape[0] == 0:
         return torch.zeros(grp, d, dtype=torch.float64), torch.zeros(grp, d, dtype=torch.float64)
@@ -100,16 +100,15 @@ def attend(q: Tensor, k: Tensor, v: Tensor, sm_scale: float, sinks: Optional[Ten
     # reach 2^-22), so a weight, over its sum, by twice that; the sums by n 2^-24
     q_err = q_off * q.double().abs().amax(-1, keepdim=True) * k.abs().sum(-1).amax() * sm_scale
     rel = 2.0 ** -8 + torch.expm1(2 * q_err) + 2 * ((d + 8) * 2.0 ** -24 * reach + 2.0 ** -20) + k.shape[0] * 2.0 ** -23
-    # rounded_sum: sum p_j (1 + e_j) v_j / sum p_j (1 + e_j) - out = sum p_j e_j (v_j - out) / sum p_j (1 + e_j), with |e_j| <=
-    # 2^-8 at most 2^-8 (sum p_j |v_j| + |out|) / (1 - 2^-8): another 2^-8 |out|, and 2^-8 of both
-    own = 2.0 ** -8 * (1 + (1 + 2.0 ** -7) * rounded_sum)
-    return out, own * out.abs() + rel * (1 + 2.0 ** -7 * rounded_sum) * (p @ v.abs())
+    # sum p_j (1 + e_j) v_j / sum p_j (1 + e_j) - out = sum p_j e_j (v_j - out) / sum p_j (1 + e_j), with |e_j| <= 2^-8 at most
+    # 2^-8 (sum p_j |v_j| + |out|) / (1 - 2^-8); the output's own rounding is 2^-8 |out| more
+    return out, 2.0 ** -8 * (2 + 2.0 ** -7) * out.abs() + rel * (1 + 2.0 ** -7) * (p @ v.abs())
 
 
 def decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, lens: Sequence[int], *, sm_scale: float,
            k_scale: Optional[Tensor] = None, v_scale: Optional[Tensor] = None, sinks: Optional[Tensor] = None, window: int = 0,
            rows: Optional[Sequence[int]] = None, blocks: Optional[Tensor] = None,
-           q_off: float = 0.0, rounded_sum: bool = False) -> tuple[Tensor, Tensor]:
+           q_off: float = 0.0) -> tuple[Tensor, Tensor]:
     """([T, H, d] float64, its error bound) of single queries over their rows, or over the columns that blocks [T, G, n]
     names."""
     T, H, d = q.shape
@@ -132,7 +131,7 @@ def decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, lens: Seq
             k, v = rows_of(k_cache, k_scale, pages, g)[seen], rows_of(v_cache, v_scale, pages, g)[seen]
             h = slice(g * grp, (g + 1) * grp)
             out[t, h], off[t, h] = attend(q[t, h], k, v, sm_scale, None if sinks is None else sinks[h],
-                                           q_off, rounded_sum)
+                                           q_off)
     return out, off
 
 
@@ -144,7 +143,7 @@ def prefill(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, q_start:
         for i in range(q_start[r + 1] - q_start[r]):
             rows.append(r)
             lens.append(prior[r] + i + 1)
-    return decode(q, k_cache, v_cache, table, lens, rows=rows, rounded_sum=True, **kw)
+    return decode(q, k_cache, v_cache, table, lens, rows=rows, **kw)
 
 
 def scores(q: Tensor, bounds: Tensor, table: Tensor, lens: Sequence[int], P: int,

@@ -7,7 +7,8 @@
 // the score's factor and V's the probability: codes go into the matrix products as they are, exact in bf16.
 //
 // Work: one workgroup per (query, KV head), or, where those do not fill the card, per (split of a query, KV head): a
-// query's splits divide its tiles evenly, and a second launch merges them. A wave takes tiles round-robin, the next one's loads in flight while it computes one.
+// query's splits divide its tiles evenly, and a second launch merges them. A wave takes tiles round-robin, the next one's
+// loads in flight while it computes one.
 // A tile is two half-tiles of 16 keys, each inside one page and one block. Lane roles (lane = 16 g4 + li):
 //   QK   S^T[key, head] = K[key, :] . Q[head, :], v_mfma_f32_16x16x32_bf16 with M = 16 keys, N = 16 heads (the group's,
 //        zero-padded): lane (g4, li) feeds key li's 16-byte chunks 4 c + g4 and head li's elements of the same dims, and
@@ -264,7 +265,7 @@ void block_decode_kernel(BlockDecodeArgs a) {
 #pragma unroll
           for (int i = 0; i < VB / 4; ++i) T.v[4 * hf + r][i] = ok ? T.v[4 * hf + r][i] : 0u;
         }
-        vs[hf] = any ? vs[hf] : 0.0f;  // (a block with no visible key here: its scale may be anything)
+        vs[hf] = any ? vs[hf] : 1.0f;  // (a block with no visible key here: its scale may be anything)
       }
     }
     float tmax = -INFINITY;
@@ -280,16 +281,26 @@ void block_decode_kernel(BlockDecodeArgs a) {
 #pragma unroll
       for (int i = 0; i < DT; ++i) acc[i] *= alpha;
     }
-    float p[8];
+    // The probabilities, times V's scale, go into the product as bf16, off by at most 2^-8 of themselves; their sum is of the
+    // same rounded values (over the scale again), so that a row which one key carries is off by nothing (8 rows of 128 to 1024
+    // keys: 2.5e-3 of the result, norm by norm, with the unrounded sum, 2.0e-3 so; the rounding of the result alone 1.6e-3).
+    uint32_t pop[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(x[i] - m_ref);
-      l_run += p[i];
-      if constexpr (FMT != kBlockBf16) p[i] *= vs[i >> 2];
+    for (int hf = 0; hf < 2; ++hf) {
+      float part = 0.0f;
+      // (a scale under the least one of a block is taken for that; NaN stays)
+      const float v = vs[hf] < kLeastBlockScale ? kLeastBlockScale : vs[hf];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float p0 = __builtin_amdgcn_exp2f(x[4 * hf + 2 * k] - m_ref), p1 = __builtin_amdgcn_exp2f(x[4 * hf + 2 * k + 1] - m_ref);
+        if constexpr (FMT != kBlockBf16) p0 *= v, p1 *= v;
+        pop[2 * hf + k] = pack_bf16x2(p0, p1);
+        float& sum = FMT != kBlockBf16 ? part : l_run;
+        sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pop[2 * hf + k]),
+                                              __builtin_bit_cast(bf16x2_t, 0x3f803f80u), sum, false);
+      }
+      if constexpr (FMT != kBlockBf16) l_run = fmaf(part, __builtin_amdgcn_rcpf(v), l_run);
     }
-    // the probabilities (times V's scale) go into the product as bf16, off by at most 2^-9 of themselves
-    const uint32_t pop[4] = {pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]),
-                             pack_bf16x2(p[6], p[7])};
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       uint32_t op[4];
@@ -533,8 +544,9 @@ extern "C" int sna_paged_decode_blocks(const void* q, const void* k_cache, const
   if (T == 0) return SNA_OK;
   if (!q || !k_cache || !v_cache || !block_table || !seq_lens || !out || (scaled && (!k_scale || !v_scale)))
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
-  if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16))
-    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: q and the caches must be 16-byte aligned", what);
+  if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(out, 4))
+    return fail(SNA_ERR_INVALID_ARGUMENT, "%s: q and the caches must be 16-byte aligned, out 4-byte", what);
+  if (table_rows < 1) return fail(SNA_ERR_INVALID_ARGUMENT, "%s: a table of no rows", what);
   if (!rows && table_rows < T)
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %d queries over a table of %d rows", what, T, table_rows);
   if (num_q_heads > 65535) return fail(SNA_ERR_INVALID_ARGUMENT, "%s: grid too large", what);

@@ -7,6 +7,10 @@
 // Work: one wave per 16 pages of a (query, KV head), 4 waves a workgroup. v_mfma_f32_16x16x32_bf16 with M = 16 pages, N =
 // 16 heads (the group's), K = 2 D: lane (g4, li) feeds page li's 8 elements from 32 s + 8 g4 in step s and head li's of the
 // same dimensions, and gets pages 4 g4 + r of head li; the heads' maximum is taken over the 16 lanes of a row.
+//
+// What bounds it: reads of 512 bytes (head dim 128) at random places, the query's length and the table before them. 64 rows of
+// 16384 keys in pages of 64, 8 KV heads: 13.9-14.8 us, 68 MB, 4.6-4.9 TB/s; one row of 131071 in pages of 32, 17 MB, 6.2. Two or
+// four groups of 16 pages a wave, all asked for at once: the same, and slower for one row (P = 128: 3.9, 5.7 and 8.1).
 #include "sna_device.h"
 #include "sna_host.h"
 
@@ -27,7 +31,7 @@ struct BlockScoreArgs {
   int64_t num_blocks;
 };
 
-template <int D, int GROUPS>
+template <int D>
 __global__ __launch_bounds__(256) void block_scores_kernel(BlockScoreArgs a) {
   constexpr int HS = D / 32, STEPS = 2 * HS;  // steps of the lower bounds, then as many of the upper ones
   const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, li = lane & 15;
@@ -38,38 +42,26 @@ __global__ __launch_bounds__(256) void block_scores_kernel(BlockScoreArgs a) {
   const int32_t g = (int32_t)(in / 8), t = (int32_t)(item / (uint32_t)a.runs);
   if (t >= a.T) return;
   const int32_t cx = (int32_t)(item - (uint32_t)t * (uint32_t)a.runs);
-  const int32_t c0 = (cx * 4 + wave) * 16 * GROUPS;  // this wave's first column
+  const int32_t c0 = cx * 64 + 16 * wave, col = c0 + li;  // this wave's first column, this lane's
   const int32_t row = a.rows ? a.rows[t] : t;
   const int32_t len = a.seq_lens[t];
   const uint16_t* qp = a.q + ((int64_t)t * a.H + g * a.group + min(li, a.group - 1)) * D + 8 * g4;
   uint4 qw[HS];
 #pragma unroll
   for (int s = 0; s < HS; ++s) qw[s] = ld16(qp + 32 * s);
-  if (c0 >= a.table_width) {
-    if (cx == 0 && g == 0 && tid == 0) a.counts[t] = (int32_t)(((int64_t)max(len, 0) + a.P - 1) / a.P);
-    return;
-  }
+  if (c0 >= a.table_width) return;
   const bool row_ok = row >= 0 && row < a.table_rows;
   const int32_t* trow = a.table + (int64_t)(row_ok ? row : 0) * a.table_stride;
-  int32_t page[GROUPS];
-#pragma unroll
-  for (int i = 0; i < GROUPS; ++i) page[i] = trow[min(c0 + 16 * i + li, a.table_width - 1)];
+  const int32_t page = trow[min(col, a.table_width - 1)];
   const int32_t count = (int32_t)(((int64_t)max(len, 0) + a.P - 1) / a.P);
   if (cx == 0 && g == 0 && tid == 0) a.counts[t] = count;
-  float* dst = a.scores + ((int64_t)t * a.G + g) * a.table_width;
-  uint32_t ok = 0;  // bit i: this lane's column of group i has a page
-  uint32_t bv[GROUPS][STEPS][4];
+  const bool ok = row_ok && col < count && col < a.table_width && page >= 0 && (int64_t)page < a.num_blocks;
+  const uint16_t* b = a.bounds + ((int64_t)(ok ? page : 0) * a.G + g) * 2 * D + 8 * g4;
+  uint32_t bv[STEPS][4];
 #pragma unroll
-  for (int i = 0; i < GROUPS; ++i) {
-    const int32_t col = c0 + 16 * i + li;
-    const bool good = row_ok && col < count && col < a.table_width && page[i] >= 0 && (int64_t)page[i] < a.num_blocks;
-    ok |= (uint32_t)good << i;
-    const uint16_t* b = a.bounds + ((int64_t)(good ? page[i] : 0) * a.G + g) * 2 * D + 8 * g4;
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      const uint4 w = ld16(b + 32 * s);  // (two loads a 128-byte line: non-temporal ones 17.2 us where these take 13.9)
-      bv[i][s][0] = w.x, bv[i][s][1] = w.y, bv[i][s][2] = w.z, bv[i][s][3] = w.w;
-    }
+  for (int s = 0; s < STEPS; ++s) {
+    const uint4 w = ld16(b + 32 * s);  // (two loads a 128-byte line: non-temporal ones 17.2 us where these take 13.9)
+    bv[s][0] = w.x, bv[s][1] = w.y, bv[s][2] = w.z, bv[s][3] = w.w;
   }
   uint32_t neg[HS][4], pos[HS][4];
 #pragma unroll
@@ -83,29 +75,27 @@ __global__ __launch_bounds__(256) void block_scores_kernel(BlockScoreArgs a) {
       pos[s][i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(v, z));
     }
   }
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < GROUPS; ++i) {
-    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < HS; ++s) {
-      acc = mfma_16x16x32_bf16(bv[i][s], neg[s], acc);
-      acc = mfma_16x16x32_bf16(bv[i][HS + s], pos[s], acc);
-    }
-    // (a lane past the group repeats its last head)
-    float best[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) best[r] = row16_max(acc[r]);
-    const float mine = li == 0 ? best[0] : (li == 1 ? best[1] : (li == 2 ? best[2] : best[3]));
-    const uint64_t okm = __ballot((ok >> i) & 1u);  // (bit li of each 16: column c0 + 16 i + li)
-    const int32_t at = 4 * g4 + li, col = c0 + 16 * i + at;
-    if (li < 4 && col < a.table_width) dst[col] = (okm >> at) & 1 ? mine : -INFINITY;
+  for (int s = 0; s < HS; ++s) {
+    acc = mfma_16x16x32_bf16(bv[s], neg[s], acc);
+    acc = mfma_16x16x32_bf16(bv[HS + s], pos[s], acc);
   }
+  // (a lane past the group repeats its last head)
+  float best[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) best[r] = row16_max(acc[r]);
+  const float mine = li == 0 ? best[0] : (li == 1 ? best[1] : (li == 2 ? best[2] : best[3]));
+  const uint64_t okm = __ballot(ok);  // (bit li of each 16: column c0 + li)
+  const int32_t at = 4 * g4 + li;
+  if (li < 4 && c0 + at < a.table_width)
+    a.scores[((int64_t)t * a.G + g) * a.table_width + c0 + at] = (okm >> at) & 1 ? mine : -INFINITY;
 }
 
 template <int D>
 static void launch_block_scores(const BlockScoreArgs& a, hipStream_t s) {
   const uint32_t items = (uint32_t)(a.T * a.runs);
-  hipLaunchKernelGGL((block_scores_kernel<D, 1>), dim3((items + 7) / 8 * 8 * a.G), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((block_scores_kernel<D>), dim3((items + 7) / 8 * 8 * a.G), dim3(256), 0, s, a);
 }
 
 }  // namespace sna
@@ -132,6 +122,7 @@ extern "C" int sna_block_scores(const void* q, const void* k_bounds, const int32
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   if (!aligned(q, 16) || !aligned(k_bounds, 16))
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: q and k_bounds must be 16-byte aligned", what);
+  if (table_rows < 1) return fail(SNA_ERR_INVALID_ARGUMENT, "%s: a table of no rows", what);
   if (!rows && table_rows < T)
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %d queries over a table of %d rows", what, T, table_rows);
   BlockScoreArgs a;

@@ -40,6 +40,7 @@ struct BlockStoreArgs {
   const int32_t* q_start;  // [R + 1], or null: token r is request r's
   const int32_t* prior;    // [R]
   int32_t R, T, G, P, bt, max_q, pages;  // pages: the most that a request's tokens can touch
+  int32_t items;  // workgroups of a KV head: R * pages, or (less) as many pages as the call can touch, found by block_item
   int64_t num_blocks;
 };
 
@@ -89,6 +90,41 @@ __device__ __forceinline__ void block_values(uint32_t w, float (&x)[4]) {
   }
 }
 
+// Request r's tokens: rows [t0, t0 + n) of the call (n = 0: none).
+__device__ __forceinline__ void block_request(const BlockStoreArgs& a, int32_t r, int32_t& t0, int32_t& n, int32_t& prior) {
+  t0 = r, n = 1;
+  if (a.q_start) {
+    t0 = a.q_start[r];
+    const int32_t t1 = min(a.q_start[r + 1], a.T);
+    n = t0 >= 0 && t1 > t0 ? min(t1 - t0, a.max_q) : 0;
+  }
+  prior = a.prior[r];
+  if (prior < 0) n = 0;
+}
+
+// The item'th page that the call touches, request by request: its request and its place among the request's pages (every lane
+// of the wave gets the same; false past the last).
+__device__ bool block_item(const BlockStoreArgs& a, int32_t item, int32_t& r_out, int32_t& j_out) {
+  const int lane = threadIdx.x & 63;
+  int32_t base = 0;
+  for (int32_t r0 = 0; r0 < a.R; r0 += 64) {  // uniform
+    int32_t t0, n = 0, prior = 0;
+    if (r0 + lane < a.R) block_request(a, r0 + lane, t0, n, prior);
+    const int32_t pages = n > 0 ? (int32_t)(((int64_t)prior + n - 1) / a.P) - prior / a.P + 1 : 0;
+    int32_t part;
+    const int32_t incl = wave_incl_scan_i32(pages, &part);
+    if (item < base + part) {
+      const uint64_t mine = __ballot(item >= base + incl - pages && item < base + incl);
+      const int32_t src = (int32_t)__builtin_amdgcn_readfirstlane(__ffsll((long long)mine) - 1);
+      r_out = r0 + src;
+      j_out = item - base - __builtin_amdgcn_readlane(incl - pages, src);
+      return true;
+    }
+    base += part;
+  }
+  return false;
+}
+
 template <int D, int FMT, int WAVES, int TEAM>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(5)))
 void kv_store_blocks_kernel(BlockStoreArgs a) {
@@ -102,18 +138,13 @@ void kv_store_blocks_kernel(BlockStoreArgs a) {
   // (KV head fastest: a page's heads, whose rows of the call lie side by side, at one time: bf16 15.2 -> 13.5 us)
   const uint32_t pj = blockIdx.x / (uint32_t)a.G;
   const int32_t g = (int32_t)(blockIdx.x - pj * a.G);
-  const int32_t r = (int32_t)(pj / (uint32_t)a.pages), j = (int32_t)pj - r * a.pages;
+  int32_t r = (int32_t)(pj / (uint32_t)a.pages), j = (int32_t)pj - r * a.pages;
+  if (a.items != a.R * a.pages && !__builtin_amdgcn_readfirstlane((int)block_item(a, (int32_t)pj, r, j))) return;
+  r = __builtin_amdgcn_readfirstlane(r), j = __builtin_amdgcn_readfirstlane(j);
 
-  // the request's tokens: rows [t0, t0 + n) of the call at positions prior ..
-  int32_t t0 = r, n = 1;
-  if (a.q_start) {
-    t0 = a.q_start[r];
-    const int32_t t1 = min(a.q_start[r + 1], a.T);
-    if (t0 < 0 || t1 <= t0) return;
-    n = min(t1 - t0, a.max_q);
-  }
-  const int32_t prior = a.prior[r];
-  if (prior < 0) return;
+  int32_t t0, n, prior;
+  block_request(a, r, t0, n, prior);
+  if (n == 0) return;
   // this workgroup's page and the positions [lo, hi) in it that the call writes
   const int64_t col = prior / a.P + (int64_t)j;
   const int64_t first = col * a.P;
@@ -309,7 +340,7 @@ void kv_store_blocks_kernel(BlockStoreArgs a) {
 
 template <int D, int FMT>
 static void launch_block_store(const BlockStoreArgs& a, hipStream_t s) {
-  const dim3 grid((uint32_t)(a.R * a.pages * a.G));
+  const dim3 grid((uint32_t)(a.items * a.G));
   // a wave holds 8 pieces of 64 * 8 elements: so many waves share a block of tokens; a workgroup takes K's and V's at once
   const int32_t waves = (a.bt * D + 8 * 512 - 1) / (8 * 512);
   if (FMT == kBlockBf16 || waves <= 1) {
@@ -390,9 +421,14 @@ extern "C" int sna_kv_store_blocks(const void* k, const void* v, int64_t k_row_s
   a.max_q = max_q_len < n_tokens ? max_q_len : n_tokens;
   a.pages = (int32_t)(((int64_t)a.max_q + page_size - 2) / page_size + 1);
   a.num_blocks = num_blocks;
-  if (((int64_t)R * a.pages + 8) * num_kv_heads >= 1 << 23)  // (a grid has under 2^32 threads)
+  // A batch of one long chunk and many short ones (a chunk between decode steps): most of R * pages workgroups would find no
+  // page, so the pages there are, at most one for every page_size tokens and two a request, are counted out instead.
+  const int64_t direct = (int64_t)R * a.pages, touched = (int64_t)n_tokens / page_size + 2 * (int64_t)R;
+  const int64_t items = direct > 4 * touched ? touched : direct;
+  if (items * num_kv_heads >= 1 << 23 || direct > INT32_MAX)  // (a grid has under 2^32 threads)
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %d requests of up to %d pages, %d heads exceed the grid", what, R, a.pages,
                 num_kv_heads);
+  a.items = (int32_t)items;
   if (head_dim == 128) launch_block_store_format<128>(a, cache_dtype, (hipStream_t)stream);
   else launch_block_store_format<64>(a, cache_dtype, (hipStream_t)stream);
   return check_launch(what);

@@ -80,6 +80,7 @@ struct PrefillArgs {
 struct PrefillBlockArgs : PrefillArgs {
   int64_t scale_page, scale_head;  // strides
   int32_t sub_magic;               // ceil(2^16 / (bt / 16)): a 16-key group's block in its page (0: one block a page)
+  int32_t items;  // > 0: the launch has so many workgroups a KV head, found by prefill_find, instead of qblocks * R
 };
 // SCALES: a BlockFormat of such a pool, or kBlockBf16 for none
 template <int SCALES>
@@ -244,6 +245,28 @@ __device__ bool prefill_item(const PrefillArgs& a, int32_t& w, int32_t& g, int32
   return found;
 }
 
+// The item'th query block there is, request by request: its request and its place among the request's (every lane of the wave
+// gets the same; false past the last).
+__device__ bool prefill_find(const PrefillArgs& a, int32_t item, int32_t& r, int32_t& bx) {
+  const int lane = threadIdx.x & 63;
+  int32_t base = 0;
+  for (int32_t r0 = 0; r0 < a.R; r0 += 64) {  // uniform
+    const int32_t S = r0 + lane < a.R ? a.q_start[r0 + lane + 1] - a.q_start[r0 + lane] : 0;
+    const int32_t n = S > 0 ? min((S + a.bq - 1) / a.bq, a.qblocks) : 0;
+    int32_t part;
+    const int32_t incl = wave_incl_scan_i32(n, &part);
+    if (item < base + part) {
+      const uint64_t mine = __ballot(item >= base + incl - n && item < base + incl);
+      const int32_t src = (int32_t)__builtin_amdgcn_readfirstlane(__ffsll((long long)mine) - 1);
+      r = r0 + src;
+      bx = item - base - __builtin_amdgcn_readlane(incl - n, src);
+      return true;
+    }
+    base += part;
+  }
+  return false;
+}
+
 // kOneTile and kHalfTile: the launch's tables name at most one tile of keys, or 32 of them (prompts of up to 64 or 32
 // tokens with no prior), so the loop's next tile, whose products it computes whether there is one or not, and the tile's
 // second sub-tile are left out (32 / 8 heads of 128, FP8 / bf16, us: 16 tokens 8.2 / 7.6 through the loop, 6.9 / 6.2 so;
@@ -286,6 +309,10 @@ void prefill_gqa_kernel(PrefillArgsOf<SCALES> a) {
                                    gridDim.x * gridDim.y * gridDim.z);
     bx = (int32_t)(lin % gridDim.x);
     r = (int32_t)((lin / gridDim.x) % gridDim.y), g = (int32_t)(lin / (gridDim.x * gridDim.y));
+    if constexpr (BLK) {
+      if (a.items > 0 && !__builtin_amdgcn_readfirstlane((int)prefill_find(a, bx, r, bx))) return;
+      r = __builtin_amdgcn_readfirstlane(r), bx = __builtin_amdgcn_readfirstlane(bx);
+    }
   }
   const int32_t qa = a.q_start[r];
   const PrefillBlock blk = prefill_block(a, a.q_start[r + 1] - qa, a.prior[r], bx);
@@ -673,7 +700,8 @@ void prefill_gqa_kernel(PrefillArgsOf<SCALES> a) {
       // tokens may never have been written
       for (int32_t i = tid; i < 2 * n * TG; i += 256) {
         const int32_t kv = i >= n * TG ? 1 : 0, u = i - kv * n * TG, key = TK * c0 + 16 * u, col = column(key);
-        const int32_t page = sm_pages[col - p0], sub = (int32_t)((uint32_t)((key - col * a.P) / 16) * (uint32_t)a.sub_magic >> 16);
+        const int32_t page = sm_pages[col - p0], in16 = (key - col * a.P) / 16;
+        const int32_t sub = (int32_t)((uint32_t)in16 * (uint32_t)a.sub_magic >> 16);
         float sc = 1.0f;
         if (page >= 0 && key < hi) sc = (kv ? a.v_scale : a.k_scale)[page * a.scale_page + g * a.scale_head + sub];
         if (kv) {
@@ -899,12 +927,17 @@ void launch_prefill(const PrefillArgsOf<SCALES>& a, hipStream_t s) {
     hipLaunchKernelGGL((prefill_gqa_kernel<D, ESZ, kSplit, SCALES>), dim3(a.slots), dim3(256), 0, s, a);
     hipLaunchKernelGGL((prefill_combine_kernel<D>), dim3(kPrefillRows * D / 1024 * a.qblocks, a.R, a.G),
                        dim3(256), 0, s, a, ESZ == 1 && SCALES == kBlockBf16);
-  } else if ((int64_t)a.table_width * a.P <= kPrefillTile / 2) {
-    hipLaunchKernelGGL((prefill_gqa_kernel<D, ESZ, kHalfTile, SCALES>), dim3(a.qblocks, a.R, a.G), dim3(256), 0, s, a);
-  } else if ((int64_t)a.table_width * a.P <= kPrefillTile) {
-    hipLaunchKernelGGL((prefill_gqa_kernel<D, ESZ, kOneTile, SCALES>), dim3(a.qblocks, a.R, a.G), dim3(256), 0, s, a);
   } else {
-    hipLaunchKernelGGL((prefill_gqa_kernel<D, ESZ, kWhole, SCALES>), dim3(a.qblocks, a.R, a.G), dim3(256), 0, s, a);
+    dim3 grid(a.qblocks, a.R, a.G);
+    if constexpr (SCALES != kBlockBf16) {
+      if (a.items > 0) grid = dim3(a.items, 1, a.G);
+    }
+    if ((int64_t)a.table_width * a.P <= kPrefillTile / 2)
+      hipLaunchKernelGGL((prefill_gqa_kernel<D, ESZ, kHalfTile, SCALES>), grid, dim3(256), 0, s, a);
+    else if ((int64_t)a.table_width * a.P <= kPrefillTile)
+      hipLaunchKernelGGL((prefill_gqa_kernel<D, ESZ, kOneTile, SCALES>), grid, dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((prefill_gqa_kernel<D, ESZ, kWhole, SCALES>), grid, dim3(256), 0, s, a);
   }
 }
 
@@ -914,15 +947,16 @@ void launch_prefill(const PrefillArgsOf<SCALES>& a, hipStream_t s) {
 struct PrefillScales {
   int64_t page_stride, head_stride;
   int32_t tokens;
+  int32_t n_queries;  // of the batch
 };
 
-static int prefill_attention(const char* what, const PrefillScales* scales, bool empty_zero, const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
-                                     const float* v_scale, const int32_t* block_table, int64_t table_stride,
-                                     int32_t table_width, const int32_t* q_start, const int32_t* prior_lens,
-                                     int32_t R, int32_t max_q_len, const float* sinks, float sm_scale, int32_t window,
-                                     void* out, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-                                     int32_t page_size, int64_t num_blocks, int32_t kv_dtype, void* workspace,
-                                     int64_t workspace_bytes, void* stream) {
+static int prefill_attention(const char* what, const PrefillScales* scales, bool empty_zero, const void* q,
+                             const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                             const int32_t* block_table, int64_t table_stride, int32_t table_width,
+                             const int32_t* q_start, const int32_t* prior_lens, int32_t R, int32_t max_q_len,
+                             const float* sinks, float sm_scale, int32_t window, void* out, int32_t num_q_heads,
+                             int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int64_t num_blocks,
+                             int32_t kv_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   if (R < 0 || max_q_len < 0 || num_q_heads < 1 || num_kv_heads < 1 || num_q_heads % num_kv_heads != 0 ||
       window < 0 || num_blocks < 1 || table_width < 1 || table_stride < table_width)
     return fail(SNA_ERR_INVALID_ARGUMENT,
@@ -1007,6 +1041,10 @@ static int prefill_attention(const char* what, const PrefillScales* scales, bool
     a.scale_head = scales->head_stride;
     const int32_t per = scales->tokens / 16;
     a.sub_magic = scales->tokens < page_size ? (65536 + per - 1) / per : 0;
+    // A batch of one long chunk and many short ones: most of qblocks * R workgroups would find no query, so the query blocks
+    // there are, at most one for every bq queries and one a request, are counted out instead.
+    const int64_t touched = (int64_t)scales->n_queries / a.bq + R;
+    a.items = qblocks * R > 4 * touched && touched <= INT32_MAX ? (int32_t)touched : 0;
     if (kv_dtype == SNA_DTYPE_INT8) {
       if (head_dim == 128) launch_prefill<128, 1, kBlockInt8>(a, s); else launch_prefill<64, 1, kBlockInt8>(a, s);
     } else {
@@ -1027,9 +1065,9 @@ extern "C" int sna_prefill_attention(const void* q, const void* k_cache, const v
                                      void* out, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                                      int32_t page_size, int64_t num_blocks, int32_t kv_dtype, void* stream) {
   ApiGuard guard;
-  return prefill_attention("prefill_attention", nullptr, false, q, k_cache, v_cache, k_scale, v_scale, block_table, table_stride, table_width, q_start,
-                           prior_lens, R, max_q_len, sinks, sm_scale, window, out, num_q_heads, num_kv_heads, head_dim,
-                           page_size, num_blocks, kv_dtype, nullptr, 0, stream);
+  return prefill_attention("prefill_attention", nullptr, false, q, k_cache, v_cache, k_scale, v_scale, block_table,
+                           table_stride, table_width, q_start, prior_lens, R, max_q_len, sinks, sm_scale, window, out,
+                           num_q_heads, num_kv_heads, head_dim, page_size, num_blocks, kv_dtype, nullptr, 0, stream);
 }
 
 extern "C" int64_t sna_prefill_workspace_bytes(int32_t R, int32_t max_q_len, int32_t num_q_heads, int32_t num_kv_heads,
@@ -1051,21 +1089,23 @@ extern "C" int sna_prefill_attention_split(const void* q, const void* k_cache, c
                                            int64_t num_blocks, int32_t kv_dtype, void* workspace,
                                            int64_t workspace_bytes, void* stream) {
   ApiGuard guard;
-  return prefill_attention("prefill_attention", nullptr, false, q, k_cache, v_cache, k_scale, v_scale, block_table, table_stride, table_width, q_start,
-                           prior_lens, R, max_q_len, sinks, sm_scale, window, out, num_q_heads, num_kv_heads, head_dim,
-                           page_size, num_blocks, kv_dtype, workspace, workspace_bytes, stream);
+  return prefill_attention("prefill_attention", nullptr, false, q, k_cache, v_cache, k_scale, v_scale, block_table,
+                           table_stride, table_width, q_start, prior_lens, R, max_q_len, sinks, sm_scale, window, out,
+                           num_q_heads, num_kv_heads, head_dim, page_size, num_blocks, kv_dtype, workspace,
+                           workspace_bytes, stream);
 }
 
 extern "C" int sna_prefill_attention_blocks(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
                                             const float* v_scale, int64_t scale_page_stride, int64_t scale_head_stride,
                                             int32_t scale_tokens, const int32_t* block_table, int64_t table_stride,
                                             int32_t table_width, const int32_t* q_start, const int32_t* prior_lens,
-                                            int32_t R, int32_t max_q_len, const float* sinks, float sm_scale,
+                                            int32_t n_queries, int32_t R, int32_t max_q_len, const float* sinks, float sm_scale,
                                             int32_t window, void* out, int32_t num_q_heads, int32_t num_kv_heads,
                                             int32_t head_dim, int32_t page_size, int64_t num_blocks, int32_t cache_dtype,
                                             void* workspace, int64_t workspace_bytes, void* stream) {
   ApiGuard guard;
-  const PrefillScales scales = {scale_page_stride, scale_head_stride, scale_tokens};
+  if (n_queries < 0) return fail(SNA_ERR_INVALID_ARGUMENT, "prefill_attention_blocks: %d queries", n_queries);
+  const PrefillScales scales = {scale_page_stride, scale_head_stride, scale_tokens, n_queries};
   return prefill_attention("prefill_attention_blocks", cache_dtype == SNA_DTYPE_BF16 ? nullptr : &scales, true, q, k_cache,
                            v_cache, k_scale, v_scale, block_table, table_stride, table_width, q_start, prior_lens, R, max_q_len,
                            sinks, sm_scale, window, out, num_q_heads, num_kv_heads, head_dim, page_size, num_blocks,

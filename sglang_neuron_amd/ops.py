@@ -1264,6 +1264,13 @@ def evict_tokens(k_cache: Tensor, v_cache: Tensor, block_table: Tensor, seq_lens
 _BLOCK_CODES = {torch.bfloat16: _lib.DTYPE_BF16, FP8: _lib.DTYPE_FP8_E4M3FN, torch.int8: _lib.DTYPE_INT8}
 
 
+def _vector(t: Tensor, dtype: torch.dtype) -> Tensor:
+    """t's elements as a contiguous vector of ``dtype``, t itself where it is one (views cost as much as a check each)."""
+    if t.dtype == dtype and t.dim() == 1 and t.is_contiguous():
+        return t
+    return t.reshape(-1).to(dtype).contiguous()
+
+
 def _block_cache(k_cache: Tensor, v_cache: Tensor, k_scale: Optional[Tensor], v_scale: Optional[Tensor]):
     """(dtype code, shape, k_scale, v_scale, their page and head strides, tokens that share a scale) of a layer's caches
     [blocks, G, page, d]: bf16, or FP8 or int8 codes with scales [blocks, G, page / tokens] fp32."""
@@ -1311,7 +1318,8 @@ def kv_store_blocks(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, bloc
 
     ``max_q_len`` bounds the chunk lengths (a host int); ``host_q_start``: a host copy of q_start, checked before the launch.
     Tokens without a page are not stored. No page may be written for two requests of a call (a cached prefix is shared by whole
-    pages only)."""
+    pages only). A page moves with its scales and bounds (copy_page_items over all their tensors); compact_tokens and
+    evict_tokens move codes between blocks, so they are for bf16 caches only."""
     dev = _on_gpu(k, v, k_cache, v_cache, block_table, prior_lens, q_start, k_scale, v_scale, k_bounds)
     code, (nb, G, P, d), ks, vs, _, _, tokens = _block_cache(k_cache, v_cache, k_scale, v_scale)
     if k.dim() != 3 or k.shape[1:] != (G, d) or v.shape != k.shape or k.dtype != torch.bfloat16 or v.dtype != k.dtype:
@@ -1330,7 +1338,7 @@ def kv_store_blocks(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, bloc
     if block_table.dim() != 2 or block_table.shape[0] < R or block_table.shape[1] < 1:
         _need(False, f"block_table must be [{R}, width], got {tuple(block_table.shape)}")
     table, stride = _strided_rows(_as(block_table, torch.int32))
-    prior = _contig(_as(prior_lens.reshape(-1), torch.int32), "prior_lens")
+    prior = _vector(prior_lens, torch.int32)
     if q_start is None:
         if T != R or max_q_len != 1:
             _need(False, f"{T} tokens of {R} requests, max_q_len {max_q_len}, and no q_start")
@@ -1339,9 +1347,11 @@ def kv_store_blocks(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, bloc
             _need(False, f"q_start must be [{R + 1}]")
         if host_q_start is not None:
             _check_q_start(host_q_start, R, T, max_q_len)
-        q_start = _contig(_as(q_start.reshape(-1), torch.int32), "q_start")
+        q_start = _vector(q_start, torch.int32)
     if T == 0 or R == 0:
         return
+    if max_q_len < 1:
+        _need(False, f"max_q_len {max_q_len} for {T} tokens")
     _launch(dev, _lib.load().sna_kv_store_blocks, "kv_store_blocks", k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), T,
             table.data_ptr(), stride, table.shape[1], _ptr(q_start), prior.data_ptr(), R, min(int(max_q_len), T),
             k_cache.data_ptr(), v_cache.data_ptr(), _ptr(ks), _ptr(vs), tokens, _ptr(k_bounds), nb, G, P, d, code)
@@ -1375,10 +1385,10 @@ def _query_rows(q: Tensor, block_table: Tensor, seq_lens: Tensor, rows: Optional
         if rows.numel() != T or block_table.dim() != 2 or block_table.shape[1] < 1:
             _need(False, f"rows must be [{T}] over a block_table [R, width], got {tuple(rows.shape)} and "
                   f"{tuple(block_table.shape)}")
-        rows = _contig(_as(rows.reshape(-1), torch.int32), "rows")
+        rows = _vector(rows, torch.int32)
     table, stride = _strided_rows(_as(block_table, torch.int32))
     q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
-    return q, table, stride, _contig(_as(seq_lens.reshape(-1), torch.int32), "seq_lens"), rows
+    return q, table, stride, _vector(seq_lens, torch.int32), rows
 
 
 def _block_attention(what, q, k_cache, v_cache, block_table, seq_lens, blocks, sm_scale, k_scale, v_scale, sinks, window, rows,
@@ -1396,11 +1406,11 @@ def _block_attention(what, q, k_cache, v_cache, block_table, seq_lens, blocks, s
         blocks = _contig(_as(blocks, torch.int32), "blocks")
         n = blocks.shape[2]
     if sinks is not None:
-        sinks = _contig(_as(sinks.reshape(-1), torch.float32), "sinks")
+        sinks = _vector(sinks, torch.float32)
         if sinks.shape[0] != H:
             _need(False, f"{sinks.shape[0]} sinks for {H} heads")
     if out is None:
-        out = torch.empty(T, H, d, dtype=torch.bfloat16, device=dev)
+        out = torch.empty_like(q)
     elif out.shape != (T, H, d) or out.dtype != torch.bfloat16 or not out.is_contiguous():
         _need(False, f"out must be contiguous [{T}, {H}, {d}] bf16, got {tuple(out.shape)} {out.dtype}")
     if T == 0:
@@ -1422,8 +1432,8 @@ def paged_decode_blocks(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table
     caches without scales too): query t sees the first seq_lens[t] keys of row t of ``block_table`` [R, width], its own
     token's, stored already, the last of them. With ``rows`` [T] it is row rows[t] instead: several tokens of a row, each at
     a length of its own (a verify step). ``window``: the last so many keys only; ``sinks`` [H] join the softmax
-    denominators. Scales may be expanded (one for all pages, say). A query that sees no key gives zeros. Returns [T, H, d]
-    bf16."""
+    denominators. Scales may be expanded (one for all pages, say). Positions past the table have no key, nor has a row outside
+    it; a query that sees no key gives zeros. Returns [T, H, d] bf16."""
     return _block_attention("paged_decode_blocks", q, k_cache, v_cache, block_table, seq_lens, None, sm_scale, k_scale,
                             v_scale, sinks, window, rows, out)
 
@@ -1468,24 +1478,26 @@ def prefill_attention_blocks(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_
         _need(False, f"block_table must be [{R}, width], got {tuple(block_table.shape)}")
     table, stride = _strided_rows(_as(block_table, torch.int32))
     q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
-    q_start = _contig(_as(q_start.reshape(-1), torch.int32), "q_start")
-    prior = _contig(_as(prior_lens.reshape(-1), torch.int32), "prior_lens")
+    q_start = _vector(q_start, torch.int32)
+    prior = _vector(prior_lens, torch.int32)
     if sinks is not None:
-        sinks = _contig(_as(sinks.reshape(-1), torch.float32), "sinks")
+        sinks = _vector(sinks, torch.float32)
         if sinks.shape[0] != H:
             _need(False, f"{sinks.shape[0]} sinks for {H} heads")
     if out is None:
-        out = torch.empty(T, H, d, dtype=torch.bfloat16, device=dev)
+        out = torch.empty_like(q)
     elif out.shape != (T, H, d) or out.dtype != torch.bfloat16 or not out.is_contiguous():
         _need(False, f"out must be contiguous [{T}, {H}, {d}] bf16, got {tuple(out.shape)} {out.dtype}")
     if T == 0 or R == 0:
         return out
+    if max_q_len < 1:
+        _need(False, f"max_q_len {max_q_len} for {T} queries")
     W, max_q_len, window = table.shape[1], min(int(max_q_len), T), min(int(window), _INT32_MAX)
     need = _prefill_workspace(R, max_q_len, H, G, d, P, W, window)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
     _launch(dev, _lib.load().sna_prefill_attention_blocks, "prefill_attention_blocks", q.data_ptr(), k_cache.data_ptr(),
             v_cache.data_ptr(), _ptr(ks), _ptr(vs), page, head, tokens, table.data_ptr(), stride, W, q_start.data_ptr(),
-            prior.data_ptr(), R, max_q_len, _ptr(sinks), sm_scale, window, out.data_ptr(), H, G, d, P, nb, code, _ptr(ws),
+            prior.data_ptr(), T, R, max_q_len, _ptr(sinks), sm_scale, window, out.data_ptr(), H, G, d, P, nb, code, _ptr(ws),
             need)
     return out
 

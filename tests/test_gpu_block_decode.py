@@ -11,7 +11,7 @@ import torch
 from oracle import blocks as ob
 from oracle import weights as ow
 from sglang_neuron_amd import ops
-from tests._block_cases import FMTS, gen, hide_unstored, pool, table_of, to, tokens
+from tests._block_cases import FMTS, gen, hide_unstored, pool, same_bits, table_of, to, tokens
 from tests.conftest import announce
 
 pytestmark = pytest.mark.gpu
@@ -112,7 +112,8 @@ def test_selected_pages(fmt, H, G, d, P, bt):
     q, kc, vc, ks, vs, table = _case(H + P, lens, H, G, d, P, bt, fmt)
     W, n = table.shape[1], 5
     g = gen(7)
-    lists = torch.stack([torch.stack([torch.randperm(max(W, n), generator=g)[:n] for _ in range(G)]) for _ in lens]).to(torch.int32)
+    lists = [torch.stack([torch.randperm(max(W, n), generator=g)[:n] for _ in range(G)]) for _ in lens]
+    lists = torch.stack(lists).to(torch.int32)
     lists[3, :, 1:3] = -1
     lists[4, 0] = -1
     lists[5, :, 0], lists[5, :, 4] = 0, 2 ** 31 - 1
@@ -243,7 +244,8 @@ def test_scores(H, G, d, P):
     for rr, ll in ((rows, at), (None, lens)):
         qq = q[:len(ll)]
         want, size, counts = ob.scores(qq, bounds, table, ll, P, rr)
-        got, n = ops.block_scores(*to(DEV, qq, bounds, table, _i32(ll)), page_size=P, rows=None if rr is None else _i32(rr).to(DEV))
+        got, n = ops.block_scores(*to(DEV, qq, bounds, table, _i32(ll)), page_size=P,
+                                  rows=None if rr is None else _i32(rr).to(DEV))
         assert n.tolist() == counts
         got = got.cpu().double()
         assert torch.equal(got == -math.inf, want == -math.inf)
@@ -322,7 +324,7 @@ def test_captured_and_replayed():
             want = step(eager)
             torch.cuda.synchronize()
             for a, c in zip((*got, *state), (*want, *eager)):
-                assert torch.equal(a.view(torch.uint8) if a.dtype == ob.FP8 else a, c.view(torch.uint8) if c.dtype == ob.FP8 else c)
+                assert same_bits(a, c)
             for x in (q, k, v):
                 x.copy_(torch.randn(x.shape, generator=g).to(torch.bfloat16))
             lens += 1

@@ -82,6 +82,18 @@ def test_chunks(fmt, G, d, P, bt, slices):
     _check(k, v, caches, scales, table, start, priors, bounds if slices else None, slices=slices)
 
 
+@pytest.mark.parametrize("fmt", list(FMTS))
+def test_one_long_chunk_among_many_tokens(fmt):
+    """The pages there are, counted out among 150 requests (some without tokens) instead of given to each."""
+    announce(f"store mixed {fmt}")
+    R, P = 150, 16
+    priors = [(7 * r) % 50 for r in range(R)]
+    counts = [0 if r % 13 == 5 else 1 for r in range(R)]
+    counts[70], counts[149] = 700, 33
+    k, v, caches, scales, table, start, bounds = _setup(41, R, 2, 64, P, 16, fmt, priors, counts)
+    _check(k, v, caches, scales, table, start, priors, bounds)
+
+
 @pytest.mark.parametrize("fmt", ["fp8", "int8"])
 def test_token_by_token_is_the_block_grown(fmt):
     """40 tokens one at a time, on a pool that held garbage: the scale only grows and every step's codes are as defined."""
