@@ -479,8 +479,8 @@ int sna_prefill_attention_split(const void *q, const void *k_cache, const void *
  *                q_start[r + 1] - 1, at positions prior_lens[r], + 1, ..; q_start NULL: row r is request r's one token.
  *   max_q_len    bounds the requests' tokens (tokens past it are not stored).
  *   scales       contiguous. For each block of a page, KV head and cache that the call writes, with
- *                  fresh = max(max |x| / top, 2^-100), top 448 (FP8) or 127 (int8), over the call's tokens of the block
- *                  (infinities not counted; a NaN makes it NaN),
+ *                  fresh = max(max |x| * r, 2^-100), r the fp32 1 / top, top 448 (FP8) or 127 (int8), over the call's tokens
+ *                  of the block (infinities not counted; a NaN makes it NaN),
  *                the scale becomes fresh where the call writes the block's first token (it starts anew), else the larger of
  *                fresh and what it was. New codes are x / scale, clamped to +-top, to nearest even; where the scale grew, the
  *                block's earlier tokens are rounded again, code * old / new. Tokens behind the written ones stay as they are.

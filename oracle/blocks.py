@@ -58,7 +58,7 @@ def append(cache: Tensor, scale: Optional[Tensor], new: Tensor, table: Tensor, q
             u, head = lo // bt, lo - lo % bt
             f = x.float()
             most = torch.where(f.isinf(), 0.0, f.abs()).amax((1, 2))  # (a NaN makes it NaN)
-            now = (most / top_of(cache.dtype)).clamp(min=LEAST_SCALE)
+            now = (most * (torch.ones(()) / top_of(cache.dtype))).clamp(min=LEAST_SCALE)
             if not first:
                 had = scale[page, :, u].clone()
                 now = torch.maximum(now, had)

@@ -3,7 +3,8 @@
 // for, the pages' key bounds (the least and the largest value of each dimension over a page's keys).
 //
 // For a block (bt tokens, one KV head, K or V apart) that the call writes from its token `lo` on:
-//   fresh = max(max |x| / top, 2^-100) over the call's tokens of the block (infinities not counted; a NaN makes it NaN)
+//   fresh = max(max |x| * (1 / top), 2^-100) over the call's tokens of the block (infinities not counted; a NaN makes it NaN;
+//           the reciprocal rounded, so no division)
 //   scale = fresh where lo = 0 (the block starts anew), else max(fresh, the scale it had)
 //   code  = round(clamp(x / scale)) of the new tokens; where the scale grew, the tokens before lo are rounded again,
 //           round(code * had / scale), so that one scale holds for the block.
@@ -250,7 +251,7 @@ void kv_store_blocks_kernel(BlockStoreArgs a) {
       tame = most < kWild;
       const float amax = bf16_bits_to_f32((uint32_t)most & 0xffffu);
       const float nan_f = __uint_as_float(0x7fc00000u);
-      s = amax != amax ? nan_f : fmaxf(amax / top, kLeastBlockScale);
+      s = amax != amax ? nan_f : fmaxf(amax * (1.0f / top), kLeastBlockScale);
       if (from > head) s = s != s || had != had ? nan_f : fmaxf(s, had);
       rs = 1.0f / s;
       // the block's earlier tokens, where the scale grew, four rows' loads in flight

@@ -1311,7 +1311,7 @@ def kv_store_blocks(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, bloc
 
     The caches hold float8_e4m3fn or int8 codes, with k_scale, v_scale [blocks, G, page / tokens] fp32 that the call keeps up:
     a code is worth code * the scale of its block of ``tokens`` tokens and KV head. A block's scale is its largest magnitude
-    over 448 or 127 (at least 2^-100): it starts anew with the block's first token and grows when a larger token comes, and the
+    times 1 / 448 or 1 / 127 (at least 2^-100): it starts anew with the block's first token and grows when a larger token comes, and the
     block's earlier tokens are then rounded again. (Infinities are clamped and do not count; a NaN makes the scale, so the
     block, NaN.) bf16 caches have no scales. ``k_bounds`` [blocks, G, 2, d] bf16, when given, is kept up as well: the least and
     the largest value of each dimension over a page's keys (block_scores reads it).
