@@ -116,6 +116,7 @@ SIGNATURES = {
     "sna_block_decode_workspace_bytes": (_I64, [_I32] * 8),
     "sna_paged_decode_blocks": (_I32, [_P, _P, _P, _P, _P, _I64, _I64, _I32, _P, _I64, _I32, _I32, _P, _P, _P, _I32, _P,
                                        _I32, _F32, _P, _I32, _I32, _I32, _I32, _I32, _I64, _I32, _P, _I64, _P]),
+    "sna_prefill_blocks_workspace_bytes": (_I64, [_I32] * 10),
     "sna_prefill_attention_blocks": (_I32, [_P, _P, _P, _P, _P, _I64, _I64, _I32, _P, _I64, _I32, _P, _P, _I32, _I32, _I32, _P,
                                             _F32, _I32, _P, _I32, _I32, _I32, _I32, _I64, _I32, _P, _I64, _P]),
     "sna_block_scores": (_I32, [_P, _P, _P, _I64, _I32, _I32, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I64, _P]),

@@ -886,9 +886,10 @@ __global__ __launch_bounds__(256) void prefill_combine_kernel(PrefillArgs a, boo
 // that the power limit allows by themselves: 352 blocks of up to 136 tiles took 201 us whole, 206 in a split launch; 376
 // of up to 24 tiles 36 and 42; requests of unequal lengths would gain, which the host does not know), too short (the
 // search and the merge launch), or past what the split counts.
-static int32_t prefill_split_slots(int64_t qblocks, int32_t R, int32_t G, int64_t bound_tiles) {
-  const int64_t base = qblocks * R * G;
-  if (base > kPrefillSplitBlocks || bound_tiles <= kPrefillNoSplit || bound_tiles > kPrefillSplitMaxTiles) return 0;
+// `most`: a bound of the batch's query blocks, qblocks * R where nothing better is known.
+static int32_t prefill_split_slots(int64_t qblocks, int32_t R, int32_t G, int64_t bound_tiles, int64_t most) {
+  const int64_t base = std::min(qblocks * R, most) * G;
+  if (base > kPrefillSplitBlocks || qblocks * R > kPrefillSplitPairs || bound_tiles <= kPrefillNoSplit || bound_tiles > kPrefillSplitMaxTiles) return 0;
   static_assert(kPrefillSplitPairs >= kPrefillSplitBlocks, "a split launch's pairs fit a wave");
   return (int32_t)std::min<int64_t>(kPrefillSlots, base * ((bound_tiles + kPrefillMinSplit - 1) / kPrefillMinSplit));
 }
@@ -906,11 +907,13 @@ int64_t prefill_bound_tiles(int32_t table_width, int32_t page_size, int32_t wind
   return (span + kPrefillTile - 1) / kPrefillTile;
 }
 
-int32_t split_slots_of(int32_t R, int32_t max_q_len, int32_t num_q_heads, int32_t num_kv_heads, int32_t page_size,
-                       int32_t table_width, int32_t window) {
+// (n_queries: of the whole batch, -1 where the caller does not say)
+int32_t split_slots_of(int32_t n_queries, int32_t R, int32_t max_q_len, int32_t num_q_heads, int32_t num_kv_heads,
+                       int32_t page_size, int32_t table_width, int32_t window) {
   const int32_t bq = kPrefillRows / (num_q_heads / num_kv_heads);
   const int64_t qblocks = ((int64_t)max_q_len + bq - 1) / bq;
-  return prefill_split_slots(qblocks, R, num_kv_heads, prefill_bound_tiles(table_width, page_size, window, bq));
+  const int64_t most = n_queries < 0 ? qblocks * R : (int64_t)n_queries / bq + R;
+  return prefill_split_slots(qblocks, R, num_kv_heads, prefill_bound_tiles(table_width, page_size, window, bq), most);
 }
 
 int64_t split_workspace_bytes(int32_t slots, int32_t R, int32_t max_q_len, int32_t num_q_heads, int32_t num_kv_heads,
@@ -1021,7 +1024,7 @@ static int prefill_attention(const char* what, const PrefillScales* scales, bool
   a.slots = 0;
   a.ws_o = a.ws_ml = nullptr;
   a.ws_item = nullptr;
-  const int32_t slots = workspace ? split_slots_of(R, max_q_len, num_q_heads, num_kv_heads, page_size, table_width,
+  const int32_t slots = workspace ? split_slots_of(scales ? scales->n_queries : -1, R, max_q_len, num_q_heads, num_kv_heads, page_size, table_width,
                                                    window) : 0;
   if (slots > 0) {
     const int64_t need = split_workspace_bytes(slots, R, max_q_len, num_q_heads, num_kv_heads, head_dim);
@@ -1070,14 +1073,28 @@ extern "C" int sna_prefill_attention(const void* q, const void* k_cache, const v
                            num_q_heads, num_kv_heads, head_dim, page_size, num_blocks, kv_dtype, nullptr, 0, stream);
 }
 
-extern "C" int64_t sna_prefill_workspace_bytes(int32_t R, int32_t max_q_len, int32_t num_q_heads, int32_t num_kv_heads,
-                                               int32_t head_dim, int32_t page_size, int32_t table_width,
-                                               int32_t window) {
+static int64_t prefill_workspace(int32_t n_queries, int32_t R, int32_t max_q_len, int32_t num_q_heads,
+                                 int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int32_t table_width,
+                                 int32_t window) {
   if (R < 1 || max_q_len < 1 || num_q_heads < 1 || num_kv_heads < 1 || num_q_heads % num_kv_heads != 0 ||
       num_q_heads / num_kv_heads > kPrefillRows || head_dim < 1 || page_size < 1 || table_width < 1 || window < 0)
     return 0;
-  const int32_t slots = split_slots_of(R, max_q_len, num_q_heads, num_kv_heads, page_size, table_width, window);
+  const int32_t slots = split_slots_of(n_queries, R, max_q_len, num_q_heads, num_kv_heads, page_size, table_width, window);
   return slots > 0 ? split_workspace_bytes(slots, R, max_q_len, num_q_heads, num_kv_heads, head_dim) : 0;
+}
+
+extern "C" int64_t sna_prefill_workspace_bytes(int32_t R, int32_t max_q_len, int32_t num_q_heads, int32_t num_kv_heads,
+                                               int32_t head_dim, int32_t page_size, int32_t table_width,
+                                               int32_t window) {
+  return prefill_workspace(-1, R, max_q_len, num_q_heads, num_kv_heads, head_dim, page_size, table_width, window);
+}
+
+extern "C" int64_t sna_prefill_blocks_workspace_bytes(int32_t n_queries, int32_t R, int32_t max_q_len,
+                                                      int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                                      int32_t page_size, int32_t table_width, int32_t window,
+                                                      int32_t cache_dtype) {
+  return prefill_workspace(cache_dtype == SNA_DTYPE_BF16 ? -1 : std::max(n_queries, 0), R, max_q_len, num_q_heads,
+                           num_kv_heads, head_dim, page_size, table_width, window);
 }
 
 extern "C" int sna_prefill_attention_split(const void* q, const void* k_cache, const void* v_cache,

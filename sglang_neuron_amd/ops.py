@@ -1451,8 +1451,8 @@ def paged_decode_selected(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tab
 
 @functools.lru_cache(maxsize=1024)
 def _prefill_workspace(*sizes: int) -> int:
-    """sna_prefill_workspace_bytes, a function of sizes alone."""
-    return _lib.load().sna_prefill_workspace_bytes(*sizes)
+    """sna_prefill_blocks_workspace_bytes, a function of sizes alone."""
+    return _lib.load().sna_prefill_blocks_workspace_bytes(*sizes)
 
 
 def prefill_attention_blocks(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, q_start: Tensor,
@@ -1493,7 +1493,7 @@ def prefill_attention_blocks(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_
     if max_q_len < 1:
         _need(False, f"max_q_len {max_q_len} for {T} queries")
     W, max_q_len, window = table.shape[1], min(int(max_q_len), T), min(int(window), _INT32_MAX)
-    need = _prefill_workspace(R, max_q_len, H, G, d, P, W, window)
+    need = _prefill_workspace(T, R, max_q_len, H, G, d, P, W, window, code)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
     _launch(dev, _lib.load().sna_prefill_attention_blocks, "prefill_attention_blocks", q.data_ptr(), k_cache.data_ptr(),
             v_cache.data_ptr(), _ptr(ks), _ptr(vs), page, head, tokens, table.data_ptr(), stride, W, q_start.data_ptr(),
