@@ -152,6 +152,9 @@ __device__ __forceinline__ PrefillBlock prefill_block(const PrefillArgs& a, int3
 // up to one workgroup a CU and 2 us with two (the card's power limit holds the chip to some 270 tiles a microsecond),
 // the partials of 32 items 1 us of the launch and the merge pass 5 us. w numbers the items KV head by KV head, then pair
 // by pair (request-major), a pair's splits in order. Every lane gets the same values; false past the last item.
+// HALF: partials of half that size (block scales at head dim 64; 24 / 4 heads, int8, 3 chunks of up to 635 after up to 1635: 53.0
+// -> 45.7 us).
+template <bool HALF>
 __device__ bool prefill_item(const PrefillArgs& a, int32_t& w, int32_t& g, int32_t& r, int32_t& bx, int32_t& split,
                              int32_t& st_out, int32_t& ns) {
   constexpr int N = kPrefillSplitPairs / 64;
@@ -208,7 +211,8 @@ __device__ bool prefill_item(const PrefillArgs& a, int32_t& w, int32_t& g, int32
     }
   // tenths of a microsecond, in 64 bits
   const int64_t whole = (int64_t)mx * 13;  // (at most one block a CU)
-  const int64_t cut = (int64_t)st * (per_head * a.G > kPrefillSlots / 2 ? 20 : 13) + 50 + per_head * a.G * 10 / 32;
+  const int64_t merge = HALF ? 40 + per_head * a.G * 10 / 64 : 50 + per_head * a.G * 10 / 32;
+  const int64_t cut = (int64_t)st * (per_head * a.G > kPrefillSlots / 2 ? 20 : 13) + merge;
   if (cut >= whole) {
     st = (uint32_t)max(mx, 1), rst = 1.0f / (float)st;
     per_head = blocks;
@@ -297,7 +301,7 @@ void prefill_gqa_kernel(PrefillArgsOf<SCALES> a) {
   int32_t bx, r, g, split = 0, split_tiles = 0, ns = 1, item = 0, note = -1;
   if constexpr (SPLIT) {
     // the same in every lane: made scalar, so what is addressed with them stays in scalar registers
-    if (!__builtin_amdgcn_readfirstlane((int)prefill_item(a, item, g, r, bx, split, split_tiles, ns))) return;
+    if (!__builtin_amdgcn_readfirstlane((int)prefill_item<BLK && D == 64>(a, item, g, r, bx, split, split_tiles, ns))) return;
     g = __builtin_amdgcn_readfirstlane(g), r = __builtin_amdgcn_readfirstlane(r);
     bx = __builtin_amdgcn_readfirstlane(bx), split = __builtin_amdgcn_readfirstlane(split);
     split_tiles = __builtin_amdgcn_readfirstlane(split_tiles), ns = __builtin_amdgcn_readfirstlane(ns);
