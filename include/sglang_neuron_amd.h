@@ -506,11 +506,12 @@ int sna_kv_store_blocks(const void *k, const void *v, int64_t k_row_stride, int6
  *                head contiguous.
  *   sinks        [num_q_heads] fp32 logits joining the softmax denominator, or NULL.
  *   out          [T, num_q_heads, head_dim] bf16, 4-byte aligned; a query that sees no key gives zeros.
- *   workspace    device, 16-byte aligned, sna_block_decode_workspace_bytes bytes (n_blocks 0: no list), any contents; calls
- *                that share one on different streams race.
+ *   workspace    device, 16-byte aligned, sna_block_decode_workspace_bytes bytes (n_blocks 0: no list; table_rows 0
+ *                unless rows and blocks are both given), any contents; calls that share one on different streams race.
  * num_q_heads / num_kv_heads <= 16. The same call gives the same bits. */
 int64_t sna_block_decode_workspace_bytes(int32_t T, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-                                         int32_t page_size, int32_t table_width, int32_t window, int32_t n_blocks);
+                                         int32_t page_size, int32_t table_width, int32_t table_rows, int32_t window,
+                                         int32_t n_blocks);
 int sna_paged_decode_blocks(const void *q, const void *k_cache, const void *v_cache, const float *k_scale,
                             const float *v_scale, int64_t scale_page_stride, int64_t scale_head_stride,
                             int32_t scale_tokens, const int32_t *block_table, int64_t table_stride, int32_t table_width,
@@ -521,8 +522,9 @@ int sna_paged_decode_blocks(const void *q, const void *k_cache, const void *v_ca
                             void *stream);
 
 /* sna_prefill_attention_split over such a pool: a batch of chunks, causal. Scales as in sna_paged_decode_blocks, the rest,
- * as in sna_prefill_attention_split, with a workspace of sna_prefill_blocks_workspace_bytes bytes. A query that sees no key gives zeros.
- * With int8 codes a query element is taken to within 2^-16 of its row's largest. n_queries: q's rows (q_start[R]). */
+ * as in sna_prefill_attention_split, with a workspace of sna_prefill_blocks_workspace_bytes bytes. A query that sees no
+ * key gives zeros. With int8 codes a query element is taken to within 2^-16 of its row's largest. n_queries: q's rows
+ * (q_start[R]). */
 int64_t sna_prefill_blocks_workspace_bytes(int32_t n_queries, int32_t R, int32_t max_q_len, int32_t num_q_heads,
                                            int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
                                            int32_t table_width, int32_t window, int32_t cache_dtype);
@@ -530,7 +532,8 @@ int sna_prefill_attention_blocks(const void *q, const void *k_cache, const void 
                                  const float *v_scale, int64_t scale_page_stride, int64_t scale_head_stride,
                                  int32_t scale_tokens, const int32_t *block_table, int64_t table_stride,
                                  int32_t table_width, const int32_t *q_start, const int32_t *prior_lens,
-                                 int32_t n_queries, int32_t R, int32_t max_q_len, const float *sinks, float sm_scale, int32_t window, void *out,
+                                 int32_t n_queries, int32_t R, int32_t max_q_len, const float *sinks, float sm_scale,
+                                 int32_t window, void *out,
                                  int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
                                  int64_t num_blocks, int32_t cache_dtype, void *workspace, int64_t workspace_bytes,
                                  void *stream);

@@ -45,7 +45,8 @@ struct BlockDecodeArgs {
   int64_t num_blocks;
   int32_t window;
   float sm_scale;
-  int32_t splits;  // of a query's tiles
+  int32_t splits;  // of a query's tiles; of a launch page by page n_blocks * segs: a partial for each listed page's 64 keys
+  int32_t segs;    // page by page: runs of 64 keys of a page
   float* ws_o;     // [T, splits, H, D] unnormalized partials
   float* ws_ml;    // [T, splits, H, 2] reference max (log2 domain) and softmax sum
   uint16_t* out;
@@ -102,6 +103,28 @@ struct BlockTile {
   int32_t pos[2];  // the halves' first positions
   bool valid[2];   // on a page of the pool, below the table's width
 };
+
+// The operand of a 16-wide d-tile of V^T over a tile's 32 keys, regrouped in registers: byte or element dt of each key's run.
+template <int D, int FMT>
+__device__ __forceinline__ void block_v_op(const BlockTile<D, FMT>& T, int dt, uint32_t (&op)[4]) {
+  if constexpr (FMT == kBlockBf16) {
+#pragma unroll
+    for (int pr = 0; pr < 4; ++pr) {
+      const uint32_t e0 = (T.v[2 * pr][dt >> 1] >> (16 * (dt & 1))) & 0xffffu;
+      const uint32_t e1 = (T.v[2 * pr + 1][dt >> 1] >> (16 * (dt & 1))) & 0xffffu;
+      op[pr] = e0 | (e1 << 16);
+    }
+  } else {
+    uint32_t c0 = 0, c1 = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      c0 |= ((T.v[e][dt >> 2] >> (8 * (dt & 3))) & 0xffu) << (8 * e);
+      c1 |= ((T.v[e + 4][dt >> 2] >> (8 * (dt & 3))) & 0xffu) << (8 * e);
+    }
+    codes_to_bf16x4<FMT>(c0, op[0], op[1]);
+    codes_to_bf16x4<FMT>(c1, op[2], op[3]);
+  }
+}
 
 // SHARED: queries of one row, which read the same pages, may be among the call's (`rows`). V then stays in the L2 (2 x 256
 // queries of 1024 selected keys, bf16: 178 -> 152 us); else it is read once, past it (64 rows of 4096 FP8 keys 87.5 us, through
@@ -304,23 +327,7 @@ void block_decode_kernel(BlockDecodeArgs a) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       uint32_t op[4];
-      if constexpr (FMT == kBlockBf16) {
-#pragma unroll
-        for (int pr = 0; pr < 4; ++pr) {
-          const uint32_t e0 = (T.v[2 * pr][dt >> 1] >> (16 * (dt & 1))) & 0xffffu;
-          const uint32_t e1 = (T.v[2 * pr + 1][dt >> 1] >> (16 * (dt & 1))) & 0xffffu;
-          op[pr] = e0 | (e1 << 16);
-        }
-      } else {
-        uint32_t c0 = 0, c1 = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          c0 |= ((T.v[e][dt >> 2] >> (8 * (dt & 3))) & 0xffu) << (8 * e);
-          c1 |= ((T.v[e + 4][dt >> 2] >> (8 * (dt & 3))) & 0xffu) << (8 * e);
-        }
-        codes_to_bf16x4<FMT>(c0, op[0], op[1]);
-        codes_to_bf16x4<FMT>(c1, op[2], op[3]);
-      }
+      block_v_op<D, FMT>(T, dt, op);
       acc[dt] = mfma_16x16x32_bf16(op, pop, acc[dt]);
     }
   };
@@ -378,10 +385,275 @@ void block_decode_kernel(BlockDecodeArgs a) {
   }
 }
 
+// Page by page, for many queries of few rows (a prompt's, each with pages of its own choice): a workgroup finds the queries
+// whose lists name one of four pages of a row, for one KV head and 64 keys of the page, keeps a page's keys as operands in
+// registers and attends 16 / group queries at a time to them, so a page is read once, not once a query, and the columns are full. A
+// partial is written for each entry of the lists and merged as splits are. Latency bounds it: a page's operands take all the
+// registers that two waves a SIMD have, and each batch waits for its queries (2 x 256 queries of 16 pages of 64, bf16, group 2:
+// 107 us of which the merge 22; one page a workgroup 137, most of it in searching the lists once for each).
+constexpr int kPageWaves = 4;  // and pages
+constexpr int kPageScan = 8;   // entries that a thread reads at a time
+constexpr int kPageStep = kPageScan * 64 * kPageWaves, kPageList = kPageStep + 1024;
+template <int D, int FMT>
+__global__ __launch_bounds__(64 * kPageWaves) __attribute__((amdgpu_waves_per_eu(2)))
+void block_pages_kernel(BlockDecodeArgs a) {
+  using Tile = BlockTile<D, FMT>;
+  constexpr int ESZ = Tile::ESZ, KB = Tile::KB, VB = Tile::VB, STEPS = D / 32, VE = D / 16, DT = D / 16, CE = 16 / ESZ;
+  const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, li = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  uint32_t idx = blockIdx.x;
+  const int32_t g = (int32_t)(idx % (uint32_t)a.G);
+  idx /= (uint32_t)a.G;
+  const int32_t seg = (int32_t)(idx % (uint32_t)a.segs);
+  idx /= (uint32_t)a.segs;
+  const uint32_t quads = ((uint32_t)a.table_width + kPageWaves - 1) / kPageWaves;
+  const int32_t c0 = (int32_t)(idx % quads) * kPageWaves, row = (int32_t)(idx / quads);
+  const int32_t keys = min(a.P - 64 * seg, 64);  // of a page's, this workgroup's
+
+  // By page: the entries t * n_blocks + i of the lists that name it, of queries that see all of the keys from the front, of
+  // queries that see some of them from the end; how many, how many of them waves have taken, the most keys that one of the
+  // latter sees.
+  __shared__ int32_t sm_e[kPageWaves][kPageList], sm_n[kPageWaves][2], sm_taken[kPageWaves][2], sm_vis[kPageWaves];
+  __shared__ int32_t sm_hit[kPageStep], sm_page[kPageWaves], sm_hits, sm_first, sm_end;
+  if (tid < kPageWaves) {
+    int32_t page = c0 + tid < a.table_width ? a.table[(int64_t)row * a.table_stride + c0 + tid] : -1;
+    if ((int64_t)page >= a.num_blocks) page = -1;
+    sm_page[tid] = page;
+    sm_n[tid][0] = sm_n[tid][1] = sm_taken[tid][0] = sm_taken[tid][1] = sm_vis[tid] = 0;
+    if (tid == 0) sm_hits = 0, sm_first = INT32_MAX, sm_end = 0;
+  }
+  __syncthreads();
+  {  // the row's queries lie in [sm_first, sm_end)
+    int32_t lo = INT32_MAX, hi = 0;
+    for (int32_t t = tid; t < a.T; t += 64 * kPageWaves)
+      if (a.rows[t] == row) lo = min(lo, t), hi = t + 1;
+    if (hi > 0) atomicMin(&sm_first, lo), atomicMax(&sm_end, hi);
+  }
+  __syncthreads();
+  const int32_t t_first = sm_first, t_end = sm_end;
+  if (t_end == 0) return;
+  auto seen = [&](int32_t t, int32_t c) { return block_len(a, a.seq_lens[t]) - (c0 + c) * a.P - 64 * seg; };
+
+  // The keys as operands in bf16: 16 keys (rows) of K by 32 of D, 16 of D by 32 keys of V. V of keys from `vis` on is zero (what
+  // was never stored may be anything).
+  struct Keys {
+    uint32_t k_op[4][STEPS][4], v_op[2][DT][4];
+    float scales[2];
+  };
+  // scales: of both tiles, in the lanes of the format's decode: K's at 0 and 16, V's at 32 and 48
+  const uint32_t k_off = (uint32_t)(li * D * ESZ + 16 * g4), v_off = (uint32_t)(4 * g4 * D * ESZ + VB * li);
+  const float* scale_base = FMT == kBlockBf16 ? nullptr : (g4 < 2 ? a.k_scale : a.v_scale) + g * a.scale_head;
+  auto load = [&](Keys& o, int32_t c, int32_t vis) {
+    const int32_t page = __builtin_amdgcn_readfirstlane(sm_page[c]);
+    const int64_t at0 = (((int64_t)page * a.G + g) * a.P + 64 * seg) * D * ESZ;
+    Tile T[2];
+#pragma unroll
+    for (int tl = 0; tl < 2; ++tl) {
+      int32_t sub[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int32_t half = 2 * tl + hf;
+        const bool in = 16 * half < keys;  // (uniform; past the page: the first half again, which is masked)
+        const uint8_t* kp = a.k_cache + at0 + (int64_t)(in ? 16 * half : 0) * D * ESZ;
+        const uint8_t* vp = a.v_cache + at0 + (int64_t)(in ? 16 * half : 0) * D * ESZ;
+        sub[hf] = (int32_t)((uint32_t)(4 * seg + (in ? half : 0)) * (uint32_t)a.sub_magic >> 16);
+#pragma unroll
+        for (int c4 = 0; c4 < KB / 16; ++c4) {
+          const uint4 w = ld16(kp + k_off + 64 * c4);
+          T[tl].k[hf][4 * c4] = w.x, T[tl].k[hf][4 * c4 + 1] = w.y, T[tl].k[hf][4 * c4 + 2] = w.z, T[tl].k[hf][4 * c4 + 3] = w.w;
+        }
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) load_run<VB, false>(vp + v_off + e4 * D * ESZ, T[tl].v[4 * hf + e4]);
+      }
+      if constexpr (FMT != kBlockBf16)
+        o.scales[tl] = scale_base[(int64_t)page * a.scale_page + (g4 & 1 ? sub[1] : sub[0])];
+    }
+#pragma unroll
+    for (int tl = 0; tl < 2; ++tl) {
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < VB / 4; ++i)
+            T[tl].v[4 * hf + r][i] = 32 * tl + 16 * hf + 4 * g4 + r < vis ? T[tl].v[4 * hf + r][i] : 0u;
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+          uint32_t(&op)[4] = o.k_op[2 * tl + hf][st];
+          if constexpr (FMT == kBlockBf16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) op[i] = T[tl].k[hf][4 * st + i];
+          } else {
+            codes_to_bf16x4<FMT>(T[tl].k[hf][2 * st], op[0], op[1]);
+            codes_to_bf16x4<FMT>(T[tl].k[hf][2 * st + 1], op[2], op[3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) block_v_op<D, FMT>(T[tl], dt, o.v_op[tl][dt]);
+    }
+  };
+
+  const float qk_scale = a.sm_scale * kLog2e;
+  // Columns [0, tpi * group): n entries from e0 on. What a query does not see counts nothing, except that a NaN or an infinity
+  // among it becomes NaN: false, and nothing is written, if `check` and the result holds one.
+  auto attend = [&](const Keys& o, int32_t c, int part, int32_t e0, int32_t n, bool check) -> bool {
+    const int32_t ce = li / a.group, hc = li - ce * a.group;
+    const bool live = ce < n;
+    const int32_t e = sm_e[c][part ? kPageList - 1 - e0 - (live ? ce : 0) : e0 + (live ? ce : 0)], t = e / a.n_blocks;
+    const int32_t vis = part ? seen(t, c) : keys;
+    uint32_t qv[STEPS][4];
+    const uint16_t* qp = a.q + ((int64_t)t * a.H + g * a.group + hc) * D;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const uint4 w = ld16(qp + CE * (4 * (8 * s / CE) + g4) + (8 * s) % CE);
+      qv[s][0] = w.x, qv[s][1] = w.y, qv[s][2] = w.z, qv[s][3] = w.w;
+    }
+    float x[2][8], m = kNegBig;
+#pragma unroll
+    for (int h4 = 0; h4 < 4; ++h4) {
+      float ks = qk_scale;
+      if constexpr (FMT != kBlockBf16)
+        ks *= __int_as_float(__builtin_amdgcn_readlane(__float_as_int(o.scales[h4 / 2]), 16 * (h4 & 1)));
+      f32x4_t sc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st) sc = mfma_16x16x32_bf16(o.k_op[h4][st], qv[st], sc);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float& y = x[h4 / 2][4 * (h4 & 1) + r];
+        y = 16 * h4 + 4 * g4 + r < vis ? sc[r] * ks : -INFINITY;
+        m = fmaxf(m, y);
+      }
+    }
+    m = max_across_groups(m);
+    float l = 0.0f;
+    f32x4_t acc[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int tl = 0; tl < 2; ++tl) {
+      uint32_t pop[4];  // (rounded and summed as in block_decode_kernel)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        float v = 1.0f, part_l = 0.0f;
+        if constexpr (FMT != kBlockBf16) {
+          v = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(o.scales[tl]), 32 + 16 * hf));
+          v = 32 * tl + 16 * hf >= vis ? 1.0f : v < kLeastBlockScale ? kLeastBlockScale : v;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float p0 = __builtin_amdgcn_exp2f(x[tl][4 * hf + 2 * k] - m);
+          float p1 = __builtin_amdgcn_exp2f(x[tl][4 * hf + 2 * k + 1] - m);
+          if constexpr (FMT != kBlockBf16) p0 *= v, p1 *= v;
+          pop[2 * hf + k] = pack_bf16x2(p0, p1);
+          part_l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pop[2 * hf + k]),
+                                                   __builtin_bit_cast(bf16x2_t, 0x3f803f80u), part_l, false);
+        }
+        l = FMT != kBlockBf16 ? fmaf(part_l, __builtin_amdgcn_rcpf(v), l) : l + part_l;
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma_16x16x32_bf16(o.v_op[tl][dt], pop, acc[dt]);
+    }
+    l = sum_across_groups(l);
+    bool nan = false;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) nan = nan || acc[dt][r] != acc[dt][r];
+    const bool redo = __builtin_amdgcn_readfirstlane((int)(check && __any(nan && live)));
+    if (live && !redo) {
+      const int64_t at = ((int64_t)e * a.segs + seg) * a.H + g * a.group + hc;
+      float* wo = a.ws_o + at * D;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int d4 = 0; d4 < VE; d4 += 4)
+          *reinterpret_cast<f32x4_t*>(wo + VE * (4 * g4 + r) + d4) =
+              f32x4_t{acc[d4][r], acc[d4 + 1][r], acc[d4 + 2][r], acc[d4 + 3][r]};
+      if (g4 == 0) *reinterpret_cast<float2*>(a.ws_ml + 2 * at) = make_float2(m, l);
+    }
+    return !redo;
+  };
+
+  const int32_t tpi = 16 / a.group;
+  constexpr int kStep = 64 * kPageWaves;
+  const int32_t entries = t_end * a.n_blocks, step_t = kStep / a.n_blocks, step_i = kStep % a.n_blocks;
+  int32_t t = t_first + tid / a.n_blocks, i = tid % a.n_blocks;
+  for (int32_t e0 = t_first * a.n_blocks; e0 < entries; e0 += kPageStep) {  // uniform in the workgroup
+    int32_t named[kPageScan];
+#pragma unroll
+    for (int u = 0; u < kPageScan; ++u) {
+      named[u] = t < t_end ? a.blocks[((int64_t)t * a.G + g) * a.n_blocks + i] : -1;
+      t += step_t, i += step_i;
+      if (i >= a.n_blocks) i -= a.n_blocks, ++t;
+    }
+#pragma unroll
+    for (int u = 0; u < kPageScan; ++u)
+      if (named[u] >= c0 && named[u] < c0 + kPageWaves)
+        sm_hit[atomicAdd(&sm_hits, 1)] = (u * kStep + tid) * kPageWaves + named[u] - c0;
+    __syncthreads();
+    for (int32_t h = tid; h < sm_hits; h += kStep) {
+      const int32_t c = sm_hit[h] % kPageWaves, e = e0 + sm_hit[h] / kPageWaves, th = e / a.n_blocks;
+      const int32_t r = a.rows[th], vis = seen(th, c);
+      if (r != row || vis <= 0 || sm_page[c] < 0) continue;
+      if (vis >= keys) {
+        sm_e[c][atomicAdd(&sm_n[c][0], 1)] = e;
+      } else {
+        sm_e[c][kPageList - 1 - atomicAdd(&sm_n[c][1], 1)] = e;
+        atomicMax(&sm_vis[c], vis);
+      }
+    }
+    __syncthreads();
+    bool flush = e0 + kPageStep >= entries;
+#pragma unroll
+    for (int c = 0; c < kPageWaves; ++c) flush = flush || sm_n[c][0] + sm_n[c][1] > kPageList - kPageStep;
+    if (tid == 0) sm_hits = 0;
+    if (flush) {
+      // The wave's next batch, of its own page first, then of the others: page c, its keys that V holds, entries from f on. After
+      // one with a NaN the same entry by entry (alone >= 0).
+      int32_t k = 0, c = 0, vis = 0, part = 0, f = 0, n = 0, alone = -1;
+      auto next = [&](bool ok) {
+        if (!ok) {
+          alone = 0;
+        } else if (alone < 0 || ++alone >= n) {
+          alone = -1, n = 0;
+          for (; k < 2 * kPageWaves; ++k) {
+            c = (wave + k / 2) % kPageWaves, part = k & 1;
+            const int32_t count = __builtin_amdgcn_readfirstlane(sm_n[c][part]);
+            if (count == 0) continue;
+            f = __builtin_amdgcn_readfirstlane(lane == 0 ? atomicAdd(&sm_taken[c][part], tpi) : 0);
+            n = min(tpi, count - f);
+            if (n > 0) break;
+          }
+          if (k == 2 * kPageWaves) return;
+        }
+        vis = __builtin_amdgcn_readfirstlane(alone >= 0 ? seen(sm_e[c][kPageList - 1 - f - alone] / a.n_blocks, c)
+                                             : part     ? sm_vis[c]
+                                                        : keys);
+      };
+      next(true);
+      while (k < 2 * kPageWaves) {
+        Keys o;
+        const int32_t at_c = c, at_vis = vis;
+        load(o, c, vis);
+        do {
+          next(attend(o, c, part, f + max(alone, 0), alone < 0 ? n : 1, part > 0 && alone < 0));
+        } while (k < 2 * kPageWaves && c == at_c && vis == at_vis);
+      }
+      __syncthreads();
+      if (tid < 2 * kPageWaves) (&sm_n[0][0])[tid] = 0, (&sm_taken[0][0])[tid] = 0;
+      if (tid < kPageWaves) sm_vis[tid] = 0;
+    }
+    __syncthreads();
+  }
+}
+
 // Merge of a query's splits, one workgroup per (query, head): out = sum_s e_s o_s / (sum_s e_s l_s + e_sink), e_s =
 // exp2(m_s - M). D / 4 lanes take a split's row in 16-byte pieces, 1024 / D splits at a time, each such group of lanes with a
 // running (M, l, o) of its own; the groups are merged in LDS.
-template <int D>
+// PAGES: split s is the keys 64 (s % segs) .. of the page that entry s / segs of the list names, and was written where the query
+// sees some of them.
+template <int D, bool PAGES>
 __global__ __launch_bounds__(256) void block_combine_kernel(BlockDecodeArgs a) {
   constexpr int LR = D / 4, NG = 256 / LR, CH = 4;
   const int32_t t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, gi = tid / LR, d = 4 * (tid % LR);
@@ -389,6 +661,17 @@ __global__ __launch_bounds__(256) void block_combine_kernel(BlockDecodeArgs a) {
   const int64_t at0 = (int64_t)t * ns * a.H + h;
   const float* wo = a.ws_o + at0 * D + d;
   const float* ml = a.ws_ml + 2 * at0;
+  const int32_t g = h / a.group, row = PAGES ? a.rows[t] : 0;
+  const bool row_ok = row >= 0 && row < a.table_rows;
+  const int32_t L = PAGES && row_ok ? block_len(a, a.seq_lens[t]) : 0;
+  const int32_t* list = PAGES ? a.blocks + ((int64_t)t * a.G + g) * a.n_blocks : nullptr;
+  auto written = [&](int32_t s) -> bool {
+    if (!PAGES) return true;
+    const int32_t e = s / a.segs, c = list[e];
+    if (c < 0 || c >= a.table_width || L - c * a.P - 64 * (s - e * a.segs) <= 0) return false;
+    const int32_t page = a.table[(int64_t)row * a.table_stride + c];
+    return page >= 0 && (int64_t)page < a.num_blocks;
+  };
   float M = kNegBig, l = 0.0f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   for (int32_t s0 = gi; s0 < ns; s0 += NG * CH) {
@@ -396,9 +679,11 @@ __global__ __launch_bounds__(256) void block_combine_kernel(BlockDecodeArgs a) {
     float2 w[CH];
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      const int64_t s = (int64_t)min(s0 + NG * k, ns - 1) * a.H;
+      const int32_t si = min(s0 + NG * k, ns - 1);
+      const int64_t s = (int64_t)si * a.H;
       x[k] = *reinterpret_cast<const f32x4_t*>(wo + s * D);
       w[k] = *reinterpret_cast<const float2*>(ml + 2 * s);
+      if (PAGES && (!written(si) || w[k].y == 0.0f)) x[k] = f32x4_t{0.f, 0.f, 0.f, 0.f}, w[k] = make_float2(kNegBig, 0.0f);
     }
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
@@ -437,7 +722,7 @@ static void launch_block_decode(const BlockDecodeArgs& a, int32_t waves, hipStre
   if (a.splits > 1) {
     if (waves == 4) hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, true, 4, SHARED>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, true, 8, SHARED>), grid, dim3(512), 0, s, a);
-    hipLaunchKernelGGL((block_combine_kernel<D>), dim3(a.T, a.H), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((block_combine_kernel<D, false>), dim3(a.T, a.H), dim3(256), 0, s, a);
   } else {
     if (waves == 4) hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, false, 4, SHARED>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, false, 8, SHARED>), grid, dim3(512), 0, s, a);
@@ -446,7 +731,12 @@ static void launch_block_decode(const BlockDecodeArgs& a, int32_t waves, hipStre
 
 template <int D, int FMT>
 static void launch_block_decode_form(const BlockDecodeArgs& a, int32_t waves, hipStream_t s) {
-  if (a.rows) {
+  if (a.segs > 0) {
+    const int32_t quads = (a.table_width + kPageWaves - 1) / kPageWaves;
+    hipLaunchKernelGGL((block_pages_kernel<D, FMT>), dim3((uint32_t)(a.table_rows * quads * a.segs * a.G)), dim3(64 * kPageWaves),
+                       0, s, a);
+    hipLaunchKernelGGL((block_combine_kernel<D, true>), dim3(a.T, a.H), dim3(256), 0, s, a);
+  } else if (a.rows) {
     if (a.blocks) launch_block_decode<D, FMT, true, true>(a, waves, s);
     else launch_block_decode<D, FMT, false, true>(a, waves, s);
   } else {
@@ -473,11 +763,26 @@ static void launch_block_decode_format(const BlockDecodeArgs& a, int32_t dtype, 
 //   rows of 4096: 89.5, two splits 93.7), above that up to three rounds of them are halved (70 of 100 to 6000: 131 and 103; 100
 //   of 500 to 2000: 61.8 and 60.8).
 // The card holds 512 workgroups of 4 waves at head dim 128 (FP8 768), 1024 at 64. A split has 4 tiles at the least.
+// table_rows: of a call whose queries share rows and take listed pages (rows and blocks given), else 0.
 struct BlockShape {
-  int32_t waves, splits;
+  int32_t waves, splits, segs;
 };
-static BlockShape block_shape(int32_t T, int32_t G, int32_t head_dim, int32_t page_size, int32_t table_width, int32_t window,
-                              int32_t n_blocks) {
+static BlockShape block_shape(int32_t T, int32_t H, int32_t G, int32_t head_dim, int32_t page_size, int32_t table_width,
+                              int32_t table_rows, int32_t window, int32_t n_blocks) {
+  if (table_rows > 0 && n_blocks > 0) {
+    // Page by page: for many queries, which a page is worth finding them for, with groups of two at most, since a partial is
+    // written for each head but K and V are read once a group. One by one | page by page, us, each query 16 pages of 64 of 8
+    // heads of 128, rows of up to 16384 keys: bf16, group 2, 2 x 64 queries 44 | 59, 2 x 128 80 | 75, 2 x 256 151 | 107, 2 x 1024
+    // 583 | 321, 4 x 64 86 | 94, 8 x 128 308 | 230; int8 509 | 317 and FP8 376 | 315 at 2 x 1024; group 1 at 2 x 256 151 | 81;
+    // pages of 128 at 2 x 512 295 | 164, of 32 at 2 x 1024 314 | 329; heads of 64 at 2 x 512 176 | 116. Group 4 at 2 x 1024:
+    // 294 | 490. A workgroup reads all of a row's lists for four pages: not for tables much wider than a page's keys are worth
+    // (1 x 1024 of 65536 keys 447 | 244). The partials stay within 1 GiB.
+    const int64_t segs = (page_size + 63) / 64, listed = (int64_t)T * n_blocks;
+    const int64_t partials = listed * segs * H * (head_dim + 2) * 4;
+    if (H <= 2 * G && page_size >= 64 && listed >= 4096 && listed >= 8 * (int64_t)table_rows * table_width &&
+        table_width <= 16 * (int64_t)page_size && partials <= 1 << 30)
+      return {4, (int32_t)(n_blocks * segs), (int32_t)segs};
+  }
   const int64_t keys = (int64_t)(n_blocks > 0 ? n_blocks : table_width) * page_size;
   const int64_t tiles = ((window > 0 ? std::min<int64_t>(keys, (int64_t)window + 31) : keys) + 31) / 32;
   const int64_t base = (int64_t)T * G, slots = head_dim == 64 ? 1024 : 512;
@@ -487,7 +792,7 @@ static BlockShape block_shape(int32_t T, int32_t G, int32_t head_dim, int32_t pa
   else if (!full) n = 1024 / base;
   else if (base > slots && base < 3 * slots) n = 2;
   n = std::max<int64_t>(1, std::min<int64_t>({n, tiles / 4, (int64_t)256}));
-  return {even && !full ? 8 : 4, (int32_t)n};
+  return {even && !full ? 8 : 4, (int32_t)n, 0};
 }
 
 }  // namespace sna
@@ -496,12 +801,12 @@ using namespace sna;
 
 extern "C" int64_t sna_block_decode_workspace_bytes(int32_t T, int32_t num_q_heads, int32_t num_kv_heads,
                                                     int32_t head_dim, int32_t page_size, int32_t table_width,
-                                                    int32_t window, int32_t n_blocks) {
+                                                    int32_t table_rows, int32_t window, int32_t n_blocks) {
   if (T < 1 || num_q_heads < 1 || num_kv_heads < 1 || head_dim < 1 || page_size < 1 || table_width < 1 || window < 0 ||
-      n_blocks < 0)
+      n_blocks < 0 || table_rows < 0)
     return 0;
-  const BlockShape b = block_shape(T, num_kv_heads, head_dim, page_size, table_width, window, n_blocks);
-  return b.splits > 1 ? (int64_t)T * b.splits * num_q_heads * (head_dim + 2) * (int64_t)sizeof(float) : 0;
+  const BlockShape b = block_shape(T, num_q_heads, num_kv_heads, head_dim, page_size, table_width, table_rows, window, n_blocks);
+  return b.splits > 1 || b.segs > 0 ? (int64_t)T * b.splits * num_q_heads * (head_dim + 2) * (int64_t)sizeof(float) : 0;
 }
 
 extern "C" int sna_paged_decode_blocks(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
@@ -579,10 +884,12 @@ extern "C" int sna_paged_decode_blocks(const void* q, const void* k_cache, const
   a.num_blocks = num_blocks;
   a.window = window;
   a.sm_scale = sm_scale;
-  const BlockShape shape = block_shape(T, num_kv_heads, head_dim, page_size, table_width, window, a.n_blocks);
+  const BlockShape shape = block_shape(T, num_q_heads, num_kv_heads, head_dim, page_size, table_width,
+                                       rows && blocks ? table_rows : 0, window, a.n_blocks);
   a.splits = shape.splits;
+  a.segs = shape.segs;
   a.ws_o = a.ws_ml = nullptr;
-  if (a.splits > 1) {
+  if (a.splits > 1 || a.segs > 0) {
     const int64_t rows_n = (int64_t)T * a.splits * num_q_heads, need = rows_n * (head_dim + 2) * (int64_t)sizeof(float);
     if (!workspace || workspace_bytes < need)
       return fail(SNA_ERR_WORKSPACE, "%s: workspace of %lld bytes, the splits need %lld", what,
@@ -592,7 +899,8 @@ extern "C" int sna_paged_decode_blocks(const void* q, const void* k_cache, const
     a.ws_o = (float*)workspace;
     a.ws_ml = a.ws_o + rows_n * head_dim;
   }
-  if ((int64_t)T * a.splits * num_kv_heads >= 1 << 23)  // (a grid has under 2^32 threads)
+  const int64_t items = a.segs > 0 ? (int64_t)table_rows * table_width * a.segs : (int64_t)T * a.splits;
+  if (items * num_kv_heads >= 1 << 23)  // (a grid has under 2^32 threads)
     return fail(SNA_ERR_INVALID_ARGUMENT, "%s: %d queries exceed the grid", what, T);
   a.out = (uint16_t*)out;
   const hipStream_t s = (hipStream_t)stream;

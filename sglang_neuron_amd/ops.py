@@ -1311,9 +1311,9 @@ def kv_store_blocks(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, bloc
 
     The caches hold float8_e4m3fn or int8 codes, with k_scale, v_scale [blocks, G, page / tokens] fp32 that the call keeps up:
     a code is worth code * the scale of its block of ``tokens`` tokens and KV head. A block's scale is its largest magnitude
-    times 1 / 448 or 1 / 127 (at least 2^-100): it starts anew with the block's first token and grows when a larger token comes, and the
-    block's earlier tokens are then rounded again. (Infinities are clamped and do not count; a NaN makes the scale, so the
-    block, NaN.) bf16 caches have no scales. ``k_bounds`` [blocks, G, 2, d] bf16, when given, is kept up as well: the least and
+    times 1 / 448 or 1 / 127 (at least 2^-100): it starts anew with the block's first token and grows when a larger token
+    comes, and the block's earlier tokens are then rounded again. (Infinities are clamped and do not count; a NaN makes the
+    scale, so the block, NaN.) bf16 caches have no scales. ``k_bounds`` [blocks, G, 2, d] bf16, when given, is kept up as well: the least and
     the largest value of each dimension over a page's keys (block_scores reads it).
 
     ``max_q_len`` bounds the chunk lengths (a host int); ``host_q_start``: a host copy of q_start, checked before the launch.
@@ -1416,7 +1416,7 @@ def _block_attention(what, q, k_cache, v_cache, block_table, seq_lens, blocks, s
     if T == 0:
         return out
     W, window = table.shape[1], min(int(window), _INT32_MAX)
-    need = _block_workspace(T, H, G, d, P, W, window, n)
+    need = _block_workspace(T, H, G, d, P, W, 0 if rows is None or blocks is None else table.shape[0], window, n)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
     _launch(dev, _lib.load().sna_paged_decode_blocks, what, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(ks),
             _ptr(vs), page, head, tokens, table.data_ptr(), stride, W, table.shape[0], _ptr(rows), lens.data_ptr(),

@@ -10,7 +10,7 @@ import torch
 
 from oracle import blocks as ob
 from oracle import weights as ow
-from sglang_neuron_amd import ops
+from sglang_neuron_amd import _lib, ops
 from tests._block_cases import FMTS, gen, hide_unstored, pool, same_bits, table_of, to, tokens
 from tests.conftest import announce
 
@@ -141,6 +141,91 @@ def test_long_lists(fmt):
     rows = [i % 2 for i in range(T)]
     got = _run(q[rows], kc, vc, ks, vs, table, [lens[r] for r in rows], blocks=lists[rows], sm_scale=0.125, rows=_i32(rows))
     _within(got[[0, 511]], want, off)
+
+
+def _by_page(T, R, W, n, H, G, d, P):
+    """Whether a call goes page by page: its workspace is a partial for each listed page's 64 keys."""
+    need = _lib.load().sna_block_decode_workspace_bytes(T, H, G, d, P, W, R, 0, n)
+    return need == T * n * -(-P // 64) * H * (d + 2) * 4
+
+
+@pytest.mark.parametrize("H,G,d,P,bt,fmt,T,n,cols", [
+    (16, 8, 128, 64, 64, "bf16", 840, 5, 8), (4, 2, 128, 64, 16, "fp8", 840, 5, 8), (3, 3, 64, 64, 32, "int8", 840, 5, 9),
+    (2, 1, 64, 80, 16, "bf16", 840, 5, 8), (2, 2, 64, 96, 32, "fp8", 840, 5, 7), (1, 1, 128, 128, 128, "bf16", 840, 5, 8),
+    (2, 1, 128, 256, 64, "int8", 840, 5, 8), (2, 1, 64, 64, 64, "bf16", 2000, 4, 3), (1, 1, 64, 64, 16, "fp8", 2000, 4, 3)])
+def test_selected_pages_of_many_queries(H, G, d, P, bt, fmt, T, n, cols):
+    """Prompts' queries: few rows, many queries a page (more than a workgroup lists at a time), lengths that end inside pages,
+    rows outside the table, pages listed twice, unordered, invalid."""
+    announce(f"selected by page {fmt} H={H} G={G} d={d} P={P} bt={bt} T={T} n={n}")
+    R = 3
+    lens = [cols * P, (cols - 1) * P + 3, 1]
+    q, kc, vc, ks, vs, table = _case(P + T, lens, H, G, d, P, bt, fmt, rows=[0] * T)
+    W = table.shape[1]
+    assert _by_page(T, R, W, n, H, G, d, P)
+    if cols > 3:
+        table[0, 2], table[1, 1] = -1, kc.shape[0] + 5
+    g = gen(T)
+    rows = (torch.rand(T, generator=g) < 0.3).long()
+    at = torch.where(rows == 0, torch.randint((cols - 1) * P - 5, cols * P + 1, (T,), generator=g),
+                     (cols - 1) * P + torch.randint(0, 4, (T,), generator=g))
+    some = torch.randperm(T, generator=g)[:12].tolist()  # (of nobody else's lengths)
+    for t, (r, n_t) in zip(some, [(2, 1), (2, 0), (-1, 9), (3, 9), (2 ** 31 - 1, 9), (0, 1), (0, -4), (0, P), (1, 16), (0, 0),
+                                  (1, 2 * P + 1), (0, 3 * P - 1)]):
+        rows[t], at[t] = r, n_t
+    lists = torch.randint(0, cols, (T, G, n), generator=g).to(torch.int32)
+    lists[::2, :, 0] = cols - 1
+    lists[1::7, :, 3] = lists[1::7, :, 1]
+    lists[2::9, 0] = -1
+    lists[4::9, :, 2], lists[5::9, :, 3] = 2 ** 31 - 1, W
+    kw = dict(sm_scale=d ** -0.5, sinks=torch.randn(H, generator=g))
+    want, off = ob.decode(q, kc, vc, table, at.tolist(), k_scale=ks, v_scale=vs, blocks=lists, rows=rows.tolist(), **kw)
+    got = _run(q, kc, vc, ks, vs, table, at.to(torch.int32), blocks=lists, rows=rows.to(torch.int32), **kw)
+    _within(got, want, off)
+    again = _run(q, kc, vc, ks, vs, table, at.to(torch.int32), blocks=lists, rows=rows.to(torch.int32), **kw)
+    assert same_bits(got, again)
+
+
+def test_selected_pages_of_many_queries_specials():
+    """Page by page, captured and replayed with other lists; NaN reaches the queries that see it and no others."""
+    announce("selected by page, graph")
+    H, G, d, P, T, R, n, cols = 4, 2, 128, 64, 1024, 2, 4, 12
+    q, kc, vc, ks, vs, table = _case(5, [cols * P] * R, H, G, d, P, 64, "bf16", rows=[0] * T, hide=False)
+    assert _by_page(T, R, table.shape[1], n, H, G, d, P)
+    g = gen(6)
+    rows = _i32([i % 2 for i in range(T)])
+    at = torch.randint(1, cols * P + 1, (T,), generator=g).to(torch.int32)
+    pick = lambda: torch.stack([torch.stack([torch.randperm(cols, generator=g)[:n] for _ in range(G)])
+                                for _ in range(T)]).to(torch.int32)
+    vc[int(table[0, 3]), 1, 7, 2] = float("nan")
+    state = to(DEV, q, kc, vc, table, at, pick(), rows)
+
+    def call():
+        s = state
+        return ops.paged_decode_selected(s[0], s[1], s[2], s[3], s[4], s[5], sm_scale=0.1, rows=s[6])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for _ in range(3):
+        lists = pick()
+        state[5].copy_(lists)
+        graph.replay()
+        eager = call()
+        torch.cuda.synchronize()
+        assert same_bits(got.isnan(), eager.isnan()) and same_bits(got.nan_to_num(), eager.nan_to_num())
+        want, off = ob.decode(q, kc, vc, table, at.tolist(), sm_scale=0.1, blocks=lists, rows=rows.tolist())
+        nan = got.isnan().cpu()
+        sees = (lists[:, 1] == 3).any(-1) & (rows == 0) & (at > 3 * P + 7)
+        assert bool(sees.any()) and torch.equal(nan[:, 2:, 2], sees[:, None].expand(T, 2))
+        nan[:, 2:, 2] = False
+        assert not bool(nan.any())
+        ok = ~got.isnan().cpu()
+        _within(torch.where(ok, got.cpu().float(), 0.0), torch.where(ok, want, 0.0), torch.where(ok, off, 0.0))
 
 
 def test_rows_and_strided_tables():

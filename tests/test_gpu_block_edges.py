@@ -175,8 +175,8 @@ def test_refusals_of_device_tensors():
     for blocks in (z(2, G, 0, dt=torch.int32), z(2, H, 3, dt=torch.int32), z(2, 3, dt=torch.int32)):
         with pytest.raises(ValueError):
             ops.paged_decode_selected(blocks=blocks, **dec)
-    pre = dict(q=q, k_cache=kc, v_cache=vc, block_table=table, q_start=start, prior_lens=one, max_q_len=1, sm_scale=1.0, k_scale=ks,
-               v_scale=vs)
+    pre = dict(q=q, k_cache=kc, v_cache=vc, block_table=table, q_start=start, prior_lens=one, max_q_len=1, sm_scale=1.0,
+               k_scale=ks, v_scale=vs)
     for change in (dict(q=z(2, 5, d)), dict(q_start=start[:2]), dict(max_q_len=0), dict(host_q_start=[0, 2, 2]),
                    dict(sinks=z(3, dt=torch.float32)), dict(out=z(3, H, d)), dict(window=-1)):
         with pytest.raises(ValueError):

@@ -121,8 +121,8 @@ def test_restaged_scales(fmt):
         # without a workspace the launch never splits
         rc = lib.sna_prefill_attention_blocks(
             dev[0].data_ptr(), dev[1].data_ptr(), dev[2].data_ptr(), dev[4].data_ptr(), dev[5].data_ptr(), ks.stride(0),
-            ks.stride(1), 16, dev[3].data_ptr(), table.shape[1], table.shape[1], q_start.data_ptr(), prior.data_ptr(), 300, 1, 300,
-            None, 0.125, window, out.data_ptr(), H, G, d, 16, kc.shape[0], 3 if fmt == "int8" else 1, None, 0,
+            ks.stride(1), 16, dev[3].data_ptr(), table.shape[1], table.shape[1], q_start.data_ptr(), prior.data_ptr(), 300, 1,
+            300, None, 0.125, window, out.data_ptr(), H, G, d, 16, kc.shape[0], 3 if fmt == "int8" else 1, None, 0,
             torch.cuda.current_stream().cuda_stream)
         _lib.check(rc, "prefill_attention_blocks")
         some = [0, 150, 299]
