@@ -18,6 +18,11 @@
 //        contiguous elements from D / 16 * li of its 8 keys).
 //   acc  lane (g4, j), d-tile t, row r: O[head j, D / 16 * (4 g4 + r) + t].
 // The softmax state is (m, l, acc) in the log2 domain, m moved only when a tile's maximum passes it by more than 8.
+//
+// What bounds it: HBM where the rows fill the card (64 rows of 4096 e4m3fn keys, 32 / 8 heads of 128, pages of 16: 87 us, 539 MB,
+// 6.2 TB/s; one row of 131071 int8 keys 48 us, the first launch at 6.0; matrix pipe 7%, VALU 38% of the cycles); the longest
+// row's share and the merge where they are ragged (128 rows of 2048 to 8192, 8 heads on one of 64, int8: 22 + 3 us for 84 MB).
+// Many queries of few rows with pages of their own go another way, block_pages_kernel.
 #include <algorithm>
 
 #include "sna_device.h"
@@ -127,7 +132,7 @@ __device__ __forceinline__ void block_v_op(const BlockTile<D, FMT>& T, int dt, u
 }
 
 // SHARED: queries of one row, which read the same pages, may be among the call's (`rows`). V then stays in the L2 (2 x 256
-// queries of 1024 selected keys, bf16: 178 -> 152 us); else it is read once, past it (64 rows of 4096 FP8 keys 87.5 us, through
+// queries of 1024 selected keys, bf16, one by one: 178 -> 152 us); else it is read once, past it (64 rows of 4096 FP8 keys 87.5 us, through
 // the L2 97). K, two loads a 128-byte line, always goes through it (past it 90; the 2 x 256 queries 244).
 template <int D, int FMT, bool SEL, bool SPLIT, int WAVES, bool SHARED>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2)))
@@ -756,7 +761,8 @@ static void launch_block_decode_format(const BlockDecodeArgs& a, int32_t dtype, 
 // table's width says little about them: it is what a graph is captured for).
 //   Queries of equal work (lists of one length; a single query): 8 waves and one round of workgroups, so the fewest partials
 //   (32 queries of 2048 selected FP8 keys, 32 / 8 heads of 128: whole rows on 8 waves 27.0 us, two splits on 4 waves 32.3, on
-//   8 32.3; one row of 131071 int8 keys: 32 splits on 8 waves 48.6, 64 on 4 50.0, 32 on 4 60.0).
+//   8 32.3; one row of 131071 int8 keys: 32 splits on 8 waves 48.6, 64 on 4 50.0, 32 on 4 60.0; both sides before K went
+//   through the L2, 24.7 and 47.8 since).
 //   Rows of unequal lengths: 4 waves, some 1024 workgroups, so that the short ones even the long ones out (24 rows of 1000 to
 //   4096 keys: 2, 4 and 8 splits on 4 waves 40.5, 33.3, 34.6 us, on 8 waves 43.2, 40.4, 47.7; 40 of 200 to 8000: whole 128, 3
 //   splits 85, 6 78; 16 of 4096: 2, 4, 8, 16 splits 31.6, 28.5, 28.9, 33.5). Where whole rows fill the card they stay whole (64
