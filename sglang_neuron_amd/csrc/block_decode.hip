@@ -132,8 +132,8 @@ __device__ __forceinline__ void block_v_op(const BlockTile<D, FMT>& T, int dt, u
 }
 
 // SHARED: queries of one row, which read the same pages, may be among the call's (`rows`). V then stays in the L2 (2 x 256
-// queries of 1024 selected keys, bf16, one by one: 178 -> 152 us); else it is read once, past it (64 rows of 4096 FP8 keys 87.5 us, through
-// the L2 97). K, two loads a 128-byte line, always goes through it (past it 90; the 2 x 256 queries 244).
+// queries of 1024 selected keys, bf16, one by one: 178 -> 152 us); else it is read once, past it (64 rows of 4096 FP8 keys 87.5
+// us, through the L2 97). K, two loads a 128-byte line, always goes through it (past it 90; the 2 x 256 queries 244).
 template <int D, int FMT, bool SEL, bool SPLIT, int WAVES, bool SHARED>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2)))
 void block_decode_kernel(BlockDecodeArgs a) {
@@ -392,8 +392,8 @@ void block_decode_kernel(BlockDecodeArgs a) {
 
 // Page by page, for many queries of few rows (a prompt's, each with pages of its own choice): a workgroup finds the queries
 // whose lists name one of four pages of a row, for one KV head and 64 keys of the page, keeps a page's keys as operands in
-// registers and attends 16 / group queries at a time to them, so a page is read once, not once a query, and the columns are full. A
-// partial is written for each entry of the lists and merged as splits are. Latency bounds it: a page's operands take all the
+// registers and attends 16 / group queries at a time to them, so a page is read once, not once a query, and the columns are full.
+// A partial is written for each entry of the lists and merged as splits are. Latency bounds it: a page's operands take all the
 // registers that two waves a SIMD have, and each batch waits for its queries (2 x 256 queries of 16 pages of 64, bf16, group 2:
 // 107 us of which the merge 22; one page a workgroup 137, most of it in searching the lists once for each).
 constexpr int kPageWaves = 4;  // and pages

@@ -893,7 +893,9 @@ __global__ __launch_bounds__(256) void prefill_combine_kernel(PrefillArgs a, boo
 // `most`: a bound of the batch's query blocks, qblocks * R where nothing better is known.
 static int32_t prefill_split_slots(int64_t qblocks, int32_t R, int32_t G, int64_t bound_tiles, int64_t most) {
   const int64_t base = std::min(qblocks * R, most) * G;
-  if (base > kPrefillSplitBlocks || qblocks * R > kPrefillSplitPairs || bound_tiles <= kPrefillNoSplit || bound_tiles > kPrefillSplitMaxTiles) return 0;
+  if (base > kPrefillSplitBlocks || qblocks * R > kPrefillSplitPairs || bound_tiles <= kPrefillNoSplit ||
+      bound_tiles > kPrefillSplitMaxTiles)
+    return 0;
   static_assert(kPrefillSplitPairs >= kPrefillSplitBlocks, "a split launch's pairs fit a wave");
   return (int32_t)std::min<int64_t>(kPrefillSlots, base * ((bound_tiles + kPrefillMinSplit - 1) / kPrefillMinSplit));
 }
@@ -984,7 +986,7 @@ static int prefill_attention(const char* what, const PrefillScales* scales, bool
                 (long long)scales->page_stride, (long long)scales->head_stride);
   if (scales ? kv_dtype != SNA_DTYPE_FP8_E4M3FN && kv_dtype != SNA_DTYPE_INT8
              : kv_dtype != SNA_DTYPE_FP8_E4M3FN && kv_dtype != SNA_DTYPE_FP8_E4M3FN_MUL && kv_dtype != SNA_DTYPE_BF16)
-    return fail(SNA_ERR_UNSUPPORTED, "%s: KV dtype %d (FP8 e4m3fn or bf16)", what, kv_dtype);
+    return fail(SNA_ERR_UNSUPPORTED, "%s: KV dtype %d (FP8 e4m3fn%s or bf16)", what, kv_dtype, empty_zero ? ", int8" : "");
   if (R == 0 || max_q_len == 0) return SNA_OK;
   if (!q || !k_cache || !v_cache || (kv_dtype != SNA_DTYPE_BF16 && (!k_scale || !v_scale)) || !block_table ||
       !q_start || !prior_lens || !out)
@@ -1028,8 +1030,9 @@ static int prefill_attention(const char* what, const PrefillScales* scales, bool
   a.slots = 0;
   a.ws_o = a.ws_ml = nullptr;
   a.ws_item = nullptr;
-  const int32_t slots = workspace ? split_slots_of(scales ? scales->n_queries : -1, R, max_q_len, num_q_heads, num_kv_heads, page_size, table_width,
-                                                   window) : 0;
+  const int32_t slots = workspace ? split_slots_of(scales ? scales->n_queries : -1, R, max_q_len, num_q_heads, num_kv_heads,
+                                                   page_size, table_width, window)
+                                  : 0;
   if (slots > 0) {
     const int64_t need = split_workspace_bytes(slots, R, max_q_len, num_q_heads, num_kv_heads, head_dim);
     if (workspace_bytes < need)

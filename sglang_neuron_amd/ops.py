@@ -1313,8 +1313,8 @@ def kv_store_blocks(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, bloc
     a code is worth code * the scale of its block of ``tokens`` tokens and KV head. A block's scale is its largest magnitude
     times 1 / 448 or 1 / 127 (at least 2^-100): it starts anew with the block's first token and grows when a larger token
     comes, and the block's earlier tokens are then rounded again. (Infinities are clamped and do not count; a NaN makes the
-    scale, so the block, NaN.) bf16 caches have no scales. ``k_bounds`` [blocks, G, 2, d] bf16, when given, is kept up as well: the least and
-    the largest value of each dimension over a page's keys (block_scores reads it).
+    scale, so the block, NaN.) bf16 caches have no scales. ``k_bounds`` [blocks, G, 2, d] bf16, when given, is kept up as
+    well: the least and the largest value of each dimension over a page's keys (block_scores reads it).
 
     ``max_q_len`` bounds the chunk lengths (a host int); ``host_q_start``: a host copy of q_start, checked before the launch.
     Tokens without a page are not stored. No page may be written for two requests of a call (a cached prefix is shared by whole
@@ -1463,7 +1463,8 @@ def prefill_attention_blocks(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_
     bf16 caches without scales too): q [T, H, d] bf16, request r's rows q_start[r] .. q_start[r + 1] at positions
     prior_lens[r] + i, causal, optionally windowed and with sinks [H]. ``max_q_len`` bounds the chunk lengths;
     ``host_q_start``: a host copy of q_start, checked before the launch. A query that sees no key gives zeros. Over int8
-    codes a query element is taken to within 2^-16 of its row's largest. Returns [T, H, d] bf16."""
+    codes a query element is taken to within 2^-16 of its row's largest. In bf16 caches a NaN or an infinity in V also reaches
+    queries of the chunk shortly before it (as in prefill_attention). Returns [T, H, d] bf16."""
     dev = _on_gpu(q, k_cache, v_cache, block_table, q_start, prior_lens, k_scale, v_scale, sinks, out)
     code, (nb, G, P, dk), ks, vs, page, head, tokens = _block_cache(k_cache, v_cache, k_scale, v_scale)
     if q.dim() != 3 or q.dtype != torch.bfloat16 or q.shape[2] != dk or q.shape[1] % G:

@@ -228,6 +228,27 @@ def test_selected_pages_of_many_queries_specials():
         _within(torch.where(ok, got.cpu().float(), 0.0), torch.where(ok, want, 0.0), torch.where(ok, off, 0.0))
 
 
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+def test_selected_pages_of_many_queries_scales(fmt):
+    """Page by page: a scale that is NaN reaches the queries that see its block and no others, whatever they share."""
+    announce(f"selected by page, NaN scales {fmt}")
+    H, G, d, P, T, R, n, cols = 2, 1, 64, 64, 1100, 2, 4, 6
+    q, kc, vc, ks, vs, table = _case(8, [cols * P] * R, H, G, d, P, 16, fmt, rows=[0] * T, hide=False)
+    assert _by_page(T, R, table.shape[1], n, H, G, d, P)
+    g = gen(9)
+    rows = torch.arange(T) % 2
+    at = torch.randint(5 * P - 20, cols * P + 1, (T,), generator=g)
+    lists = torch.randint(0, cols, (T, G, n), generator=g).to(torch.int32)
+    want, off = ob.decode(q, kc, vc, table, at.tolist(), k_scale=ks, v_scale=vs, sm_scale=0.1, blocks=lists, rows=rows.tolist())
+    ks[int(table[0, 5]), 0, 2] = float("nan")
+    vs[int(table[1, 5]), 0, 1] = float("nan")
+    got = _run(q, kc, vc, ks, vs, table, at.to(torch.int32), sm_scale=0.1, blocks=lists, rows=rows.to(torch.int32)).cpu()
+    sees = (lists[:, 0] == 5).any(-1) & (at > 5 * P + torch.where(rows == 0, 32, 16))
+    assert bool(sees.any()) and bool((~sees & (lists[:, 0] == 5).any(-1) & (at > 5 * P)).any())
+    assert bool(got[sees].isnan().all())
+    _within(got[~sees], want[~sees], off[~sees])
+
+
 def test_rows_and_strided_tables():
     """Several queries of a row at lengths of their own; rows outside the table see nothing; tables that are views."""
     announce("decode rows, strides")

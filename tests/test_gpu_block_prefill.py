@@ -178,6 +178,17 @@ def test_missing_pages_and_nan(fmt):
         assert float(((out - want).abs() - off)[clean].max()) <= 1e-30
 
 
+@pytest.mark.parametrize("d,lens", [(64, (9, 40)), (128, (60, 3)), (64, (700, 300))])
+def test_bf16_rows_without_pages(d, lens):
+    """bf16 caches: requests whose table names no page give zeros, whatever the output held, the others their attention."""
+    announce(f"bf16 without pages {d} {lens}")
+    q, kc, vc, ks, vs, table, start = _case(9, [0, 5], list(lens), 4, 2, d, 16, 16, "bf16", extra=1)
+    table[0, :] = -1
+    out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device=DEV)
+    got = _check((q, kc, vc, ks, vs, table, start), [0, 5], "bf16", sm_scale=0.125, out=out)
+    assert bool((got[:lens[0]] == 0).all())
+
+
 def test_sinks_without_end():
     announce("prefill sinks")
     priors, counts = [0], [20]
