@@ -511,7 +511,7 @@ int sna_kv_store_blocks(const void *k, const void *v, int64_t k_row_stride, int6
  * num_q_heads / num_kv_heads <= 16. The same call gives the same bits. */
 int64_t sna_block_decode_workspace_bytes(int32_t T, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                                          int32_t page_size, int32_t table_width, int32_t table_rows, int32_t window,
-                                         int32_t n_blocks);
+                                         int32_t n_blocks, int32_t cache_dtype);
 int sna_paged_decode_blocks(const void *q, const void *k_cache, const void *v_cache, const float *k_scale,
                             const float *v_scale, int64_t scale_page_stride, int64_t scale_head_stride,
                             int32_t scale_tokens, const int32_t *block_table, int64_t table_stride, int32_t table_width,

@@ -113,7 +113,7 @@ SIGNATURES = {
                                 _P, _I32, _I32, _I32, _I32, _P, _P, _P, _I64, _I64, _I32, _P, _I64, _P]),
     "sna_kv_store_blocks": (_I32, [_P, _P, _I64, _I64, _I32, _P, _I64, _I32, _P, _P, _I32, _I32, _P, _P, _P, _P, _I32, _P, _I64, _I32,
                                    _I32, _I32, _I32, _P]),
-    "sna_block_decode_workspace_bytes": (_I64, [_I32] * 9),
+    "sna_block_decode_workspace_bytes": (_I64, [_I32] * 10),
     "sna_paged_decode_blocks": (_I32, [_P, _P, _P, _P, _P, _I64, _I64, _I32, _P, _I64, _I32, _I32, _P, _P, _P, _I32, _P,
                                        _I32, _F32, _P, _I32, _I32, _I32, _I32, _I32, _I64, _I32, _P, _I64, _P]),
     "sna_prefill_blocks_workspace_bytes": (_I64, [_I32] * 10),

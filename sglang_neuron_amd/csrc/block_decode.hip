@@ -395,7 +395,8 @@ void block_decode_kernel(BlockDecodeArgs a) {
 // registers and attends 16 / group queries at a time to them, so a page is read once, not once a query, and the columns are full.
 // A partial is written for each entry of the lists and merged as splits are. Latency bounds it: a page's operands take all the
 // registers that two waves a SIMD have, and each batch waits for its queries (2 x 256 queries of 16 pages of 64, bf16, group 2:
-// 107 us of which the merge 22; one page a workgroup 137, most of it in searching the lists once for each).
+// 94 us, of which the search 20 and the merge 13; with one page a workgroup 30 more, the lists searched once for each; the first
+// and last pages, which most lists name, before the others 9 more).
 constexpr int kPageWaves = 4;  // and pages
 constexpr int kPageScan = 8;   // entries that a thread reads at a time
 constexpr int kPageStep = kPageScan * 64 * kPageWaves, kPageList = kPageStep + 1024;
@@ -568,13 +569,31 @@ void block_pages_kernel(BlockDecodeArgs a) {
     const bool redo = __builtin_amdgcn_readfirstlane((int)(check && __any(nan && live)));
     if (live && !redo) {
       const int64_t at = ((int64_t)e * a.segs + seg) * a.H + g * a.group + hc;
+      // A lane holds D / 4 elements in a row, so that a store of all lanes' quarters would touch 64 lines: four lane groups
+      // transpose their quads of elements among each other, and each stores one of four that follow each other (107 -> 102 us).
       float* wo = a.ws_o + at * D;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int c0 = 0; c0 < D / 16; c0 += 4) {
+        uint32_t y[4][4];  // [quad c0 + o of the lane's, its element], then [quad c0 + g4 of lane group o's, ..]
 #pragma unroll
-        for (int d4 = 0; d4 < VE; d4 += 4)
-          *reinterpret_cast<f32x4_t*>(wo + VE * (4 * g4 + r) + d4) =
-              f32x4_t{acc[d4][r], acc[d4 + 1][r], acc[d4 + 2][r], acc[d4 + 3][r]};
+        for (int w = 0; w < 4; ++w) {
+#pragma unroll
+          for (int o = 0; o < 4; ++o) y[o][w] = __float_as_uint(acc[(4 * (c0 + o) + w) % VE][(4 * (c0 + o) + w) / VE]);
+#pragma unroll
+          for (int o = 0; o < 2; ++o) {
+            const auto z = __builtin_amdgcn_permlane32_swap(y[o][w], y[o + 2][w], false, false);
+            y[o][w] = (uint32_t)z[0], y[o + 2][w] = (uint32_t)z[1];
+          }
+#pragma unroll
+          for (int o = 0; o < 4; o += 2) {
+            const auto z = __builtin_amdgcn_permlane16_swap(y[o][w], y[o + 1][w], false, false);
+            y[o][w] = (uint32_t)z[0], y[o + 1][w] = (uint32_t)z[1];
+          }
+        }
+#pragma unroll
+        for (int o = 0; o < 4; ++o)
+          *reinterpret_cast<uint4*>(wo + D / 4 * o + 4 * (c0 + g4)) = make_uint4(y[o][0], y[o][1], y[o][2], y[o][3]);
+      }
       if (g4 == 0) *reinterpret_cast<float2*>(a.ws_ml + 2 * at) = make_float2(m, l);
     }
     return !redo;
@@ -656,9 +675,7 @@ void block_pages_kernel(BlockDecodeArgs a) {
 // Merge of a query's splits, one workgroup per (query, head): out = sum_s e_s o_s / (sum_s e_s l_s + e_sink), e_s =
 // exp2(m_s - M). D / 4 lanes take a split's row in 16-byte pieces, 1024 / D splits at a time, each such group of lanes with a
 // running (M, l, o) of its own; the groups are merged in LDS.
-// PAGES: split s is the keys 64 (s % segs) .. of the page that entry s / segs of the list names, and was written where the query
-// sees some of them.
-template <int D, bool PAGES>
+template <int D>
 __global__ __launch_bounds__(256) void block_combine_kernel(BlockDecodeArgs a) {
   constexpr int LR = D / 4, NG = 256 / LR, CH = 4;
   const int32_t t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, gi = tid / LR, d = 4 * (tid % LR);
@@ -666,17 +683,6 @@ __global__ __launch_bounds__(256) void block_combine_kernel(BlockDecodeArgs a) {
   const int64_t at0 = (int64_t)t * ns * a.H + h;
   const float* wo = a.ws_o + at0 * D + d;
   const float* ml = a.ws_ml + 2 * at0;
-  const int32_t g = h / a.group, row = PAGES ? a.rows[t] : 0;
-  const bool row_ok = row >= 0 && row < a.table_rows;
-  const int32_t L = PAGES && row_ok ? block_len(a, a.seq_lens[t]) : 0;
-  const int32_t* list = PAGES ? a.blocks + ((int64_t)t * a.G + g) * a.n_blocks : nullptr;
-  auto written = [&](int32_t s) -> bool {
-    if (!PAGES) return true;
-    const int32_t e = s / a.segs, c = list[e];
-    if (c < 0 || c >= a.table_width || L - c * a.P - 64 * (s - e * a.segs) <= 0) return false;
-    const int32_t page = a.table[(int64_t)row * a.table_stride + c];
-    return page >= 0 && (int64_t)page < a.num_blocks;
-  };
   float M = kNegBig, l = 0.0f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   for (int32_t s0 = gi; s0 < ns; s0 += NG * CH) {
@@ -684,11 +690,9 @@ __global__ __launch_bounds__(256) void block_combine_kernel(BlockDecodeArgs a) {
     float2 w[CH];
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      const int32_t si = min(s0 + NG * k, ns - 1);
-      const int64_t s = (int64_t)si * a.H;
+      const int64_t s = (int64_t)min(s0 + NG * k, ns - 1) * a.H;
       x[k] = *reinterpret_cast<const f32x4_t*>(wo + s * D);
       w[k] = *reinterpret_cast<const float2*>(ml + 2 * s);
-      if (PAGES && (!written(si) || w[k].y == 0.0f)) x[k] = f32x4_t{0.f, 0.f, 0.f, 0.f}, w[k] = make_float2(kNegBig, 0.0f);
     }
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
@@ -721,13 +725,73 @@ __global__ __launch_bounds__(256) void block_combine_kernel(BlockDecodeArgs a) {
       f32_to_bf16_bits(a0 * inv) | f32_to_bf16_bits(a1 * inv) << 16;
 }
 
+// The same of the partials page by page, one wave per (query, head): split s is the keys 64 (s % segs) .. of the page that entry
+// s / segs of the list names, and was written where the query sees some of them. 64 splits at a time, each lane looks one up;
+// D / 4 lanes take a split's row. (2 x 256 queries of 16 pages, 16 heads of 128: a workgroup per (query, head), each lane with
+// look-ups of its own, 22 us; 13 so.)
+template <int D>
+__global__ __launch_bounds__(256) void block_pages_combine_kernel(BlockDecodeArgs a) {
+  constexpr int LR = D / 4, NG = 64 / LR, CH = 8;
+  const int lane = threadIdx.x & 63, gi = lane / LR, d = 4 * (lane % LR);
+  const int32_t item = (int32_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  if (item >= a.T * a.H) return;
+  const int32_t t = item / a.H, h = item - t * a.H, ns = a.splits, row = a.rows[t];
+  const int32_t L = row >= 0 && row < a.table_rows ? block_len(a, a.seq_lens[t]) : 0;
+  const int32_t* list = a.blocks + ((int64_t)t * a.G + h / a.group) * a.n_blocks;
+  const int64_t at0 = (int64_t)t * ns * a.H + h;
+  const float* wo = a.ws_o + at0 * D + d;
+  const float* ml = a.ws_ml + 2 * at0;
+  float M = kNegBig, l = 0.0f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (int32_t s0 = 0; s0 < ns; s0 += 64) {  // uniform
+    const int32_t s = s0 + lane, e = s / a.segs;
+    float m = kNegBig, sum = 0.0f;
+    bool written = false;
+    if (s < ns) {
+      const int32_t c = list[e];
+      const float2 w = *reinterpret_cast<const float2*>(ml + (int64_t)2 * s * a.H);
+      if (c >= 0 && c < a.table_width && L - c * a.P - 64 * (s - e * a.segs) > 0) {
+        const int32_t page = a.table[(int64_t)row * a.table_stride + c];
+        written = page >= 0 && (int64_t)page < a.num_blocks && w.y != 0.0f;
+        if (written) m = w.x, sum = w.y;
+      }
+    }
+    const float m_new = fmaxf(M, wave_max(m)), keep = __builtin_amdgcn_exp2f(M - m_new);
+    const float f = __builtin_amdgcn_exp2f(m - m_new);
+    M = m_new;
+    l = l * keep + wave_sum(sum * f);
+    o *= keep;
+    const uint64_t some = __ballot(written);
+    for (int32_t i0 = 0; i0 < min(ns - s0, 64); i0 += NG * CH) {
+      f32x4_t x[CH];
+#pragma unroll
+      for (int k = 0; k < CH; ++k)
+        x[k] = *reinterpret_cast<const f32x4_t*>(wo + (int64_t)min(s0 + i0 + NG * k + gi, ns - 1) * a.H * D);
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        const int32_t i = i0 + NG * k + gi;  // below 64 + NG * CH
+        const float fi = __shfl(f, i & 63);
+        if (i < 64 && (some >> (i & 63) & 1)) o += x[k] * fi;
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) o[r] = D == 128 ? xor32_partner_sum(o[r]) : sum_across_groups(o[r]);
+  if (a.sinks) l += __builtin_amdgcn_exp2f(a.sinks[h] * kLog2e - M);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (gi == 0)
+    *reinterpret_cast<uint2*>(a.out + ((int64_t)t * a.H + h) * D + d) =
+        make_uint2(f32_to_bf16_bits(o[0] * inv) | f32_to_bf16_bits(o[1] * inv) << 16,
+                   f32_to_bf16_bits(o[2] * inv) | f32_to_bf16_bits(o[3] * inv) << 16);
+}
+
 template <int D, int FMT, bool SEL, bool SHARED>
 static void launch_block_decode(const BlockDecodeArgs& a, int32_t waves, hipStream_t s) {
   const dim3 grid((uint32_t)(a.T * a.splits * a.G));
   if (a.splits > 1) {
     if (waves == 4) hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, true, 4, SHARED>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, true, 8, SHARED>), grid, dim3(512), 0, s, a);
-    hipLaunchKernelGGL((block_combine_kernel<D, false>), dim3(a.T, a.H), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((block_combine_kernel<D>), dim3(a.T, a.H), dim3(256), 0, s, a);
   } else {
     if (waves == 4) hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, false, 4, SHARED>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((block_decode_kernel<D, FMT, SEL, false, 8, SHARED>), grid, dim3(512), 0, s, a);
@@ -740,7 +804,7 @@ static void launch_block_decode_form(const BlockDecodeArgs& a, int32_t waves, hi
     const int32_t quads = (a.table_width + kPageWaves - 1) / kPageWaves;
     hipLaunchKernelGGL((block_pages_kernel<D, FMT>), dim3((uint32_t)(a.table_rows * quads * a.segs * a.G)), dim3(64 * kPageWaves),
                        0, s, a);
-    hipLaunchKernelGGL((block_combine_kernel<D, true>), dim3(a.T, a.H), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((block_pages_combine_kernel<D>), dim3((uint32_t)((a.T * a.H + 3) / 4)), dim3(256), 0, s, a);
   } else if (a.rows) {
     if (a.blocks) launch_block_decode<D, FMT, true, true>(a, waves, s);
     else launch_block_decode<D, FMT, false, true>(a, waves, s);
@@ -774,19 +838,23 @@ struct BlockShape {
   int32_t waves, splits, segs;
 };
 static BlockShape block_shape(int32_t T, int32_t H, int32_t G, int32_t head_dim, int32_t page_size, int32_t table_width,
-                              int32_t table_rows, int32_t window, int32_t n_blocks) {
+                              int32_t table_rows, int32_t window, int32_t n_blocks, int32_t esz) {
   if (table_rows > 0 && n_blocks > 0) {
-    // Page by page: for many queries, which a page is worth finding them for, with groups of two at most, since a partial is
-    // written for each head but K and V are read once a group. One by one | page by page, us, each query 16 pages of 64 of 8
-    // heads of 128, rows of up to 16384 keys: bf16, group 2, 2 x 64 queries 44 | 59, 2 x 128 80 | 75, 2 x 256 151 | 107, 2 x 1024
-    // 583 | 321, 4 x 64 86 | 94, 8 x 128 308 | 230; int8 509 | 317 and FP8 376 | 315 at 2 x 1024; group 1 at 2 x 256 151 | 81;
-    // pages of 128 at 2 x 512 295 | 164, of 32 at 2 x 1024 314 | 329; heads of 64 at 2 x 512 176 | 116. Group 4 at 2 x 1024:
-    // 294 | 490. A workgroup reads all of a row's lists for four pages: not for tables much wider than a page's keys are worth
-    // (1 x 1024 of 65536 keys 447 | 244). The partials stay within 1 GiB.
+    // Page by page: for many queries, which a page is worth finding them for, with groups of three at most, since a partial is
+    // written for each head but K and V are read once a group. One by one | page by page, us, each query 16 pages of 64, heads
+    // of 128, rows of up to 16384 keys:
+    //   bf16, 8 KV heads, group 2: 2 x 64 queries 44 | 54, 2 x 128 80 | 70, 2 x 256 151 | 94, 2 x 1024 579 | 247, 4 x 64 86 | 90,
+    //   8 x 128 307 | 200, 1 x 1024 of 65536 keys 447 | 217; 2 KV heads, 2 x 512 77 | 77;
+    //   8 KV heads, group 1 at 2 x 256 150 | 74; group 3 at 2 x 128 80 | 81, 2 x 256 152 | 119; group 4 at 2 x 1024 292 | 321;
+    //   FP8, group 2: 2 x 256 100 | 81, 2 x 1024 373 | 231, 2 KV heads at 2 x 512 54 | 72, group 3 at 2 x 256 100 | 106, 2 x 1024
+    //   377 | 356; int8 at 2 x 1024: group 2 507 | 231, group 3 511 | 359;
+    //   pages of 128 at 2 x 512 294 | 139, of 32 at 2 x 256 86 | 111; heads of 64 at 2 x 512 176 | 90.
+    // A workgroup reads all of a row's lists for four pages: not for tables much wider than a page's keys are worth. The partials
+    // stay within 1 GiB.
     const int64_t segs = (page_size + 63) / 64, listed = (int64_t)T * n_blocks;
     const int64_t partials = listed * segs * H * (head_dim + 2) * 4;
-    if (H <= 2 * G && page_size >= 64 && listed >= 4096 && listed >= 8 * (int64_t)table_rows * table_width &&
-        table_width <= 16 * (int64_t)page_size && partials <= 1 << 30)
+    if (H <= 3 * G && page_size >= 64 && listed * G * esz >= (H <= 2 * G ? 1 : 2) << 16 &&
+        listed >= 8 * (int64_t)table_rows * table_width && table_width <= 16 * (int64_t)page_size && partials <= 1 << 30)
       return {4, (int32_t)(n_blocks * segs), (int32_t)segs};
   }
   const int64_t keys = (int64_t)(n_blocks > 0 ? n_blocks : table_width) * page_size;
@@ -807,11 +875,13 @@ using namespace sna;
 
 extern "C" int64_t sna_block_decode_workspace_bytes(int32_t T, int32_t num_q_heads, int32_t num_kv_heads,
                                                     int32_t head_dim, int32_t page_size, int32_t table_width,
-                                                    int32_t table_rows, int32_t window, int32_t n_blocks) {
+                                                    int32_t table_rows, int32_t window, int32_t n_blocks,
+                                                    int32_t cache_dtype) {
   if (T < 1 || num_q_heads < 1 || num_kv_heads < 1 || head_dim < 1 || page_size < 1 || table_width < 1 || window < 0 ||
       n_blocks < 0 || table_rows < 0)
     return 0;
-  const BlockShape b = block_shape(T, num_q_heads, num_kv_heads, head_dim, page_size, table_width, table_rows, window, n_blocks);
+  const BlockShape b = block_shape(T, num_q_heads, num_kv_heads, head_dim, page_size, table_width, table_rows, window, n_blocks,
+                                   cache_dtype == SNA_DTYPE_BF16 ? 2 : 1);
   return b.splits > 1 || b.segs > 0 ? (int64_t)T * b.splits * num_q_heads * (head_dim + 2) * (int64_t)sizeof(float) : 0;
 }
 
@@ -891,7 +961,7 @@ extern "C" int sna_paged_decode_blocks(const void* q, const void* k_cache, const
   a.window = window;
   a.sm_scale = sm_scale;
   const BlockShape shape = block_shape(T, num_q_heads, num_kv_heads, head_dim, page_size, table_width,
-                                       rows && blocks ? table_rows : 0, window, a.n_blocks);
+                                       rows && blocks ? table_rows : 0, window, a.n_blocks, scaled ? 1 : 2);
   a.splits = shape.splits;
   a.segs = shape.segs;
   a.ws_o = a.ws_ml = nullptr;

@@ -1416,7 +1416,8 @@ def _block_attention(what, q, k_cache, v_cache, block_table, seq_lens, blocks, s
     if T == 0:
         return out
     W, window = table.shape[1], min(int(window), _INT32_MAX)
-    need = _block_workspace(T, H, G, d, P, W, 0 if rows is None or blocks is None else table.shape[0], window, n)
+    need = _block_workspace(T, H, G, d, P, W, 0 if rows is None or blocks is None else table.shape[0], window, n,
+                            code)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
     _launch(dev, _lib.load().sna_paged_decode_blocks, what, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(ks),
             _ptr(vs), page, head, tokens, table.data_ptr(), stride, W, table.shape[0], _ptr(rows), lens.data_ptr(),

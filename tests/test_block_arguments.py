@@ -74,21 +74,24 @@ def test_decode_refusals(change, code, text):
 
 def test_decode_workspace_sizes():
     fn = _lib.load().sna_block_decode_workspace_bytes
-    good = (600, 4, 2, 128, 32, 4, 0, 0, 0)
+    bf16, fp8 = _lib.DTYPE_BF16, _lib.DTYPE_FP8_E4M3FN
+    good = (600, 4, 2, 128, 32, 4, 0, 0, 0, fp8)
     assert fn(*good) == 0
-    few = fn(1, 32, 8, 128, 16, 8192, 0, 0, 0)
+    few = fn(1, 32, 8, 128, 16, 8192, 0, 0, 0, fp8)
     assert few > 0 and few % (32 * 130 * 4) == 0
-    assert fn(1, 32, 8, 128, 16, 8192, 0, 128, 0) < few and 0 < fn(1, 32, 8, 128, 16, 8192, 0, 0, 64) <= few
+    assert fn(1, 32, 8, 128, 16, 8192, 0, 128, 0, fp8) < few and 0 < fn(1, 32, 8, 128, 16, 8192, 0, 0, 64, fp8) <= few
     for at, bad in ((0, 0), (1, 0), (4, 0), (5, 0), (6, -1), (7, -1), (8, -1)):
         assert fn(*good[:at], bad, *good[at + 1:]) == 0
     # the most that any size asks for: 256 splits a query
-    assert fn(512, 4, 1, 64, 4096, 2 ** 19, 0, 0, 0) <= 512 * 256 * 4 * 66 * 4
+    assert fn(512, 4, 1, 64, 4096, 2 ** 19, 0, 0, 0, fp8) <= 512 * 256 * 4 * 66 * 4
     # page by page, of 2 rows: a partial for each listed page's 64 keys, of at most 1 GiB
-    assert fn(512, 16, 8, 128, 64, 256, 2, 0, 16) == 512 * 16 * 16 * 130 * 4
-    assert fn(512, 16, 8, 128, 160, 100, 2, 0, 16) == 512 * 16 * 3 * 16 * 130 * 4
-    for other in ((512, 16, 8, 128, 64, 256, 0, 0, 16), (512, 16, 4, 128, 64, 256, 2, 0, 16), (512, 16, 8, 128, 48, 256, 2, 0, 16),
-                  (512, 16, 8, 128, 64, 1025, 2, 0, 16), (255, 16, 8, 128, 64, 256, 2, 0, 16),
-                  (2 ** 14, 16, 8, 128, 64, 256, 2, 0, 16)):
+    assert fn(512, 16, 8, 128, 64, 256, 2, 0, 16, bf16) == 512 * 16 * 16 * 130 * 4
+    assert fn(512, 16, 8, 128, 160, 100, 2, 0, 16, fp8) == 512 * 16 * 3 * 16 * 130 * 4
+    assert fn(512, 24, 8, 128, 64, 256, 2, 0, 16, bf16) == 512 * 16 * 24 * 130 * 4
+    for other in ((512, 16, 8, 128, 64, 256, 0, 0, 16, bf16), (512, 16, 4, 128, 64, 256, 2, 0, 16, bf16),
+                  (512, 24, 8, 128, 64, 256, 2, 0, 16, fp8), (512, 16, 8, 128, 48, 256, 2, 0, 16, bf16),
+                  (512, 16, 8, 128, 64, 1025, 2, 0, 16, bf16), (255, 16, 8, 128, 64, 256, 2, 0, 16, bf16),
+                  (511, 16, 8, 128, 64, 256, 2, 0, 16, fp8), (2 ** 14, 16, 8, 128, 64, 256, 2, 0, 16, bf16)):
         assert fn(*other) < other[0] * other[8] * 16 * 130 * 4
 
 
