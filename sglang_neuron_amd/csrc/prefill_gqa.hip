@@ -555,7 +555,7 @@ void prefill_gqa_kernel(PrefillArgsOf<SCALES> a) {
   // The exponents of a tile's raw scores relative to the row's reference maximum (log2 domain), in place, and the lane's
   // largest. BLK: log2 of the group's V scale is in them, so that the probabilities come out times it, without a product
   // each (24 / 4 heads of 64, int8, 3 chunks of up to 635 tokens: 41.3 -> 39.7 us; 32 / 8 heads of 128, FP8, 4 x 2048 after
-  // 2048: 416 -> 413, among other kernels 392); the largest is without it.
+  // 2048: 416 -> 413, among other kernels 392-412); the largest is without it.
   float mx = -INFINITY;
   float v_inv[TG];  // BLK: 1 / the V scales of the tile's groups, 0 for a group that this lane's row does not see
   // (i: the tile's place among the staged ones)
