@@ -482,8 +482,9 @@ int sna_prefill_attention_split(const void *q, const void *k_cache, const void *
  *                  fresh = max(max |x| * r, 2^-100), r the fp32 1 / top, top 448 (FP8) or 127 (int8), over the call's tokens
  *                  of the block (infinities not counted; a NaN makes it NaN),
  *                the scale becomes fresh where the call writes the block's first token (it starts anew), else the larger of
- *                fresh and what it was. New codes are x / scale, clamped to +-top, to nearest even; where the scale grew, the
- *                block's earlier tokens are rounded again, code * old / new. Tokens behind the written ones stay as they are.
+ *                fresh and what it was. New codes are x / scale, clamped to +-top, to nearest even (under a scale that is NaN or
+ *                infinite some code that is a number); where the scale grew, the block's earlier tokens are rounded again,
+ *                code * old / new. Tokens behind the written ones stay as they are.
  *   k_bounds     [num_blocks, num_kv_heads, 2, head_dim] bf16 or NULL: the least and the largest value of each dimension
  *                over a page's keys (the k given, before any rounding), likewise started anew by a page's first token. A NaN
  *                widens nothing.

@@ -248,12 +248,14 @@ void kv_store_blocks_kernel(BlockStoreArgs a) {
         most = __builtin_amdgcn_readfirstlane(most | wild);
       }
       if (pieces == 0) continue;
-      tame = most < kWild;
       const float amax = bf16_bits_to_f32((uint32_t)most & 0xffffu);
       const float nan_f = __uint_as_float(0x7fc00000u);
       s = amax != amax ? nan_f : fmaxf(amax * (1.0f / top), kLeastBlockScale);
       if (from > head) s = s != s || had != had ? nan_f : fmaxf(s, had);
       rs = 1.0f / s;
+      // (a block whose scale was no number gives quotients that are none: clamped they are codes that are numbers, which a
+      // probability of 0 times gives 0, so that the block reaches nobody who does not see it)
+      tame = most < kWild && s < INFINITY;
       // the block's earlier tokens, where the scale grew, four rows' loads in flight
       if (from > head && s > had) {
         for (int32_t at0 = head + part * RP + row0; at0 < from; at0 += 4 * TEAM * RP) {

@@ -178,6 +178,41 @@ def test_missing_pages_and_nan(fmt):
         assert float(((out - want).abs() - off)[clean].max()) <= 1e-30
 
 
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_stores_behind_a_nan_token(d, fmt):
+    """A NaN token makes its block NaN; tokens that later calls store in that block reach nobody who does not see it: queries
+    whose window has left it, and earlier queries of a chunk that two calls stored."""
+    announce(f"prefill behind a NaN token {fmt} d={d}")
+    G, H, P, n = 2, 4, 16, 240
+    g = gen(d)
+    table = (torch.randperm(n // P, generator=g) + 1).to(torch.int32).view(1, -1)
+    tab = table.to(DEV)
+    for window, nan_at, calls in ((20, 36, (36, 37, n)), (0, 50, (52, n))):
+        caches = [torch.zeros(n // P + 1, G, P, d, dtype=FMTS[fmt], device=DEV) for _ in range(2)]
+        scales = [torch.zeros(n // P + 1, G, 1, device=DEV) for _ in range(2)]
+        k, v = (tokens(g, n, G, d).to(torch.bfloat16) for _ in range(2))
+        k[nan_at, 0, 3] = v[nan_at, 0, 7] = math.nan
+        at = 0
+        for end in calls:
+            ops.kv_store_blocks(k[at:end].to(DEV), v[at:end].to(DEV), *caches, tab, _i32([at]).to(DEV),
+                                q_start=_i32([0, end - at]).to(DEV), max_q_len=end - at, k_scale=scales[0], v_scale=scales[1])
+            at = end
+        prior = calls[-2] if window else 0
+        q = torch.randn(n - prior, H, d, generator=g).to(torch.bfloat16)
+        args = (q, *(c.cpu() for c in caches), *(s.cpu() for s in scales), table, [0, n - prior])
+        got = _run(*args, [prior], sm_scale=0.125, window=window).cpu().double()
+        want, off = ob.prefill(q, *args[1:3], table, [0, n - prior], [prior], sm_scale=0.125, k_scale=args[3], v_scale=args[4],
+                               window=window, q_off=2.0 ** -16 * 1.02 if fmt == "int8" else 0.0)
+        first = nan_at - nan_at % P  # the block that is NaN, for KV head 0
+        sees = torch.tensor([prior + i >= first and (window == 0 or prior + i - window + 1 < first + P) for i in range(n - prior)])
+        assert bool(got[sees, :H // G].isnan().all())
+        clean = torch.ones(n - prior, H, dtype=torch.bool)
+        clean[sees, :H // G] = False
+        assert bool(torch.isfinite(got[clean]).all()), int(got[clean].isnan().any(-1).sum())
+        assert float(((got - want).abs() - off)[clean].max()) <= 1e-30
+
+
 @pytest.mark.parametrize("d,lens", [(64, (9, 40)), (128, (60, 3)), (64, (700, 300))])
 def test_bf16_rows_without_pages(d, lens):
     """bf16 caches: requests whose table names no page give zeros, whatever the output held, the others their attention."""

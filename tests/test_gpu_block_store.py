@@ -145,6 +145,29 @@ def test_special_elements(fmt):
         assert torch.equal(got[4].cpu().float() + 0.0, bounds.float() + 0.0)
 
 
+@pytest.mark.parametrize("bt", [16, 64, 128])  # a wave, two and four waves a block
+@pytest.mark.parametrize("had", [math.nan, math.inf])
+def test_no_code_is_nan_behind_a_scale_that_is_no_number(bt, had):
+    """Finite tokens behind a block whose scale is NaN (a NaN token before them) or infinite: the scale stays, and their e4m3fn
+    codes are numbers, so that a product with a probability of 0 is 0."""
+    announce(f"store behind a scale of {had} bt={bt}")
+    G, d, P = 2, 128, 128
+    g = gen(bt)
+    caches = [torch.zeros(3, G, P, d, dtype=FMTS["fp8"], device=DEV) for _ in range(2)]
+    scales = [torch.full((3, G, P // bt), had, device=DEV) for _ in range(2)]
+    table = torch.tensor([[1, 2]], dtype=torch.int32, device=DEV)
+    at = 5
+    for n in (1, 9, 120):
+        k, v = (tokens(g, n, G, d).to(torch.bfloat16).to(DEV) for _ in range(2))
+        ops.kv_store_blocks(k, v, *caches, table, torch.tensor([at], dtype=torch.int32, device=DEV),
+                            q_start=torch.tensor([0, n], dtype=torch.int32, device=DEV), max_q_len=n, k_scale=scales[0],
+                            v_scale=scales[1])
+        at += n
+        for c, s in zip(caches, scales):
+            assert bool(((c.view(torch.uint8) & 0x7F) != 0x7F).all()), n
+            assert bool((s[1, :, 0].isnan() if math.isnan(had) else s[1, :, 0].isinf()).all())
+
+
 @pytest.mark.parametrize("fmt", ["int8", "bf16"])
 def test_tokens_without_a_page_are_not_stored(fmt):
     """Entries outside the pool, columns past the table, chunks longer than max_q_len, a negative position."""
