@@ -542,8 +542,9 @@ int sna_prefill_attention_blocks(const void *q, const void *k_cache, const void 
 
 /* The score of each page of a query's row, from the pages' key bounds: scores[t, g, c] = max over KV head g's query heads of
  * sum_d max(q_d lo_d, q_d hi_d), which no key of the page in column c exceeds; -inf past the row's pages and on invalid
- * ones. scores [T, num_kv_heads, table_width] fp32; counts [T] int32: the rows' pages, ceil(seq_lens / page_size), for a
- * selection by the scores (sna_select_tokens). The other arguments as above. */
+ * ones. A product with an element q_d = 0 is 0, infinite bounds included (where q_d takes one the score is infinite), and a
+ * head whose sum is NaN counts only where all of them are. scores [T, num_kv_heads, table_width] fp32; counts [T] int32: the
+ * rows' pages, ceil(seq_lens / page_size), for a selection by the scores (sna_select_tokens). The other arguments as above. */
 int sna_block_scores(const void *q, const void *k_bounds, const int32_t *block_table, int64_t table_stride,
                      int32_t table_width, int32_t table_rows, const int32_t *rows, const int32_t *seq_lens, float *scores,
                      int32_t *counts, int32_t T, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,

@@ -148,7 +148,8 @@ def prefill(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, q_start:
 
 def scores(q: Tensor, bounds: Tensor, table: Tensor, lens: Sequence[int], P: int,
            rows: Optional[Sequence[int]] = None) -> tuple[Tensor, Tensor, list[int]]:
-    """([T, G, W] float64 scores, the sums of magnitudes that their rounding errors are relative to, the rows' pages)."""
+    """([T, G, W] float64 scores, the sums of magnitudes that their rounding errors are relative to, the rows' pages). A product
+    with a query element of 0 is 0, whatever the bounds; a head whose sum is NaN counts only where all of them are."""
     T, H, d = q.shape
     nb, G = bounds.shape[:2]
     grp, W = H // G, table.shape[1]
@@ -166,7 +167,8 @@ def scores(q: Tensor, bounds: Tensor, table: Tensor, lens: Sequence[int], P: int
             for g in range(G):
                 x = q[t, g * grp:(g + 1) * grp].double()
                 lo, hi = bounds[page, g, 0].double(), bounds[page, g, 1].double()
-                each = torch.maximum(x * lo, x * hi)
-                out[t, g, c] = each.sum(-1).max()
+                each = torch.where(x == 0, 0.0, torch.maximum(x * lo, x * hi))
+                heads = each.sum(-1)
+                out[t, g, c] = heads.max() if bool(heads.isnan().all()) else heads[~heads.isnan()].max()
                 size[t, g, c] = each.abs().sum(-1).max()
     return out, size, counts

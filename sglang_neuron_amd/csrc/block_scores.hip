@@ -1,7 +1,8 @@
 // Score of a row's pages for a query, from the bounds of each page's keys: no key k with lo <= k <= hi (dimension by
 // dimension) gives a head more than sum_d max(q_d lo_d, q_d hi_d), and
 //   score[t, g, c] = max over the query heads of KV head g of that sum for the page in column c of the query's table row,
-// -inf past the row's pages and on invalid ones. As max(q lo, q hi) is q hi for q >= 0 and q lo for q <= 0, the sum is the
+// -inf past the row's pages and on invalid ones; a product with a query element of 0 is 0, and a head whose sum is NaN counts
+// only where all of them are. As max(q lo, q hi) is q hi for q >= 0 and q lo for q <= 0, the sum is the
 // product of the page's [lo, hi] with [min(q, 0), max(q, 0)]: 2 D long, on the matrix cores.
 //
 // Work: one wave per 16 pages of a (query, KV head), 4 waves a workgroup. v_mfma_f32_16x16x32_bf16 with M = 16 pages, N =
@@ -30,6 +31,36 @@ struct BlockScoreArgs {
   int32_t runs;  // workgroups of a (query, KV head)
   int64_t num_blocks;
 };
+
+// The sums of a lane's pages (4 g4 + r, whose bounds are at the lanes' `at`) and head (elements qp) by their definition, one
+// element after the other: where bounds are infinite (infinite keys; lo = inf, hi = -inf: a dimension whose keys are all NaN),
+// as their products with the zeros of [min(q, 0), max(q, 0)] are NaN.
+template <int D>
+__device__ __forceinline__ f32x4_t block_scores_defined(const uint16_t* bounds, int64_t at, const uint16_t* qp) {
+  const int lane = threadIdx.x & 63, g4 = lane >> 4;
+  f32x4_t sums = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int r = 0; r < 4; ++r) {
+    const int src = 16 * g4 + 4 * g4 + r;
+    const uint16_t* b = bounds + __shfl((long long)at, src);
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int d = 0; d < D; d += 8) {
+      const uint4 wl = ld16(b + d), wh = ld16(b + D + d), wq = ld16(qp + d);
+      const uint32_t l[4] = {wl.x, wl.y, wl.z, wl.w}, h[4] = {wh.x, wh.y, wh.z, wh.w}, q[4] = {wq.x, wq.y, wq.z, wq.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int up = e & 1 ? 0 : 16;  // an element's bits to the upper half
+        const float f = __uint_as_float(q[e >> 1] << up & 0xffff0000u);
+        const float lo = __uint_as_float(l[e >> 1] << up & 0xffff0000u), hi = __uint_as_float(h[e >> 1] << up & 0xffff0000u);
+        sum += f == 0.0f ? 0.0f : fmaxf(f * lo, f * hi);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sums[k] = r == k ? sum : sums[k];
+  }
+  return sums;
+}
 
 template <int D>
 __global__ __launch_bounds__(256) void block_scores_kernel(BlockScoreArgs a) {
@@ -81,12 +112,16 @@ __global__ __launch_bounds__(256) void block_scores_kernel(BlockScoreArgs a) {
     acc = mfma_16x16x32_bf16(bv[s], neg[s], acc);
     acc = mfma_16x16x32_bf16(bv[HS + s], pos[s], acc);
   }
+  const uint64_t okm = __ballot(ok);  // (bit li of each 16: column c0 + li)
+  bool infinite = false;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) infinite |= !(fabsf(acc[r]) < INFINITY) && (okm >> (4 * g4 + r) & 1);
+  if (__any(infinite)) acc = block_scores_defined<D>(a.bounds, b - a.bounds - 8 * g4, qp - 8 * g4);
   // (a lane past the group repeats its last head)
   float best[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) best[r] = row16_max(acc[r]);
   const float mine = li == 0 ? best[0] : (li == 1 ? best[1] : (li == 2 ? best[2] : best[3]));
-  const uint64_t okm = __ballot(ok);  // (bit li of each 16: column c0 + li)
   const int32_t at = 4 * g4 + li;
   if (li < 4 && c0 + at < a.table_width)
     a.scores[((int64_t)t * a.G + g) * a.table_width + c0 + at] = (okm >> at) & 1 ? mine : -INFINITY;

@@ -1509,7 +1509,9 @@ def block_scores(q: Tensor, k_bounds: Tensor, block_table: Tensor, seq_lens: Ten
     """What a page can give a query at the most: (scores [T, G, width] fp32, counts [T] int32), scores[t, g, c] the largest,
     over the query heads of KV head g, of sum_d max(q_d lo_d, q_d hi_d) with the bounds ``k_bounds`` [blocks, G, 2, d] bf16
     (kv_store_blocks) of the page in column c of query t's table row; -inf past the row's ceil(seq_lens / page_size) = counts
-    pages and where the table names no page. The other arguments are paged_decode_blocks'."""
+    pages and where the table names no page. A product with q_d = 0 is 0; where a head takes an infinite key's bound, or one of
+    a dimension whose keys are all NaN, its sum is infinite; a head whose sum is NaN counts only where all of them are. The
+    other arguments are paged_decode_blocks'."""
     dev = _on_gpu(q, k_bounds, block_table, seq_lens, rows)
     q, table, stride, lens, rows = _query_rows(q, block_table, seq_lens, rows)
     T, H, d = q.shape

@@ -360,6 +360,79 @@ def test_scores(H, G, d, P):
         assert bool(((got - want).abs()[ok] <= 2 * d * 2.0 ** -24 * size[ok]).all())
 
 
+@pytest.mark.parametrize("H,G,d,P", [(4, 2, 128, 16), (3, 3, 64, 48), (16, 1, 64, 64), (10, 2, 128, 128)])
+def test_scores_of_infinite_bounds(H, G, d, P):
+    """Pages with infinite keys and with dimensions that are NaN in every key, as the writer leaves their bounds, among ordinary
+    ones; query elements of 0, infinite and NaN. Infinite and NaN scores are the definition's, the others as near as ever."""
+    announce(f"scores, infinite bounds H={H} G={G} d={d} P={P}")
+    lens, inf = [64 * P, 3 * P, 20 * P], math.inf
+    g = gen(P + 1)
+    table, nb = table_of(g, lens, P)
+    b = tokens(g, nb, G, 3, d)
+    bounds = torch.stack([b.amin(2), b.amax(2)], 2).to(torch.bfloat16)
+    kinds = [(-inf, None), (None, inf), (-inf, inf), (inf, -inf), (inf, inf), (-inf, -inf)]
+    for c in range(64):  # (every third page of row 0, one to three dimensions of each KV head; all pages of row 1)
+        for r in range(2):
+            if (r == 0 and c % 3) or (r == 1 and c > 2):
+                continue
+            for gg in range(G):
+                for at in torch.randperm(d, generator=g)[:1 + c % 3].tolist():
+                    lo, hi = kinds[int(torch.randint(len(kinds), (1,), generator=g))]
+                    page = int(table[r, c])
+                    if lo is not None:
+                        bounds[page, gg, 0, at] = lo
+                    if hi is not None:
+                        bounds[page, gg, 1, at] = hi
+    rows = [0, 0, 0, 1, 1, 2, 2]
+    q = torch.randn(len(rows), H, d, generator=g).to(torch.bfloat16)
+    q[1, :, ::2] = 0.0
+    q[1, :, 1::4] = -0.0
+    q[2, 0, 5], q[2, H - 1, 7], q[4, 0, 1], q[6, H - 1, 2] = math.nan, inf, math.nan, -inf
+    at = [lens[r] for r in rows]
+    want, size, counts = ob.scores(q, bounds, table, at, P, rows)
+    got, n = ops.block_scores(*to(DEV, q, bounds, table, _i32(at)), page_size=P, rows=_i32(rows).to(DEV))
+    assert n.tolist() == counts
+    got = got.cpu().double()
+    assert torch.equal(got.isnan(), want.isnan()), (int(got.isnan().sum()), int(want.isnan().sum()))
+    fin = torch.isfinite(want)
+    assert torch.equal(got[~fin & ~want.isnan()], want[~fin & ~want.isnan()])
+    assert int((want == inf).sum()) > 20 and int(fin.sum()) > 20
+    # (a finite score among heads whose own sums are infinite: its magnitudes are at most those of all finite bounds)
+    fb = torch.where(bounds.double().isinf(), 0.0, bounds.double())
+    for t, r in enumerate(rows):
+        for gg in range(G):
+            for c in range(counts[t]):
+                if fin[t, gg, c]:
+                    x = torch.nan_to_num(q[t, gg * (H // G):(gg + 1) * (H // G)].double(), posinf=0.0, neginf=0.0)
+                    most = float((x.abs() @ fb[int(table[r, c]), gg].abs().amax(0)).max())
+                    assert abs(float(got[t, gg, c] - want[t, gg, c])) <= 2 * d * 2.0 ** -24 * most
+
+
+def test_a_page_of_infinite_keys_is_selected():
+    """Stored with bounds: an infinite key's page scores what its other heads and elements give, or is the first of all."""
+    announce("selection, infinite keys")
+    G, d, P, keep = 1, 64, 16, 3
+    g = gen(8)
+    k = torch.randint(-4, 5, (10 * P, G, d), generator=g).to(torch.bfloat16)
+    k[5 * P + 3, 0, 7] = math.inf    # q's element 7 is positive: page 5 is the first of all
+    k[7 * P, 0, 9] = -math.inf       # q's element 9 is positive: page 7 by its other elements
+    caches = [torch.zeros(11, G, P, d, dtype=torch.int8, device=DEV) for _ in range(2)]
+    scales = [torch.zeros(11, G, 1, device=DEV) for _ in range(2)]
+    bounds = torch.zeros(11, G, 2, d, dtype=torch.bfloat16, device=DEV)
+    table = (torch.randperm(10, generator=g) + 1).to(torch.int32).view(1, 10)
+    ops.kv_store_blocks(k.to(DEV), k.to(DEV).nan_to_num(posinf=0.0, neginf=0.0), *caches, table.to(DEV), _i32([0]).to(DEV),
+                        q_start=_i32([0, 10 * P]).to(DEV), max_q_len=10 * P, k_scale=scales[0], v_scale=scales[1],
+                        k_bounds=bounds)
+    q = torch.randint(1, 5, (1, 2, d), generator=g).to(torch.bfloat16)
+    want, _, pages = ob.scores(q, bounds.cpu(), table, [10 * P], P)
+    assert want[0, 0, 5] == math.inf and bool(torch.isfinite(want[0, 0, 7]))
+    got, _ = ops.block_scores(q.to(DEV), bounds, table.to(DEV), _i32([10 * P]).to(DEV), page_size=P)
+    assert torch.equal(got.cpu().double(), want)  # (small whole numbers: exact)
+    chosen, _ = ow.select_tokens(want.float(), pages, keep, 0, 0)
+    sel = ops.select_blocks(q.to(DEV), bounds, table.to(DEV), _i32([10 * P]).to(DEV), keep=keep, page_size=P, first=0, recent=0)
+    assert torch.equal(sel.cpu(), chosen) and 5 in chosen[0, 0].tolist()
+
+
 def test_writer_to_selection_to_attention():
     """The operators as they are used: chunks, then tokens, appended with bounds; each query's pages selected; attention over
     them. Scores of small whole numbers are exact, so the selection has to be the definition's."""

@@ -70,6 +70,23 @@ def test_bounds_hold_every_key():
     assert ob.scores(q, bounds, table, [0], 16)[2] == [0]
 
 
+def test_scores_of_infinite_bounds():
+    """A bound that a query element does not take, or takes times 0, does not count; one that counts makes the score infinite."""
+    inf = math.inf
+    # of two dimensions: (lo, hi) of each page
+    pages = [([-inf, -1.0], [2.0, 3.0]), ([-1.0, -1.0], [inf, 3.0]), ([inf, -1.0], [-inf, 3.0]), ([-inf, -1.0], [-inf, 3.0])]
+    bounds = torch.tensor([[lo, hi] for lo, hi in pages]).to(torch.bfloat16).view(4, 1, 2, 2)
+    table = torch.arange(4).view(1, 4)
+    for q, want in (([1.0, 1.0], [5.0, inf, inf, -inf]), ([-1.0, 1.0], [inf, 4.0, inf, inf]), ([0.0, -2.0], [2.0] * 4)):
+        s, _, _ = ob.scores(torch.tensor(q, dtype=torch.bfloat16).view(1, 1, 2), bounds, table, [64], 16)
+        assert s.reshape(-1).tolist() == want
+    # infinities of both signs are no number: the head counts only where it is alone
+    bounds = torch.tensor([[-inf, 1.0], [-inf, inf]]).to(torch.bfloat16).view(1, 1, 2, 2)
+    q = torch.tensor([[1.0, 1.0], [0.0, -2.0]], dtype=torch.bfloat16).view(1, 2, 2)
+    assert ob.scores(q, bounds, table[:, :1], [16], 16)[0].item() == -2.0
+    assert ob.scores(q[:, :1], bounds, table[:, :1], [16], 16)[0].isnan().all()
+
+
 def test_attention_of_equal_keys():
     G, d, P = 1, 8, 16
     table = torch.tensor([[2, 1]])
