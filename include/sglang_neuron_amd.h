@@ -701,7 +701,8 @@ int sna_window_table(const int32_t *table, int64_t table_stride, int32_t table_w
 
 /* A pool's regions as its get_contiguous_buf_infos gives them (host arrays of n_regions): region r is region_lens[r]
  * bytes at device address region_ptrs[r], page p its item_lens[r] bytes at region_ptrs[r] + p * item_lens[r]
- * (addresses and item sizes multiples of 16, items under 2 GiB, under 2^31 items a region). pages: device int32
+ * (addresses and item sizes multiples of 16, for sna_page_items_copy of 4, so that a page's scales move too; items under
+ * 2 GiB, under 2^31 items a region). pages: device int32
  * [n_pages]. Every call moves whole items, one workgroup per (page, region), in launches of up to 96 regions on
  * `stream`.
  * Replaces: the page-item addressing of NeuronMHATokenToKVPool.get_contiguous_buf_infos (mem_cache/memory_pool.py:

@@ -14,7 +14,8 @@
 //   copy:    item (r, src_pages[i]) of the source regions to item (r, dst_pages[i]) of the destination regions
 //            (the transfer's WRITE list on one GPU).
 // One workgroup per (item, region), 16-byte non-temporal loads and stores (every byte is touched once); HBM-bound:
-// 2 bytes of traffic per byte moved.
+// 2 bytes of traffic per byte moved. A copy also takes items and addresses that are multiples of 4 (the scales of a page whose
+// blocks of tokens carry them: 4 bytes and up), word by word; a wire buffer's regions start on 16 bytes.
 
 #include <cstring>
 #include <vector>
@@ -29,9 +30,9 @@ constexpr int kItemRegions = 96;
 
 struct ItemRegion {
   uint64_t src, dst;         // base addresses of the item arrays read and written
-  int32_t item;              // bytes per item (a multiple of 16)
+  int32_t item;              // bytes per item (a multiple of 16, of 4 where words is set)
   int32_t src_cap, dst_cap;  // items in each array
-  int32_t pad;
+  int32_t words;             // moved 4 bytes at a time
 };
 static_assert(sizeof(ItemRegion) == 32, "a 32-byte region record");
 
@@ -48,6 +49,13 @@ __global__ __launch_bounds__(256) void page_items_kernel(PageItemsArgs a) {
   const int64_t sp = a.src_pages ? (int64_t)a.src_pages[i] : i;
   const int64_t dp = a.dst_pages ? (int64_t)a.dst_pages[i] : i;
   if (dp < 0 || dp >= g.dst_cap) return;  // (uniform) nowhere to write
+  if (g.words) {  // (uniform; copies only)
+    if (sp < 0 || sp >= g.src_cap) return;
+    const uint32_t* s = reinterpret_cast<const uint32_t*>(g.src + (uint64_t)sp * (uint64_t)g.item);
+    uint32_t* d = reinterpret_cast<uint32_t*>(g.dst + (uint64_t)dp * (uint64_t)g.item);
+    for (int32_t v = threadIdx.x; v < g.item >> 2; v += 256) d[v] = s[v];
+    return;
+  }
   typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
   u32x4_t* dst = reinterpret_cast<u32x4_t*>(g.dst + (uint64_t)dp * (uint64_t)g.item);
   const int32_t n = g.item >> 4;  // 16-byte vectors
@@ -75,15 +83,15 @@ namespace {
 
 // Validates the host region description; *total_item_bytes = the bytes of one page over all regions.
 int check_regions(const char* what, const uint64_t* ptrs, const int64_t* lens, const int64_t* item_lens,
-                  int32_t n_regions, int64_t* total_item_bytes) {
+                  int32_t n_regions, int unit, int64_t* total_item_bytes) {
   int64_t total = 0;
   for (int32_t r = 0; r < n_regions; ++r) {
-    if (!ptrs[r] || item_lens[r] <= 0 || item_lens[r] % 16 != 0 || ptrs[r] % 16 != 0 || lens[r] < 0 ||
+    if (!ptrs[r] || item_lens[r] <= 0 || item_lens[r] % unit != 0 || ptrs[r] % unit != 0 || lens[r] < 0 ||
         item_lens[r] > 0x7fffffffLL || lens[r] / item_lens[r] > 0x7fffffffLL)
       return fail(SNA_ERR_INVALID_ARGUMENT,
                   "%s: region %d (address %llx, %lld bytes, items of %lld bytes): the address and the item size "
-                  "must be non-zero multiples of 16, items under 2 GiB and fewer than 2^31 of them",
-                  what, r, (unsigned long long)ptrs[r], (long long)lens[r], (long long)item_lens[r]);
+                  "must be non-zero multiples of %d, items under 2 GiB and fewer than 2^31 of them",
+                  what, r, (unsigned long long)ptrs[r], (long long)lens[r], (long long)item_lens[r], unit);
     total += item_lens[r];
   }
   if (total_item_bytes) *total_item_bytes = total;
@@ -133,7 +141,7 @@ int sna_page_items_pack(const uint64_t* region_ptrs, const int64_t* region_lens,
   if (!region_ptrs || !region_lens || !item_lens || !pages || !wire)
     return fail(SNA_ERR_INVALID_ARGUMENT, "page_items_pack: null pointer");
   int64_t per_page = 0;
-  if (int rc = check_regions("page_items_pack", region_ptrs, region_lens, item_lens, n_regions, &per_page)) return rc;
+  if (int rc = check_regions("page_items_pack", region_ptrs, region_lens, item_lens, n_regions, 16, &per_page)) return rc;
   if (!aligned(wire, 16)) return fail(SNA_ERR_INVALID_ARGUMENT, "page_items_pack: the wire buffer must be 16-B aligned");
   if (wire_bytes < per_page * n_pages)
     return fail(SNA_ERR_WORKSPACE, "page_items_pack: a wire buffer of %lld bytes, the items need %lld",
@@ -161,7 +169,7 @@ int sna_page_items_unpack(const void* wire, int64_t wire_bytes, const uint64_t* 
   if (!region_ptrs || !region_lens || !item_lens || !pages || !wire)
     return fail(SNA_ERR_INVALID_ARGUMENT, "page_items_unpack: null pointer");
   int64_t per_page = 0;
-  if (int rc = check_regions("page_items_unpack", region_ptrs, region_lens, item_lens, n_regions, &per_page))
+  if (int rc = check_regions("page_items_unpack", region_ptrs, region_lens, item_lens, n_regions, 16, &per_page))
     return rc;
   if (!aligned(wire, 16))
     return fail(SNA_ERR_INVALID_ARGUMENT, "page_items_unpack: the wire buffer must be 16-B aligned");
@@ -190,14 +198,15 @@ int sna_page_items_copy(const uint64_t* src_ptrs, const int64_t* src_lens, const
   if (n_regions == 0 || n_pages == 0) return SNA_OK;
   if (!src_ptrs || !src_lens || !dst_ptrs || !dst_lens || !item_lens || !src_pages || !dst_pages)
     return fail(SNA_ERR_INVALID_ARGUMENT, "page_items_copy: null pointer");
-  if (int rc = check_regions("page_items_copy", src_ptrs, src_lens, item_lens, n_regions, nullptr)) return rc;
-  if (int rc = check_regions("page_items_copy", dst_ptrs, dst_lens, item_lens, n_regions, nullptr)) return rc;
+  if (int rc = check_regions("page_items_copy", src_ptrs, src_lens, item_lens, n_regions, 4, nullptr)) return rc;
+  if (int rc = check_regions("page_items_copy", dst_ptrs, dst_lens, item_lens, n_regions, 4, nullptr)) return rc;
   return launch_items("page_items_copy", n_regions, n_pages, src_pages, dst_pages, 0, (hipStream_t)stream,
                       [&](PageItemsArgs& a, int32_t r0, int32_t nr) {
                         for (int32_t j = 0; j < nr; ++j) {
                           const int32_t r = r0 + j;
+                          const int32_t words = (src_ptrs[r] | dst_ptrs[r] | (uint64_t)item_lens[r]) % 16 != 0;
                           a.r[j] = {src_ptrs[r], dst_ptrs[r], (int32_t)item_lens[r],
-                                    (int32_t)(src_lens[r] / item_lens[r]), (int32_t)(dst_lens[r] / item_lens[r]), 0};
+                                    (int32_t)(src_lens[r] / item_lens[r]), (int32_t)(dst_lens[r] / item_lens[r]), words};
                         }
                       });
 }

@@ -1735,7 +1735,8 @@ def unpack_page_items(wire: Tensor, infos, pages: Tensor) -> None:
 def copy_page_items(src_infos, dst_infos, src_pages: Tensor, dst_pages: Tensor) -> None:
     """The transfer's WRITE list on one GPU: item (r, src_pages[i]) of the source pool's regions to item (r,
     dst_pages[i]) of the destination's (disaggregation/state_transfer.py:9-10), items of the source's item_lens[r]
-    bytes (a destination page holding several source items is addressed in source-item units). A page outside its
+    bytes (a destination page holding several source items is addressed in source-item units). Items and addresses are
+    multiples of 4 bytes (a page's scales are a region like its codes), of 16 they move faster. A page outside its
     region is skipped; ``dst_pages`` must be distinct."""
     dev = _on_gpu(src_pages, dst_pages)
     sp, dp = _pages(src_pages, "copy_page_items"), _pages(dst_pages, "copy_page_items")

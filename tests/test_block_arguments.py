@@ -3,6 +3,8 @@ followed, and tensors lie on the meta device where a device is asked for."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -126,6 +128,24 @@ PREFILL = [("q", A), ("k_cache", A), ("v_cache", A), ("ks", A), ("vs", A), ("s_p
 ])
 def test_prefill_refusals(change, code, text):
     _refused("sna_prefill_attention_blocks", PREFILL, change, code, text)
+
+
+@pytest.mark.parametrize("src,dst,item", [(A, 2 * A, 6), (A, 2 * A, 2), (A + 2, 2 * A, 4), (A, 2 * A + 1, 4), (A, 2 * A, 0)])
+def test_page_copies_of_broken_words(src, dst, item):
+    """Pages' scales are copied as items of whole words (on whole words)."""
+    lens, items = (ctypes.c_int64 * 1)(64), (ctypes.c_int64 * 1)(item)
+    rc = _lib.load().sna_page_items_copy((ctypes.c_uint64 * 1)(src), lens, (ctypes.c_uint64 * 1)(dst), lens, items, 1, A, A, 3,
+                                         None)
+    assert rc == -1 and "multiples of 4" in _lib.last_error()
+
+
+@pytest.mark.parametrize("item", [4, 24])
+def test_wire_buffers_hold_whole_vectors(item):
+    lens, items, ptrs = (ctypes.c_int64 * 1)(96), (ctypes.c_int64 * 1)(item), (ctypes.c_uint64 * 1)(A)
+    lib = _lib.load()
+    for rc in (lib.sna_page_items_pack(ptrs, lens, items, 1, A, 2, A, 4096, None),
+               lib.sna_page_items_unpack(A, 4096, ptrs, lens, items, 1, A, 2, None)):
+        assert rc == -1 and "multiples of 16" in _lib.last_error()
 
 
 def test_int8_is_for_blocks_only():

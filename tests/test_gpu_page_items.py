@@ -121,6 +121,59 @@ def test_copy_into_replicated_pages():
     assert torch.equal(dst.cpu(), want)
 
 
+def test_copy_of_small_items():
+    """Items and addresses that are multiples of 4 bytes only, beside a region of whole vectors: bytes around them stay."""
+    announce("page items copy, multiples of 4")
+    g = torch.Generator().manual_seed(9)
+    items, offs = [4, 12, 20, 1028, 64, 64, 4112], [0, 4, 8, 0, 4, 0, 12]
+    src = [torch.randint(0, 256, (o + il * 9 + 4,), dtype=torch.uint8, generator=g) for il, o in zip(items, offs)]
+    dst = [torch.randint(0, 256, (o + il * 7 + 4,), dtype=torch.uint8, generator=g) for il, o in zip(items, offs)]
+    sp, dp = torch.tensor([8, 0, 9, 3, 5, -1], dtype=torch.int32), torch.tensor([1, 6, 2, 7, 0, 3], dtype=torch.int32)
+    ds, dd = [t.to(DEV) for t in src], [t.to(DEV) for t in dst]
+    infos = [([t.data_ptr() + o for t, o in zip(ts, offs)], [il * n for il in items], items) for ts, n in ((ds, 9), (dd, 7))]
+    ops.copy_page_items(*infos, sp.to(DEV), dp.to(DEV))
+    opi.copy([t[o:o + il * 9] for t, o, il in zip(src, offs, items)], [t[o:o + il * 7] for t, o, il in zip(dst, offs, items)],
+             items, sp.tolist(), dp.tolist())
+    for a, b in zip(dd, dst):
+        assert torch.equal(a.cpu(), b)
+
+
+@pytest.mark.parametrize("G,P,bt", [(1, 16, 16), (3, 64, 64), (2, 64, 32), (5, 128, 128), (8, 64, 16)])
+@pytest.mark.parametrize("dtype", [torch.int8, FP8])
+def test_pages_move_with_their_block_scales(G, P, bt, dtype):
+    """A cache whose blocks of tokens carry scales: pages copied to others with scales and bounds, 4 bytes of scales a page and
+    up. What is attended, and what the next tokens make of a page that is not full, is the same on both."""
+    announce(f"page items copy, block scales G={G} P={P} bt={bt} {dtype}")
+    g = torch.Generator().manual_seed(G)
+    d, n = 64, 2 * P + 5
+    caches = [torch.zeros(8, G, P, d, dtype=dtype, device=DEV) for _ in range(2)]
+    scales = [torch.zeros(8, G, P // bt, device=DEV) for _ in range(2)]
+    bounds = torch.zeros(8, G, 2, d, dtype=torch.bfloat16, device=DEV)
+    q = torch.randn(1, 2 * G, d, generator=g).to(torch.bfloat16).to(DEV)
+
+    def i32(v):
+        return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+    def store(table, at, k, v):
+        ops.kv_store_blocks(k, v, *caches, table, i32([at]), q_start=i32([0, k.shape[0]]), max_q_len=k.shape[0],
+                            k_scale=scales[0], v_scale=scales[1], k_bounds=bounds)
+    old, new = i32([[5, 1, 6]]), i32([[2, 7, 3]])
+    store(old, 0, *(torch.randn(n, G, d, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2)))
+    tensors = [*caches, *scales, bounds]
+    infos = ([t.data_ptr() for t in tensors], [t.numel() * t.element_size() for t in tensors],
+             [t[0].numel() * t.element_size() for t in tensors])
+    ops.copy_page_items(infos, infos, old[0], new[0])
+    more = [(3 * torch.randn(4, G, d, generator=g)).to(torch.bfloat16).to(DEV) for _ in range(2)]
+    got = []
+    for table in (old, new):
+        store(table, n, *more)
+        out = ops.paged_decode_blocks(q, *caches, table, i32([n + 4]), sm_scale=0.125, k_scale=scales[0], v_scale=scales[1])
+        s, _ = ops.block_scores(q, bounds, table, i32([n + 4]), page_size=P)
+        got.append((out.cpu(), s.cpu()))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    assert bool((got[0][0] != 0).any())
+
+
 def test_transfer_then_decode_matches():
     """A request's pages moved from a 'prefill' pool to other pages of a 'decode' pool (every layer's K and V): a GQA
     decode over the destination table gives exactly the source's output."""
