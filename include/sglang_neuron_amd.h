@@ -524,7 +524,7 @@ int sna_paged_decode_blocks(const void *q, const void *k_cache, const void *v_ca
 
 /* sna_prefill_attention_split over such a pool: a batch of chunks, causal. Scales as in sna_paged_decode_blocks, the rest,
  * as in sna_prefill_attention_split, with a workspace of sna_prefill_blocks_workspace_bytes bytes. A query that sees no
- * key gives zeros. With int8 codes a query element is taken to within 2^-16 of its row's largest. A V element that is no
+ * key gives zeros. With int8 codes a query element is taken to within 1.56e-5 of its row's largest. A V element that is no
  * finite number (bf16; e4m3fn codes of NaN, which sna_kv_store_blocks never writes) also reaches earlier queries of the
  * chunk, those that share its matrix products. n_queries: q's rows (q_start[R]). */
 int64_t sna_prefill_blocks_workspace_bytes(int32_t n_queries, int32_t R, int32_t max_q_len, int32_t num_q_heads,

@@ -12,6 +12,9 @@ from torch import Tensor
 
 FP8 = torch.float8_e4m3fn
 LEAST_SCALE = 2.0 ** -100
+# What a prompt's query element over int8 codes is off by, of its row's largest: half a step of 32600, the quotient 32600 / largest
+# and its product with the element rounded (2^-24 each, of up to 32600 steps), the step's size rounded (2^-24).
+INT8_QUERY_OFF = (0.5 + 32600 * 2.0 ** -23) / 32600 + 2.0 ** -24
 
 
 def top_of(dtype: torch.dtype) -> float:

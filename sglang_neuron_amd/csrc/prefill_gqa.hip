@@ -387,7 +387,8 @@ void prefill_gqa_kernel(PrefillArgsOf<SCALES> a) {
       }
   }
   // int8 codes take the query as whole numbers too, on v_mfma_i32_32x32x32_i8: the row times 32600 / its absolute maximum,
-  // to nearest (an element is off by at most 2^-16 of that maximum), as 256 hi + lo with hi and lo int8. The dot product
+  // to nearest, as 256 hi + lo with hi and lo int8 (an element is off by at most 1.56e-5 of that maximum: half a step of 32600,
+  // and the roundings of the quotient, its product and the unit, 2^-24 each). The dot product
   // with the codes is then exact: |256 sum hi k + sum lo k| < 2^30. An element that is no number makes the row NaN.
   float q_unit = 1.0f;
   if constexpr (INT8) {

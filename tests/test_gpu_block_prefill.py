@@ -203,7 +203,7 @@ def test_stores_behind_a_nan_token(d, fmt):
         args = (q, *(c.cpu() for c in caches), *(s.cpu() for s in scales), table, [0, n - prior])
         got = _run(*args, [prior], sm_scale=0.125, window=window).cpu().double()
         want, off = ob.prefill(q, *args[1:3], table, [0, n - prior], [prior], sm_scale=0.125, k_scale=args[3], v_scale=args[4],
-                               window=window, q_off=2.0 ** -16 * 1.02 if fmt == "int8" else 0.0)
+                               window=window, q_off=ob.INT8_QUERY_OFF if fmt == "int8" else 0.0)
         first = nan_at - nan_at % P  # the block that is NaN, for KV head 0
         sees = torch.tensor([prior + i >= first and (window == 0 or prior + i - window + 1 < first + P) for i in range(n - prior)])
         assert bool(got[sees, :H // G].isnan().all())

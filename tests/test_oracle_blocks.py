@@ -87,6 +87,21 @@ def test_scores_of_infinite_bounds():
     assert ob.scores(q[:, :1], bounds, table[:, :1], [16], 16)[0].isnan().all()
 
 
+def test_int8_query_rounding():
+    """The whole numbers that a prompt's queries become over int8 codes, step by step in fp32: every bf16 element up to 4 octaves
+    below every largest one of an octave. The stated bound holds, and 2^-16 would not."""
+    top = (1 + torch.arange(128) / 128.0).to(torch.float32)
+    x = torch.cat([top * 2.0 ** -e for e in range(5)])
+    worst = 0.0
+    for amp in top:
+        v = x[x <= amp]
+        n = torch.round(v * (torch.tensor(32600.0) / amp))
+        assert float(n.max()) == 32600
+        value = n.double() * (amp / torch.tensor(32600.0)).double()
+        worst = max(worst, float(((value - v.double()).abs() / amp.double()).max()))
+    assert 2.0 ** -16 < worst <= ob.INT8_QUERY_OFF < 1.56e-5
+
+
 def test_attention_of_equal_keys():
     G, d, P = 1, 8, 16
     table = torch.tensor([[2, 1]])
