@@ -525,8 +525,9 @@ int sna_paged_decode_blocks(const void *q, const void *k_cache, const void *v_ca
 /* sna_prefill_attention_split over such a pool: a batch of chunks, causal. Scales as in sna_paged_decode_blocks, the rest,
  * as in sna_prefill_attention_split, with a workspace of sna_prefill_blocks_workspace_bytes bytes. A query that sees no
  * key gives zeros. With int8 codes a query element is taken to within 1.56e-5 of its row's largest. A V element that is no
- * finite number (bf16; e4m3fn codes of NaN, which sna_kv_store_blocks never writes) also reaches earlier queries of the
- * chunk, those that share its matrix products. n_queries: q's rows (q_start[R]). */
+ * finite number (bf16; e4m3fn codes of NaN, which sna_kv_store_blocks never writes) also reaches queries of the chunk that do
+ * not see it but share its matrix products: up to 128 / group queries before it and, with a window, up to 128 / group + 63
+ * behind the last one that sees it. n_queries: q's rows (q_start[R]). */
 int64_t sna_prefill_blocks_workspace_bytes(int32_t n_queries, int32_t R, int32_t max_q_len, int32_t num_q_heads,
                                            int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
                                            int32_t table_width, int32_t window, int32_t cache_dtype);

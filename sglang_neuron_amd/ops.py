@@ -1465,7 +1465,8 @@ def prefill_attention_blocks(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_
     prior_lens[r] + i, causal, optionally windowed and with sinks [H]. ``max_q_len`` bounds the chunk lengths;
     ``host_q_start``: a host copy of q_start, checked before the launch. A query that sees no key gives zeros. Over int8
     codes a query element is taken to within 1.56e-5 of its row's largest. In bf16 caches a NaN or an infinity in V also reaches
-    queries of the chunk shortly before it (as in prefill_attention). Returns [T, H, d] bf16."""
+    queries that do not see it but share its matrix products (as in prefill_attention): up to 128 / group queries before it and,
+    with a window, up to 128 / group + 63 behind the last one that sees it. Returns [T, H, d] bf16."""
     dev = _on_gpu(q, k_cache, v_cache, block_table, q_start, prior_lens, k_scale, v_scale, sinks, out)
     code, (nb, G, P, dk), ks, vs, page, head, tokens = _block_cache(k_cache, v_cache, k_scale, v_scale)
     if q.dim() != 3 or q.dtype != torch.bfloat16 or q.shape[2] != dk or q.shape[1] % G:
