@@ -542,8 +542,9 @@ int sna_prefill_attention_blocks(const void *q, const void *k_cache, const void 
                                  void *stream);
 
 /* The score of each page of a query's row, from the pages' key bounds: scores[t, g, c] = max over KV head g's query heads of
- * sum_d max(q_d lo_d, q_d hi_d), which no key of the page in column c exceeds; -inf past the row's pages and on invalid
- * ones. A product with an element q_d = 0 is 0, infinite bounds included (where q_d takes one the score is infinite), and a
+ * sum_d max(q_d lo_d, q_d hi_d), which no key of the page in column c exceeds as it was given (as 8-bit codes hold it, each
+ * element is off by up to 2^-4 of itself, e4m3fn, or 2^-10 of its block's scale where that is more, or by half a scale, int8,
+ * and as much again each time the scale grew since); -inf past the row's pages and on invalid ones. A product with an element q_d = 0 is 0, infinite bounds included (where q_d takes one the score is infinite), and a
  * head whose sum is NaN counts only where all of them are. scores [T, num_kv_heads, table_width] fp32; counts [T] int32: the
  * rows' pages, ceil(seq_lens / page_size), for a selection by the scores (sna_select_tokens). The other arguments as above. */
 int sna_block_scores(const void *q, const void *k_bounds, const int32_t *block_table, int64_t table_stride,

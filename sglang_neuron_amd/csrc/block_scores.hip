@@ -1,5 +1,5 @@
 // Score of a row's pages for a query, from the bounds of each page's keys: no key k with lo <= k <= hi (dimension by
-// dimension) gives a head more than sum_d max(q_d lo_d, q_d hi_d), and
+// dimension, as given) gives a head more than sum_d max(q_d lo_d, q_d hi_d), and
 //   score[t, g, c] = max over the query heads of KV head g of that sum for the page in column c of the query's table row,
 // -inf past the row's pages and on invalid ones; a product with a query element of 0 is 0, and a head whose sum is NaN counts
 // only where all of them are. As max(q lo, q hi) is q hi for q >= 0 and q lo for q <= 0, the sum is the

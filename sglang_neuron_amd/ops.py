@@ -1507,12 +1507,14 @@ def prefill_attention_blocks(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_
 
 def block_scores(q: Tensor, k_bounds: Tensor, block_table: Tensor, seq_lens: Tensor, *, page_size: int,
                  rows: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
-    """What a page can give a query at the most: (scores [T, G, width] fp32, counts [T] int32), scores[t, g, c] the largest,
-    over the query heads of KV head g, of sum_d max(q_d lo_d, q_d hi_d) with the bounds ``k_bounds`` [blocks, G, 2, d] bf16
+    """What a page's keys can give a query at the most: (scores [T, G, width] fp32, counts [T] int32), scores[t, g, c] the
+    largest, over the query heads of KV head g, of sum_d max(q_d lo_d, q_d hi_d) with the bounds ``k_bounds`` [blocks, G, 2, d] bf16
     (kv_store_blocks) of the page in column c of query t's table row; -inf past the row's ceil(seq_lens / page_size) = counts
-    pages and where the table names no page. A product with q_d = 0 is 0; where a head takes an infinite key's bound, or one of
-    a dimension whose keys are all NaN, its sum is infinite; a head whose sum is NaN counts only where all of them are. The
-    other arguments are paged_decode_blocks'."""
+    pages and where the table names no page. The bounds are of the keys as given: the codes of an FP8 or int8 cache hold each
+    element to within 2^-4 of itself (or 2^-10 of its block's scale) or half a scale, and to as much again each time the scale
+    grew since, so a key as attended can exceed its page's score by that, times |q_d|. A product with q_d = 0 is 0; where a head
+    takes an infinite key's bound, or one of a dimension whose keys are all NaN, its sum is infinite; a head whose sum is NaN
+    counts only where all of them are. The other arguments are paged_decode_blocks'."""
     dev = _on_gpu(q, k_bounds, block_table, seq_lens, rows)
     q, table, stride, lens, rows = _query_rows(q, block_table, seq_lens, rows)
     T, H, d = q.shape

@@ -70,6 +70,42 @@ def test_bounds_hold_every_key():
     assert ob.scores(q, bounds, table, [0], 16)[2] == [0]
 
 
+@pytest.mark.parametrize("dtype", [ob.FP8, torch.int8])
+def test_cached_keys_pass_their_bounds_by_their_roundings(dtype):
+    """Scores bound the keys as given. A cached key passes its page's by no more than its codes' roundings, one for each scale
+    that its block has had (their halves of a step: 2^-4 of the element or 2^-10 of the scale, half a scale), and some do."""
+    g = gen(4)
+    for seed in range(20):
+        cache, scale = torch.zeros(2, 1, 16, 8).to(dtype), torch.zeros(2, 1, 1)
+        bounds, table = torch.zeros(2, 1, 2, 8, dtype=torch.bfloat16), torch.tensor([[1]])
+        keys = (torch.randn(16, 1, 8, generator=g) * torch.linspace(1, 1 + seed / 4, 16).view(16, 1, 1)).to(torch.bfloat16)
+        slack = torch.zeros(16, 8, dtype=torch.float64)
+        for at in range(16):
+            had = float(scale[1])
+            ob.append(cache, scale, keys[at:at + 1], table, [0, 1], [at], bounds)
+            s = float(scale[1])
+            x = keys[:at + 1, 0].double().abs() + slack[:at + 1]
+            half = torch.maximum(x * 2.0 ** -4, torch.tensor(s * 2.0 ** -10)) if dtype == ob.FP8 else torch.full_like(x, s / 2)
+            slack[:at] += half[:at] if s > had else 0.0
+            slack[at] = half[at]
+        q = torch.randn(1, 1, 8, generator=g).to(torch.bfloat16)
+        score = ob.scores(q, bounds, table, [16], 16)[0][0, 0, 0]
+        got = (cache[1, 0].double() * float(scale[1])) @ q[0, 0].double()
+        assert bool(((keys[:, 0].double() @ q[0, 0].double()) <= score).all())
+        assert bool((got <= score + (1 + 2.0 ** -20) * (slack @ q[0, 0].double().abs())).all())
+    # the one key of a page passes its score by the rounding of its second element, for a query of that or the other sign
+    cache, scale = torch.zeros(2, 1, 16, 8).to(dtype), torch.zeros(2, 1, 1)
+    bounds = torch.zeros(2, 1, 2, 8, dtype=torch.bfloat16)
+    key = torch.zeros(1, 1, 8, dtype=torch.bfloat16)
+    key[0, 0, 0], key[0, 0, 1] = 100.0, 1.2
+    ob.append(cache, scale, key, torch.tensor([[1]]), [0, 1], [0], bounds)
+    q = torch.zeros(2, 1, 8, dtype=torch.bfloat16)
+    q[0, 0, 1], q[1, 0, 1] = 1.0, -1.0
+    score = ob.scores(q, bounds, torch.tensor([[1], [1]]), [1, 1], 16)[0][:, 0, 0]
+    got = q[:, 0].double() @ (cache[1, 0, 0].double() * float(scale[1]))
+    assert int((got > score).sum()) == 1
+
+
 def test_scores_of_infinite_bounds():
     """A bound that a query element does not take, or takes times 0, does not count; one that counts makes the score infinite."""
     inf = math.inf
