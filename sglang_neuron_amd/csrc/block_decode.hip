@@ -830,8 +830,10 @@ static void launch_block_decode_format(const BlockDecodeArgs& a, int32_t dtype, 
 //   Rows of unequal lengths: 4 waves, some 1024 workgroups, so that the short ones even the long ones out (24 rows of 1000 to
 //   4096 keys: 2, 4 and 8 splits on 4 waves 40.5, 33.3, 34.6 us, on 8 waves 43.2, 40.4, 47.7; 40 of 200 to 8000: whole 128, 3
 //   splits 85, 6 78; 16 of 4096: 2, 4, 8, 16 splits 31.6, 28.5, 28.9, 33.5). Where whole rows fill the card they stay whole (64
-//   rows of 4096: 89.5, two splits 93.7), above that up to three rounds of them are halved (70 of 100 to 6000: 131 and 103; 100
-//   of 500 to 2000: 61.8 and 60.8).
+//   rows of 4096: 82.4, two splits 85.7, four 84.9; 56 such rows 74.0, 80.4, 75.1; of 1024 keys 25.7, 29.8, 30.5), above that up to
+//   three rounds of them are halved (70 of 100 to 6000: 131 and 103; 100 of 500 to 2000: 61.8 and 60.8). Ragged rows pay for
+//   staying whole: 64 of 100 to 6000 whole, two and four splits 91.2, 91.5, 77.7, in bf16 158, 145, 134; 63 of 500 and one of 16384
+//   217, 160, 87. What a launch knows beforehand does not tell the two kinds apart.
 // The card holds 512 workgroups of 4 waves at head dim 128 (FP8 768), 1024 at 64. A split has 4 tiles at the least.
 // table_rows: of a call whose queries share rows and take listed pages (rows and blocks given), else 0.
 struct BlockShape {

@@ -153,7 +153,8 @@ __device__ __forceinline__ PrefillBlock prefill_block(const PrefillArgs& a, int3
 // the partials of 32 items 1 us of the launch and the merge pass 5 us. w numbers the items KV head by KV head, then pair
 // by pair (request-major), a pair's splits in order. Every lane gets the same values; false past the last item.
 // HALF: partials of half that size (block scales at head dim 64; 24 / 4 heads, int8, 3 chunks of up to 635 after up to 1635: 53.0
-// -> 45.7 us).
+// -> 45.7 us, of 300 to 635 39.1 -> 37.1; the two prices seldom choose differently: 11 other batches of int8 and 12 of FP8, 24 / 4
+// and 8 / 1 heads, one to four chunks of 64 to 2048 after 0 to 7680, are within 1% by either, as are 12 of head dim 128).
 template <bool HALF>
 __device__ bool prefill_item(const PrefillArgs& a, int32_t& w, int32_t& g, int32_t& r, int32_t& bx, int32_t& split,
                              int32_t& st_out, int32_t& ns) {
