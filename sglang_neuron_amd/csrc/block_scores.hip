@@ -35,6 +35,8 @@ struct BlockScoreArgs {
 // The sums of a lane's pages (4 g4 + r, whose bounds are at the lanes' `at`) and head (elements qp) by their definition, one
 // element after the other: where bounds are infinite (infinite keys; lo = inf, hi = -inf: a dimension whose keys are all NaN),
 // as their products with the zeros of [min(q, 0), max(q, 0)] are NaN.
+// Its loads wait for each other: 64 rows of 16384 keys, 15 us, take 65 with such a bound in every 16th page, 75 in every page; as
+// products of cleaned bounds and of counts of the infinite ones it took 95 registers, where 58 keep 8 waves a SIMD for all calls.
 template <int D>
 __device__ __forceinline__ f32x4_t block_scores_defined(const uint16_t* bounds, int64_t at, const uint16_t* qp) {
   const int lane = threadIdx.x & 63, g4 = lane >> 4;
