@@ -10,7 +10,7 @@
 // same dimensions, and gets pages 4 g4 + r of head li; the heads' maximum is taken over the 16 lanes of a row.
 //
 // What bounds it: reads of 512 bytes (head dim 128) at random places, the query's length and the table before them. 64 rows of
-// 16384 keys in pages of 64, 8 KV heads: 13.9-14.8 us, 68 MB, 4.6-4.9 TB/s; one row of 131071 in pages of 32, 17 MB, 6.2. Two or
+// 16384 keys in pages of 64, 8 KV heads: 12.9-14.1 us, 68 MB, 4.8-5.3 TB/s; one row of 131071 in pages of 32, 17 MB, 6.2. Two or
 // four groups of 16 pages a wave, all asked for at once: the same, and slower for one row (P = 128: 3.9, 5.7 and 8.1).
 #include "sna_device.h"
 #include "sna_host.h"
